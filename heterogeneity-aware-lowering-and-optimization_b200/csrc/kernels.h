@@ -272,4 +272,36 @@ int nms(int B, int C, int N, int max_sel, float iou_thr, float score_thr, int bo
 int yolo_postprocess(int cls, const int* S3, const void* const* heads, int dt, const int* nchw3, const unsigned* anchors18, const unsigned* img_w,
                      const unsigned* img_h, float* boxes, float* scores, int* sel, int* cnt, float* info, unsigned* num, cudaStream_t stream);
 
+// ---- a decoder's serving step ----
+// Rows (token, head) of `channels` values whose first 2 * pairs channels turn by position * frequency (kernels_rotary.cu).  Part 0: `heads`
+// rows of each of batch * tokens tokens; parts 1 and 2 (batch 1): kv_heads rows of keys, which turn, and of values, which do not,
+// to the page and place that slots[token] names, if the cache has it.
+struct TurnGeom {
+  const void* src[3];
+  void* dst[3];
+  int64_t s_batch, s_token[3], s_head[3], d_batch, d_token, d_head, c_page, c_token, c_head;
+  int batch, tokens, heads, kv_heads, channels, pairs, interleaved, pages, page_size;
+  int heads_outside;               // rows of one head lie closer together than those of one token
+  const int* positions;            // [axes][batch * tokens]
+  const long long* slots;
+  uint64_t frequency[128];         // turns per position in units of 2^-64
+  unsigned char axis[128];
+};
+int turn_rows(const TurnGeom& g, int dt, cudaStream_t stream);
+
+// Attention of `queries` tokens per sequence over a paged cache (kernels_paged_attention.cu); strides in elements.
+struct PagedAttention {
+  int dt, batch, queries, heads, kv_heads, channels, pages, page_size, prefix_length, table_width;
+  float scale;
+  int64_t c_page, c_head, c_token, q_batch, q_token, q_head, y_batch, y_token, y_head;
+};
+int64_t paged_attention_workspace(const PagedAttention& a);
+int paged_attention(const PagedAttention& a, const void* key_cache, const void* value_cache, const void* q, const int* prefix_pages, const int* page_table,
+                    const int* lengths, void* y, void* workspace, cudaStream_t stream);
+
+// The next token of each row of logits (kernels_sample.cu).
+constexpr int kMaxVocab = 1 << 18;
+int sample(int dt, int rows, int vocab, int64_t row, const void* logits, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+           const float* uniform, int* tokens, cudaStream_t stream);
+
 }  // namespace b200

@@ -1,0 +1,395 @@
+// Attention over a paged cache whose sequences share their first positions.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 16, kStep = 32;   // rows of a tile; positions a warp takes at a time
+constexpr int kRing = 3;                                                    // units of kStep rows of keys or of values, per warp
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  PagedAttention a;
+  const void *k, *v, *q;
+  const int *prefix_pages, *page_table, *lengths;
+  void* y;
+  float* part;                       // [rows][slots][channels], then float2 [rows][slots]: maximum (of base-2 exponents) and sum
+  float2* stat;
+  int group, rows;                   // query heads of a cache head; rows of one cache head = batch * queries * group
+  int prefix_chunk, prefix_chunks, own_chunk, own_chunks, slots;
+  int prefix_tiles, own_tiles;       // tiles of 16 rows: over all rows, and over those of one sequence
+  float scale_log2e;
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {   // adds the values as rounded
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    sum += f.x + f.y;
+    return *(const uint32_t*)&h;
+  }
+  static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+};
+template <> struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const uint32_t u = *(const uint32_t*)&h;
+    sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+    return u;
+  }
+  static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes, or zeros (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool any) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(any ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  return x;
+}
+__device__ __forceinline__ int own_length(const Params& p, int b) {
+  const long long cap = (long long)p.a.table_width * p.a.page_size;
+  const int n = p.lengths[b];
+  return n < 0 ? 0 : n > cap ? (int)cap : n;
+}
+
+// A tile of up to 16 rows (query, query head) of one cache head against one chunk of positions, of the prefix or of one sequence.
+// Bound by the cache's bytes: 16 rows do 16 products for each two bytes read, far below what the tensor cores could do, so that the
+// kernel's work is to keep loads in flight.  Each warp has positions and a ring of its own: no warp waits for another until
+// the end.  The ring's units alternate keys and values of 32 positions; two of the three are always in flight.
+// Softmax runs over positions with maximum and sum per row; the weights are rounded to the cache's type for the second product, and the
+// sum is taken of the rounded ones, so that the result is an average of values with weights that add up to one.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kPieces = D / 8, kUnit = kStep * D * 2;   // 16-byte pieces of a row; bytes of a unit
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+  // what this block works on
+  int item = blockIdx.x;
+  const int prefix_items = p.prefix_tiles * p.prefix_chunks;
+  const bool own = item >= prefix_items;
+  const int* pages;
+  int row0, n_rows, begin, end, slot, length = 0;
+  if (!own) {
+    const int chunk = item / p.prefix_tiles, tile = item - chunk * p.prefix_tiles;
+    row0 = tile * kRows;
+    n_rows = min(kRows, p.rows - row0);
+    begin = chunk * p.prefix_chunk;
+    end = min(begin + p.prefix_chunk, p.a.prefix_length);
+    pages = p.prefix_pages;
+    slot = chunk;
+  } else {
+    item -= prefix_items;
+    const int b = item % p.a.batch, rest = item / p.a.batch, chunk = rest / p.own_tiles, tile = rest - chunk * p.own_tiles;
+    const int per = p.a.queries * p.group;
+    row0 = b * per + tile * kRows;
+    n_rows = min(kRows, per - tile * kRows);
+    length = own_length(p, b);
+    begin = chunk * p.own_chunk;
+    end = min(begin + p.own_chunk, length);
+    if (begin >= end) return;   // (the sum over slots knows)
+    pages = p.page_table + (int64_t)b * p.a.table_width;
+    slot = p.prefix_chunks + chunk;
+  }
+  // the rows this lane has a share of: row0 + lane / 4 and + 8
+  int limit[2];
+  uint32_t qa[D / 16][4];
+  {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (lane >> 2) + 8 * h;
+      const bool live = r < n_rows;
+      const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
+      limit[h] = !live ? 0 : own ? length - p.a.queries + j + 1 : p.a.prefix_length;
+      const T* q = (const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qa[k][h] = live ? *(const uint32_t*)(q + k * 16 + (lane & 3) * 2) : 0u;
+        qa[k][h + 2] = live ? *(const uint32_t*)(q + k * 16 + 8 + (lane & 3) * 2) : 0u;
+      }
+    }
+  }
+  // positions below `all` are seen by every row of the tile
+  int all = own ? length - p.a.queries + row0 / p.group % p.a.queries + 1 : p.a.prefix_length;
+  const int n_steps = (end - begin + kStep - 1) / kStep;
+  const uint32_t ring = shared_address(smem) + warp * (kRing * kUnit);
+
+  const T *kc = (const T*)p.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.v + (int64_t)head * p.a.c_head;
+  int64_t off = -1;
+  // unit u: keys (u even) or values (u odd) of this warp's step u / 2; returns which of the 32 positions can be seen at all
+  auto issue = [&](int u) -> uint32_t {
+    uint32_t seen = 0;
+    const int step = warp + (u >> 1) * kWarps;
+    if (step < n_steps) {
+      if (!(u & 1)) {
+        const int pos = begin + step * kStep + lane;
+        off = -1;
+        if (pos < end) {
+          const int n = pos / p.a.page_size, page = pages[n];
+          if (page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos - n * p.a.page_size) * p.a.c_token;
+        }
+        seen = __ballot_sync(~0u, off >= 0);
+      }
+      const T* base = (u & 1) ? vc : kc;
+      const uint32_t dst = ring + (u % kRing) * kUnit;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
+        const int64_t o = __shfl_sync(~0u, off, r);
+        copy16(dst + r * (D * 2) + ((c ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
+      }
+    }
+    copies_commit();
+    return seen;
+  };
+
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+  uint32_t seen = issue(0);
+  issue(1);
+  uint32_t next = issue(2);
+  for (int i = 0, step = warp; step < n_steps; ++i, step += kWarps) {
+    const int at = begin + step * kStep;
+    copies_wait<2>();
+    __syncwarp();
+    const uint32_t ku = ring + (2 * i % kRing) * kUnit, vu = ring + ((2 * i + 1) % kRing) * kUnit;
+    float s[kStep / 8][4];
+#pragma unroll
+    for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
+#pragma unroll
+    for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {   // 8 positions x 32 channels
+        uint32_t b[4];
+        const int r = n * 8 + (lane & 7), c = k * 4 + (lane >> 3);
+        ldmatrix4<false>(b, ku + r * (D * 2) + ((c ^ (r & 7)) << 4));
+        Mma<T>::run(s[n], qa[2 * k], b[0], b[1]);
+        Mma<T>::run(s[n], qa[2 * k + 1], b[2], b[3]);
+      }
+    __syncwarp();
+    issue(2 * i + 3);
+    // scores in powers of two; a position that is not seen has none
+    const bool masked = seen != ~0u || at + kStep > all;
+    float mx[2] = {m[0], m[1]};
+#pragma unroll
+    for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int pos = n * 8 + (lane & 3) * 2 + (k & 1);
+        s[n][k] *= p.scale_log2e;
+        if (masked && (!(seen >> pos & 1) || at + pos >= limit[k >> 1])) s[n][k] = -INFINITY;
+        mx[k >> 1] = fmaxf(mx[k >> 1], s[n][k]);
+      }
+    float base[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 2));
+      base[h] = mx[h] == -INFINITY ? 0.f : mx[h];
+      const float corr = exp2_fast(m[h] - base[h]);   // 0 at first
+      m[h] = mx[h];
+      l[h] *= corr;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= corr; o[n][2 * h + 1] *= corr; }
+    }
+    uint32_t pa[kStep / 16][4];
+#pragma unroll
+    for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        pa[n >> 1][(n & 1) * 2 + h] = Mma<T>::pack(exp2_fast(s[n][2 * h] - base[h]), exp2_fast(s[n][2 * h + 1] - base[h]), l[h]);
+    copies_wait<2>();
+    __syncwarp();
+    if (at + kStep <= all || !own) {
+#pragma unroll
+      for (int k = 0; k < kStep / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {   // 16 positions x 16 channels
+          uint32_t b[4];
+          const int r = k * 16 + (lane & 15), c = n * 2 + (lane >> 4);
+          ldmatrix4<true>(b, vu + r * (D * 2) + ((c ^ (r & 7)) << 4));
+          Mma<T>::run(o[2 * n], pa[k], b[0], b[1]);
+          Mma<T>::run(o[2 * n + 1], pa[k], b[2], b[3]);
+        }
+    } else {
+      // Positions that later queries of the tile see and earlier ones do not: a weight of zero does not hide an infinity there, so each
+      // query has its product with the values that it sees, and the other rows take nothing of it.
+      const int q0 = row0 / p.group, q1 = (row0 + n_rows - 1) / p.group;
+      for (int qi = q0; qi <= q1; ++qi) {
+        const int lim = length - p.a.queries + qi % p.a.queries + 1 - at;
+        const bool mine[2] = {(row0 + (lane >> 2)) / p.group == qi, (row0 + (lane >> 2) + 8) / p.group == qi};
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k) {
+          const int pos = k * 16 + (lane & 3) * 2;
+          const uint32_t keep0 = (pos < lim ? 0xffffu : 0u) | (pos + 1 < lim ? 0xffff0000u : 0u), keep1 = (pos + 8 < lim ? 0xffffu : 0u) | (pos + 9 < lim ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            uint32_t b[4];
+            const int r = k * 16 + (lane & 15), c = n * 2 + (lane >> 4);
+            ldmatrix4<true>(b, vu + r * (D * 2) + ((c ^ (r & 7)) << 4));
+            float t[2][4] = {};
+            Mma<T>::run(t[0], pa[k], b[0] & keep0, b[1] & keep1);
+            Mma<T>::run(t[1], pa[k], b[2] & keep0, b[3] & keep1);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (mine[(x & 3) >> 1]) o[2 * n + (x >> 2)][x & 3] += t[x >> 2][x & 3];
+          }
+        }
+      }
+    }
+    __syncwarp();
+    seen = next;
+    next = issue(2 * i + 4);
+  }
+  copies_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(~0u, l[h], 1);
+    l[h] += __shfl_xor_sync(~0u, l[h], 2);
+  }
+  // ---- the four warps' results become one ----
+  __syncthreads();
+  float* so = (float*)smem;                                 // [warp][16 rows][D + 4]: the padding spreads rows over the banks
+  float2* sm = (float2*)(so + kWarps * kRows * (D + 4));    // [warp][16]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) *(float2*)&so[(warp * kRows + r) * (D + 4) + n * 8 + (lane & 3) * 2] = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    if ((lane & 3) == 0) sm[warp * kRows + r] = make_float2(m[h], l[h]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 st = sm[w * kRows + r];
+      const float f = exp2_fast(st.x - base);
+      const float4 x = *(const float4*)&so[(w * kRows + r) * (D + 4) + c];
+      sum += f * st.y;
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    const int row = row0 + r;
+    const int64_t at = ((int64_t)head * p.rows + row) * p.slots + slot;
+    *(float4*)(p.part + at * D + c) = acc;
+    if (c == 0) p.stat[at] = make_float2(top, sum);
+  }
+}
+
+// The sum over a row's slots; a warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);   // head * rows + row
+  if (id >= (int64_t)p.rows * p.a.kv_heads) return;
+  const int head = (int)(id / p.rows), row = (int)(id - (int64_t)head * p.rows);
+  const int g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
+  const int used = p.prefix_chunks + (p.own_chunks ? (own_length(p, b) + p.own_chunk - 1) / p.own_chunk : 0);
+  const float2* stat = p.stat + id * p.slots;
+  const float* part = p.part + id * p.slots * D;
+  constexpr int N = D / 32;
+  float top = -INFINITY;
+  for (int i = lane; i < used; i += 32) top = fmaxf(top, stat[i].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
+  for (int i = 0; i < used; ++i) {
+    const float2 st = stat[i];
+    const float f = exp2_fast(st.x - base);
+    sum += f * st.y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] += f * part[(int64_t)i * D + lane * N + k];
+  }
+  T* y = (T*)p.y + b * p.a.y_batch + j * p.a.y_token + (int64_t)(head * p.group + g) * p.a.y_head + lane * N;
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[k] = Mma<T>::narrow(sum == 0.f ? 0.f : acc[k] / sum);
+}
+
+Params plan(const PagedAttention& a) {
+  Params p{};
+  p.a = a;
+  p.group = a.heads / a.kv_heads;
+  p.rows = a.batch * a.queries * p.group;
+  p.scale_log2e = a.scale * kLog2e;
+  p.prefix_tiles = (p.rows + kRows - 1) / kRows;
+  p.own_tiles = (a.queries * p.group + kRows - 1) / kRows;
+  const int64_t own_max = (int64_t)a.table_width * a.page_size;
+  auto chunk_of = [&](int64_t positions, int64_t tiles) {
+    int64_t chunk = 4096;
+    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < 2 * 148) chunk /= 2;
+    return (int)chunk;
+  };
+  p.prefix_chunk = chunk_of(a.prefix_length, p.prefix_tiles);
+  p.prefix_chunks = (a.prefix_length + p.prefix_chunk - 1) / p.prefix_chunk;
+  p.own_chunk = chunk_of(own_max, (int64_t)p.own_tiles * a.batch);
+  p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
+  p.slots = p.prefix_chunks + p.own_chunks;
+  return p;
+}
+
+template <typename T, int D> int launch(const Params& p, cudaStream_t stream) {
+  const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
+  if (items >= (1ll << 31)) return -1;
+  constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
+  if (items) {
+    if (cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
+    tile_kernel<T, D><<<dim3((unsigned)items, (unsigned)p.a.kv_heads), kThreads, smem, stream>>>(p);
+  }
+  const int64_t ids = (int64_t)p.rows * p.a.kv_heads;
+  join_kernel<T, D><<<(unsigned)((ids + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace
+
+int64_t paged_attention_workspace(const PagedAttention& a) {
+  if (a.batch == 0) return 0;
+  const Params p = plan(a);
+  return (int64_t)p.rows * a.kv_heads * p.slots * ((int64_t)a.channels * 4 + 8);
+}
+
+int paged_attention(const PagedAttention& a, const void* key_cache, const void* value_cache, const void* q, const int* prefix_pages, const int* page_table, const int* lengths,
+                    void* y, void* workspace, cudaStream_t stream) {
+  Params p = plan(a);
+  p.k = key_cache; p.v = value_cache; p.q = q; p.y = y;
+  p.prefix_pages = prefix_pages; p.page_table = page_table; p.lengths = lengths;
+  p.part = (float*)workspace;
+  p.stat = (float2*)(p.part + (int64_t)p.rows * a.kv_heads * p.slots * a.channels);
+  if (a.dt == DT_F16) return a.channels == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);
+  return a.channels == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);
+}
+
+}  // namespace b200

@@ -81,6 +81,48 @@ class ConvDesc(C.Structure):
                [("alpha", C.c_float), ("res_scale", C.c_float), ("out_scale", C.c_float), ("out_multiply", C.c_int)]
 
 
+class RotarySpec(C.Structure):
+    """odla_b200_rotary_spec; see rotary_spec()."""
+    _fields_ = [("pairs", C.c_int), ("interleaved", C.c_int), ("axes", C.c_int), ("axis", C.c_ubyte * 128), ("frequency", C.c_double * 128)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "tokens", "heads", "channels")] + \
+               [(n, C.c_longlong) for n in ("x_batch", "x_token", "x_head", "y_batch", "y_token", "y_head")]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "pages", "page_size", "heads", "channels")] + [(n, C.c_longlong) for n in ("page", "head", "token")]
+
+
+class AppendDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("tokens", "heads")] + \
+               [(n, C.c_longlong) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "y_token", "y_head")]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "queries", "heads", "prefix_length", "table_width")] + [("scale", C.c_float)] + \
+               [(n, C.c_longlong) for n in ("q_batch", "q_token", "q_head", "y_batch", "y_token", "y_head")]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "rows", "vocab")] + [("row", C.c_longlong)]
+
+
+def rotary_spec(frequency, axis=None, interleaved=False):
+    """The odla_b200_rotary_spec whose pair i turns by position[axis[i]] * frequency[i] radians (axis None: one axis)."""
+    frequency = [float(f) for f in frequency]
+    axis = [0] * len(frequency) if axis is None else [int(a) for a in axis]
+    if len(axis) != len(frequency) or len(frequency) > 128:
+        raise ValueError("rotary_spec: at most 128 pairs, one axis for each")
+    if any(a < 0 or a > 3 for a in axis):
+        raise ValueError("rotary_spec: axes are 0 ... 3")
+    s = RotarySpec(pairs=len(frequency), interleaved=int(bool(interleaved)), axes=max(axis, default=0) + 1)
+    for i, (f, a) in enumerate(zip(frequency, axis)):
+        s.frequency[i], s.axis[i] = f, a
+    return s
+
+
 def shape(dims):
     s = Shape()
     s.size = len(dims)
@@ -188,6 +230,11 @@ _OPTIONAL = {
     "odla_b200_conv_umma": (C.c_int, [C.POINTER(ConvDesc), _V, _V, _V, _V, _V, _V, _V]),
     "odla_b200_attention": (C.c_int, [C.c_int, _V, _V, _V, _V, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, _V]),
     "odla_b200_reduce_mean_noalloc": (C.c_int, [_V, _V, C.c_int, C.POINTER(C.c_longlong), C.c_int, C.POINTER(C.c_int), C.c_int, _V]),
+    "odla_b200_rotary": (C.c_int, [C.POINTER(RotarySpec), C.POINTER(RotaryDesc), _V, _V, _V, _V]),
+    "odla_b200_paged_append": (C.c_int, [C.POINTER(PagedCache), _V, _V, C.POINTER(AppendDesc), C.POINTER(RotarySpec), _V, _V, _V, _V, _V, _V, _V]),
+    "odla_b200_paged_attention_workspace": (C.c_longlong, [C.POINTER(PagedCache), C.POINTER(PagedAttentionDesc)]),
+    "odla_b200_paged_attention": (C.c_int, [C.POINTER(PagedCache), _V, _V, C.POINTER(PagedAttentionDesc), _V, _V, _V, _V, _V, _V, C.c_longlong, _V]),
+    "odla_b200_sample": (C.c_int, [C.POINTER(SampleDesc), _V, _V, _V, _V, _V, _V, _V, _V]),
     "odla_cpuref_UsesReference": (C.c_int, []),
     "odla_cpuref_Threads": (C.c_int, []),
     "odla_cpuref_GetAccumulators": (C.c_longlong, [_V, C.c_char_p, _V, C.c_longlong]),

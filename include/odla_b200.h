@@ -493,6 +493,112 @@ int odla_b200_attention(int dtype, const void* q, const void* k, const void* v, 
 int odla_b200_reduce_mean_noalloc(const void* x, void* y, int dtype, const long long* dims, int rank,
                                   const int* axes, int n_axes, void* stream);
 
+/* ---- serving a decoder ---------------------------------------------------------------------
+ * Four raw entry points for what a decoder does between its matrix products; none has a counterpart in the reference,
+ * whose models have no cache.  odla_b200_paged_append turns the new tokens' queries and keys by their positions and puts
+ * keys and values into a paged cache, odla_b200_paged_attention reads the cache, odla_b200_sample chooses the next tokens
+ * from the logits; odla_b200_rotary turns tensors that no cache keeps (an encoder over pictures or clips).
+ *
+ * They take DEVICE pointers on the current device, only enqueue kernels on `stream` (a cudaStream_t as void*, NULL = the default
+ * stream, of the same device) and allocate nothing, so they can be captured into a CUDA graph; descriptors are host memory
+ * and are read during the call.  dtype: 0 = fp32, 1 = fp16, 2 = bf16.  Strides count elements and are not negative; channels are
+ * contiguous.  Any strides and any pointers aligned to the element are served; 16-byte alignment of pointers and
+ * strides is faster (odla_b200_paged_attention asks for it).  They return 0, -1 (bad argument, nothing enqueued) or -2 (CUDA
+ * error).  Zero tokens, sequences or rows are a valid call that does nothing. */
+
+/* Which channels turn, and how fast.  Pair i is channels (2i, 2i + 1) of a head when `interleaved`, else (i, i + pairs); channels
+ * from 2 * pairs on stay as they are.  It turns by position[axis[i]] * frequency[i] radians (any finite frequency; positions
+ * are int32 and may be negative), reduced exactly, so that far positions are as accurate as near ones:
+ *   (a, b) -> (a cos - b sin, a sin + b cos).
+ * Opposite frequencies turn back. */
+#define ODLA_B200_MAX_ROTARY_PAIRS 128
+typedef struct {
+  int pairs;        /* 0 ... 128 */
+  int interleaved;
+  int axes;         /* 1 ... 4 */
+  unsigned char axis[ODLA_B200_MAX_ROTARY_PAIRS];   /* of each pair, below `axes` */
+  double frequency[ODLA_B200_MAX_ROTARY_PAIRS];     /* radians per position */
+} odla_b200_rotary_spec;
+
+typedef struct {
+  int dtype;
+  int batch, tokens, heads, channels;                /* channels 1 ... 1024 */
+  long long x_batch, x_token, x_head;                /* x[b * x_batch + t * x_token + h * x_head + channel] */
+  long long y_batch, y_token, y_head;
+} odla_b200_rotary_desc;
+
+/* y = x turned.  positions: [axes][batch * tokens].  y may be x with the same strides; other overlaps are not allowed. */
+int odla_b200_rotary(const odla_b200_rotary_spec* spec, const odla_b200_rotary_desc* desc, const void* x, void* y,
+                     const int* positions, void* stream);
+
+/* A paged cache: keys and values each hold `pages` pages of `page_size` positions,
+ * cache[p * page + i * token + h * head + channel]: both [pages][page_size][heads][channels] and [pages][heads][page_size][channels]
+ * are such layouts.  A slot is p * page_size + i. */
+typedef struct {
+  int dtype;
+  int pages, page_size, heads, channels;
+  long long page, head, token;
+} odla_b200_paged_cache;
+
+/* The new tokens of a step, of any number of sequences: token t has query rows q[t * q_token + h * q_head] (heads of them, 0 for none)
+ * and key and value rows k[t * k_token + h * k_head], v[...] (cache->heads of them); all three may be column groups of one
+ * projection's rows. */
+typedef struct {
+  int tokens, heads;
+  long long q_token, q_head, k_token, k_head, v_token, v_head, y_token, y_head;
+} odla_b200_append_desc;
+
+/* Queries and keys turned (spec NULL: not turned), queries to q_out (y strides; q_out may be q with the same strides), keys and values
+ * to slot slots[t] of the caches.  positions: [axes][tokens], may be NULL without spec.  A token whose slot is negative, or not a slot of
+ * the cache, is not kept (its queries are still turned): that is how a padded batch ends.  Two tokens of one call must not
+ * name the same slot. */
+int odla_b200_paged_append(const odla_b200_paged_cache* cache, void* key_cache, void* value_cache, const odla_b200_append_desc* desc,
+                           const odla_b200_rotary_spec* spec, const void* q, const void* k, const void* v, void* q_out,
+                           const int* positions, const long long* slots, void* stream);
+
+/* Attention of the last `queries` tokens of each of `batch` sequences (1 when decoding, more when drafted tokens are checked).
+ * Every sequence begins with the same prefix_length positions, which lie on prefix_pages[0 ...]; sequence b goes on with
+ * lengths[b] positions of its own on page_table[b * table_width ...], the last `queries` of them the tokens that ask.  Query j
+ * sees the prefix and own positions 0 ... lengths[b] - queries + j.  Query heads come in equal groups, one for each head
+ * of the cache. */
+typedef struct {
+  int batch, queries, heads;
+  int prefix_length, table_width;
+  float scale;
+  long long q_batch, q_token, q_head, y_batch, y_token, y_head;
+} odla_b200_paged_attention_desc;
+
+/* y = softmax(scale * q k^T) v over what each query sees, the prefix read once for the whole batch.  dtype fp16 or bf16,
+ * channels 64 or 128, q, y, caches 16-byte aligned with strides that are multiples of 8 elements, heads a multiple of
+ * cache->heads.  A query that sees nothing gets zeros (lengths[b] <= 0 and no prefix: a padded batch).  Own lengths beyond
+ * table_width pages count as table_width pages; positions on a page that the cache does not have (a negative entry) are
+ * not seen.  What the cache holds in slots that no query sees may be anything, NaN included.
+ * lengths, page_table and prefix_pages are device memory and read when the kernels run, so a captured call follows them.
+ * workspace: odla_b200_paged_attention_workspace(cache, desc) bytes (16-byte aligned; -1 for arguments that the call refuses), which need not
+ * be cleared; calls that may run at the same time need one each.  A bounded wait inside the kernel that expires gives rows of NaN. */
+long long odla_b200_paged_attention_workspace(const odla_b200_paged_cache* cache, const odla_b200_paged_attention_desc* desc);
+int odla_b200_paged_attention(const odla_b200_paged_cache* cache, const void* key_cache, const void* value_cache,
+                              const odla_b200_paged_attention_desc* desc, const void* q, const int* prefix_pages,
+                              const int* page_table, const int* lengths, void* y, void* workspace, long long workspace_bytes,
+                              void* stream);
+
+/* One token for each row of logits, logits[r * row + i], i < vocab (at most 262144).  temperature, top_k, top_p, min_p: [rows], each may be
+ * NULL (1, 0, 1, 0: no effect); uniform: [rows], random numbers in [0, 1).  Ties go to the lower index throughout.
+ *   A logit that is NaN or minus infinity is never chosen; a row without any other gives -1.  temperature <= 0 takes the
+ *   largest logit.  Otherwise w = exp((l - max l) / temperature) and these tokens are kept: the top_k largest logits (top_k <= 0: all);
+ *   of those, in descending order, each before which less than top_p of their sum of w has passed (top_p >= 1: all; the
+ *   first always); of those, the ones with w >= min_p (above 1 counts as 1).  With W the sum of w over the tokens kept, the choice is
+ *   the first kept token, by index, at which the running sum of w exceeds uniform * W (the first kept token for uniform <= 0, the last
+ *   one when rounding leaves none).
+ * w is held as a 64-bit whole number of units of 2^-44 of the largest, so that sums do not depend on their order. */
+typedef struct {
+  int dtype;
+  int rows, vocab;
+  long long row;
+} odla_b200_sample_desc;
+int odla_b200_sample(const odla_b200_sample_desc* desc, const void* logits, const float* temperature, const int* top_k,
+                     const float* top_p, const float* min_p, const float* uniform, int* tokens, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
