@@ -2,9 +2,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <algorithm>
+#include <cstdlib>
 
 #include "kernels.h"
+#include "umma_ptx.cuh"
 
 namespace b200 {
 namespace {
@@ -23,11 +24,15 @@ struct Params {
   int group, rows;                   // query heads of a cache head; rows of one cache head = batch * queries * group
   int prefix_chunk, prefix_chunks, own_chunk, own_chunks, slots;
   int prefix_tiles, own_tiles;       // tiles of 16 rows: over all rows, and over those of one sequence
+  int wide_tiles;                    // tiles of 256 rows for the tensor-core kernel, which then takes the prefix; 0: tile_kernel does
   float scale_log2e;
+  uint32_t spin_limit;
+  int test_skip_stage;               // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
 
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -41,6 +46,7 @@ template <> struct Mma<__half> {
   static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 };
 template <> struct Mma<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -306,6 +312,275 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   }
 }
 
+// ---------------------------------------------------------- the prefix on the tensor cores ----
+// Up to 256 rows (query, query head) of one cache head against one chunk of the prefix, 128 positions at a time: two tiles of
+// 128 rows, so that the products of one tile run under the softmax of the other.  S = Q K^T goes to tensor memory; a thread per
+// row turns it into weights, which replace it there as the A operand of O += P V.  O stays in tensor memory over the whole chunk: a
+// row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
+// rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
+// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks).
+// Warps 0-3 and 4-7: softmax of a tile each; 8-11: loads; 12: products.  Keys and values arrive by 16-byte asynchronous copies into
+// the layout the products read (rows of 64 channels, 128-byte swizzle), because a page may end anywhere inside a step; the ring
+// alternates units of 128 keys and 128 values.
+constexpr int kWideRows = 256, kWideStep = 128, kWideRing = 4, kWideThreads = 13 * 32;
+constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
+
+struct WideShared {
+  uint64_t full[kWideRing], empty[kWideRing], q_full, s_full[2], p_full[2], o_done[2], drained;
+  uint32_t seen[4][4];   // which of a step's positions can be seen; a step's words are written at most two steps ahead
+  uint32_t tmem;
+  int abort;
+};
+__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+               "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ WideShared w;
+  constexpr int kBoxes = D / 64, kPieces = D / 8;
+  constexpr uint32_t kUnit = kBoxes * kBox;
+  const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem, s_ring = smem + 2 * kUnit;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y;
+  const int chunk = blockIdx.x / p.wide_tiles, row0 = (blockIdx.x - chunk * p.wide_tiles) * kWideRows;
+  const int n_rows = min(kWideRows, p.rows - row0), tiles = n_rows > 128 ? 2 : 1;
+  const int begin = chunk * p.prefix_chunk, end = min(begin + p.prefix_chunk, p.a.prefix_length), steps = (end - begin + kWideStep - 1) / kWideStep;
+  const uint32_t columns = tiles == 2 ? 512u : 256u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWideRing; ++i) { mbar_init(&w.full[i], 4); mbar_init(&w.empty[i], 1); }
+    mbar_init(&w.q_full, 4 * tiles);
+    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
+    mbar_init(&w.drained, 1);
+    w.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_proxy();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = w.tmem;
+  volatile int* abort_flag = &w.abort;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, nullptr, 0, p.spin_limit); };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, wait(bar, parity)); };   // one answer for the warp
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------- softmax ----
+    const int tile = warp >> 2, quarter = warp & 3, r = tile * 128 + quarter * 32 + lane;
+    if (tile < tiles) {
+      const bool live = r < n_rows;
+      const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
+      const uint4* q = (const uint4*)((const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head);
+      // (a negative scale becomes the sign of the queries: the largest score is then the largest product)
+      const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
+      const uint32_t s_row = s_q + tile * kUnit + (r & 127) * 128;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        uint4 u = live ? q[c] : make_uint4(0, 0, 0, 0);
+        u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_row + (c >> 3) * kBox + (((c & 7) ^ (r & 7)) << 4)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+      }
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w.q_full);
+      const float scale = fabsf(p.scale_log2e);
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16, t_s = tmem + tile * 128 + lanes, t_o = tmem + tiles * 128 + tile * D + lanes;
+      float reference = -INFINITY, sum = 0.f;
+      bool ok = true;
+      for (int i = 0; i < steps; ++i) {
+        if (!warp_wait(&w.s_full[tile], i & 1)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t seen[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) seen[c] = *(volatile uint32_t*)&w.seen[i & 3][c];
+        const bool whole = (seen[0] & seen[1] & seen[2] & seen[3]) == ~0u;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(t_s + c * 32, v);
+          tmem_ld_wait();
+          if (whole) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(v[k]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) if (seen[c] >> k & 1) mx = fmaxf(mx, __uint_as_float(v[k]));
+          }
+        }
+        mx = mx == -INFINITY ? mx : mx * scale;   // (a scale of zero keeps it a number)
+        const bool passed = mx > (i ? reference + 8.f : -INFINITY);
+        if (__any_sync(~0u, passed)) {
+          const float next = passed ? mx : reference, corr = passed ? exp2_fast(reference - mx) : 1.f;
+          reference = next;
+          sum *= corr;
+          if (i) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld32(t_o + c * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t u[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(v[h * 16 + k]) * corr);
+                tmem_st16(t_o + c * 32 + h * 16, u);
+              }
+            }
+            tmem_st_wait();
+          }
+        }
+        const float base = reference == -INFINITY ? 0.f : reference;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32], u[16];
+          tmem_ld32(t_s + c * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float e[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              e[h] = exp2_fast(fmaf(__uint_as_float(v[2 * k + h]), scale, -base));
+              if (!whole && !(seen[c] >> (2 * k + h) & 1)) e[h] = 0.f;
+            }
+            u[k] = Mma<T>::pack(e[0], e[1], sum);
+          }
+          tmem_st16(t_s + c * 16, u);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w.p_full[tile]);
+      }
+      if (ok) ok = warp_wait(&w.o_done[tile], 0);
+      tc_fence_after();
+      const int64_t at = ((int64_t)head * p.rows + row) * p.slots + chunk;
+      if (live) p.stat[at] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld32(t_o + c * 32, v);
+          tmem_ld_wait();
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *(float4*)(p.part + at * D + c * 32 + k * 4) =
+                  make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  } else if (warp < 12) {
+    // --------------------------------------------------------------------- loads ----
+    const int part = warp - 8;
+    const T *kc = (const T*)p.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.v + (int64_t)head * p.a.c_head;
+    int64_t off = -1;
+    bool ok = true;
+    auto announce = [&](int u) {
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0 && !(p.test_skip_stage && blockIdx.x == 0 && u == 1)) mbar_arrive(&w.full[u % kWideRing]);
+    };
+    int u = 0;
+    for (; u < 2 * steps; ++u) {
+      if (!warp_wait(&w.empty[u % kWideRing], ((u / kWideRing) & 1) ^ 1)) { ok = false; break; }
+      if (!(u & 1)) {
+        const int pos = begin + (u >> 1) * kWideStep + part * 32 + lane;
+        off = -1;
+        if (pos < end) {
+          const int n = pos / p.a.page_size, page = p.prefix_pages[n];
+          if (page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos - n * p.a.page_size) * p.a.c_token;
+        }
+        const uint32_t seen = __ballot_sync(~0u, off >= 0);
+        if (lane == 0) *(volatile uint32_t*)&w.seen[(u >> 1) & 3][part] = seen;
+      }
+      const T* base = (u & 1) ? vc : kc;
+      const uint32_t dst = s_ring + (u % kWideRing) * kUnit + part * 32 * 128;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
+        const int64_t o = __shfl_sync(~0u, off, r);
+        copy16(dst + (c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
+      }
+      copies_commit();
+      if (u >= 2) { copies_wait<2>(); announce(u - 2); }
+    }
+    copies_wait<0>();
+    if (ok) {
+      if (u >= 2) announce(u - 2);
+      announce(u - 1);
+    }
+  } else if (elect_one()) {
+    // ------------------------------------------------------------------ products ----
+    const uint32_t fmt = Mma<T>::kBf16 ? 1u : 0u, common = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
+    const uint32_t idesc_s = common | ((uint32_t)(kWideStep >> 3) << 17), idesc_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // (V lies with channels innermost)
+    const uint64_t hi = (uint64_t)(((8u * 128u) >> 4) | (1u << 14) | (2u << 29)) << 32;
+    // the distance between two boxes of channels is only read for V, whose 64-channel groups are a box apart
+    auto desc = [&](uint32_t at, uint32_t lead) { return hi | ((uint64_t)lead << 16) | (uint64_t)((at & 0x3FFFF) >> 4); };
+    bool ok = wait(&w.q_full, 0);
+    auto scores = [&](int i, int t) {   // S_t = Q_t K_i^T
+      const uint32_t k = s_ring + (2 * i % kWideRing) * kUnit, q = s_q + t * kUnit;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n)
+        umma_f16(tmem + t * 128, desc(q + (n >> 2) * kBox + (n & 3) * 32, 1), desc(k + (n >> 2) * kBox + (n & 3) * 32, 1), idesc_s, n ? 1u : 0u);
+      umma_commit(&w.s_full[t]);
+    };
+    if (ok) ok = wait(&w.full[0], 0);
+    if (ok) {
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) scores(0, t);
+      umma_commit(&w.empty[0]);
+    }
+    for (int i = 0; i < steps && ok; ++i) {
+      const int vu = 2 * i + 1, ku = 2 * i + 2;
+      const bool more = i + 1 < steps;
+      for (int t = 0; t < tiles && ok; ++t) {
+        if (t == 0) ok = wait(&w.full[vu % kWideRing], (vu / kWideRing) & 1);
+        ok = ok && wait(&w.p_full[t], i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = s_ring + (vu % kWideRing) * kUnit;
+#pragma unroll
+        for (int n = 0; n < kWideStep / 16; ++n)
+          umma_tmem_a(tmem + tiles * 128 + t * D, tmem + t * 128 + n * 8, desc(v + n * 2048, kBox >> 4), idesc_o, (i || n) ? 1u : 0u);
+        if (t == tiles - 1) umma_commit(&w.empty[vu % kWideRing]);
+        if (!more) { umma_commit(&w.o_done[t]); continue; }
+        if (t == 0) ok = wait(&w.full[ku % kWideRing], (ku / kWideRing) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        scores(i + 1, t);
+        if (t == tiles - 1) umma_commit(&w.empty[ku % kWideRing]);
+      }
+    }
+    if (!ok) { umma_commit(&w.drained); await_landing(&w.drained, 0); }   // products in flight end before their memory goes
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+  }
+}
+
 // The sum over a row's slots; a warp per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
@@ -352,7 +627,21 @@ Params plan(const PagedAttention& a) {
     while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < 2 * 148) chunk /= 2;
     return (int)chunk;
   };
-  p.prefix_chunk = chunk_of(a.prefix_length, p.prefix_tiles);
+  if (a.prefix_length && p.rows > kRows) {
+    // Blocks of equal work on 148 SMs: the number of chunks with the shortest estimate of waves of steps (1.4 us each, 3 us at both ends) and of
+    // the partial results' way to memory and back.
+    p.wide_tiles = (p.rows + kWideRows - 1) / kWideRows;
+    const int tiles = p.wide_tiles * a.kv_heads, all = (a.prefix_length + kWideStep - 1) / kWideStep;
+    double best = 1e30;
+    for (int c = 1; c <= all && c <= 64; ++c) {
+      const int steps = (all + c - 1) / c;
+      const double us = (double)((tiles * (int64_t)c + 147) / 148) * (steps * 1.4 + 3.0) + (double)c * p.rows * a.kv_heads * a.channels * 8 / 5e6;
+      if (us < best) { best = us; p.prefix_chunk = steps * kWideStep; }
+    }
+    p.prefix_tiles = 0;
+  } else {
+    p.prefix_chunk = chunk_of(a.prefix_length, p.prefix_tiles);
+  }
   p.prefix_chunks = (a.prefix_length + p.prefix_chunk - 1) / p.prefix_chunk;
   p.own_chunk = chunk_of(own_max, (int64_t)p.own_tiles * a.batch);
   p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
@@ -363,6 +652,11 @@ Params plan(const PagedAttention& a) {
 template <typename T, int D> int launch(const Params& p, cudaStream_t stream) {
   const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
   if (items >= (1ll << 31)) return -1;
+  if (p.wide_tiles) {
+    constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
+    if (cudaFuncSetAttribute(prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide) != cudaSuccess) { cudaGetLastError(); return -2; }
+    prefix_kernel<T, D><<<dim3((unsigned)(p.wide_tiles * p.prefix_chunks), (unsigned)p.a.kv_heads), kWideThreads, wide, stream>>>(p);
+  }
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
   if (items) {
     if (cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
@@ -386,6 +680,9 @@ int paged_attention(const PagedAttention& a, const void* key_cache, const void* 
   Params p = plan(a);
   p.k = key_cache; p.v = value_cache; p.q = q; p.y = y;
   p.prefix_pages = prefix_pages; p.page_table = page_table; p.lengths = lengths;
+  p.spin_limit = kSpinLimit;
+  p.test_skip_stage = getenv("ODLA_B200_TEST_SKIP_STAGE") != nullptr;
+  if (const char* e = getenv("ODLA_B200_TEST_SPIN_LIMIT")) { const long v = atol(e); if (v >= 64 && v <= (1l << 18)) p.spin_limit = (uint32_t)v; }
   p.part = (float*)workspace;
   p.stat = (float2*)(p.part + (int64_t)p.rows * a.kv_heads * p.slots * a.channels);
   if (a.dt == DT_F16) return a.channels == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);

@@ -157,6 +157,19 @@ def check_attention(odla, lib, case, prefix, scale=None, **kw):
     return y
 
 
+def test_attention_a_wait_that_runs_out_gives_nan_and_the_next_call_is_exact(odla, gpu_lib, monkeypatch):
+    """The hook leaves one unit of the first block's ring unannounced; the products' wait for it ends after 256 attempts."""
+    case = attention_case(1, 24, 1, 8, 2, 128, 16, 600, [30] * 24)
+    monkeypatch.setenv("ODLA_B200_TEST_SKIP_STAGE", "1")
+    monkeypatch.setenv("ODLA_B200_TEST_SPIN_LIMIT", "256")
+    y = R.call_attention(odla, gpu_lib, *case[:4], 600, *case[4:], R.scale_of(128))
+    torch.cuda.synchronize()
+    assert torch.isnan(y).all()
+    monkeypatch.delenv("ODLA_B200_TEST_SKIP_STAGE")
+    monkeypatch.delenv("ODLA_B200_TEST_SPIN_LIMIT")
+    check_attention(odla, gpu_lib, case, 600)
+
+
 SHAPES = [  # batch, queries, heads, kv heads, channels, page, prefix, own lengths
     (1, 1, 1, 1, 64, 16, 0, [1]),
     (1, 1, 2, 1, 128, 16, 1, [0]),
@@ -169,6 +182,9 @@ SHAPES = [  # batch, queries, heads, kv heads, channels, page, prefix, own lengt
     (6, 1, 32, 1, 128, 64, 513, [65, 0, 3, 200, 1, 64]),
     (9, 4, 8, 1, 128, 16, 1025, [4 + 11 * i for i in range(9)]),
     (33, 1, 8, 1, 64, 1, 260, [i % 5 for i in range(33)]),
+    (34, 1, 8, 1, 128, 24, 1500, [i % 7 for i in range(34)]),
+    (70, 2, 4, 1, 128, 16, 129, [2 + i % 9 for i in range(70)]),
+    (24, 1, 6, 1, 64, 100, 2049, [0] * 24),
 ]
 
 
