@@ -24,7 +24,9 @@ struct Params {
   int group, rows;                   // query heads of a cache head; rows of one cache head = batch * queries * group
   int prefix_chunk, prefix_chunks, own_chunk, own_chunks, slots;
   int prefix_tiles, own_tiles;       // tiles of 16 rows: over all rows, and over those of one sequence
-  int wide_tiles;                    // tiles of 256 rows for the tensor-core kernel, which then takes the prefix; 0: tile_kernel does
+  // The tensor-core kernel's tiles of 256 rows: over all rows, for the prefix, and over those of one sequence, for the own positions that all
+  // its queries see (the last queries - 1 positions remain for tile_kernel, in the last slot).  0: tile_kernel takes them all.
+  int wide_tiles, own_wide_tiles, own_wide_chunks, own_wide_chunk;
   float scale_log2e;
   uint32_t spin_limit;
   int test_skip_stage;               // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
@@ -37,13 +39,16 @@ template <> struct Mma<__half> {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t*)&h;
+  }
   static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {   // adds the values as rounded
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
     sum += f.x + f.y;
     return *(const uint32_t*)&h;
   }
-  static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
 };
 template <> struct Mma<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
@@ -51,13 +56,16 @@ template <> struct Mma<__nv_bfloat16> {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t*)&h;
+  }
   static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     const uint32_t u = *(const uint32_t*)&h;
     sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
     return u;
   }
-  static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -81,6 +89,10 @@ __device__ __forceinline__ int own_length(const Params& p, int b) {
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
 
+// Own positions that every query of the sequence sees.
+__device__ __forceinline__ int common_length(const Params& p, int length) { return max(0, length - p.a.queries + 1); }
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // A tile of up to 16 rows (query, query head) of one cache head against one chunk of positions, of the prefix or of one sequence.
 // Bound by the cache's bytes: 16 rows do 16 products for each two bytes read, far below what the tensor cores could do, so that the
 // kernel's work is to keep loads in flight.  Each warp has positions and a ring of its own: no warp waits for another until
@@ -92,6 +104,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kPieces = D / 8, kUnit = kStep * D * 2;   // 16-byte pieces of a row; bytes of a unit
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+  launch_dependents();
   // what this block works on
   int item = blockIdx.x;
   const int prefix_items = p.prefix_tiles * p.prefix_chunks;
@@ -113,11 +126,11 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     row0 = b * per + tile * kRows;
     n_rows = min(kRows, per - tile * kRows);
     length = own_length(p, b);
-    begin = chunk * p.own_chunk;
+    begin = chunk * p.own_chunk + (p.own_wide_tiles ? common_length(p, length) : 0);
     end = min(begin + p.own_chunk, length);
     if (begin >= end) return;   // (the sum over slots knows)
     pages = p.page_table + (int64_t)b * p.a.table_width;
-    slot = p.prefix_chunks + chunk;
+    slot = p.prefix_chunks + p.own_wide_chunks + chunk;
   }
   // the rows this lane has a share of: row0 + lane / 4 and + 8
   int limit[2];
@@ -319,12 +332,14 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
 // rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
 // is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks).
-// Warps 0-3 and 4-7: softmax of a tile each; 8-11: loads; 12: products.  Keys and values arrive by 16-byte asynchronous copies into
+// Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values arrive by 16-byte asynchronous copies into
 // the layout the products read (rows of 64 channels, 128-byte swizzle), because a page may end anywhere inside a step; the ring
 // alternates units of 128 keys and 128 values.
-constexpr int kWideRows = 256, kWideStep = 128, kWideRing = 4, kWideThreads = 13 * 32;
+constexpr int kWideRows = 256, kWideStep = 128, kWideRing = 4, kLoaders = 2, kWideThreads = 12 * 32;
 constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
 
+struct True { static constexpr bool value = true; };
+struct False { static constexpr bool value = false; };
 struct WideShared {
   uint64_t full[kWideRing], empty[kWideRing], q_full, s_full[2], p_full[2], o_done[2], drained;
   uint32_t seen[4][4];   // which of a step's positions can be seen; a step's words are written at most two steps ahead
@@ -343,23 +358,53 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// The wait for a load, naming its registers so that no read of them is scheduled above it.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ WideShared w;
   constexpr int kBoxes = D / 64, kPieces = D / 8;
   constexpr uint32_t kUnit = kBoxes * kBox;
   const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem, s_ring = smem + 2 * kUnit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y;
-  const int chunk = blockIdx.x / p.wide_tiles, row0 = (blockIdx.x - chunk * p.wide_tiles) * kWideRows;
-  const int n_rows = min(kWideRows, p.rows - row0), tiles = n_rows > 128 ? 2 : 1;
-  const int begin = chunk * p.prefix_chunk, end = min(begin + p.prefix_chunk, p.a.prefix_length), steps = (end - begin + kWideStep - 1) / kWideStep;
+  launch_dependents();
+  int row0, n_rows, begin, end, slot;
+  const int* pages;
+  if ((int)blockIdx.x < p.wide_tiles * p.prefix_chunks) {
+    const int chunk = blockIdx.x / p.wide_tiles;
+    row0 = (blockIdx.x - chunk * p.wide_tiles) * kWideRows;
+    n_rows = min(kWideRows, p.rows - row0);
+    begin = chunk * p.prefix_chunk;
+    end = min(begin + p.prefix_chunk, p.a.prefix_length);
+    pages = p.prefix_pages;
+    slot = chunk;
+  } else {
+    const int item = blockIdx.x - p.wide_tiles * p.prefix_chunks, b = item % p.a.batch, rest = item / p.a.batch;
+    const int chunk = rest / p.own_wide_tiles, tile = rest - chunk * p.own_wide_tiles, per = p.a.queries * p.group;
+    row0 = b * per + tile * kWideRows;
+    n_rows = min(kWideRows, per - tile * kWideRows);
+    begin = chunk * p.own_wide_chunk;
+    end = min(begin + p.own_wide_chunk, common_length(p, own_length(p, b)));
+    if (begin >= end) { grid_dependency_wait(); return; }
+    pages = p.page_table + (int64_t)b * p.a.table_width;
+    slot = p.prefix_chunks + chunk;
+  }
+  const int tiles = n_rows > 128 ? 2 : 1, steps = (end - begin + kWideStep - 1) / kWideStep;
   const uint32_t columns = tiles == 2 ? 512u : 256u;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWideRing; ++i) { mbar_init(&w.full[i], 4); mbar_init(&w.empty[i], 1); }
+    for (int i = 0; i < kWideRing; ++i) { mbar_init(&w.full[i], kLoaders * 33); mbar_init(&w.empty[i], 1); }
     mbar_init(&w.q_full, 4 * tiles);
     for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
     mbar_init(&w.drained, 1);
@@ -367,7 +412,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_proxy();
   }
-  if (warp == 12) {
+  if (warp == 8 + kLoaders) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -410,19 +455,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
         for (int c = 0; c < 4; ++c) seen[c] = *(volatile uint32_t*)&w.seen[i & 3][c];
         const bool whole = (seen[0] & seen[1] & seen[2] & seen[3]) == ~0u;
         float mx = -INFINITY;
+        auto largest = [&](auto all) {
+          uint32_t v[2][32];
+          tmem_ld32(t_s, v[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld32(t_s + c * 32, v);
-          tmem_ld_wait();
-          if (whole) {
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait32(v[c & 1]);
+            if (c < 3) tmem_ld32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+            float m2[2] = {mx, mx};
 #pragma unroll
-            for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(v[k]));
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) if (seen[c] >> k & 1) mx = fmaxf(mx, __uint_as_float(v[k]));
+            for (int k = 0; k < 32; ++k)
+              if (decltype(all)::value || (seen[c] >> k & 1)) m2[k & 1] = fmaxf(m2[k & 1], __uint_as_float(v[c & 1][k]));
+            mx = fmaxf(m2[0], m2[1]);
           }
-        }
+        };
+        if (whole) largest(True()); else largest(False());
         mx = mx == -INFINITY ? mx : mx * scale;   // (a scale of zero keeps it a number)
         const bool passed = mx > (i ? reference + 8.f : -INFINITY);
         if (__any_sync(~0u, passed)) {
@@ -434,7 +481,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
             for (int c = 0; c < D / 32; ++c) {
               uint32_t v[32];
               tmem_ld32(t_o + c * 32, v);
-              tmem_ld_wait();
+              tmem_ld_wait32(v);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 uint32_t u[16];
@@ -447,23 +494,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
           }
         }
         const float base = reference == -INFINITY ? 0.f : reference;
+        auto weights = [&](auto all) {
+          uint32_t v[2][32], u[16];
+          float part[2] = {0.f, 0.f};
+          tmem_ld32(t_s, v[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], u[16];
-          tmem_ld32(t_s + c * 32, v);
-          tmem_ld_wait();
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait32(v[c & 1]);
+            if (c < 3) tmem_ld32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float e[2];
+            for (int k = 0; k < 16; ++k) {
+              float e[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              e[h] = exp2_fast(fmaf(__uint_as_float(v[2 * k + h]), scale, -base));
-              if (!whole && !(seen[c] >> (2 * k + h) & 1)) e[h] = 0.f;
+              for (int h = 0; h < 2; ++h) {
+                e[h] = exp2_fast(fmaf(__uint_as_float(v[c & 1][2 * k + h]), scale, -base));
+                if (!decltype(all)::value && !(seen[c] >> (2 * k + h) & 1)) e[h] = 0.f;
+                part[h] += e[h];
+              }
+              u[k] = Mma<T>::pack(e[0], e[1]);
             }
-            u[k] = Mma<T>::pack(e[0], e[1], sum);
+            tmem_st16(t_s + c * 16, u);   // (over scores that have been read)
           }
-          tmem_st16(t_s + c * 16, u);
-        }
+          sum += part[0] + part[1];
+        };
+        if (whole) weights(True()); else weights(False());
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -471,14 +525,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
       }
       if (ok) ok = warp_wait(&w.o_done[tile], 0);
       tc_fence_after();
-      const int64_t at = ((int64_t)head * p.rows + row) * p.slots + chunk;
+      const int64_t at = ((int64_t)head * p.rows + row) * p.slots + slot;
       if (live) p.stat[at] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
       if (ok) {
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
           tmem_ld32(t_o + c * 32, v);
-          tmem_ld_wait();
+          tmem_ld_wait32(v);
           if (live) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -489,53 +543,63 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
       }
       tc_fence_before();
     }
-  } else if (warp < 12) {
+  } else if (warp < 8 + kLoaders) {
     // --------------------------------------------------------------------- loads ----
     const int part = warp - 8;
     const T *kc = (const T*)p.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.v + (int64_t)head * p.a.c_head;
-    int64_t off = -1;
-    bool ok = true;
-    auto announce = [&](int u) {
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0 && !(p.test_skip_stage && blockIdx.x == 0 && u == 1)) mbar_arrive(&w.full[u % kWideRing]);
+    // where this lane's positions of a step lie, or -1; the page numbers of the step after are asked for one step early
+    constexpr int kEach = 4 / kLoaders;   // groups of 32 positions
+    int page[kEach];
+    int64_t off[kEach];
+    auto position = [&](int step, int h) { return begin + step * kWideStep + (part * kEach + h) * 32 + lane; };
+    auto ask = [&](int step) {
+#pragma unroll
+      for (int h = 0; h < kEach; ++h) page[h] = position(step, h) < end ? pages[position(step, h) / p.a.page_size] : -1;
     };
-    int u = 0;
-    for (; u < 2 * steps; ++u) {
-      if (!warp_wait(&w.empty[u % kWideRing], ((u / kWideRing) & 1) ^ 1)) { ok = false; break; }
+    ask(0);
+    for (int u = 0; u < 2 * steps; ++u) {
+      if (!warp_wait(&w.empty[u % kWideRing], ((u / kWideRing) & 1) ^ 1)) break;
       if (!(u & 1)) {
-        const int pos = begin + (u >> 1) * kWideStep + part * 32 + lane;
-        off = -1;
-        if (pos < end) {
-          const int n = pos / p.a.page_size, page = p.prefix_pages[n];
-          if (page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos - n * p.a.page_size) * p.a.c_token;
+#pragma unroll
+        for (int h = 0; h < kEach; ++h) {
+          off[h] = page[h] >= 0 && page[h] < p.a.pages ? page[h] * p.a.c_page + (int64_t)(position(u >> 1, h) % p.a.page_size) * p.a.c_token : -1;
+          const uint32_t seen = __ballot_sync(~0u, off[h] >= 0);
+          if (lane == 0) *(volatile uint32_t*)&w.seen[(u >> 1) & 3][part * kEach + h] = seen;
         }
-        const uint32_t seen = __ballot_sync(~0u, off >= 0);
-        if (lane == 0) *(volatile uint32_t*)&w.seen[(u >> 1) & 3][part] = seen;
+        ask((u >> 1) + 1);
       }
       const T* base = (u & 1) ? vc : kc;
-      const uint32_t dst = s_ring + (u % kWideRing) * kUnit + part * 32 * 128;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
-        const int64_t o = __shfl_sync(~0u, off, r);
-        copy16(dst + (c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
+      for (int h = 0; h < kEach; ++h) {
+        const uint32_t dst = s_ring + (u % kWideRing) * kUnit + (part * kEach + h) * 32 * 128;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
+          const int64_t o = __shfl_sync(~0u, off[h], r);
+          copy16(dst + (c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
+        }
       }
-      copies_commit();
-      if (u >= 2) { copies_wait<2>(); announce(u - 2); }
+      // Each thread's copies announce themselves when they have landed, so that this warp goes on to the next unit at once (announcing
+      // units after a wait for them two units later cost 6300 clocks a step); lane 0's own arrival publishes `seen`.
+      if (!(p.test_skip_stage && blockIdx.x == 0 && u == 1)) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&w.full[u % kWideRing])) : "memory");
+        if (lane == 0) mbar_arrive(&w.full[u % kWideRing]);
+      }
     }
-    copies_wait<0>();
-    if (ok) {
-      if (u >= 2) announce(u - 2);
-      announce(u - 1);
-    }
-  } else if (elect_one()) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 8 + kLoaders && elect_one()) {
     // ------------------------------------------------------------------ products ----
     const uint32_t fmt = Mma<T>::kBf16 ? 1u : 0u, common = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
     const uint32_t idesc_s = common | ((uint32_t)(kWideStep >> 3) << 17), idesc_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // (V lies with channels innermost)
     const uint64_t hi = (uint64_t)(((8u * 128u) >> 4) | (1u << 14) | (2u << 29)) << 32;
     // the distance between two boxes of channels is only read for V, whose 64-channel groups are a box apart
     auto desc = [&](uint32_t at, uint32_t lead) { return hi | ((uint64_t)lead << 16) | (uint64_t)((at & 0x3FFFF) >> 4); };
+    // (keys and values were written by copies of other threads, which the barrier has told of: the fence makes them visible to the products)
+    auto landed = [&](int u) {
+      const bool there = wait(&w.full[u % kWideRing], (u / kWideRing) & 1);
+      fence_async_proxy();
+      return there;
+    };
     bool ok = wait(&w.q_full, 0);
     auto scores = [&](int i, int t) {   // S_t = Q_t K_i^T
       const uint32_t k = s_ring + (2 * i % kWideRing) * kUnit, q = s_q + t * kUnit;
@@ -544,7 +608,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
         umma_f16(tmem + t * 128, desc(q + (n >> 2) * kBox + (n & 3) * 32, 1), desc(k + (n >> 2) * kBox + (n & 3) * 32, 1), idesc_s, n ? 1u : 0u);
       umma_commit(&w.s_full[t]);
     };
-    if (ok) ok = wait(&w.full[0], 0);
+    if (ok) ok = landed(0);
     if (ok) {
       tc_fence_after();
       for (int t = 0; t < tiles; ++t) scores(0, t);
@@ -554,7 +618,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
       const int vu = 2 * i + 1, ku = 2 * i + 2;
       const bool more = i + 1 < steps;
       for (int t = 0; t < tiles && ok; ++t) {
-        if (t == 0) ok = wait(&w.full[vu % kWideRing], (vu / kWideRing) & 1);
+        if (t == 0) ok = landed(vu);
         ok = ok && wait(&w.p_full[t], i & 1);
         if (!ok) break;
         tc_fence_after();
@@ -564,7 +628,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
           umma_tmem_a(tmem + tiles * 128 + t * D, tmem + t * 128 + n * 8, desc(v + n * 2048, kBox >> 4), idesc_o, (i || n) ? 1u : 0u);
         if (t == tiles - 1) umma_commit(&w.empty[vu % kWideRing]);
         if (!more) { umma_commit(&w.o_done[t]); continue; }
-        if (t == 0) ok = wait(&w.full[ku % kWideRing], (ku / kWideRing) & 1);
+        if (t == 0) ok = landed(ku);
         if (!ok) break;
         tc_fence_after();
         scores(i + 1, t);
@@ -575,42 +639,73 @@ __global__ void __launch_bounds__(kWideThreads, 1) prefix_kernel(const __grid_co
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8 + kLoaders) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
   }
+  grid_dependency_wait();   // the end of this grid is the end of tile_kernel's, which it may have started under
 }
 
-// The sum over a row's slots; a warp per row.
+// The sum over a row's slots; a warp per row.  Lanes read the statistics of 32 slots at once, and the partial results in groups of eight
+// independent loads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
   const int lane = threadIdx.x & 31;
   const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);   // head * rows + row
-  if (id >= (int64_t)p.rows * p.a.kv_heads) return;
-  const int head = (int)(id / p.rows), row = (int)(id - (int64_t)head * p.rows);
+  const bool live = id < (int64_t)p.rows * p.a.kv_heads;
+  const int head = live ? (int)(id / p.rows) : 0, row = live ? (int)(id - (int64_t)head * p.rows) : 0;
   const int g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
-  const int used = p.prefix_chunks + (p.own_chunks ? (own_length(p, b) + p.own_chunk - 1) / p.own_chunk : 0);
+  const int length = live ? own_length(p, b) : 0;   // (an input: nothing before this kernel writes it)
+  grid_dependency_wait();
+  if (!live) return;
+  // slots that were written: all of the prefix's, as many of the sequence's as it has positions for, and that of the last positions
+  const int span = p.own_wide_tiles ? common_length(p, length) : length, chunk = p.own_wide_tiles ? p.own_wide_chunk : p.own_chunk;
+  const int first = p.prefix_chunks + (span > 0 ? (span + chunk - 1) / chunk : 0);
+  const bool tail = p.own_wide_tiles && p.own_chunks && length > span;
+  const int used = first + (tail ? 1 : 0);
+  auto slot_of = [&](int i) { return i < first ? i : p.prefix_chunks + p.own_wide_chunks; };
   const float2* stat = p.stat + id * p.slots;
-  const float* part = p.part + id * p.slots * D;
+  const float* part = p.part + id * p.slots * D + lane * (D / 32);
   constexpr int N = D / 32;
-  float top = -INFINITY;
-  for (int i = lane; i < used; i += 32) top = fmaxf(top, stat[i].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, acc[N];
+  float top = -INFINITY, sum = 0.f, acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  for (int i = 0; i < used; ++i) {
-    const float2 st = stat[i];
-    const float f = exp2_fast(st.x - base);
-    sum += f * st.y;
+  for (int i0 = 0; i0 < used; i0 += 32) {
+    const int i = i0 + lane, n = min(32, used - i0);
+    const float2 st = i < used ? stat[slot_of(i)] : make_float2(-INFINITY, 0.f);
+    float mx = fmaxf(top, st.x);
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] += f * part[(int64_t)i * D + lane * N + k];
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+    const float base = mx == -INFINITY ? 0.f : mx, f = i < used ? exp2_fast(st.x - base) : 0.f, corr = exp2_fast(top - base);
+    top = mx;
+    float s = f * st.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    sum = sum * corr + s;
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] *= corr;
+    for (int m = 0; m < n; m += 8) {
+      float x[8][N];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float* src = part + (int64_t)slot_of(i0 + min(m + e, n - 1)) * D;
+        if constexpr (N == 4) { const float4 v = *(const float4*)src; x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w; }
+        else { const float2 v = *(const float2*)src; x[e][0] = v.x; x[e][1] = v.y; }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = __shfl_sync(~0u, f, (m + e) & 31);
+        if (m + e < n) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += w * x[e][k];
+        }
+      }
+    }
   }
   T* y = (T*)p.y + b * p.a.y_batch + j * p.a.y_token + (int64_t)(head * p.group + g) * p.a.y_head + lane * N;
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int k = 0; k < N; ++k) y[k] = Mma<T>::narrow(sum == 0.f ? 0.f : acc[k] / sum);
+  for (int k = 0; k < N; k += 2) *(uint32_t*)(y + k) = Mma<T>::pack(acc[k] * inverse, acc[k + 1] * inverse);
 }
 
 Params plan(const PagedAttention& a) {
@@ -643,28 +738,54 @@ Params plan(const PagedAttention& a) {
     p.prefix_chunk = chunk_of(a.prefix_length, p.prefix_tiles);
   }
   p.prefix_chunks = (a.prefix_length + p.prefix_chunk - 1) / p.prefix_chunk;
-  p.own_chunk = chunk_of(own_max, (int64_t)p.own_tiles * a.batch);
-  p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
-  p.slots = p.prefix_chunks + p.own_chunks;
+  const int64_t per = (int64_t)a.queries * p.group;
+  if (per > kRows && own_max > kWideStep) {
+    p.own_wide_tiles = (int)((per + kWideRows - 1) / kWideRows);
+    const int64_t all = (own_max + kWideStep - 1) / kWideStep, tiles = (int64_t)p.own_wide_tiles * a.batch * a.kv_heads;
+    int64_t steps = 32;
+    while (steps > 4 && tiles * ((all + steps - 1) / steps) < 2 * 148) steps /= 2;
+    p.own_wide_chunk = (int)steps * kWideStep;
+    p.own_wide_chunks = (int)((all + steps - 1) / steps);
+    p.own_chunk = (a.queries - 1 + kStep - 1) / kStep * kStep;
+    p.own_chunks = a.queries > 1 ? 1 : 0;
+  } else {
+    p.own_chunk = chunk_of(own_max, (int64_t)p.own_tiles * a.batch);
+    p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
+  }
+  p.slots = p.prefix_chunks + p.own_wide_chunks + p.own_chunks;
   return p;
 }
 
+template <typename F> bool start(F* fn, dim3 grid, int threads, size_t smem, bool overlap, const Params& p, cudaStream_t stream) {
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return false; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, fn, p) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
+}
+
+// Up to three launches: tiles of 16 rows, wide tiles, the sum.  The wide kernel starts while the last blocks of the first still run (neither
+// reads what the other writes) and ends no earlier; the sum waits for the kernel in front of it.
 template <typename T, int D> int launch(const Params& p, cudaStream_t stream) {
   const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
-  if (items >= (1ll << 31)) return -1;
-  if (p.wide_tiles) {
-    constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
-    if (cudaFuncSetAttribute(prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)wide) != cudaSuccess) { cudaGetLastError(); return -2; }
-    prefix_kernel<T, D><<<dim3((unsigned)(p.wide_tiles * p.prefix_chunks), (unsigned)p.a.kv_heads), kWideThreads, wide, stream>>>(p);
-  }
+  const int64_t wide_items = (int64_t)p.wide_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_wide_tiles * p.own_wide_chunks;
+  if (items >= (1ll << 31) || wide_items >= (1ll << 31)) return -1;
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
-  if (items) {
-    if (cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
-    tile_kernel<T, D><<<dim3((unsigned)items, (unsigned)p.a.kv_heads), kThreads, smem, stream>>>(p);
-  }
+  constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
+  const unsigned heads = (unsigned)p.a.kv_heads;
+  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, false, p, stream)) return -2;
+  if (wide_items && !start(wide_kernel<T, D>, dim3((unsigned)wide_items, heads), kWideThreads, wide, items > 0, p, stream)) return -2;
   const int64_t ids = (int64_t)p.rows * p.a.kv_heads;
-  join_kernel<T, D><<<(unsigned)((ids + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  return start(join_kernel<T, D>, dim3((unsigned)((ids + kWarps - 1) / kWarps)), kThreads, 0, items + wide_items > 0, p, stream) ? 0 : -2;
 }
 
 }  // namespace
