@@ -5,6 +5,7 @@
 #include <cstdlib>
 
 #include "kernels.h"
+#include "tensor_maps.h"
 #include "umma_ptx.cuh"
 
 namespace b200 {
@@ -28,6 +29,7 @@ struct Params {
   // its queries see (the last queries - 1 positions remain for tile_kernel, in the last slot).  0: tile_kernel takes them all.
   int wide_tiles, own_wide_tiles, own_wide_chunks, own_wide_chunk;
   float scale_log2e;
+  int box_shift;                     // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
   uint32_t spin_limit;
   int test_skip_stage;               // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
@@ -332,9 +334,11 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
 // rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
 // is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks).
-// Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values arrive by 16-byte asynchronous copies into
-// the layout the products read (rows of 64 channels, 128-byte swizzle), because a page may end anywhere inside a step; the ring
-// alternates units of 128 keys and 128 values.
+// Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values lie as
+// the products read them (rows of 64 channels, 128-byte swizzle); the ring alternates units of 128 keys and 128 values.  They arrive by
+// TMA in boxes of as many positions as divide both a page and a step, where those are at least the swizzle's eight; pages of other
+// sizes, and the last step of a range, whose unseen values have to be zeros, by 16-byte asynchronous copies with an address for each
+// position (as the only way they held a step at 4500 clocks).
 constexpr int kWideRows = 256, kWideStep = 128, kWideRing = 4, kLoaders = 2, kWideThreads = 12 * 32;
 constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
 
@@ -369,10 +373,16 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int channel, int position, int head, int page) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"((uint64_t)map),
+               "r"(smem_u32(bar)), "r"(channel), "r"(position), "r"(head), "r"(page)
+               : "memory");
+}
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWideThreads, 1)
+wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ WideShared w;
   constexpr int kBoxes = D / 64, kPieces = D / 8;
@@ -404,6 +414,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const int tiles = n_rows > 128 ? 2 : 1, steps = (end - begin + kWideStep - 1) / kWideStep;
   const uint32_t columns = tiles == 2 ? 512u : 256u;
   if (threadIdx.x == 0) {
+    if (p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
     for (int i = 0; i < kWideRing; ++i) { mbar_init(&w.full[i], kLoaders * 33); mbar_init(&w.empty[i], 1); }
     mbar_init(&w.q_full, 4 * tiles);
     for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
@@ -547,46 +558,80 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     // --------------------------------------------------------------------- loads ----
     const int part = warp - 8;
     const T *kc = (const T*)p.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.v + (int64_t)head * p.a.c_head;
-    // where this lane's positions of a step lie, or -1; the page numbers of the step after are asked for one step early
+    // Page numbers are asked for one step early: of the box that this lane brings, or of the positions whose copies it knows the address of.
     constexpr int kEach = 4 / kLoaders;   // groups of 32 positions
-    int page[kEach];
+    int page[kEach], box_page = -1;
     int64_t off[kEach];
+    const int boxes = p.box_shift ? kWideStep >> p.box_shift : 0;
+    auto by_box = [&](int step) { return p.box_shift && begin + (step + 1) * kWideStep <= end; };
     auto position = [&](int step, int h) { return begin + step * kWideStep + (part * kEach + h) * 32 + lane; };
     auto ask = [&](int step) {
+      if (by_box(step)) {
+        if (lane < boxes) box_page = pages[(begin + step * kWideStep + (lane << p.box_shift)) / p.a.page_size];
+      } else {
 #pragma unroll
-      for (int h = 0; h < kEach; ++h) page[h] = position(step, h) < end ? pages[position(step, h) / p.a.page_size] : -1;
+        for (int h = 0; h < kEach; ++h) page[h] = position(step, h) < end ? pages[position(step, h) / p.a.page_size] : -1;
+      }
     };
+    int box_coord = 0, box_at = 0, loaded = 0;
     ask(0);
-    for (int u = 0; u < 2 * steps; ++u) {
+    for (int u = 0; u < 2 * steps; loaded = ++u) {
+      const int step = u >> 1;
+      uint64_t* full = &w.full[u % kWideRing];
+      const uint32_t dst = s_ring + (u % kWideRing) * kUnit;
       if (!warp_wait(&w.empty[u % kWideRing], ((u / kWideRing) & 1) ^ 1)) break;
+      const bool skip = p.test_skip_stage && blockIdx.x == 0 && u == 1;
+      if (by_box(step)) {
+        if (!(u & 1)) {
+          const bool there = box_page >= 0 && box_page < p.a.pages;
+          box_coord = there ? box_page : p.a.pages;   // (past the last page: zeros)
+          box_at = (begin + step * kWideStep + (lane << p.box_shift)) % p.a.page_size;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t seen = __ballot_sync(~0u, __shfl_sync(~0u, there, (h * 32 + lane) >> p.box_shift));
+            if (lane == 0 && part == 0) *(volatile uint32_t*)&w.seen[step & 3][h] = seen;
+          }
+          ask(step + 1);
+        }
+        if (skip) continue;
+        mbar_arrive(full);
+        if (lane == 0) { if (part == 0) mbar_expect_tx(full, kUnit); else mbar_arrive(full); }
+        if (part == 0 && lane < boxes) {
+#pragma unroll
+          for (int c = 0; c < kBoxes; ++c) load_box(dst + c * kBox + (lane << p.box_shift) * 128, (u & 1) ? &values : &keys, full, c * 64, box_at, head, box_coord);
+        }
+        continue;
+      }
       if (!(u & 1)) {
 #pragma unroll
         for (int h = 0; h < kEach; ++h) {
-          off[h] = page[h] >= 0 && page[h] < p.a.pages ? page[h] * p.a.c_page + (int64_t)(position(u >> 1, h) % p.a.page_size) * p.a.c_token : -1;
+          off[h] = page[h] >= 0 && page[h] < p.a.pages ? page[h] * p.a.c_page + (int64_t)(position(step, h) % p.a.page_size) * p.a.c_token : -1;
           const uint32_t seen = __ballot_sync(~0u, off[h] >= 0);
-          if (lane == 0) *(volatile uint32_t*)&w.seen[(u >> 1) & 3][part * kEach + h] = seen;
+          if (lane == 0) *(volatile uint32_t*)&w.seen[step & 3][part * kEach + h] = seen;
         }
-        ask((u >> 1) + 1);
+        ask(step + 1);
       }
       const T* base = (u & 1) ? vc : kc;
 #pragma unroll
       for (int h = 0; h < kEach; ++h) {
-        const uint32_t dst = s_ring + (u % kWideRing) * kUnit + (part * kEach + h) * 32 * 128;
+        const uint32_t row0_at = dst + (part * kEach + h) * 32 * 128;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
           const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
           const int64_t o = __shfl_sync(~0u, off[h], r);
-          copy16(dst + (c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
+          copy16(row0_at + (c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
         }
       }
-      // Each thread's copies announce themselves when they have landed, so that this warp goes on to the next unit at once (announcing
-      // units after a wait for them two units later cost 6300 clocks a step); lane 0's own arrival publishes `seen`.
-      if (!(p.test_skip_stage && blockIdx.x == 0 && u == 1)) {
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&w.full[u % kWideRing])) : "memory");
-        if (lane == 0) mbar_arrive(&w.full[u % kWideRing]);
+      // Each thread's copies announce themselves when they have landed, so that this warp goes on to the next unit at once; lane 0's own
+      // arrival publishes `seen`.
+      if (!skip) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
+        if (lane == 0) mbar_arrive(full);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (*abort_flag && lane == 0)
+      for (int i = 0; i < kWideRing; ++i) await_landing(&w.full[i], loaded > i ? (uint32_t)((loaded - 1 - i) / kWideRing & 1) : 1u);   // boxes in flight land before their memory goes
   } else if (warp == 8 + kLoaders && elect_one()) {
     // ------------------------------------------------------------------ products ----
     const uint32_t fmt = Mma<T>::kBf16 ? 1u : 0u, common = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
@@ -756,7 +801,7 @@ Params plan(const PagedAttention& a) {
   return p;
 }
 
-template <typename F> bool start(F* fn, dim3 grid, int threads, size_t smem, bool overlap, const Params& p, cudaStream_t stream) {
+template <typename F, typename... Args> bool start(F* fn, dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t stream, const Args&... args) {
   if (smem > 48 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return false; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -768,24 +813,44 @@ template <typename F> bool start(F* fn, dim3 grid, int threads, size_t smem, boo
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = overlap ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, fn, p) == cudaSuccess) return true;
+  if (cudaLaunchKernelEx(&cfg, fn, args...) == cudaSuccess) return true;
   cudaGetLastError();
   return false;
 }
 
+// Boxes of 64 channels and `positions` positions of one head and page.  False where the strides are none that TMA takes.
+bool box_map(CUtensorMap* m, const Params& p, const void* base, int positions) {
+  if (!load_driver_entry_points()) return false;
+  // (the stride of a dimension of one entry is never used, but has to be valid)
+  auto bytes = [](int64_t stride, int extent) { return extent == 1 && stride == 0 ? (cuuint64_t)16 : (cuuint64_t)stride * 2; };
+  const cuuint64_t dims[4] = {(cuuint64_t)p.a.channels, (cuuint64_t)p.a.page_size, (cuuint64_t)p.a.kv_heads, (cuuint64_t)p.a.pages};
+  const cuuint64_t strides[3] = {bytes(p.a.c_token, p.a.page_size), bytes(p.a.c_head, p.a.kv_heads), bytes(p.a.c_page, p.a.pages)};
+  for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return false;
+  const cuuint32_t box[4] = {64, (cuuint32_t)positions, 1, 1}, step[4] = {1, 1, 1, 1};
+  return g_encode_tiled(m, p.a.dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)base, dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Up to three launches: tiles of 16 rows, wide tiles, the sum.  The wide kernel starts while the last blocks of the first still run (neither
 // reads what the other writes) and ends no earlier; the sum waits for the kernel in front of it.
-template <typename T, int D> int launch(const Params& p, cudaStream_t stream) {
+template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
   const int64_t wide_items = (int64_t)p.wide_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_wide_tiles * p.own_wide_chunks;
   if (items >= (1ll << 31) || wide_items >= (1ll << 31)) return -1;
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
   constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
   const unsigned heads = (unsigned)p.a.kv_heads;
-  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, false, p, stream)) return -2;
-  if (wide_items && !start(wide_kernel<T, D>, dim3((unsigned)wide_items, heads), kWideThreads, wide, items > 0, p, stream)) return -2;
+  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, false, stream, p)) return -2;
+  if (wide_items) {
+    CUtensorMap keys{}, values{};
+    p.box_shift = 0;
+    int shift = 0;
+    while (shift < 7 && p.a.page_size % (2 << shift) == 0) ++shift;
+    if (shift >= 3 && box_map(&keys, p, p.k, 1 << shift) && box_map(&values, p, p.v, 1 << shift)) p.box_shift = shift;
+    if (!start(wide_kernel<T, D>, dim3((unsigned)wide_items, heads), kWideThreads, wide, items > 0, stream, p, keys, values)) return -2;
+  }
   const int64_t ids = (int64_t)p.rows * p.a.kv_heads;
-  return start(join_kernel<T, D>, dim3((unsigned)((ids + kWarps - 1) / kWarps)), kThreads, 0, items + wide_items > 0, p, stream) ? 0 : -2;
+  return start(join_kernel<T, D>, dim3((unsigned)((ids + kWarps - 1) / kWarps)), kThreads, 0, items + wide_items > 0, stream, p) ? 0 : -2;
 }
 
 }  // namespace
