@@ -43,8 +43,20 @@ template <> struct Keys<__nv_bfloat16> {
   static __device__ __forceinline__ float value(Key k) { return __uint_as_float((uint32_t)((k >> 15) ? k & 0x7fff : (uint16_t)~k) << 16); }
 };
 
+constexpr int kBins = 2048, kList = 2048, kListTopK = 1024;
+constexpr float kBinsPerE = 32.f;         // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
+
 struct Shared {
-  double table[64];                       // 2^(j / 64)
+  double table[256];                      // 2^(j / 256)
+  // The direct way: a histogram (counts, or masses), then a list of (key, ~index), and what every warp of the cluster has summed.
+  union { uint32_t hist[kBins]; unsigned long long list[kList]; };
+  unsigned long long weight[kListTopK];   // of the list's first, by rank (top-k)
+  unsigned long long all[kMaxCluster * kWarps], below[kMaxCluster * kWarps], taken[kMaxCluster * kWarps];
+  double share;
+  unsigned long long before;
+  double target;
+  unsigned long long cut_entry;
+  int n_list, found, owner, ok;
   unsigned long long warp_sum[kWarps], cta_sum, best;
   uint32_t lo[2][256], hi[2][256];        // histograms: counts in lo, or masses in both words
   unsigned long long total[256], above, in_bin;
@@ -52,21 +64,20 @@ struct Shared {
   int cut, pick;
 };
 
-// exp(x) for x <= 0, by a table of 2^(j/64) and the exponential series up to the fifth power on |r| <= ln 2 / 128 (P. T. P. Tang's
-// table-driven method, 1989): the next term is below 4e-17.  Below exp(-700): 0.
-__device__ __forceinline__ double exp_below(double x, const double* table) {
-  if (!(x > -700.0)) return 0.0;
+// exp(d * inverse) for d <= 0, with scale = inverse * 256 / ln 2: a table of 2^(j/256) and the exponential series up to the third power on
+// |r| <= ln 2 / 512 (P. T. P. Tang's table-driven method, 1989); the next term is below 1.4e-13, and in a sum of many weights, of
+// either size, less.  Ten operations in 64 bits, two clocks of a scheduler each, are what a weight costs; a table of 64 takes two more.
+__device__ __forceinline__ double exp_below(double d, double scale, const double* table) {
+  const double z = d * scale;
+  if (!(z > -258000.0)) return 0.0;                            // below exp(-698)
   const double shift = 6755399441055744.0;                     // 1.5 * 2^52: adding it rounds to a whole number
-  const double z = fma(x, 92.332482616893656877, shift);       // 64 / ln 2
-  const int n = __double2loint(z);
-  const double r = fma(z - shift, -0.010830424696249145, x);   // ln 2 / 64; its rounding costs |x| * 1.2e-16
-  double p = fma(r, 1.0 / 120, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  const double t = table[n & 63];
-  return p * __hiloint2double(__double2hiint(t) + ((n >> 6) << 20), __double2loint(t));
+  const double m = z + shift, g = z - (m - shift);
+  const int n = __double2loint(m);
+  constexpr double c = 0.69314718055994530942 / 256;
+  double p = fma(g, c * c * c / 6, c * c / 2);
+  p = fma(p, g, c) * g;
+  const double t = table[n & 255], w = __hiloint2double(__double2hiint(t) + ((n >> 8) << 20), __double2loint(t));
+  return fma(w, p, w);
 }
 // Weights are summed as whole numbers of 2^-44 of the largest: 2^18 of them stay inside 62 bits, and the sums do not depend on
 // their order.
@@ -94,6 +105,318 @@ struct Row {
   int top_k;
 };
 
+// Sum over the block's threads before this one, and over all of them.
+template <typename V> __device__ __forceinline__ V block_scan(V mine, V* warps, V& total, int lane, int warp) {
+  V upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V u = __shfl_up_sync(~0u, upto, o);
+    if (lane >= o) upto += u;
+  }
+  const V previous = __shfl_up_sync(~0u, upto, 1);
+  __syncthreads();
+  if (lane == 31) warps[warp] = upto;
+  __syncthreads();
+  V before = 0;
+  total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before = total;
+    total += warps[w];
+  }
+  return lane ? before + previous : before;   // (the same sums, in the same order, as the thread in front of this one ends with)
+}
+// Largest first; n2 a power of two, entries from n on are zeros.
+__device__ __forceinline__ void sort_list(unsigned long long* list, int n2, int tid) {
+  for (int k = 2; k <= n2; k <<= 1)
+    for (int j = k >> 1; j; j >>= 1) {
+      __syncthreads();
+      for (int i = tid; i < n2 / 2; i += kThreads) {
+        const int a = 2 * i - (i & (j - 1)), b = a + j;
+        const unsigned long long x = list[a], y = list[b];
+        if ((x < y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+      }
+    }
+  __syncthreads();
+}
+
+// What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them, of
+// counts for top-k or of masses (32-bit, relative to the bin's middle: good to 2^-16) for top-p, finds the bin of the last
+// kept token.
+//   top-k up to 1024: all tokens down to that bin go to a list of the first CTA, which sorts it and does the rest alone.
+//   otherwise: every CTA sums exact weights, over all tokens, over those in higher bins, and of the latter, warp by warp, over those that
+//   min-p keeps; tokens in the bin itself go to the list.  The first CTA sorts it, finds the last token kept, and which
+//   warp's stretch of the row the choice lies in; that stretch's CTA finds it there.
+// The histogram of masses only proposes the bin: the exact sums have to confirm it.  Returns false, with nothing written, where that fails, the list
+// is full (many equal logits), or a parameter is out of this way's range (top-k above 1024, uniform outside (0, 1), temperature, infinities).
+// All CTAs of a cluster take the same branches.
+template <typename T>
+__device__ __forceinline__ bool direct(Shared& s, cg::cluster_group& cluster, const typename Keys<T>::Key* keys, const Row& r, typename Keys<T>::Key top_key, double scale, int vocab,
+                                       int slice, int row, int* tokens) {
+  using K = Keys<T>;
+  using Key = typename K::Key;
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
+  const float topf = K::value(top_key), per_unit = kBinsPerE / r.temperature;
+  const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
+  if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(topf) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kListTopK)) return false;
+  const double top = (double)topf;
+  auto weight = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)K::value(k) - top, scale, s.table); };
+  Shared* first = cluster.map_shared_rank(&s, 0);
+  // the bin, as a float: nearest to (top - logit) * per_unit, which grows as logits fall
+  auto place = [&](Key k) { return fminf((topf - K::value(k)) * per_unit, (float)(kBins - 1)); };
+  auto bin_of = [&](float at) { return (int)(__float_as_uint(at + 8388608.f) & 0x7fffffu); };
+  int bin = -1;
+  if (by_count || by_mass) {
+    for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
+    if (tid == 0) { s.found = -1; s.n_list = 0; }
+    __syncthreads();
+    struct alignas(4 * sizeof(Key)) Four { Key k[4]; };
+    for (int i = tid; i < slice / 4; i += kThreads) {
+      const Four f = ((const Four*)keys)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (f.k[j]) {
+          const float at = place(f.k[j]);
+          const int b = bin_of(at);
+          uint32_t add = 1;
+          if (!by_count) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
+            const float x = ((float)b - at) * (1.f / kBinsPerE);
+            add = __float_as_uint(fmaf(fmaf(fmaf(x, 1.f / 6, 0.5f), x, 1.f), x * 65536.f, 65536.f + 8388608.f)) & 0x7fffffu;
+          }
+          atomicAdd(&s.hist[b], add);
+        }
+    }
+    cluster.sync();
+    // each CTA adds up its share of the bins
+    const int share = kBins / ranks, each = share > kThreads ? share / kThreads : 1, b0 = rank * share + tid * each;
+    const bool mine = tid * each < share;
+    double v[kBins / kThreads], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / kThreads; ++j) {
+      v[j] = 0;
+      if (mine && j < each) {
+        unsigned long long n = 0;
+        for (int k = 0; k < ranks; ++k) n += cluster.map_shared_rank(&s, k)->hist[b0 + j];
+        v[j] = (double)n;
+        if (!by_count) v[j] *= (double)exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE));
+      }
+      sum += v[j];
+    }
+    double total;
+    const double before = block_scan(sum, (double*)s.warp_sum, total, lane, warp);
+    if (tid == 0) s.share = total;
+    cluster.sync();
+    double offset = 0, everything = 0;
+    for (int k = 0; k < ranks; ++k) {
+      if (k == rank) offset = everything;
+      everything += cluster.map_shared_rank(&s, k)->share;
+    }
+    const double need = by_count ? (double)r.top_k : (double)r.top_p * everything;
+    double run = offset + before;
+#pragma unroll
+    for (int j = 0; j < kBins / kThreads; ++j) {
+      if (run < need && need <= run + v[j])
+        for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->found = b0 + j;
+      run += v[j];
+    }
+    cluster.sync();
+    bin = s.found;
+    if (bin < 0 || bin == kBins - 1) return false;   // (fewer tokens than k; a mark that rounding put between two bins; weights of no units)
+  }
+  auto push = [&](bool any, Key k, int i) {
+    const uint32_t who = __ballot_sync(~0u, any);
+    if (!who) return;
+    int at = 0;
+    if (lane == __ffs(who) - 1) at = atomicAdd(&first->n_list, __popc(who));
+    at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
+    if (any && at < kList) first->list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(base + i);
+  };
+  const int sub = slice / kWarps, warp_base = warp * sub;
+  const double least = (double)r.min_p;
+  if (by_count) {
+    for (int i = lane; i < sub; i += 32) {
+      const Key k = keys[warp_base + i];
+      push(k && bin_of(place(k)) <= bin, k, warp_base + i);
+    }
+  } else {
+    // (below this no weight passes min-p, with room for the roundings of 32 bits)
+    const float last = by_mass ? (float)(kBins - 1) : r.min_p > 0.f ? fminf(-kBinsPerE * logf(r.min_p) + 1.f, (float)(kBins - 1)) : (float)(kBins - 1);
+    unsigned long long all = 0, below = 0, taken = 0;
+    for (int i = lane; i < sub; i += 32) {
+      const Key k = keys[warp_base + i];
+      const float at = k ? place(k) : (float)kBins;
+      bool listed = false;
+      if (at < last) {
+        const double w = weight(k);
+        const unsigned long long u = units(w);
+        const int b = bin_of(at);
+        all += u;
+        if (!by_mass || b < bin) {
+          below += u;
+          if (w >= least) taken += u;
+        } else {
+          listed = b == bin;
+        }
+      }
+      if (by_mass) push(listed, k, warp_base + i);
+    }
+    all = warp_sum(all); below = warp_sum(below); taken = warp_sum(taken);
+    if (lane == 0) { first->all[rank * kWarps + warp] = all; first->below[rank * kWarps + warp] = below; first->taken[rank * kWarps + warp] = taken; }
+  }
+  cluster.sync();
+  if (by_count || by_mass) {
+    const bool full = first->n_list > kList;
+    cluster.sync();   // (the first CTA goes on, and the others may leave)
+    if (full) return false;
+  }
+  // exact weights of the sorted list, four entries per thread; entries from `limit` on do not count
+  unsigned long long unit[4], sum = 0, total = 0, run = 0;
+  double w[4];
+  auto weigh = [&](int limit) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid * 4 + j;
+      w[j] = i < limit ? weight((Key)(s.list[i] >> 32)) : 0.0;
+      unit[j] = i < limit ? units(w[j]) : 0;
+      sum += unit[j];
+    }
+    run = block_scan(sum, s.warp_sum, total, lane, warp);
+  };
+  auto sorted = [&]() {
+    const int n = s.n_list;
+    int n2 = 2;
+    while (n2 < n) n2 *= 2;
+    for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
+    sort_list(s.list, n2, tid);
+    return n;
+  };
+  if (by_count) {
+    if (rank) return true;
+    sorted();
+    weigh(r.top_k);
+    const double mark = by_mass ? (double)r.top_p * (double)total : 0.0;
+    unsigned long long kept = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = tid * 4 + j;
+      if (i < r.top_k && (i == 0 || ((!by_mass || (double)run < mark) && w[j] >= least))) {
+        kept += unit[j];
+        s.weight[i] = unit[j];
+      } else if (i < kListTopK) {
+        s.weight[i] = 0;
+      }
+      run += unit[j];
+    }
+    block_scan(kept, s.warp_sum, total, lane, warp);
+    // by index, six bits at a time: the digit at which the running sum passes the target
+    const double target = (double)r.uniform * (double)total;
+    uint32_t prefix = 0;
+    unsigned long long before = 0;
+    for (int shift = 12; shift >= 0; shift -= 6) {
+      if (tid < 64) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+      __syncthreads();
+      for (int i = tid; i < r.top_k; i += kThreads) {
+        const uint32_t index = ~(uint32_t)s.list[i];
+        const unsigned long long u = s.weight[i];
+        if (u && index >> (shift + 6) == prefix) {
+          const int d = (index >> shift) & 63;
+          const uint32_t lo = (uint32_t)u, old = atomicAdd(&s.lo[0][d], lo), up = (uint32_t)(u >> 32) + (old + lo < old ? 1u : 0u);
+          if (up) atomicAdd(&s.hi[0][d], up);
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const unsigned long long x = ((unsigned long long)s.hi[0][2 * lane] << 32) + s.lo[0][2 * lane], y = ((unsigned long long)s.hi[0][2 * lane + 1] << 32) + s.lo[0][2 * lane + 1];
+        const unsigned long long upto = before + warp_scan(x + y, lane), from = upto - x - y;
+        const uint32_t ballot = __ballot_sync(~0u, (double)upto > target);
+        if (lane == __ffs(ballot) - 1) {
+          const bool second = !((double)(from + x) > target);
+          s.bin = prefix << 6 | (uint32_t)(2 * lane + second);
+          s.above = second ? from + x : from;
+        }
+      }
+      __syncthreads();
+      prefix = s.bin;
+      before = s.above;
+    }
+    if (tid == 0) tokens[row] = (int)prefix;
+    return true;
+  }
+  if (rank == 0) {
+    // the sums of all warps, in index order
+    const int n_warps = ranks * kWarps;
+    const unsigned long long all = tid < n_warps ? s.all[tid] : 0, below = tid < n_warps ? s.below[tid] : 0;
+    unsigned long long sum_all, sum_below;
+    block_scan(all, s.warp_sum, sum_all, lane, warp);
+    block_scan(below, s.warp_sum, sum_below, lane, warp);
+    if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; }
+    if (by_mass) {
+      const int n = sorted();
+      weigh(n);
+      const double mark = (double)r.top_p * (double)sum_all;
+      run += sum_below;
+      // (kept entries are the first ones; the last of them ends the kept tokens)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = tid * 4 + j;
+        const bool kept = i < n && ((double)run < mark || (i == 0 && sum_below == 0));
+        const bool next = i + 1 < n && (double)(run + unit[j]) < mark;
+        if (kept) {
+          const unsigned long long entry = s.list[i];
+          if (!next) s.cut_entry = entry;
+          const uint32_t index = ~(uint32_t)entry;
+          if (w[j] >= least) atomicAdd(&s.taken[index / (uint32_t)sub], unit[j]);
+        }
+        run += unit[j];
+      }
+      if (tid == 0 && !((sum_below == 0 || (double)sum_below < mark) && mark <= (double)(sum_below + total))) s.ok = 0;
+    }
+    __syncthreads();
+    const unsigned long long taken = tid < n_warps ? s.taken[tid] : 0;
+    unsigned long long sum_taken;
+    const unsigned long long before = block_scan(taken, s.warp_sum, sum_taken, lane, warp);
+    const double target = (double)r.uniform * (double)sum_taken;
+    if (!((double)before > target) && (double)(before + taken) > target)
+      for (int k = 0; k < ranks; ++k) {
+        Shared* o = cluster.map_shared_rank(&s, k);
+        o->owner = tid; o->before = before; o->target = target;
+      }
+    __syncthreads();
+    if (tid < ranks && tid) { Shared* o = cluster.map_shared_rank(&s, tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
+  }
+  cluster.sync();
+  if (!s.ok) return false;
+  if (s.owner / kWarps != rank) return true;
+  // the stretch of one warp, now by all warps of its CTA
+  const Key cut = (Key)(s.cut_entry >> 32);
+  const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
+  auto chosen = [&](int i) -> unsigned long long {
+    if (i >= sub) return 0;
+    const Key k = keys[stretch + i];
+    if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
+    const double w = weight(k);
+    return w >= least ? units(w) : 0;
+  };
+  unsigned long long mine = 0;
+  for (int i = warp * part + lane; i < (warp + 1) * part; i += 32) mine += chosen(i);
+  mine = warp_sum(mine);
+  __syncthreads();
+  if (lane == 0) s.warp_sum[warp] = mine;
+  __syncthreads();
+  unsigned long long before = s.before;
+  for (int k = 0; k < warp; ++k) before += s.warp_sum[k];
+  if ((double)before > s.target || !((double)(before + mine) > s.target)) return true;
+  for (int i = warp * part; i < (warp + 1) * part; i += 32) {
+    const unsigned long long upto = before + warp_scan(chosen(i + lane), lane);
+    const uint32_t ballot = __ballot_sync(~0u, (double)upto > s.target);
+    if (ballot) {
+      if (lane == __ffs(ballot) - 1) tokens[row] = base + stretch + i + lane;
+      break;
+    }
+    before = __shfl_sync(~0u, upto, 31);
+  }
+  return true;
+}
+
 // One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps as keys in shared memory.
 //   1. the largest key (and, of those, the lowest index);
 //   2. top-k and top-p, each a search for the key t and, among the tokens with that key, the last index c that are still kept: a
@@ -114,8 +437,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   const int base = rank * slice;
   const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
 
-  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
-  if (tid < 256) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+  if (tid < 256) { s.table[tid] = exp2((double)tid / 256.0); s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
   // ---- 1. keys, and the largest ----
   unsigned long long best = 0;
   const T* src = logits + (int64_t)row * row_stride + base;
@@ -158,8 +480,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
     cluster.sync();   // nobody leaves while a peer may still read its shared memory
     return;
   }
-  const double top = (double)K::value(top_key), inverse = 1.0 / (double)r.temperature;
-  auto weight = [&](Key k) { return k == top_key ? 1.0 : exp_below(((double)K::value(k) - top) * inverse, s.table); };
+  const double top = (double)K::value(top_key), scale = 369.32993046757462708 / (double)r.temperature;   // 256 / ln 2
+  auto weight = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)K::value(k) - top, scale, s.table); };
+  if (direct<T>(s, cluster, keys, r, top_key, scale, vocab, slice, row, tokens)) return;
 
   // Kept so far: key > t, or key == t and index <= c.
   Key t = 1;

@@ -305,6 +305,22 @@ def test_sample(odla, gpu_lib, dtype, rows, vocab, pad):
     check_sample(odla, gpu_lib, logits, (None, None, None, None), u, dtype)
 
 
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("spread", [0.05, 1.0, 20.0])
+@pytest.mark.parametrize("rows,vocab", [(64, 3000), (24, 50001), (150, 32000)])
+def test_sample_each_filter_alone_and_together(odla, gpu_lib, dtype, spread, rows, vocab):
+    """Flat, ordinary and steep rows; top-k on both sides of 1024, top-p from nearly nothing to nearly all."""
+    g = gen(rows, vocab, int(spread * 100), dtype)
+    logits = (spread * torch.randn((rows, vocab), generator=g, device="cuda")).to(R.TORCH[dtype])
+    u = torch.rand(rows, generator=g, device="cuda")
+
+    def pick(values, dtype=torch.float32):
+        return torch.tensor(values, dtype=dtype, device="cuda")[torch.randint(0, len(values), (rows,), generator=g, device="cuda")]
+    T, k, p, m = pick([0.2, 0.7, 1.0, 1.7]), pick([1, 3, 40, 1000, 1024, 1025, 2000, 10 ** 6], torch.int32), pick([0.01, 0.3, 0.8, 0.95, 0.999, 0.999999]), pick([1e-6, 0.01, 0.2, 0.9])
+    for params in ((T, None, None, None), (T, k, None, None), (T, None, p, None), (T, None, None, m), (T, None, p, m), (T, k, p, None), (T, k, p, m)):
+        check_sample(odla, gpu_lib, logits, params, u, dtype)
+
+
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("vocab", [100, 4096, 40000])
 def test_sample_ties(odla, gpu_lib, dtype, vocab):
