@@ -12,52 +12,77 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 128;
+constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
 
 // Logits as keys that compare like them: whole numbers, larger for larger logits, 0 for those that are never chosen (NaN, -inf).
 // -0 becomes +0: equal logits must have equal keys.
-template <typename T> struct Keys;
-template <> struct Keys<float> {
-  using Key = uint32_t;
-  static constexpr int kBits = 32;
-  static __device__ __forceinline__ Key key(float v) {
-    const uint32_t b = __float_as_uint(v + 0.f);
-    return v > -INFINITY ? ((b >> 31) ? ~b : b | 0x80000000u) : 0u;
-  }
-  static __device__ __forceinline__ float value(Key k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
-};
 template <int INF> __device__ __forceinline__ uint16_t half_key(uint16_t b) {   // INF: the type's bits of infinity
   const uint32_t m = b & 0x7fffu;
   if (m > INF || b == (0x8000u | INF)) return 0;
   return (b >> 15) && m ? (uint16_t)~b : (uint16_t)(m | 0x8000u);
 }
-template <> struct Keys<__half> {
+template <typename T> struct Logits;
+template <> struct Logits<float> {
+  using Key = uint32_t;
+  static constexpr int kBits = 32;
+  static __device__ __forceinline__ float dead() { return -INFINITY; }
+  static __device__ __forceinline__ Key key(float v) {
+    const uint32_t b = __float_as_uint(v + 0.f);
+    return v > -INFINITY ? ((b >> 31) ? ~b : b | 0x80000000u) : 0u;
+  }
+  static __device__ __forceinline__ float value(Key k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+  static __device__ __forceinline__ float widen(float v) { return v; }
+  static __device__ __forceinline__ float largest(const uint4& u) {   // of 16 bytes; a NaN loses
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+};
+template <> struct Logits<__half> {
   using Key = uint16_t;
   static constexpr int kBits = 16;
+  static __device__ __forceinline__ __half dead() { return __ushort_as_half(0xfc00); }
   static __device__ __forceinline__ Key key(__half v) { return half_key<0x7c00>(__half_as_ushort(v)); }
   static __device__ __forceinline__ float value(Key k) { return __half2float(__ushort_as_half((k >> 15) ? k & 0x7fff : (uint16_t)~k)); }
+  static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ float largest(const uint4& u) {
+    const __half2* h = (const __half2*)&u;
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
 };
-template <> struct Keys<__nv_bfloat16> {
+template <> struct Logits<__nv_bfloat16> {
   using Key = uint16_t;
   static constexpr int kBits = 16;
+  static __device__ __forceinline__ __nv_bfloat16 dead() { return __ushort_as_bfloat16(0xff80); }
   static __device__ __forceinline__ Key key(__nv_bfloat16 v) { return half_key<0x7f80>(__bfloat16_as_ushort(v)); }
   static __device__ __forceinline__ float value(Key k) { return __uint_as_float((uint32_t)((k >> 15) ? k & 0x7fff : (uint16_t)~k) << 16); }
+  static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ float largest(const uint4& u) {
+    const __nv_bfloat162* h = (const __nv_bfloat162*)&u;
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
 };
-
-constexpr int kBins = 2048, kList = 2048, kListTopK = 1024;
-constexpr float kBinsPerE = 32.f;         // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
+// 16 bytes of logits.
+template <typename T> struct alignas(16) Piece {
+  static constexpr int N = 16 / sizeof(T);
+  T e[N];
+};
 
 struct Shared {
   double table[256];                      // 2^(j / 256)
-  // The direct way: a histogram (counts, or masses), then a list of (key, ~index), and what every warp of the cluster has summed.
+  // The direct way: a histogram (counts, or masses), then a list of (key, ~index); what every warp of the cluster has summed.
   union { uint32_t hist[kBins]; unsigned long long list[kList]; };
-  unsigned long long weight[kListTopK];   // of the list's first, by rank (top-k)
-  unsigned long long all[kMaxCluster * kWarps], below[kMaxCluster * kWarps], taken[kMaxCluster * kWarps];
-  double share;
-  unsigned long long before;
-  double target;
-  unsigned long long cut_entry;
-  int n_list, found, owner, ok;
-  unsigned long long warp_sum[kWarps], cta_sum, best;
+  union {
+    unsigned long long weight[kTopK];     // of the list's first, by rank (top-k)
+    uint32_t bucket[kBins];
+  };
+  unsigned long long below[kMaxCluster * kWarps], taken[kMaxCluster * kWarps], all[kMaxCluster];
+  unsigned long long warp_sum[kWarps], cta_sum, before, cut_entry;
+  float warp_top[kWarps], tops[kMaxCluster];
+  double shares[kMaxCluster], target;
+  int listed[kMaxCluster], n_list, found, owner, ok, crowded, token;
+  // The general way.
   uint32_t lo[2][256], hi[2][256];        // histograms: counts in lo, or masses in both words
   unsigned long long total[256], above, in_bin;
   uint32_t bin;
@@ -100,6 +125,12 @@ __device__ __forceinline__ unsigned long long warp_scan(unsigned long long v, in
   return v;
 }
 
+// Adds a weight to a sum of two words.
+__device__ __forceinline__ void add_units(uint32_t* lo, uint32_t* hi, unsigned long long u) {
+  const uint32_t l = (uint32_t)u, old = atomicAdd(lo, l), up = (uint32_t)(u >> 32) + (old + l < old ? 1u : 0u);
+  if (up) atomicAdd(hi, up);
+}
+
 struct Row {
   float temperature, top_p, min_p, uniform;
   int top_k;
@@ -139,189 +170,283 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, int n2, int 
   __syncthreads();
 }
 
-// What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them, of
-// counts for top-k or of masses (32-bit, relative to the bin's middle: good to 2^-16) for top-p, finds the bin of the last
-// kept token.
-//   top-k up to 1024: all tokens down to that bin go to a list of the first CTA, which sorts it and does the rest alone.
-//   otherwise: every CTA sums exact weights, over all tokens, over those in higher bins, and of the latter, warp by warp, over those that
-//   min-p keeps; tokens in the bin itself go to the list.  The first CTA sorts it, finds the last token kept, and which
-//   warp's stretch of the row the choice lies in; that stretch's CTA finds it there.
-// The histogram of masses only proposes the bin: the exact sums have to confirm it.  Returns false, with nothing written, where that fails, the list
-// is full (many equal logits), or a parameter is out of this way's range (top-k above 1024, uniform outside (0, 1), temperature, infinities).
-// All CTAs of a cluster take the same branches.
-template <typename T>
-__device__ __forceinline__ bool direct(Shared& s, cg::cluster_group& cluster, const typename Keys<T>::Key* keys, const Row& r, typename Keys<T>::Key top_key, double scale, int vocab,
-                                       int slice, int row, int* tokens) {
-  using K = Keys<T>;
-  using Key = typename K::Key;
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
-  const float topf = K::value(top_key), per_unit = kBinsPerE / r.temperature;
-  const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
-  if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(topf) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kListTopK)) return false;
-  const double top = (double)topf;
-  auto weight = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)K::value(k) - top, scale, s.table); };
-  Shared* first = cluster.map_shared_rank(&s, 0);
-  // the bin, as a float: nearest to (top - logit) * per_unit, which grows as logits fall
-  auto place = [&](Key k) { return fminf((topf - K::value(k)) * per_unit, (float)(kBins - 1)); };
-  auto bin_of = [&](float at) { return (int)(__float_as_uint(at + 8388608.f) & 0x7fffffu); };
-  int bin = -1;
-  if (by_count || by_mass) {
+// A CTA's part of a row: `slice` logits in shared memory, of which those past the row's end never count.
+template <typename T, int RANKS> struct Part {
+  Shared& s;
+  cg::cluster_group cluster;
+  const T* logits;
+  unsigned long long* spare;   // kList entries
+  Row r;
+  float top;                   // the row's largest logit
+  double scale;                // 256 / (ln 2 * temperature)
+  int vocab, slice, base, rank, row;
+  int* tokens;
+
+  using L = Logits<T>;
+  using Key = typename L::Key;
+  __device__ __forceinline__ Shared* peer(int k) { return cluster.map_shared_rank(&s, k); }
+  __device__ __forceinline__ double weight(float v) const { return exp_below((double)v - (double)top, scale, s.table); }
+
+  // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them finds
+  // the bin of the last kept token.
+  //   top-k up to 1024: a histogram of the largest logit of each 16 bytes (the k-th largest of those has at least k tokens above it, and rarely
+  //   many more; of every logit where that did not hold, or the row is short).  All tokens down to that bin go to a list of the first CTA,
+  //   which sorts it and does the rest alone.
+  //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 2^-16), for top-p; then every CTA sums exact weights,
+  //   over all tokens, over those in higher bins, and of the latter, warp by warp, over those that min-p keeps; tokens in the bin itself
+  //   go to the list.  The first CTA sorts it, finds the last token kept, and which warp's stretch of the row the choice lies in; that
+  //   stretch's CTA finds it there.
+  // The histogram of masses only proposes the bin: the exact sums have to confirm it.  Returns false, with nothing written, where that fails,
+  // the list is full (many equal logits), or a parameter is out of this way's range (top-k above 1024, uniform outside (0, 1),
+  // temperature, infinities).  All CTAs of a cluster take the same branches.
+  __device__ __forceinline__ bool direct() {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float per_unit = kBinsPerE / r.temperature;
+    const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
+    if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(top) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kTopK)) return false;
+    if (by_count) {
+      if (vocab / Piece<T>::N >= 2 * r.top_k) {
+        const int n = top_k<true>(per_unit);
+        if (n >= 0) return true;
+        if (n == -1) return false;
+      }
+      return top_k<false>(per_unit) >= 0;
+    }
+    int bin = kBins;
+    if (by_mass) {
+      bin = find_bin<false, false>(per_unit, (double)r.top_p);
+      if (bin < 0 || bin == kBins - 1) return false;   // (a mark that rounding put between two bins; weights of no units)
+    }
+    return sum_and_choose(per_unit, by_mass, bin, lane, warp, tid);
+  }
+
+  // The bin, as a float: nearest to (top - logit) * per_unit, which grows as logits fall; the last one for NaN and -inf.
+  __device__ __forceinline__ float place(float v, float per_unit) const { return fminf((top - v) * per_unit, (float)(kBins - 1)); }
+  static __device__ __forceinline__ int bin_of(float at) { return (int)(__float_as_uint(at + 8388608.f) & 0x7fffffu); }
+
+  // The bin in which the sum over bins passes `need` (a count, or a share of the mass), or -1.
+  template <bool COUNT, bool GROUPS> __device__ __forceinline__ int find_bin(float per_unit, double need) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
-    if (tid == 0) { s.found = -1; s.n_list = 0; }
+    if (tid == 0) s.found = -1;
     __syncthreads();
-    struct alignas(4 * sizeof(Key)) Four { Key k[4]; };
-    for (int i = tid; i < slice / 4; i += kThreads) {
-      const Four f = ((const Four*)keys)[i];
+    for (int i = tid; i < slice / Piece<T>::N; i += kThreads) {
+      const Piece<T> x = ((const Piece<T>*)logits)[i];
+      if constexpr (GROUPS) {
+        const int b = bin_of(place(L::largest(*(const uint4*)&x), per_unit));
+        if (b < kBins - 1) atomicAdd(&s.hist[b], 1u);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (f.k[j]) {
-          const float at = place(f.k[j]);
+        for (int j = 0; j < Piece<T>::N; ++j) {
+          const float at = place(L::widen(x.e[j]), per_unit);
           const int b = bin_of(at);
           uint32_t add = 1;
-          if (!by_count) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
-            const float x = ((float)b - at) * (1.f / kBinsPerE);
-            add = __float_as_uint(fmaf(fmaf(fmaf(x, 1.f / 6, 0.5f), x, 1.f), x * 65536.f, 65536.f + 8388608.f)) & 0x7fffffu;
+          if (!COUNT) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
+            const float d = ((float)b - at) * (1.f / kBinsPerE);
+            add = __float_as_uint(fmaf(fmaf(fmaf(d, 1.f / 6, 0.5f), d, 1.f), d * 65536.f, 65536.f + 8388608.f)) & 0x7fffffu;
           }
-          atomicAdd(&s.hist[b], add);
+          if (b < kBins - 1) atomicAdd(&s.hist[b], add);
         }
+      }
     }
     cluster.sync();
     // each CTA adds up its share of the bins
-    const int share = kBins / ranks, each = share > kThreads ? share / kThreads : 1, b0 = rank * share + tid * each;
-    const bool mine = tid * each < share;
-    double v[kBins / kThreads], sum = 0;
+    constexpr int kShare = kBins / RANKS, kEach = kShare > kThreads ? kShare / kThreads : 1;
+    const int b0 = rank * kShare + tid * kEach;
+    double v[kEach], sum = 0;
 #pragma unroll
-    for (int j = 0; j < kBins / kThreads; ++j) {
+    for (int j = 0; j < kEach; ++j) {
       v[j] = 0;
-      if (mine && j < each) {
-        unsigned long long n = 0;
-        for (int k = 0; k < ranks; ++k) n += cluster.map_shared_rank(&s, k)->hist[b0 + j];
-        v[j] = (double)n;
-        if (!by_count) v[j] *= (double)exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE));
+      if (tid * kEach < kShare) {
+        uint32_t n[RANKS];
+#pragma unroll
+        for (int k = 0; k < RANKS; ++k) n[k] = peer(k)->hist[b0 + j];
+        unsigned long long m = 0;
+#pragma unroll
+        for (int k = 0; k < RANKS; ++k) m += n[k];
+        v[j] = (double)m;
+        if (!COUNT) v[j] *= (double)exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE));
       }
       sum += v[j];
     }
     double total;
     const double before = block_scan(sum, (double*)s.warp_sum, total, lane, warp);
-    if (tid == 0) s.share = total;
+    if (tid < RANKS) peer(tid)->shares[rank] = total;
     cluster.sync();
     double offset = 0, everything = 0;
-    for (int k = 0; k < ranks; ++k) {
+#pragma unroll
+    for (int k = 0; k < RANKS; ++k) {
       if (k == rank) offset = everything;
-      everything += cluster.map_shared_rank(&s, k)->share;
+      everything += s.shares[k];
     }
-    const double need = by_count ? (double)r.top_k : (double)r.top_p * everything;
+    const double mark = COUNT ? need : need * everything;
     double run = offset + before;
 #pragma unroll
-    for (int j = 0; j < kBins / kThreads; ++j) {
-      if (run < need && need <= run + v[j])
-        for (int k = 0; k < ranks; ++k) cluster.map_shared_rank(&s, k)->found = b0 + j;
+    for (int j = 0; j < kEach; ++j) {
+      if (run < mark && mark <= run + v[j])
+        for (int k = 0; k < RANKS; ++k) peer(k)->found = b0 + j;
       run += v[j];
     }
     cluster.sync();
-    bin = s.found;
-    if (bin < 0 || bin == kBins - 1) return false;   // (fewer tokens than k; a mark that rounding put between two bins; weights of no units)
+    return s.found;
   }
-  auto push = [&](bool any, Key k, int i) {
-    const uint32_t who = __ballot_sync(~0u, any);
-    if (!who) return;
-    int at = 0;
-    if (lane == __ffs(who) - 1) at = atomicAdd(&first->n_list, __popc(who));
-    at = __shfl_sync(~0u, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-    if (any && at < kList) first->list[at] = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(base + i);
-  };
-  const int sub = slice / kWarps, warp_base = warp * sub;
-  const double least = (double)r.min_p;
-  if (by_count) {
-    for (int i = lane; i < sub; i += 32) {
-      const Key k = keys[warp_base + i];
-      push(k && bin_of(place(k)) <= bin, k, warp_base + i);
-    }
-  } else {
-    // (below this no weight passes min-p, with room for the roundings of 32 bits)
-    const float last = by_mass ? (float)(kBins - 1) : r.min_p > 0.f ? fminf(-kBinsPerE * logf(r.min_p) + 1.f, (float)(kBins - 1)) : (float)(kBins - 1);
-    unsigned long long all = 0, below = 0, taken = 0;
-    for (int i = lane; i < sub; i += 32) {
-      const Key k = keys[warp_base + i];
-      const float at = k ? place(k) : (float)kBins;
-      bool listed = false;
-      if (at < last) {
-        const double w = weight(k);
-        const unsigned long long u = units(w);
-        const int b = bin_of(at);
-        all += u;
-        if (!by_mass || b < bin) {
-          below += u;
-          if (w >= least) taken += u;
-        } else {
-          listed = b == bin;
-        }
+
+  // Appends to this CTA's list the logits of a piece that `mask` names; all lanes of the warp take part.
+  __device__ __forceinline__ void append(uint32_t mask, const Piece<T>& x, int at, int lane) {
+    if (!__any_sync(~0u, mask)) return;
+    int n = __popc(mask), upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(~0u, upto, o); if (lane >= o) upto += u; }
+    int start = 0;
+    if (lane == 31) start = atomicAdd(&s.n_list, upto);
+    start = __shfl_sync(~0u, start, 31) + upto - n;
+#pragma unroll
+    for (int j = 0; j < Piece<T>::N; ++j)
+      if (mask >> j & 1) {
+        if (start < kList) s.list[start] = ((unsigned long long)L::key(x.e[j]) << 32) | (uint32_t)~(uint32_t)(base + at + j);
+        ++start;
       }
-      if (by_mass) push(listed, k, warp_base + i);
+  }
+  // The CTAs' lists, one after the other in the first one's memory.  Returns their length; above kList they are not there.
+  __device__ __forceinline__ int collect() {
+    const int tid = threadIdx.x, n = s.n_list;   // (after a barrier)
+    if (tid < RANKS) peer(tid)->listed[rank] = n;
+    cluster.sync();
+    int offset = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < RANKS; ++k) {
+      if (k == rank) offset = all;
+      all += s.listed[k];
     }
-    all = warp_sum(all); below = warp_sum(below); taken = warp_sum(taken);
-    if (lane == 0) { first->all[rank * kWarps + warp] = all; first->below[rank * kWarps + warp] = below; first->taken[rank * kWarps + warp] = taken; }
+    if (all <= kList) {
+      if (rank) {
+        Shared* first = peer(0);
+        for (int i = tid; i < n; i += kThreads) first->list[offset + i] = s.list[i];
+      }
+    }
+    cluster.sync();
+    return all;
   }
-  cluster.sync();
-  if (by_count || by_mass) {
-    const bool full = first->n_list > kList;
-    cluster.sync();   // (the first CTA goes on, and the others may leave)
-    if (full) return false;
+  // The first CTA's list, largest first: by bins, and inside a bin by counting, or, where a bin is crowded, by exchanges.
+  __device__ __forceinline__ void sort(int n, float per_unit) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < kBins; i += kThreads) s.bucket[i] = 0;
+    if (tid == 0) s.crowded = 0;
+    __syncthreads();
+    unsigned long long entry[kList / kThreads];
+    int b[kList / kThreads];
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      const int i = j * kThreads + tid;
+      if (i < n) {
+        entry[j] = s.list[i];
+        b[j] = bin_of(place(L::value((Key)(entry[j] >> 32)), per_unit));
+        if (atomicAdd(&s.bucket[b[j]], 1u) >= kBucket) s.crowded = 1;
+      }
+    }
+    __syncthreads();
+    if (s.crowded) {
+      int n2 = 2;
+      while (n2 < n) n2 *= 2;
+      for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
+      sort_list(s.list, n2, tid);
+      return;
+    }
+    uint32_t mine[kBins / kThreads], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < kBins / kThreads; ++j) sum += mine[j] = s.bucket[tid * (kBins / kThreads) + j];
+    uint32_t run = block_scan(sum, (uint32_t*)s.warp_sum, total, lane, warp);
+#pragma unroll
+    for (int j = 0; j < kBins / kThreads; ++j) { s.bucket[tid * (kBins / kThreads) + j] = run; run += mine[j]; }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j)
+      if (j * kThreads + tid < n) spare[atomicAdd(&s.bucket[b[j]], 1u)] = entry[j];
+    __syncthreads();
+    // (each bucket now names its end, which is the next one's beginning)
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j)
+      if (j * kThreads + tid < n) {
+        const uint32_t from = b[j] ? s.bucket[b[j] - 1] : 0u, to = s.bucket[b[j]];
+        uint32_t rank_of = from;
+        for (uint32_t i = from; i < to; ++i) rank_of += spare[i] > entry[j];
+        s.list[rank_of] = entry[j];
+      }
+    __syncthreads();
   }
-  // exact weights of the sorted list, four entries per thread; entries from `limit` on do not count
-  unsigned long long unit[4], sum = 0, total = 0, run = 0;
-  double w[4];
-  auto weigh = [&](int limit) {
+
+  // Returns 0 when the token is written, -1 when the row has to go the general way, -2 when more tokens than fit lie in the groups' bin.
+  template <bool GROUPS> __device__ __forceinline__ int top_k(float per_unit) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int bin = find_bin<true, GROUPS>(per_unit, (double)r.top_k);
+    if (bin < 0) return GROUPS ? -2 : -1;   // (fewer than k of them outside the last bin)
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    for (int i = tid; i < slice / Piece<T>::N; i += kThreads) {   // (whole warps: a slice is a multiple of 32 pieces)
+      const Piece<T> x = ((const Piece<T>*)logits)[i];
+      uint32_t mask = 0;
+      if (bin_of(place(L::largest(*(const uint4*)&x), per_unit)) <= bin) {
+#pragma unroll
+        for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
+      }
+      append(mask, x, i * Piece<T>::N, lane);
+    }
+    __syncthreads();
+    const int n = collect();
+    if (n > kList) return GROUPS ? -2 : -1;
+    if (rank) return 0;
+    sort(n, per_unit);
+    // the first top_k of the sorted list, four entries per thread
+    const bool by_mass = r.top_p < 1.f;
+    const double least = (double)r.min_p;
+    unsigned long long unit[4], sum = 0, total;
+    double w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = tid * 4 + j;
-      w[j] = i < limit ? weight((Key)(s.list[i] >> 32)) : 0.0;
-      unit[j] = i < limit ? units(w[j]) : 0;
-      sum += unit[j];
+      w[j] = i < r.top_k ? weight(L::value((Key)(s.list[i] >> 32))) : 0.0;
+      sum += unit[j] = i < r.top_k ? units(w[j]) : 0;
     }
-    run = block_scan(sum, s.warp_sum, total, lane, warp);
-  };
-  auto sorted = [&]() {
-    const int n = s.n_list;
-    int n2 = 2;
-    while (n2 < n) n2 *= 2;
-    for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
-    sort_list(s.list, n2, tid);
-    return n;
-  };
-  if (by_count) {
-    if (rank) return true;
-    sorted();
-    weigh(r.top_k);
+    unsigned long long run = block_scan(sum, s.warp_sum, total, lane, warp), kept = 0;
     const double mark = by_mass ? (double)r.top_p * (double)total : 0.0;
-    unsigned long long kept = 0;
+    int n_kept = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = tid * 4 + j;
-      if (i < r.top_k && (i == 0 || ((!by_mass || (double)run < mark) && w[j] >= least))) {
-        kept += unit[j];
-        s.weight[i] = unit[j];
-      } else if (i < kListTopK) {
-        s.weight[i] = 0;
-      }
+      const bool keep = i < r.top_k && (i == 0 || ((!by_mass || (double)run < mark) && w[j] >= least));
+      if (keep) { kept += unit[j]; n_kept = i + 1; }
+      if (i < kTopK) s.weight[i] = keep ? unit[j] : 0;
       run += unit[j];
     }
+    if (tid == 0) { s.pick = 0; s.token = INT_MAX; }
     block_scan(kept, s.warp_sum, total, lane, warp);
-    // by index, six bits at a time: the digit at which the running sum passes the target
+    if (n_kept) atomicMax(&s.pick, n_kept);
+    __syncthreads();
+    n_kept = s.pick;
     const double target = (double)r.uniform * (double)total;
+    if (n_kept <= kFew) {   // four threads for each: the sum over those of lower or the same index
+      const int i = tid >> 2;
+      const uint32_t index = i < n_kept ? ~(uint32_t)s.list[i] : 0u;
+      unsigned long long upto = 0;
+      for (int j = tid & 3; j < n_kept; j += 4)
+        if (~(uint32_t)s.list[j] <= index) upto += s.weight[j];
+      upto += __shfl_xor_sync(~0u, upto, 1);
+      upto += __shfl_xor_sync(~0u, upto, 2);
+      if (i < n_kept && (double)upto > target) atomicMin(&s.token, (int)index);
+      __syncthreads();
+      if (tid == 0) tokens[row] = s.token;
+      return 0;
+    }
+    // by index, six bits at a time: the digit at which the running sum passes the target
     uint32_t prefix = 0;
     unsigned long long before = 0;
     for (int shift = 12; shift >= 0; shift -= 6) {
       if (tid < 64) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
       __syncthreads();
-      for (int i = tid; i < r.top_k; i += kThreads) {
+      for (int i = tid; i < n_kept; i += kThreads) {
         const uint32_t index = ~(uint32_t)s.list[i];
         const unsigned long long u = s.weight[i];
-        if (u && index >> (shift + 6) == prefix) {
-          const int d = (index >> shift) & 63;
-          const uint32_t lo = (uint32_t)u, old = atomicAdd(&s.lo[0][d], lo), up = (uint32_t)(u >> 32) + (old + lo < old ? 1u : 0u);
-          if (up) atomicAdd(&s.hi[0][d], up);
-        }
+        if (u && index >> (shift + 6) == prefix) add_units(&s.lo[0][(index >> shift) & 63], &s.hi[0][(index >> shift) & 63], u);
       }
       __syncthreads();
       if (warp == 0) {
@@ -339,257 +464,221 @@ __device__ __forceinline__ bool direct(Shared& s, cg::cluster_group& cluster, co
       before = s.above;
     }
     if (tid == 0) tokens[row] = (int)prefix;
-    return true;
+    return 0;
   }
-  if (rank == 0) {
-    // the sums of all warps, in index order
-    const int n_warps = ranks * kWarps;
-    const unsigned long long all = tid < n_warps ? s.all[tid] : 0, below = tid < n_warps ? s.below[tid] : 0;
-    unsigned long long sum_all, sum_below;
-    block_scan(all, s.warp_sum, sum_all, lane, warp);
-    block_scan(below, s.warp_sum, sum_below, lane, warp);
-    if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; }
-    if (by_mass) {
-      const int n = sorted();
-      weigh(n);
-      const double mark = (double)r.top_p * (double)sum_all;
-      run += sum_below;
-      // (kept entries are the first ones; the last of them ends the kept tokens)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = tid * 4 + j;
-        const bool kept = i < n && ((double)run < mark || (i == 0 && sum_below == 0));
-        const bool next = i + 1 < n && (double)(run + unit[j]) < mark;
-        if (kept) {
-          const unsigned long long entry = s.list[i];
-          if (!next) s.cut_entry = entry;
-          const uint32_t index = ~(uint32_t)entry;
-          if (w[j] >= least) atomicAdd(&s.taken[index / (uint32_t)sub], unit[j]);
-        }
-        run += unit[j];
-      }
-      if (tid == 0 && !((sum_below == 0 || (double)sum_below < mark) && mark <= (double)(sum_below + total))) s.ok = 0;
-    }
+
+  __device__ __forceinline__ bool sum_and_choose(float per_unit, bool by_mass, int bin, int lane, int warp, int tid) {
+    constexpr int N = Piece<T>::N;
+    Shared* first = peer(0);
+    const int sub = slice / kWarps, warp_base = warp * sub;   // a warp's stretch
+    const double least = (double)r.min_p;
+    if (tid == 0) s.n_list = 0;
     __syncthreads();
-    const unsigned long long taken = tid < n_warps ? s.taken[tid] : 0;
-    unsigned long long sum_taken;
-    const unsigned long long before = block_scan(taken, s.warp_sum, sum_taken, lane, warp);
-    const double target = (double)r.uniform * (double)sum_taken;
-    if (!((double)before > target) && (double)(before + taken) > target)
-      for (int k = 0; k < ranks; ++k) {
-        Shared* o = cluster.map_shared_rank(&s, k);
-        o->owner = tid; o->before = before; o->target = target;
-      }
-    __syncthreads();
-    if (tid < ranks && tid) { Shared* o = cluster.map_shared_rank(&s, tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
-  }
-  cluster.sync();
-  if (!s.ok) return false;
-  if (s.owner / kWarps != rank) return true;
-  // the stretch of one warp, now by all warps of its CTA
-  const Key cut = (Key)(s.cut_entry >> 32);
-  const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
-  auto chosen = [&](int i) -> unsigned long long {
-    if (i >= sub) return 0;
-    const Key k = keys[stretch + i];
-    if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
-    const double w = weight(k);
-    return w >= least ? units(w) : 0;
-  };
-  unsigned long long mine = 0;
-  for (int i = warp * part + lane; i < (warp + 1) * part; i += 32) mine += chosen(i);
-  mine = warp_sum(mine);
-  __syncthreads();
-  if (lane == 0) s.warp_sum[warp] = mine;
-  __syncthreads();
-  unsigned long long before = s.before;
-  for (int k = 0; k < warp; ++k) before += s.warp_sum[k];
-  if ((double)before > s.target || !((double)(before + mine) > s.target)) return true;
-  for (int i = warp * part; i < (warp + 1) * part; i += 32) {
-    const unsigned long long upto = before + warp_scan(chosen(i + lane), lane);
-    const uint32_t ballot = __ballot_sync(~0u, (double)upto > s.target);
-    if (ballot) {
-      if (lane == __ffs(ballot) - 1) tokens[row] = base + stretch + i + lane;
-      break;
-    }
-    before = __shfl_sync(~0u, upto, 31);
-  }
-  return true;
-}
-
-// One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps as keys in shared memory.
-//   1. the largest key (and, of those, the lowest index);
-//   2. top-k and top-p, each a search for the key t and, among the tokens with that key, the last index c that are still kept: a
-//      histogram of counts, or of masses, over 8 bits of the keys at a time from the top;
-//   3. the sum of what is kept, and the place where the running sum passes uniform * W.
-// Sums over CTAs go through distributed shared memory in rank order; index order is rank order, then warp order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, const float* temperature,
-                                                          const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
-  using K = Keys<T>;
-  using Key = typename K::Key;
-  extern __shared__ __align__(16) uint8_t dynamic[];
-  Key* keys = (Key*)dynamic;
-  __shared__ Shared s;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = rank * slice;
-  const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
-
-  if (tid < 256) { s.table[tid] = exp2((double)tid / 256.0); s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
-  // ---- 1. keys, and the largest ----
-  unsigned long long best = 0;
-  const T* src = logits + (int64_t)row * row_stride + base;
-  const int here = max(0, min(slice, vocab - base));
-  auto put = [&](int i, T v) {
-    const Key k = K::key(v);
-    keys[i] = k;
-    const unsigned long long b = ((unsigned long long)k << 32) | (uint32_t)~(uint32_t)(base + i);
-    if (k && b > best) best = b;
-  };
-  constexpr int VEC = 16 / sizeof(T);
-  int done = 0;
-  if (vec) {
-    done = here / VEC * VEC;
-#pragma unroll 2
-    for (int i = tid * VEC; i < done; i += kThreads * VEC) {
-      const uint4 u = *(const uint4*)(src + i);
-      T e[VEC];
-      *(uint4*)e = u;
+    {
+      // (where only min-p chooses, no weight past this place passes it, with room for the roundings of 32 bits)
+      const float last = by_mass || !(r.min_p > 0.f) ? (float)(kBins - 1) : fminf(-kBinsPerE * logf(r.min_p) + 1.f, (float)(kBins - 1));
+      const float floor = top - 70.f * r.temperature;   // no units; NaN and -inf become this
+      unsigned long long all = 0, below = 0, taken = 0;
+      for (int i = warp_base / N + lane; i < (warp_base + sub) / N; i += 32) {
+        const Piece<T> x = ((const Piece<T>*)logits)[i];
+        uint32_t mask = 0;
+        if (place(L::largest(*(const uint4*)&x), per_unit) < last) {
+          double w[N];
+          float at[N];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) put(i + j, e[j]);
-    }
-  }
-  for (int i = done + tid; i < here; i += kThreads) put(i, src[i]);
-  for (int i = here + tid; i < slice; i += kThreads) keys[i] = 0;
+          for (int j = 0; j < N; ++j) {
+            const float v = fmaxf(L::widen(x.e[j]), floor);
+            at[j] = place(v, per_unit);
+            w[j] = weight(v);
+          }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) { const unsigned long long v = __shfl_xor_sync(~0u, best, o); if (v > best) best = v; }
-  if (lane == 0) s.warp_sum[warp] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) if (s.warp_sum[w] > best) best = s.warp_sum[w];
-    s.best = best;
-  }
-  cluster.sync();
-  best = 0;
-  for (int k = 0; k < ranks; ++k) { const unsigned long long v = cluster.map_shared_rank(&s, k)->best; if (v > best) best = v; }
-  const Key top_key = (Key)(best >> 32);
-  if (top_key == 0 || !(r.temperature > 0.f)) {
-    if (rank == 0 && tid == 0) tokens[row] = top_key == 0 ? -1 : (int)~(uint32_t)best;
-    cluster.sync();   // nobody leaves while a peer may still read its shared memory
-    return;
-  }
-  const double top = (double)K::value(top_key), scale = 369.32993046757462708 / (double)r.temperature;   // 256 / ln 2
-  auto weight = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)K::value(k) - top, scale, s.table); };
-  if (direct<T>(s, cluster, keys, r, top_key, scale, vocab, slice, row, tokens)) return;
-
-  // Kept so far: key > t, or key == t and index <= c.
-  Key t = 1;
-  int c = INT_MAX, buffer = 0;
-  auto kept = [&](Key k, int i) { return k > t || (k == t && i <= c); };
-  // The key at which counts, or masses, summed from the largest key down, reach the mark; `above` is the sum over the larger keys
-  // and `in_bin` the sum at the key itself.
-  auto search = [&](bool mass, auto reached, bool share_of, double share, unsigned long long& above_out, unsigned long long& bin_out, double& mark) -> Key {
-    Key prefix = 0;
-    unsigned long long above = 0, in_bin = 0;
-    for (int shift = K::kBits - 8; shift >= 0; shift -= 8) {
-      for (int i = tid; i < slice; i += kThreads) {
-        const Key k = keys[i];
-        if (k && (shift + 8 == K::kBits || (uint32_t)k >> (shift + 8) == (uint32_t)prefix) && kept(k, base + i)) {
-          const int b = ((uint32_t)k >> shift) & 255;
-          if (mass) {
-            const unsigned long long u = units(weight(k));
-            if (u) {
-              const uint32_t lo = (uint32_t)u, old = atomicAdd(&s.lo[buffer][b], lo), up = (uint32_t)(u >> 32) + (old + lo < old ? 1u : 0u);
-              if (up) atomicAdd(&s.hi[buffer][b], up);
+          for (int j = 0; j < N; ++j) {
+            const unsigned long long u = units(w[j]);
+            const int b = bin_of(at[j]);
+            all += u;
+            if (b < bin) {
+              below += u;
+              if (w[j] >= least) taken += u;
             }
-          } else {
-            atomicAdd(&s.lo[buffer][b], 1u);
+            mask |= (b == bin ? 1u : 0u) << j;
           }
         }
+        if (by_mass && mask) append_some(mask, x, i * N);
       }
-      cluster.sync();
-      if (tid < 256) {
-        unsigned long long v = 0;
-        for (int k = 0; k < ranks; ++k) {
-          const Shared* o = cluster.map_shared_rank(&s, k);
-          v += ((unsigned long long)o->hi[buffer][tid] << 32) + o->lo[buffer][tid];
-        }
-        s.total[tid] = v;
-        s.lo[buffer ^ 1][tid] = 0;
-        s.hi[buffer ^ 1][tid] = 0;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        unsigned long long mine = 0;
-        for (int j = 0; j < 8; ++j) mine += s.total[255 - lane * 8 - j];
-        const unsigned long long upto = warp_scan(mine, lane);
-        if (share_of && shift + 8 == K::kBits) mark = share * (double)__shfl_sync(~0u, upto, 31);
-        unsigned long long run = above + upto - mine;
-        if (!reached(run, mark) && reached(run + mine, mark))
-          for (int j = 0; j < 8; ++j) {
-            const unsigned long long v = s.total[255 - lane * 8 - j];
-            if (reached(run + v, mark)) { s.bin = (uint32_t)(255 - lane * 8 - j); s.above = run; s.in_bin = v; break; }
-            run += v;
-          }
-      }
-      __syncthreads();
-      prefix = (Key)((uint32_t)prefix << 8 | s.bin);
-      above = s.above;
-      in_bin = s.in_bin;
-      buffer ^= 1;
+      all = warp_sum(all); below = warp_sum(below); taken = warp_sum(taken);
+      if (lane == 0) { s.warp_sum[warp] = all; first->below[rank * kWarps + warp] = below; first->taken[rank * kWarps + warp] = taken; }
     }
-    above_out = above;
-    bin_out = in_bin;
-    return prefix;
-  };
-  // The index of the n-th kept token, by index, whose key is `key`.
-  const int sub = slice / kWarps, warp_base = warp * sub;
-  auto nth = [&](Key key, int n) -> int {
-    int mine = 0;
-    for (int i = lane; i < sub; i += 32) mine += keys[warp_base + i] == key && kept(key, base + warp_base + i);
-    const unsigned long long count = warp_sum((unsigned long long)mine);
-    __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = count;
-    if (tid == 0) s.cut = -1;
     __syncthreads();
     if (tid == 0) {
       unsigned long long v = 0;
-      for (int w = 0; w < kWarps; ++w) v += s.warp_sum[w];
-      s.cta_sum = v;
+      for (int k = 0; k < kWarps; ++k) v += s.warp_sum[k];
+      first->all[rank] = v;
+    }
+    int n = 0;
+    if (by_mass) {
+      n = collect();
+      if (n > kList) return false;
+    } else {
+      cluster.sync();
+    }
+    if (rank == 0) {
+      // the sums of all warps, in index order
+      constexpr int kAll = RANKS * kWarps;
+      unsigned long long sum_all = 0, sum_below, total = 0;
+#pragma unroll
+      for (int k = 0; k < RANKS; ++k) sum_all += s.all[k];
+      if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; }
+      if (by_mass) {
+        block_scan(tid < kAll ? s.below[tid] : 0ull, s.warp_sum, sum_below, lane, warp);
+        sort(n, per_unit);
+        unsigned long long unit[4], sum = 0;
+        double w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = tid * 4 + j;
+          w[j] = i < n ? weight(L::value((Key)(s.list[i] >> 32))) : 0.0;
+          sum += unit[j] = i < n ? units(w[j]) : 0;
+        }
+        unsigned long long run = sum_below + block_scan(sum, s.warp_sum, total, lane, warp);
+        const double mark = (double)r.top_p * (double)sum_all;
+        // (kept entries are the first ones; the last of them ends the kept tokens)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = tid * 4 + j;
+          const bool keep = i < n && ((double)run < mark || (i == 0 && sum_below == 0));
+          if (keep) {
+            const unsigned long long entry = s.list[i];
+            if (!(i + 1 < n && (double)(run + unit[j]) < mark)) s.cut_entry = entry;
+            if (w[j] >= least) atomicAdd(&s.taken[~(uint32_t)entry / (uint32_t)sub], unit[j]);
+          }
+          run += unit[j];
+        }
+        if (tid == 0 && !((sum_below == 0 || (double)sum_below < mark) && mark <= (double)(sum_below + total))) s.ok = 0;
+      }
+      __syncthreads();
+      const unsigned long long taken = tid < kAll ? s.taken[tid] : 0;
+      unsigned long long sum_taken;
+      const unsigned long long before = block_scan(taken, s.warp_sum, sum_taken, lane, warp);
+      const double target = (double)r.uniform * (double)sum_taken;
+      if (!((double)before > target) && (double)(before + taken) > target)
+        for (int k = 0; k < RANKS; ++k) { Shared* o = peer(k); o->owner = tid; o->before = before; o->target = target; }
+      if (tid && tid < RANKS) { Shared* o = peer(tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
     }
     cluster.sync();
-    long long before = 0;
-    for (int k = 0; k < rank; ++k) before += (long long)cluster.map_shared_rank(&s, k)->cta_sum;
-    for (int w = 0; w < warp; ++w) before += (long long)s.warp_sum[w];
-    if (before < n && before + (long long)count >= n)
-      for (int i = 0; i < sub; i += 32) {
-        const bool hit = keys[warp_base + i + lane] == key && kept(key, base + warp_base + i + lane);
-        const uint32_t ballot = __ballot_sync(~0u, hit);
-        const int upto = (int)before + __popc(ballot & (0xffffffffu >> (31 - lane)));
-        if (hit && upto == n) s.cut = base + warp_base + i + lane;
-        before += __popc(ballot);
-        if (before >= n) break;
+    if (!s.ok) return false;
+    if (s.owner / kWarps != rank) return true;
+    // the stretch of one warp, now by all warps of its CTA
+    const Key cut = (Key)(s.cut_entry >> 32);
+    const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
+    auto chosen = [&](int i) -> unsigned long long {
+      if (i >= sub) return 0;
+      const T x = logits[stretch + i];
+      const Key k = L::key(x);
+      if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
+      const double w = weight(L::widen(x));
+      return w >= least ? units(w) : 0;
+    };
+    unsigned long long mine = 0;
+    for (int i = warp * part + lane; i < (warp + 1) * part; i += 32) mine += chosen(i);
+    mine = warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) s.warp_sum[warp] = mine;
+    __syncthreads();
+    unsigned long long before = s.before;
+    for (int k = 0; k < warp; ++k) before += s.warp_sum[k];
+    if ((double)before > s.target || !((double)(before + mine) > s.target)) return true;
+    for (int i = warp * part; i < (warp + 1) * part; i += 32) {
+      const unsigned long long upto = before + warp_scan(chosen(i + lane), lane);
+      const uint32_t ballot = __ballot_sync(~0u, (double)upto > s.target);
+      if (ballot) {
+        if (lane == __ffs(ballot) - 1) tokens[row] = base + stretch + i + lane;
+        break;
       }
-    cluster.sync();
-    int found = -1;
-    for (int k = 0; k < ranks; ++k) found = max(found, cluster.map_shared_rank(&s, k)->cut);
-    cluster.sync();
-    return found;
-  };
+      before = __shfl_sync(~0u, upto, 31);
+    }
+    return true;
+  }
+  // The same one logit at a time, for lanes that may be fewer than a warp.
+  __device__ __forceinline__ void append_some(uint32_t mask, const Piece<T>& x, int at) {
+#pragma unroll
+    for (int j = 0; j < Piece<T>::N; ++j)
+      if (mask >> j & 1) {
+        const int i = atomicAdd(&s.n_list, 1);
+        if (i < kList) s.list[i] = ((unsigned long long)L::key(x.e[j]) << 32) | (uint32_t)~(uint32_t)(base + at + j);
+      }
+  }
 
-  // ---- 2. top-k, top-p ----
-  unsigned long long above = 0, in_bin = 0;
-  double mark = 0.0;
-  if (r.top_k > 0 && r.top_k < vocab) {
-    // (with fewer live logits than k no sum reaches the mark: everything stays)
-    unsigned long long live = 0;
-    {
+  // Any row: one search for top-k and one for top-p, each over 8 bits of the keys at a time from the top.
+  __device__ __noinline__ void general() {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = RANKS;
+    const Key top_key = key_of_top();
+    auto weight_of = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)L::value(k) - (double)top, scale, s.table); };
+    // Kept so far: key > t, or key == t and index <= c.
+    Key t = 1;
+    int c = INT_MAX, buffer = 0;
+    auto kept = [&](Key k, int i) { return k > t || (k == t && i <= c); };
+    // The key at which counts, or masses, summed from the largest key down, reach the mark; `above` is the sum over the larger keys
+    // and `in_bin` the sum at the key itself.
+    auto search = [&](bool mass, auto reached, bool share_of, double share, unsigned long long& above_out, unsigned long long& bin_out, double& mark) -> Key {
+      Key prefix = 0;
+      unsigned long long above = 0, in_bin = 0;
+      for (int shift = L::kBits - 8; shift >= 0; shift -= 8) {
+        for (int i = tid; i < slice; i += kThreads) {
+          const Key k = L::key(logits[i]);
+          if (k && (shift + 8 == L::kBits || (uint32_t)k >> (shift + 8) == (uint32_t)prefix) && kept(k, base + i)) {
+            const int b = ((uint32_t)k >> shift) & 255;
+            if (mass) {
+              const unsigned long long u = units(weight_of(k));
+              if (u) add_units(&s.lo[buffer][b], &s.hi[buffer][b], u);
+            } else {
+              atomicAdd(&s.lo[buffer][b], 1u);
+            }
+          }
+        }
+        cluster.sync();
+        if (tid < 256) {
+          unsigned long long v = 0;
+          for (int k = 0; k < ranks; ++k) {
+            const Shared* o = cluster.map_shared_rank(&s, k);
+            v += ((unsigned long long)o->hi[buffer][tid] << 32) + o->lo[buffer][tid];
+          }
+          s.total[tid] = v;
+          s.lo[buffer ^ 1][tid] = 0;
+          s.hi[buffer ^ 1][tid] = 0;
+        }
+        __syncthreads();
+        if (warp == 0) {
+          unsigned long long mine = 0;
+          for (int j = 0; j < 8; ++j) mine += s.total[255 - lane * 8 - j];
+          const unsigned long long upto = warp_scan(mine, lane);
+          if (share_of && shift + 8 == L::kBits) mark = share * (double)__shfl_sync(~0u, upto, 31);
+          unsigned long long run = above + upto - mine;
+          if (!reached(run, mark) && reached(run + mine, mark))
+            for (int j = 0; j < 8; ++j) {
+              const unsigned long long v = s.total[255 - lane * 8 - j];
+              if (reached(run + v, mark)) { s.bin = (uint32_t)(255 - lane * 8 - j); s.above = run; s.in_bin = v; break; }
+              run += v;
+            }
+        }
+        __syncthreads();
+        prefix = (Key)((uint32_t)prefix << 8 | s.bin);
+        above = s.above;
+        in_bin = s.in_bin;
+        buffer ^= 1;
+      }
+      above_out = above;
+      bin_out = in_bin;
+      return prefix;
+    };
+    // The index of the n-th kept token, by index, whose key is `key`.
+    const int sub = slice / kWarps, warp_base = warp * sub;
+    auto nth = [&](Key key, int n) -> int {
       int mine = 0;
-      for (int i = tid; i < slice; i += kThreads) mine += keys[i] != 0;
-      const unsigned long long n = warp_sum((unsigned long long)mine);
-      if (lane == 0) s.warp_sum[warp] = n;
+      for (int i = lane; i < sub; i += 32) mine += L::key(logits[warp_base + i]) == key && kept(key, base + warp_base + i);
+      const unsigned long long count = warp_sum((unsigned long long)mine);
+      __syncthreads();
+      if (lane == 0) s.warp_sum[warp] = count;
+      if (tid == 0) s.cut = -1;
       __syncthreads();
       if (tid == 0) {
         unsigned long long v = 0;
@@ -597,96 +686,196 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
         s.cta_sum = v;
       }
       cluster.sync();
-      for (int k = 0; k < ranks; ++k) live += cluster.map_shared_rank(&s, k)->cta_sum;
+      long long before = 0;
+      for (int k = 0; k < rank; ++k) before += (long long)cluster.map_shared_rank(&s, k)->cta_sum;
+      for (int w = 0; w < warp; ++w) before += (long long)s.warp_sum[w];
+      if (before < n && before + (long long)count >= n)
+        for (int i = 0; i < sub; i += 32) {
+          const bool hit = L::key(logits[warp_base + i + lane]) == key && kept(key, base + warp_base + i + lane);
+          const uint32_t ballot = __ballot_sync(~0u, hit);
+          const int upto = (int)before + __popc(ballot & (0xffffffffu >> (31 - lane)));
+          if (hit && upto == n) s.cut = base + warp_base + i + lane;
+          before += __popc(ballot);
+          if (before >= n) break;
+        }
       cluster.sync();
+      int found = -1;
+      for (int k = 0; k < ranks; ++k) found = max(found, cluster.map_shared_rank(&s, k)->cut);
+      cluster.sync();
+      return found;
+    };
+
+    // ---- 2. top-k, top-p ----
+    unsigned long long above = 0, in_bin = 0;
+    double mark = 0.0;
+    if (r.top_k > 0 && r.top_k < vocab) {
+      // (with fewer live logits than k no sum reaches the mark: everything stays)
+      unsigned long long live = 0;
+      {
+        int mine = 0;
+        for (int i = tid; i < slice; i += kThreads) mine += L::key(logits[i]) != 0;
+        const unsigned long long n = warp_sum((unsigned long long)mine);
+        if (lane == 0) s.warp_sum[warp] = n;
+        __syncthreads();
+        if (tid == 0) {
+          unsigned long long v = 0;
+          for (int w = 0; w < kWarps; ++w) v += s.warp_sum[w];
+          s.cta_sum = v;
+        }
+        cluster.sync();
+        for (int k = 0; k < ranks; ++k) live += cluster.map_shared_rank(&s, k)->cta_sum;
+        cluster.sync();
+      }
+      if ((unsigned long long)r.top_k < live) {
+        const unsigned long long need = (unsigned long long)r.top_k;
+        const Key found = search(false, [need](unsigned long long v, double) { return v >= need; }, false, 0.0, above, in_bin, mark);
+        const int ties = (int)(need - above);
+        const int last = (unsigned long long)ties < in_bin ? nth(found, ties) : INT_MAX;
+        t = found;
+        c = last;
+      }
     }
-    if ((unsigned long long)r.top_k < live) {
-      const unsigned long long need = (unsigned long long)r.top_k;
-      const Key found = search(false, [need](unsigned long long v, double) { return v >= need; }, false, 0.0, above, in_bin, mark);
-      const int ties = (int)(need - above);
-      const int last = (unsigned long long)ties < in_bin ? nth(found, ties) : INT_MAX;
+    if (r.top_p < 1.f) {
+      const double p = (double)fmaxf(r.top_p, 0.f);
+      const Key found = search(true, [](unsigned long long v, double m) { return (double)v >= m && v > 0; }, true, p, above, in_bin, mark);
+      // (the mark is known to warp 0)
+      const unsigned long long w = units(weight_of(found));
+      if (tid == 0) {
+        long long j = w ? (long long)((mark - (double)above) / (double)w) : 1;
+        if (j < 1) j = 1;
+        while (j > 1 && (double)(above + (unsigned long long)(j - 1) * w) >= mark) --j;
+        while ((double)(above + (unsigned long long)j * w) < mark) ++j;
+        s.pick = (int)j;
+      }
+      __syncthreads();
+      const int ties = s.pick;
+      const int old = found == t ? c : INT_MAX;
+      const int last = (unsigned long long)ties * w < in_bin ? nth(found, ties) : old;
       t = found;
       c = last;
     }
-  }
-  if (r.top_p < 1.f) {
-    const double p = (double)fmaxf(r.top_p, 0.f);
-    const Key found = search(true, [](unsigned long long v, double m) { return (double)v >= m && v > 0; }, true, p, above, in_bin, mark);
-    // (the mark is known to warp 0)
-    const unsigned long long w = units(weight(found));
-    if (tid == 0) {
-      long long j = w ? (long long)((mark - (double)above) / (double)w) : 1;
-      if (j < 1) j = 1;
-      while (j > 1 && (double)(above + (unsigned long long)(j - 1) * w) >= mark) --j;
-      while ((double)(above + (unsigned long long)j * w) < mark) ++j;
-      s.pick = (int)j;
-    }
-    __syncthreads();
-    const int ties = s.pick;
-    const int old = found == t ? c : INT_MAX;
-    const int last = (unsigned long long)ties * w < in_bin ? nth(found, ties) : old;
-    t = found;
-    c = last;
-  }
 
-  // ---- 3. the choice ----
-  const double least = (double)r.min_p;
-  auto chosen_weight = [&](int i, bool& is_kept) -> unsigned long long {
-    const Key k = keys[i];
-    is_kept = false;
-    if (!k || !kept(k, base + i)) return 0;
-    const double w = weight(k);
-    is_kept = w >= least;
-    return is_kept ? units(w) : 0;
-  };
-  unsigned long long sum = 0;
-  int lowest = INT_MAX, highest = -1;
-  for (int i = lane; i < sub; i += 32) {
-    bool is_kept;
-    sum += chosen_weight(warp_base + i, is_kept);
-    if (is_kept) { lowest = min(lowest, base + warp_base + i); highest = base + warp_base + i; }
-  }
-  sum = warp_sum(sum);
-  __syncthreads();
-  if (tid == 0) { s.pick = r.uniform > 0.f ? -1 : INT_MAX; s.cut = -1; }
-  if (lane == 0) s.warp_sum[warp] = sum;
-  __syncthreads();
-  if (!(r.uniform > 0.f)) atomicMin(&s.pick, lowest);
-  atomicMax(&s.cut, highest);
-  if (tid == 0) {
-    unsigned long long v = 0;
-    for (int w = 0; w < kWarps; ++w) v += s.warp_sum[w];
-    s.cta_sum = v;
-  }
-  cluster.sync();
-  unsigned long long before = 0, all = 0;
-  int first = INT_MAX, last = -1;
-  for (int k = 0; k < ranks; ++k) {
-    const Shared* o = cluster.map_shared_rank(&s, k);
-    if (k < rank) before += o->cta_sum;
-    all += o->cta_sum;
-    first = min(first, o->pick);
-    last = max(last, o->cut);
-  }
-  const double target = (double)r.uniform * (double)all;
-  if (!(r.uniform > 0.f) || !((double)all > target)) {
-    if (rank == 0 && tid == 0) tokens[row] = !(r.uniform > 0.f) ? first : last;
-  } else {
-    for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
-    if (!((double)before > target) && (double)(before + sum) > target)
-      for (int i = 0; i < sub; i += 32) {
-        bool is_kept;
-        const unsigned long long upto = before + warp_scan(chosen_weight(warp_base + i + lane, is_kept), lane);
-        const uint32_t ballot = __ballot_sync(~0u, (double)upto > target);
-        if (ballot) {
-          if (lane == __ffs(ballot) - 1) tokens[row] = base + warp_base + i + lane;
-          break;
+    // ---- 3. the choice ----
+    const double least = (double)r.min_p;
+    auto chosen_weight = [&](int i, bool& is_kept) -> unsigned long long {
+      const Key k = L::key(logits[i]);
+      is_kept = false;
+      if (!k || !kept(k, base + i)) return 0;
+      const double w = weight_of(k);
+      is_kept = w >= least;
+      return is_kept ? units(w) : 0;
+    };
+    unsigned long long sum = 0;
+    int lowest = INT_MAX, highest = -1;
+    for (int i = lane; i < sub; i += 32) {
+      bool is_kept;
+      sum += chosen_weight(warp_base + i, is_kept);
+      if (is_kept) { lowest = min(lowest, base + warp_base + i); highest = base + warp_base + i; }
+    }
+    sum = warp_sum(sum);
+    __syncthreads();
+    if (tid == 0) { s.pick = r.uniform > 0.f ? -1 : INT_MAX; s.cut = -1; }
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    if (!(r.uniform > 0.f)) atomicMin(&s.pick, lowest);
+    atomicMax(&s.cut, highest);
+    if (tid == 0) {
+      unsigned long long v = 0;
+      for (int w = 0; w < kWarps; ++w) v += s.warp_sum[w];
+      s.cta_sum = v;
+    }
+    cluster.sync();
+    unsigned long long before = 0, all = 0;
+    int first = INT_MAX, last = -1;
+    for (int k = 0; k < ranks; ++k) {
+      const Shared* o = cluster.map_shared_rank(&s, k);
+      if (k < rank) before += o->cta_sum;
+      all += o->cta_sum;
+      first = min(first, o->pick);
+      last = max(last, o->cut);
+    }
+    const double target = (double)r.uniform * (double)all;
+    if (!(r.uniform > 0.f) || !((double)all > target)) {
+      if (rank == 0 && tid == 0) tokens[row] = !(r.uniform > 0.f) ? first : last;
+    } else {
+      for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
+      if (!((double)before > target) && (double)(before + sum) > target)
+        for (int i = 0; i < sub; i += 32) {
+          bool is_kept;
+          const unsigned long long upto = before + warp_scan(chosen_weight(warp_base + i + lane, is_kept), lane);
+          const uint32_t ballot = __ballot_sync(~0u, (double)upto > target);
+          if (ballot) {
+            if (lane == __ffs(ballot) - 1) tokens[row] = base + warp_base + i + lane;
+            break;
+          }
+          before = __shfl_sync(~0u, upto, 31);
         }
-        before = __shfl_sync(~0u, upto, 31);
-      }
+    }
+    cluster.sync();
+  }
+  __device__ __forceinline__ Key key_of_top() const { return L::key(narrow()); }
+  __device__ __forceinline__ T narrow() const { return (T)top; }
+};
+
+// One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps in shared memory.
+template <typename T, int RANKS>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, const float* temperature,
+                                                          const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
+  using L = Logits<T>;
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  __shared__ Shared s;
+  constexpr int N = Piece<T>::N;
+  T* mine = (T*)(dynamic + kList * 8);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), row = blockIdx.x / RANKS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
+  const T* src = logits + (int64_t)row * row_stride + base;
+  const int here = max(0, min(slice, vocab - base)), whole = vec ? here / N * N : 0;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = tid * N; i < whole; i += kThreads * N) {
+    const uint4 u = *(const uint4*)(src + i);
+    *(uint4*)(mine + i) = u;
+    top = fmaxf(top, L::largest(u));
+  }
+  for (int i = whole + tid; i < slice; i += kThreads) {
+    const T v = i < here ? src[i] : L::dead();
+    mine[i] = v;
+    top = fmaxf(top, L::widen(v));
+  }
+  const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
+  if (tid < 256) { s.table[tid] = exp2((double)tid / 256.0); s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  if (lane == 0) s.warp_top[warp] = top;
+  if (tid == 0) s.token = INT_MAX;
+  __syncthreads();
+  if (tid < RANKS) {
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s.warp_top[k]);
+    cluster.map_shared_rank(&s, tid)->tops[rank] = top;
   }
   cluster.sync();
+#pragma unroll
+  for (int k = 0; k < RANKS; ++k) top = fmaxf(top, s.tops[k]);
+  top += 0.f;   // (of two zeros the positive one)
+  if (!(top > -INFINITY) || !(r.temperature > 0.f)) {
+    // nothing to choose from, or the lowest index of the largest logit
+    if (top > -INFINITY) {
+      int at = INT_MAX;
+      for (int i = tid; i < slice; i += kThreads)
+        if (L::widen(mine[i]) == top) { at = base + i; break; }
+      at = __reduce_min_sync(~0u, at);
+      if (lane == 0 && at < INT_MAX) atomicMin(&cluster.map_shared_rank(&s, 0)->token, at);
+      cluster.sync();
+    }
+    if (rank == 0 && tid == 0) tokens[row] = top > -INFINITY ? s.token : -1;
+    return;
+  }
+  Part<T, RANKS> part{s, cluster, mine, (unsigned long long*)dynamic, r, top, 369.32993046757462708 /* 256 / ln 2 */ / (double)r.temperature, vocab, slice, base, rank, row, tokens};
+  if (!part.direct()) part.general();
 }
+
+template <typename T> auto kernel_of(int ranks) { return ranks == 1 ? sample_kernel<T, 1> : ranks == 2 ? sample_kernel<T, 2> : ranks == 4 ? sample_kernel<T, 4> : sample_kernel<T, 8>; }
 
 template <typename T>
 int launch(int rows, int vocab, int64_t row, const void* logits, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens,
@@ -695,9 +884,9 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
   auto slice_of = [&](int n) { return ((vocab + n - 1) / n + kThreads - 1) / kThreads * kThreads; };
   while (ranks < kMaxCluster && (slice_of(ranks) * sizeof(T) > 64 * 1024 || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
   const int slice = slice_of(ranks);
-  const size_t smem = (size_t)slice * sizeof(T);
+  const size_t smem = (size_t)slice * sizeof(T) + kList * 8;
   const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
-  auto* fn = sample_kernel<T>;
+  auto* fn = kernel_of<T>(ranks);
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * (unsigned)ranks);
