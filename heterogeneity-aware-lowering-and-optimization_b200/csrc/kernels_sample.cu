@@ -11,6 +11,7 @@ namespace b200 {
 namespace {
 namespace cg = cooperative_groups;
 
+// (A slice is at most 64 logits per thread: 2^18 over 8 CTAs of 512 threads.)
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
 constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 128;
 constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
@@ -69,39 +70,43 @@ template <typename T> struct alignas(16) Piece {
   T e[N];
 };
 
+constexpr int kTable = 32, kCopies = 16;
 struct Shared {
-  double table[256];                      // 2^(j / 256)
+  double table[kTable][kCopies];          // 2^(j / 32), a copy for each pair of banks
   // The direct way: a histogram (counts, or masses), then a list of (key, ~index); what every warp of the cluster has summed.
   union { uint32_t hist[kBins]; unsigned long long list[kList]; };
   union {
+    unsigned long long spare[kList];      // while the list is sorted
     unsigned long long weight[kTopK];     // of the list's first, by rank (top-k)
-    uint32_t bucket[kBins];
+    struct {                              // the general way
+      uint32_t lo[2][256], hi[2][256];    // histograms: counts in lo, or masses in both words
+      unsigned long long total[256];
+    };
   };
+  uint32_t bucket[kBins];
   unsigned long long below[kMaxCluster * kWarps], taken[kMaxCluster * kWarps], all[kMaxCluster];
-  unsigned long long warp_sum[kWarps], cta_sum, before, cut_entry;
+  unsigned long long warp_sum[kWarps], cta_sum, before, cut_entry, above, in_bin;
   float warp_top[kWarps], tops[kMaxCluster];
   double shares[kMaxCluster], target;
-  int listed[kMaxCluster], n_list, found, owner, ok, crowded, token;
-  // The general way.
-  uint32_t lo[2][256], hi[2][256];        // histograms: counts in lo, or masses in both words
-  unsigned long long total[256], above, in_bin;
-  uint32_t bin;
-  int cut, pick;
+  uint32_t low_key, high_key, bin, digit_lo[64], digit_hi[64];
+  int listed[kMaxCluster], found, owner, ok, crowded, token, cut, pick;
 };
 
-// exp(d * inverse) for d <= 0, with scale = inverse * 256 / ln 2: a table of 2^(j/256) and the exponential series up to the third power on
-// |r| <= ln 2 / 512 (P. T. P. Tang's table-driven method, 1989); the next term is below 1.4e-13, and in a sum of many weights, of
-// either size, less.  Ten operations in 64 bits, two clocks of a scheduler each, are what a weight costs; a table of 64 takes two more.
-__device__ __forceinline__ double exp_below(double d, double scale, const double* table) {
+// exp(d * inverse) for d <= 0, with scale = inverse * 32 / ln 2: a table of 2^(j/32) and the exponential series up to the fourth power on
+// |r| <= ln 2 / 64 (P. T. P. Tang's table-driven method, 1989); the next term is below 1.3e-12, a fifth of that on average over r, and in sums
+// of many weights, of either size, less.  Eleven operations in 64 bits, two clocks of a scheduler each, are what a weight costs.  (A table of
+// 256 entries and two operations fewer were slower: 32 lanes at random places of it meet in the same banks.)
+__device__ __forceinline__ double exp_below(double d, double scale, const Shared& s) {
   const double z = d * scale;
-  if (!(z > -258000.0)) return 0.0;                            // below exp(-698)
+  if (!(z > -32250.0)) return 0.0;                             // below exp(-698)
   const double shift = 6755399441055744.0;                     // 1.5 * 2^52: adding it rounds to a whole number
   const double m = z + shift, g = z - (m - shift);
   const int n = __double2loint(m);
-  constexpr double c = 0.69314718055994530942 / 256;
-  double p = fma(g, c * c * c / 6, c * c / 2);
+  constexpr double c = 0.69314718055994530942 / 32;
+  double p = fma(g, c * c * c * c / 24, c * c * c / 6);
+  p = fma(p, g, c * c / 2);
   p = fma(p, g, c) * g;
-  const double t = table[n & 255], w = __hiloint2double(__double2hiint(t) + ((n >> 8) << 20), __double2loint(t));
+  const double t = s.table[n & 31][threadIdx.x & 15], w = __hiloint2double(__double2hiint(t) + ((n >> 5) << 20), __double2loint(t));
   return fma(w, p, w);
 }
 // Weights are summed as whole numbers of 2^-44 of the largest: 2^18 of them stay inside 62 bits, and the sums do not depend on
@@ -110,6 +115,8 @@ __device__ __forceinline__ unsigned long long units(double w) {
   const double whole = fma(w, 17592186044416.0, 4503599627370496.0);   // 2^44 w + 2^52, rounded to a whole number
   return (unsigned long long)__double_as_longlong(whole) & 0xfffffffffffffull;
 }
+// The same as a double; sums of up to 256 of them are exact.
+__device__ __forceinline__ double units_exact(double w) { return fma(w, 17592186044416.0, 4503599627370496.0) - 4503599627370496.0; }
 
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
 #pragma unroll
@@ -175,17 +182,16 @@ template <typename T, int RANKS> struct Part {
   Shared& s;
   cg::cluster_group cluster;
   const T* logits;
-  unsigned long long* spare;   // kList entries
   Row r;
   float top;                   // the row's largest logit
-  double scale;                // 256 / (ln 2 * temperature)
+  double scale;                // 32 / (ln 2 * temperature)
   int vocab, slice, base, rank, row;
   int* tokens;
 
   using L = Logits<T>;
   using Key = typename L::Key;
   __device__ __forceinline__ Shared* peer(int k) { return cluster.map_shared_rank(&s, k); }
-  __device__ __forceinline__ double weight(float v) const { return exp_below((double)v - (double)top, scale, s.table); }
+  __device__ __forceinline__ double weight(float v) const { return exp_below((double)v - (double)top, scale, s); }
 
   // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them finds
   // the bin of the last kept token.
@@ -291,25 +297,23 @@ template <typename T, int RANKS> struct Part {
     return s.found;
   }
 
-  // Appends to this CTA's list the logits of a piece that `mask` names; all lanes of the warp take part.
-  __device__ __forceinline__ void append(uint32_t mask, const Piece<T>& x, int at, int lane) {
-    if (!__any_sync(~0u, mask)) return;
-    int n = __popc(mask), upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(~0u, upto, o); if (lane >= o) upto += u; }
-    int start = 0;
-    if (lane == 31) start = atomicAdd(&s.n_list, upto);
-    start = __shfl_sync(~0u, start, 31) + upto - n;
-#pragma unroll
-    for (int j = 0; j < Piece<T>::N; ++j)
-      if (mask >> j & 1) {
-        if (start < kList) s.list[start] = ((unsigned long long)L::key(x.e[j]) << 32) | (uint32_t)~(uint32_t)(base + at + j);
-        ++start;
-      }
+  // Puts on this CTA's list the logits that `mask` names: bit m of thread t is element m % N of its piece m / N, pieces `first` + (m / N) * `step`.
+  // The first kList bits of the row's order need not come first: the list is sorted later.  Returns how many there are.
+  __device__ __forceinline__ int enlist(unsigned long long mask, int first, int step) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int all;
+    int at = block_scan(__popcll(mask), (int*)s.warp_sum, all, lane, warp);
+    while (mask) {
+      const int m = __ffsll((long long)mask) - 1, i = (first + m / Piece<T>::N * step) * Piece<T>::N + m % Piece<T>::N;
+      mask &= mask - 1;
+      if (at < kList) s.list[at] = ((unsigned long long)L::key(logits[i]) << 32) | (uint32_t)~(uint32_t)(base + i);
+      ++at;
+    }
+    return all;
   }
-  // The CTAs' lists, one after the other in the first one's memory.  Returns their length; above kList they are not there.
-  __device__ __forceinline__ int collect() {
-    const int tid = threadIdx.x, n = s.n_list;   // (after a barrier)
+  // The CTAs' lists of n entries, one after the other in the first one's memory.  Returns their length; above kList they are not there.
+  __device__ __forceinline__ int collect(int n) {
+    const int tid = threadIdx.x;
     if (tid < RANKS) peer(tid)->listed[rank] = n;
     cluster.sync();
     int offset = 0, all = 0;
@@ -327,8 +331,9 @@ template <typename T, int RANKS> struct Part {
     cluster.sync();
     return all;
   }
-  // The first CTA's list, largest first: by bins, and inside a bin by counting, or, where a bin is crowded, by exchanges.
-  __device__ __forceinline__ void sort(int n, float per_unit) {
+  // The first CTA's list, largest first: entries go to buckets by `place_of`, which never puts a smaller entry before a larger one; inside a bucket
+  // they are counted, or, where one is crowded, all are sorted by exchanges.
+  template <typename F> __device__ __forceinline__ void sort(int n, F place_of) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < kBins; i += kThreads) s.bucket[i] = 0;
     if (tid == 0) s.crowded = 0;
@@ -340,7 +345,7 @@ template <typename T, int RANKS> struct Part {
       const int i = j * kThreads + tid;
       if (i < n) {
         entry[j] = s.list[i];
-        b[j] = bin_of(place(L::value((Key)(entry[j] >> 32)), per_unit));
+        b[j] = place_of(entry[j]);
         if (atomicAdd(&s.bucket[b[j]], 1u) >= kBucket) s.crowded = 1;
       }
     }
@@ -361,7 +366,7 @@ template <typename T, int RANKS> struct Part {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kList / kThreads; ++j)
-      if (j * kThreads + tid < n) spare[atomicAdd(&s.bucket[b[j]], 1u)] = entry[j];
+      if (j * kThreads + tid < n) s.spare[atomicAdd(&s.bucket[b[j]], 1u)] = entry[j];
     __syncthreads();
     // (each bucket now names its end, which is the next one's beginning)
 #pragma unroll
@@ -369,10 +374,54 @@ template <typename T, int RANKS> struct Part {
       if (j * kThreads + tid < n) {
         const uint32_t from = b[j] ? s.bucket[b[j] - 1] : 0u, to = s.bucket[b[j]];
         uint32_t rank_of = from;
-        for (uint32_t i = from; i < to; ++i) rank_of += spare[i] > entry[j];
+        for (uint32_t i = from; i < to; ++i) rank_of += s.spare[i] > entry[j];
         s.list[rank_of] = entry[j];
       }
     __syncthreads();
+  }
+  __device__ __forceinline__ float value_of(unsigned long long entry) const { return L::value((Key)(entry >> 32)); }
+
+  // The choice from a list of up to 128 entries in any order, four threads for each: three rounds in which every entry looks at all others.
+  __device__ __forceinline__ void choose_from_few(int n) {
+    const int tid = threadIdx.x, i = tid >> 2;
+    const bool live = i < n;
+    const unsigned long long entry = live ? s.list[i] : 0;
+    const double w = live ? weight(value_of(entry)) : 0.0;
+    const unsigned long long unit = units(w);
+    if (live && (tid & 3) == 0) s.weight[i] = unit;
+    if (tid == 0) s.token = INT_MAX;
+    __syncthreads();
+    auto quad = [](unsigned long long v) { v += __shfl_xor_sync(~0u, v, 1); return v + __shfl_xor_sync(~0u, v, 2); };
+    // rank, and the weight of all larger ones; both in one sum: up to 128 of 2^44 units and of 2^56
+    unsigned long long sum = 0;
+    for (int j = tid & 3; j < n; j += 4)
+      if (s.list[j] > entry) sum += s.weight[j] + (1ull << 56);
+    sum = quad(sum);
+    const int place_in = (int)(sum >> 56);
+    const unsigned long long larger = sum & ((1ull << 56) - 1);
+    bool keep = live && place_in < r.top_k;
+    if (r.top_p < 1.f) {
+      __syncthreads();
+      if (live && (tid & 3) == 0 && !keep) s.weight[i] = 0;
+      __syncthreads();
+      unsigned long long total = 0;
+      for (int j = 0; j < n; ++j) total += s.weight[j];
+      keep = keep && (place_in == 0 || (double)larger < (double)r.top_p * (double)total);
+    }
+    keep = keep && w >= (double)r.min_p;
+    __syncthreads();
+    if (live && (tid & 3) == 0) s.weight[i] = keep ? unit : 0;
+    __syncthreads();
+    unsigned long long upto = 0, total = 0;
+    for (int j = tid & 3; j < n; j += 4) {
+      total += s.weight[j];
+      if (~(uint32_t)s.list[j] <= ~(uint32_t)entry) upto += s.weight[j];
+    }
+    upto = quad(upto);
+    total = quad(total);
+    if (keep && (double)upto > (double)r.uniform * (double)total) atomicMin(&s.token, (int)~(uint32_t)entry);
+    __syncthreads();
+    if (tid == 0) tokens[row] = s.token;
   }
 
   // Returns 0 when the token is written, -1 when the row has to go the general way, -2 when more tokens than fit lie in the groups' bin.
@@ -380,22 +429,23 @@ template <typename T, int RANKS> struct Part {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int bin = find_bin<true, GROUPS>(per_unit, (double)r.top_k);
     if (bin < 0) return GROUPS ? -2 : -1;   // (fewer than k of them outside the last bin)
-    if (tid == 0) s.n_list = 0;
-    __syncthreads();
-    for (int i = tid; i < slice / Piece<T>::N; i += kThreads) {   // (whole warps: a slice is a multiple of 32 pieces)
+    unsigned long long named = 0;
+    int shift = 0;
+#pragma unroll 4
+    for (int i = tid; i < slice / Piece<T>::N; i += kThreads, shift += Piece<T>::N) {
       const Piece<T> x = ((const Piece<T>*)logits)[i];
-      uint32_t mask = 0;
       if (bin_of(place(L::largest(*(const uint4*)&x), per_unit)) <= bin) {
+        uint32_t mask = 0;
 #pragma unroll
         for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
+        named |= (unsigned long long)mask << shift;
       }
-      append(mask, x, i * Piece<T>::N, lane);
     }
-    __syncthreads();
-    const int n = collect();
+    const int n = collect(enlist(named, tid, kThreads));
     if (n > kList) return GROUPS ? -2 : -1;
     if (rank) return 0;
-    sort(n, per_unit);
+    if (n <= kFew) { choose_from_few(n); return 0; }
+    sort(n, [&](unsigned long long e) { return bin_of(place(value_of(e), per_unit)); });
     // the first top_k of the sorted list, four entries per thread
     const bool by_mass = r.top_p < 1.f;
     const double least = (double)r.min_p;
@@ -404,7 +454,7 @@ template <typename T, int RANKS> struct Part {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = tid * 4 + j;
-      w[j] = i < r.top_k ? weight(L::value((Key)(s.list[i] >> 32))) : 0.0;
+      w[j] = i < r.top_k ? weight(value_of(s.list[i])) : 0.0;
       sum += unit[j] = i < r.top_k ? units(w[j]) : 0;
     }
     unsigned long long run = block_scan(sum, s.warp_sum, total, lane, warp), kept = 0;
@@ -418,39 +468,26 @@ template <typename T, int RANKS> struct Part {
       if (i < kTopK) s.weight[i] = keep ? unit[j] : 0;
       run += unit[j];
     }
-    if (tid == 0) { s.pick = 0; s.token = INT_MAX; }
+    if (tid == 0) s.pick = 0;
     block_scan(kept, s.warp_sum, total, lane, warp);
     if (n_kept) atomicMax(&s.pick, n_kept);
     __syncthreads();
     n_kept = s.pick;
     const double target = (double)r.uniform * (double)total;
-    if (n_kept <= kFew) {   // four threads for each: the sum over those of lower or the same index
-      const int i = tid >> 2;
-      const uint32_t index = i < n_kept ? ~(uint32_t)s.list[i] : 0u;
-      unsigned long long upto = 0;
-      for (int j = tid & 3; j < n_kept; j += 4)
-        if (~(uint32_t)s.list[j] <= index) upto += s.weight[j];
-      upto += __shfl_xor_sync(~0u, upto, 1);
-      upto += __shfl_xor_sync(~0u, upto, 2);
-      if (i < n_kept && (double)upto > target) atomicMin(&s.token, (int)index);
-      __syncthreads();
-      if (tid == 0) tokens[row] = s.token;
-      return 0;
-    }
     // by index, six bits at a time: the digit at which the running sum passes the target
     uint32_t prefix = 0;
     unsigned long long before = 0;
     for (int shift = 12; shift >= 0; shift -= 6) {
-      if (tid < 64) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+      if (tid < 64) { s.digit_lo[tid] = 0; s.digit_hi[tid] = 0; }
       __syncthreads();
       for (int i = tid; i < n_kept; i += kThreads) {
         const uint32_t index = ~(uint32_t)s.list[i];
         const unsigned long long u = s.weight[i];
-        if (u && index >> (shift + 6) == prefix) add_units(&s.lo[0][(index >> shift) & 63], &s.hi[0][(index >> shift) & 63], u);
+        if (u && index >> (shift + 6) == prefix) add_units(&s.digit_lo[(index >> shift) & 63], &s.digit_hi[(index >> shift) & 63], u);
       }
       __syncthreads();
       if (warp == 0) {
-        const unsigned long long x = ((unsigned long long)s.hi[0][2 * lane] << 32) + s.lo[0][2 * lane], y = ((unsigned long long)s.hi[0][2 * lane + 1] << 32) + s.lo[0][2 * lane + 1];
+        const unsigned long long x = ((unsigned long long)s.digit_hi[2 * lane] << 32) + s.digit_lo[2 * lane], y = ((unsigned long long)s.digit_hi[2 * lane + 1] << 32) + s.digit_lo[2 * lane + 1];
         const unsigned long long upto = before + warp_scan(x + y, lane), from = upto - x - y;
         const uint32_t ballot = __ballot_sync(~0u, (double)upto > target);
         if (lane == __ffs(ballot) - 1) {
@@ -472,51 +509,54 @@ template <typename T, int RANKS> struct Part {
     Shared* first = peer(0);
     const int sub = slice / kWarps, warp_base = warp * sub;   // a warp's stretch
     const double least = (double)r.min_p;
-    if (tid == 0) s.n_list = 0;
-    __syncthreads();
+    unsigned long long named = 0;
     {
       // (where only min-p chooses, no weight past this place passes it, with room for the roundings of 32 bits)
       const float last = by_mass || !(r.min_p > 0.f) ? (float)(kBins - 1) : fminf(-kBinsPerE * logf(r.min_p) + 1.f, (float)(kBins - 1));
       const float floor = top - 70.f * r.temperature;   // no units; NaN and -inf become this
-      unsigned long long all = 0, below = 0, taken = 0;
-      for (int i = warp_base / N + lane; i < (warp_base + sub) / N; i += 32) {
+      const bool every = !(r.min_p > 0.f);              // min-p keeps all
+      // a thread's sums of units are exact as doubles (64 logits at most); integer additions of two words would cost as much as the weights
+      double all = 0, below = 0, taken = 0;
+      int shift = 0;
+      for (int i = warp_base / N + lane; i < (warp_base + sub) / N; i += 32, shift += N) {
         const Piece<T> x = ((const Piece<T>*)logits)[i];
-        uint32_t mask = 0;
         if (place(L::largest(*(const uint4*)&x), per_unit) < last) {
           double w[N];
-          float at[N];
+          int b[N];
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             const float v = fmaxf(L::widen(x.e[j]), floor);
-            at[j] = place(v, per_unit);
+            b[j] = (int)__float_as_uint(place(v, per_unit) + 8388608.f) - 0x4b000000;
             w[j] = weight(v);
           }
+          uint32_t mask = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const unsigned long long u = units(w[j]);
-            const int b = bin_of(at[j]);
+            const double u = units_exact(w[j]);
             all += u;
-            if (b < bin) {
+            if (b[j] < bin) {
               below += u;
-              if (w[j] >= least) taken += u;
+              if (!every && w[j] >= least) taken += u;
             }
-            mask |= (b == bin ? 1u : 0u) << j;
+            mask |= (b[j] == bin ? 1u : 0u) << j;
           }
+          named |= (unsigned long long)mask << shift;
         }
-        if (by_mass && mask) append_some(mask, x, i * N);
       }
-      all = warp_sum(all); below = warp_sum(below); taken = warp_sum(taken);
-      if (lane == 0) { s.warp_sum[warp] = all; first->below[rank * kWarps + warp] = below; first->taken[rank * kWarps + warp] = taken; }
+      if (every) taken = below;
+      const unsigned long long sum_all = warp_sum((unsigned long long)all), sum_below = warp_sum((unsigned long long)below), sum_taken = warp_sum((unsigned long long)taken);
+      if (lane == 0) { s.bucket[2 * warp] = (uint32_t)sum_all; s.bucket[2 * warp + 1] = (uint32_t)(sum_all >> 32); first->below[rank * kWarps + warp] = sum_below; first->taken[rank * kWarps + warp] = sum_taken; }
     }
+    int n = 0;
+    if (by_mass) n = enlist(named, warp_base / N + lane, 32);
     __syncthreads();
     if (tid == 0) {
       unsigned long long v = 0;
-      for (int k = 0; k < kWarps; ++k) v += s.warp_sum[k];
+      for (int k = 0; k < kWarps; ++k) v += ((unsigned long long)s.bucket[2 * k + 1] << 32) + s.bucket[2 * k];
       first->all[rank] = v;
     }
-    int n = 0;
     if (by_mass) {
-      n = collect();
+      n = collect(n);
       if (n > kList) return false;
     } else {
       cluster.sync();
@@ -530,13 +570,22 @@ template <typename T, int RANKS> struct Part {
       if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; }
       if (by_mass) {
         block_scan(tid < kAll ? s.below[tid] : 0ull, s.warp_sum, sum_below, lane, warp);
-        sort(n, per_unit);
+        // one bin's tokens: buckets by key and, between equal keys, by index
+        if (tid == 0) { s.low_key = ~0u; s.high_key = 0; }
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) { const uint32_t k = (uint32_t)(s.list[i] >> 32); atomicMin(&s.low_key, k); atomicMax(&s.high_key, k); }
+        __syncthreads();
+        const uint32_t high = s.high_key;
+        const double spread = (double)kBins / ((double)(high - s.low_key) + 1.0);
+        sort(n, [&](unsigned long long e) {
+          return min(kBins - 1, (int)(((double)(high - (uint32_t)(e >> 32)) + (double)(~(uint32_t)e) * (1.0 / kMaxVocab)) * spread));
+        });
         unsigned long long unit[4], sum = 0;
         double w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = tid * 4 + j;
-          w[j] = i < n ? weight(L::value((Key)(s.list[i] >> 32))) : 0.0;
+          w[j] = i < n ? weight(value_of(s.list[i])) : 0.0;
           sum += unit[j] = i < n ? units(w[j]) : 0;
         }
         unsigned long long run = sum_below + block_scan(sum, s.warp_sum, total, lane, warp);
@@ -598,21 +647,13 @@ template <typename T, int RANKS> struct Part {
     }
     return true;
   }
-  // The same one logit at a time, for lanes that may be fewer than a warp.
-  __device__ __forceinline__ void append_some(uint32_t mask, const Piece<T>& x, int at) {
-#pragma unroll
-    for (int j = 0; j < Piece<T>::N; ++j)
-      if (mask >> j & 1) {
-        const int i = atomicAdd(&s.n_list, 1);
-        if (i < kList) s.list[i] = ((unsigned long long)L::key(x.e[j]) << 32) | (uint32_t)~(uint32_t)(base + at + j);
-      }
-  }
-
   // Any row: one search for top-k and one for top-p, each over 8 bits of the keys at a time from the top.
   __device__ __noinline__ void general() {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = RANKS;
     const Key top_key = key_of_top();
-    auto weight_of = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)L::value(k) - (double)top, scale, s.table); };
+    if (tid < 256) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+    __syncthreads();
+    auto weight_of = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)L::value(k) - (double)top, scale, s); };
     // Kept so far: key > t, or key == t and index <= c.
     Key t = 1;
     int c = INT_MAX, buffer = 0;
@@ -825,7 +866,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared s;
   constexpr int N = Piece<T>::N;
-  T* mine = (T*)(dynamic + kList * 8);
+  T* mine = (T*)dynamic;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), row = blockIdx.x / RANKS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
   const T* src = logits + (int64_t)row * row_stride + base;
@@ -843,7 +884,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
     top = fmaxf(top, L::widen(v));
   }
   const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
-  if (tid < 256) { s.table[tid] = exp2((double)tid / 256.0); s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
+  s.table[tid / kCopies][tid % kCopies] = exp2((double)(tid / kCopies) / kTable);   // (as many entries as threads)
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
   if (lane == 0) s.warp_top[warp] = top;
@@ -871,7 +912,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
     if (rank == 0 && tid == 0) tokens[row] = top > -INFINITY ? s.token : -1;
     return;
   }
-  Part<T, RANKS> part{s, cluster, mine, (unsigned long long*)dynamic, r, top, 369.32993046757462708 /* 256 / ln 2 */ / (double)r.temperature, vocab, slice, base, rank, row, tokens};
+  Part<T, RANKS> part{s, cluster, mine, r, top, 46.166241308446828384 /* 32 / ln 2 */ / (double)r.temperature, vocab, slice, base, rank, row, tokens};
   if (!part.direct()) part.general();
 }
 
@@ -884,7 +925,7 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
   auto slice_of = [&](int n) { return ((vocab + n - 1) / n + kThreads - 1) / kThreads * kThreads; };
   while (ranks < kMaxCluster && (slice_of(ranks) * sizeof(T) > 64 * 1024 || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
   const int slice = slice_of(ranks);
-  const size_t smem = (size_t)slice * sizeof(T) + kList * 8;
+  const size_t smem = (size_t)slice * sizeof(T);
   const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
   auto* fn = kernel_of<T>(ranks);
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
