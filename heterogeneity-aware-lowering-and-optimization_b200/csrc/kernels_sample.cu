@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <climits>
+#include <cmath>
 
 #include "kernels.h"
 
@@ -11,9 +12,9 @@ namespace b200 {
 namespace {
 namespace cg = cooperative_groups;
 
-// (A slice is at most 64 logits per thread: 2^18 over 8 CTAs of 512 threads.)
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
-constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 128;
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 256;
+constexpr int kSlice = 64 * kThreads;   // logits of a CTA at most: a thread names its own by the bits of one word
 constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
 
 // Logits as keys that compare like them: whole numbers, larger for larger logits, 0 for those that are never chosen (NaN, -inf).
@@ -71,7 +72,8 @@ template <typename T> struct alignas(16) Piece {
 };
 
 constexpr int kTable = 32, kCopies = 16;
-struct Shared {
+struct Powers { double of[kTable]; };   // 2^(j / 32)
+struct alignas(16) Shared {
   double table[kTable][kCopies];          // 2^(j / 32), a copy for each pair of banks
   // The direct way: a histogram (counts, or masses), then a list of (key, ~index); what every warp of the cluster has summed.
   union { uint32_t hist[kBins]; unsigned long long list[kList]; };
@@ -87,7 +89,8 @@ struct Shared {
   unsigned long long below[kMaxCluster * kWarps], taken[kMaxCluster * kWarps], all[kMaxCluster];
   unsigned long long warp_sum[kWarps], cta_sum, before, cut_entry, above, in_bin;
   float warp_top[kWarps], tops[kMaxCluster];
-  double shares[kMaxCluster], target;
+  unsigned long long shares[kMaxCluster];
+  double target;
   uint32_t low_key, high_key, bin, digit_lo[64], digit_hi[64];
   int listed[kMaxCluster], found, owner, ok, crowded, token, cut, pick;
 };
@@ -143,25 +146,25 @@ struct Row {
   int top_k;
 };
 
-// Sum over the block's threads before this one, and over all of them.
+// Sum over the block's threads before this one, and over all of them (whole numbers; the block has as many warps as a warp has lanes).
 template <typename V> __device__ __forceinline__ V block_scan(V mine, V* warps, V& total, int lane, int warp) {
-  V upto = mine;
+  static_assert(kWarps == 32, "a lane per warp");
+  auto scan = [lane](V v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const V u = __shfl_up_sync(~0u, upto, o);
-    if (lane >= o) upto += u;
-  }
-  const V previous = __shfl_up_sync(~0u, upto, 1);
+    for (int o = 1; o < 32; o <<= 1) {
+      const V u = __shfl_up_sync(~0u, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  const V upto = scan(mine);
   __syncthreads();
   if (lane == 31) warps[warp] = upto;
   __syncthreads();
-  V before = 0;
-  total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = total;
-    total += warps[w];
-  }
-  return lane ? before + previous : before;   // (the same sums, in the same order, as the thread in front of this one ends with)
+  const V all = scan(warps[lane]);
+  total = __shfl_sync(~0u, all, 31);
+  const V before = __shfl_sync(~0u, all, (warp + 31) & 31);
+  return (warp ? before : 0) + upto - mine;
 }
 // Largest first; n2 a power of two, entries from n on are zeros.
 __device__ __forceinline__ void sort_list(unsigned long long* list, int n2, int tid) {
@@ -179,23 +182,27 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, int n2, int 
 
 // A CTA's part of a row: `slice` logits in shared memory, of which those past the row's end never count.
 template <typename T, int RANKS> struct Part {
+  static constexpr int kGroups = 8, kPer = kSlice / kThreads / Piece<T>::N / kGroups;
   Shared& s;
   cg::cluster_group cluster;
-  const T* logits;
+  const T* logits;             // in shared memory, or, where they do not fit, the caller's
   Row r;
   float top;                   // the row's largest logit
+  float group[kGroups];        // the largest of kPer pieces: of this thread's pieces tid + (g * kPer + i) * kThreads
   double scale;                // 32 / (ln 2 * temperature)
-  int vocab, slice, base, rank, row;
+  int vocab, slice, limit, base, rank, row;   // logits[i] may be read below `limit`, whole pieces; the rest of a slice counts as dead
   int* tokens;
 
   using L = Logits<T>;
   using Key = typename L::Key;
-  __device__ __forceinline__ Shared* peer(int k) { return cluster.map_shared_rank(&s, k); }
+  __device__ __forceinline__ Shared* peer(int k) { return RANKS == 1 ? &s : cluster.map_shared_rank(&s, k); }
+  __device__ __forceinline__ void sync_row() { if (RANKS == 1) __syncthreads(); else cluster.sync(); }
+  __device__ __forceinline__ T logit(int i) const { return i < limit ? logits[i] : L::dead(); }
   __device__ __forceinline__ double weight(float v) const { return exp_below((double)v - (double)top, scale, s); }
 
   // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them finds
   // the bin of the last kept token.
-  //   top-k up to 1024: a histogram of the largest logit of each 16 bytes (the k-th largest of those has at least k tokens above it, and rarely
+  //   top-k up to 1024: a histogram of the largest logits of small groups, kept in registers (the k-th largest of those has at least k tokens above it, and rarely
   //   many more; of every logit where that did not hold, or the row is short).  All tokens down to that bin go to a list of the first CTA,
   //   which sorts it and does the rest alone.
   //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 2^-16), for top-p; then every CTA sums exact weights,
@@ -211,7 +218,7 @@ template <typename T, int RANKS> struct Part {
     const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
     if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(top) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kTopK)) return false;
     if (by_count) {
-      if (vocab / Piece<T>::N >= 2 * r.top_k) {
+      if (vocab / (kPer * Piece<T>::N) >= 2 * r.top_k) {
         const int n = top_k<true>(per_unit);
         if (n >= 0) return true;
         if (n == -1) return false;
@@ -236,12 +243,16 @@ template <typename T, int RANKS> struct Part {
     for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
     if (tid == 0) s.found = -1;
     __syncthreads();
-    for (int i = tid; i < slice / Piece<T>::N; i += kThreads) {
-      const Piece<T> x = ((const Piece<T>*)logits)[i];
-      if constexpr (GROUPS) {
-        const int b = bin_of(place(L::largest(*(const uint4*)&x), per_unit));
+    if constexpr (GROUPS) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int b = bin_of(place(group[g], per_unit));
         if (b < kBins - 1) atomicAdd(&s.hist[b], 1u);
-      } else {
+      }
+    } else {
+#pragma unroll 2
+      for (int i = tid; i < limit / Piece<T>::N; i += kThreads) {
+        const Piece<T> x = ((const Piece<T>*)logits)[i];
 #pragma unroll
         for (int j = 0; j < Piece<T>::N; ++j) {
           const float at = place(L::widen(x.e[j]), per_unit);
@@ -255,11 +266,11 @@ template <typename T, int RANKS> struct Part {
         }
       }
     }
-    cluster.sync();
+    sync_row();
     // each CTA adds up its share of the bins
     constexpr int kShare = kBins / RANKS, kEach = kShare > kThreads ? kShare / kThreads : 1;
     const int b0 = rank * kShare + tid * kEach;
-    double v[kEach], sum = 0;
+    unsigned long long v[kEach], sum = 0;   // counts, or masses in units of 2^-40 (a bin holds at most 2^18 of them)
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       v[j] = 0;
@@ -267,33 +278,31 @@ template <typename T, int RANKS> struct Part {
         uint32_t n[RANKS];
 #pragma unroll
         for (int k = 0; k < RANKS; ++k) n[k] = peer(k)->hist[b0 + j];
-        unsigned long long m = 0;
 #pragma unroll
-        for (int k = 0; k < RANKS; ++k) m += n[k];
-        v[j] = (double)m;
-        if (!COUNT) v[j] *= (double)exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE));
+        for (int k = 0; k < RANKS; ++k) v[j] += n[k];
+        if (!COUNT) v[j] = (unsigned long long)((float)v[j] * exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE) + 24.f));
       }
       sum += v[j];
     }
-    double total;
-    const double before = block_scan(sum, (double*)s.warp_sum, total, lane, warp);
+    unsigned long long total;
+    const unsigned long long before = block_scan(sum, s.warp_sum, total, lane, warp);
     if (tid < RANKS) peer(tid)->shares[rank] = total;
-    cluster.sync();
-    double offset = 0, everything = 0;
+    sync_row();
+    unsigned long long offset = 0, everything = 0;
 #pragma unroll
     for (int k = 0; k < RANKS; ++k) {
       if (k == rank) offset = everything;
       everything += s.shares[k];
     }
-    const double mark = COUNT ? need : need * everything;
-    double run = offset + before;
+    const double mark = COUNT ? need : need * (double)everything;
+    unsigned long long run = offset + before;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      if (run < mark && mark <= run + v[j])
+      if ((double)run < mark && mark <= (double)(run + v[j]))
         for (int k = 0; k < RANKS; ++k) peer(k)->found = b0 + j;
       run += v[j];
     }
-    cluster.sync();
+    sync_row();
     return s.found;
   }
 
@@ -315,7 +324,7 @@ template <typename T, int RANKS> struct Part {
   __device__ __forceinline__ int collect(int n) {
     const int tid = threadIdx.x;
     if (tid < RANKS) peer(tid)->listed[rank] = n;
-    cluster.sync();
+    sync_row();
     int offset = 0, all = 0;
 #pragma unroll
     for (int k = 0; k < RANKS; ++k) {
@@ -328,7 +337,7 @@ template <typename T, int RANKS> struct Part {
         for (int i = tid; i < n; i += kThreads) first->list[offset + i] = s.list[i];
       }
     }
-    cluster.sync();
+    sync_row();
     return all;
   }
   // The first CTA's list, largest first: entries go to buckets by `place_of`, which never puts a smaller entry before a larger one; inside a bucket
@@ -430,11 +439,26 @@ template <typename T, int RANKS> struct Part {
     const int bin = find_bin<true, GROUPS>(per_unit, (double)r.top_k);
     if (bin < 0) return GROUPS ? -2 : -1;   // (fewer than k of them outside the last bin)
     unsigned long long named = 0;
-    int shift = 0;
-#pragma unroll 4
-    for (int i = tid; i < slice / Piece<T>::N; i += kThreads, shift += Piece<T>::N) {
-      const Piece<T> x = ((const Piece<T>*)logits)[i];
-      if (bin_of(place(L::largest(*(const uint4*)&x), per_unit)) <= bin) {
+    if constexpr (GROUPS) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        if (bin_of(place(group[g], per_unit)) <= bin) {
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) {
+            const int i = tid + (g * kPer + k) * kThreads;
+            if (i < limit / Piece<T>::N) {
+              const Piece<T> x = ((const Piece<T>*)logits)[i];
+              uint32_t mask = 0;
+#pragma unroll
+              for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
+              named |= (unsigned long long)mask << ((g * kPer + k) * Piece<T>::N);
+            }
+          }
+        }
+    } else {
+      int shift = 0;
+      for (int i = tid; i < limit / Piece<T>::N; i += kThreads, shift += Piece<T>::N) {
+        const Piece<T> x = ((const Piece<T>*)logits)[i];
         uint32_t mask = 0;
 #pragma unroll
         for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
@@ -446,30 +470,21 @@ template <typename T, int RANKS> struct Part {
     if (rank) return 0;
     if (n <= kFew) { choose_from_few(n); return 0; }
     sort(n, [&](unsigned long long e) { return bin_of(place(value_of(e), per_unit)); });
-    // the first top_k of the sorted list, four entries per thread
+    // the first top_k of the sorted list, an entry per thread
     const bool by_mass = r.top_p < 1.f;
     const double least = (double)r.min_p;
-    unsigned long long unit[4], sum = 0, total;
-    double w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * 4 + j;
-      w[j] = i < r.top_k ? weight(value_of(s.list[i])) : 0.0;
-      sum += unit[j] = i < r.top_k ? units(w[j]) : 0;
-    }
-    unsigned long long run = block_scan(sum, s.warp_sum, total, lane, warp), kept = 0;
+    static_assert(kTopK <= kThreads, "an entry per thread");
+    const bool inside = tid < r.top_k;
+    const double w = inside ? weight(value_of(s.list[tid])) : 0.0;
+    const unsigned long long unit = inside ? units(w) : 0;
+    unsigned long long total;
+    const unsigned long long run = block_scan(unit, s.warp_sum, total, lane, warp);
     const double mark = by_mass ? (double)r.top_p * (double)total : 0.0;
-    int n_kept = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = tid * 4 + j;
-      const bool keep = i < r.top_k && (i == 0 || ((!by_mass || (double)run < mark) && w[j] >= least));
-      if (keep) { kept += unit[j]; n_kept = i + 1; }
-      if (i < kTopK) s.weight[i] = keep ? unit[j] : 0;
-      run += unit[j];
-    }
+    const bool keep = inside && (tid == 0 || ((!by_mass || (double)run < mark) && w >= least));
+    int n_kept = keep ? tid + 1 : 0;
+    if (tid < kTopK) s.weight[tid] = keep ? unit : 0;
     if (tid == 0) s.pick = 0;
-    block_scan(kept, s.warp_sum, total, lane, warp);
+    block_scan(keep ? unit : 0ull, s.warp_sum, total, lane, warp);
     if (n_kept) atomicMax(&s.pick, n_kept);
     __syncthreads();
     n_kept = s.pick;
@@ -518,7 +533,7 @@ template <typename T, int RANKS> struct Part {
       // a thread's sums of units are exact as doubles (64 logits at most); integer additions of two words would cost as much as the weights
       double all = 0, below = 0, taken = 0;
       int shift = 0;
-      for (int i = warp_base / N + lane; i < (warp_base + sub) / N; i += 32, shift += N) {
+      for (int i = warp_base / N + lane; i < min(warp_base + sub, limit) / N; i += 32, shift += N) {
         const Piece<T> x = ((const Piece<T>*)logits)[i];
         if (place(L::largest(*(const uint4*)&x), per_unit) < last) {
           double w[N];
@@ -559,7 +574,7 @@ template <typename T, int RANKS> struct Part {
       n = collect(n);
       if (n > kList) return false;
     } else {
-      cluster.sync();
+      sync_row();
     }
     if (rank == 0) {
       // the sums of all warps, in index order
@@ -580,11 +595,12 @@ template <typename T, int RANKS> struct Part {
         sort(n, [&](unsigned long long e) {
           return min(kBins - 1, (int)(((double)(high - (uint32_t)(e >> 32)) + (double)(~(uint32_t)e) * (1.0 / kMaxVocab)) * spread));
         });
-        unsigned long long unit[4], sum = 0;
-        double w[4];
+        constexpr int kMine = kList / kThreads;
+        unsigned long long unit[kMine], sum = 0;
+        double w[kMine];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = tid * 4 + j;
+        for (int j = 0; j < kMine; ++j) {
+          const int i = tid * kMine + j;
           w[j] = i < n ? weight(value_of(s.list[i])) : 0.0;
           sum += unit[j] = i < n ? units(w[j]) : 0;
         }
@@ -592,8 +608,8 @@ template <typename T, int RANKS> struct Part {
         const double mark = (double)r.top_p * (double)sum_all;
         // (kept entries are the first ones; the last of them ends the kept tokens)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = tid * 4 + j;
+        for (int j = 0; j < kMine; ++j) {
+          const int i = tid * kMine + j;
           const bool keep = i < n && ((double)run < mark || (i == 0 && sum_below == 0));
           if (keep) {
             const unsigned long long entry = s.list[i];
@@ -613,7 +629,7 @@ template <typename T, int RANKS> struct Part {
         for (int k = 0; k < RANKS; ++k) { Shared* o = peer(k); o->owner = tid; o->before = before; o->target = target; }
       if (tid && tid < RANKS) { Shared* o = peer(tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
     }
-    cluster.sync();
+    sync_row();
     if (!s.ok) return false;
     if (s.owner / kWarps != rank) return true;
     // the stretch of one warp, now by all warps of its CTA
@@ -621,7 +637,7 @@ template <typename T, int RANKS> struct Part {
     const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
     auto chosen = [&](int i) -> unsigned long long {
       if (i >= sub) return 0;
-      const T x = logits[stretch + i];
+      const T x = logit(stretch + i);
       const Key k = L::key(x);
       if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
       const double w = weight(L::widen(x));
@@ -665,7 +681,7 @@ template <typename T, int RANKS> struct Part {
       unsigned long long above = 0, in_bin = 0;
       for (int shift = L::kBits - 8; shift >= 0; shift -= 8) {
         for (int i = tid; i < slice; i += kThreads) {
-          const Key k = L::key(logits[i]);
+          const Key k = L::key(logit(i));
           if (k && (shift + 8 == L::kBits || (uint32_t)k >> (shift + 8) == (uint32_t)prefix) && kept(k, base + i)) {
             const int b = ((uint32_t)k >> shift) & 255;
             if (mass) {
@@ -715,7 +731,7 @@ template <typename T, int RANKS> struct Part {
     const int sub = slice / kWarps, warp_base = warp * sub;
     auto nth = [&](Key key, int n) -> int {
       int mine = 0;
-      for (int i = lane; i < sub; i += 32) mine += L::key(logits[warp_base + i]) == key && kept(key, base + warp_base + i);
+      for (int i = lane; i < sub; i += 32) mine += L::key(logit(warp_base + i)) == key && kept(key, base + warp_base + i);
       const unsigned long long count = warp_sum((unsigned long long)mine);
       __syncthreads();
       if (lane == 0) s.warp_sum[warp] = count;
@@ -732,7 +748,7 @@ template <typename T, int RANKS> struct Part {
       for (int w = 0; w < warp; ++w) before += (long long)s.warp_sum[w];
       if (before < n && before + (long long)count >= n)
         for (int i = 0; i < sub; i += 32) {
-          const bool hit = L::key(logits[warp_base + i + lane]) == key && kept(key, base + warp_base + i + lane);
+          const bool hit = L::key(logit(warp_base + i + lane)) == key && kept(key, base + warp_base + i + lane);
           const uint32_t ballot = __ballot_sync(~0u, hit);
           const int upto = (int)before + __popc(ballot & (0xffffffffu >> (31 - lane)));
           if (hit && upto == n) s.cut = base + warp_base + i + lane;
@@ -754,7 +770,7 @@ template <typename T, int RANKS> struct Part {
       unsigned long long live = 0;
       {
         int mine = 0;
-        for (int i = tid; i < slice; i += kThreads) mine += L::key(logits[i]) != 0;
+        for (int i = tid; i < slice; i += kThreads) mine += L::key(logit(i)) != 0;
         const unsigned long long n = warp_sum((unsigned long long)mine);
         if (lane == 0) s.warp_sum[warp] = n;
         __syncthreads();
@@ -799,7 +815,7 @@ template <typename T, int RANKS> struct Part {
     // ---- 3. the choice ----
     const double least = (double)r.min_p;
     auto chosen_weight = [&](int i, bool& is_kept) -> unsigned long long {
-      const Key k = L::key(logits[i]);
+      const Key k = L::key(logit(i));
       is_kept = false;
       if (!k || !kept(k, base + i)) return 0;
       const double w = weight_of(k);
@@ -858,33 +874,50 @@ template <typename T, int RANKS> struct Part {
   __device__ __forceinline__ T narrow() const { return (T)top; }
 };
 
-// One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps in shared memory.
+// One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps in shared memory; where they do not fit
+// (`keep` is 0) the passes after the first read them from the caller's memory again, mostly from L2.  CTAs are few and large: what a row costs beside
+// its loads and weights is a chain of barriers, and a cluster's barrier costs several times a block's.
 template <typename T, int RANKS>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, const float* temperature,
-                                                          const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
+__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
+                                                          const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
   using L = Logits<T>;
+  using P = Part<T, RANKS>;
   extern __shared__ __align__(16) uint8_t dynamic[];
-  __shared__ Shared s;
+  Shared& s = *(Shared*)dynamic;
   constexpr int N = Piece<T>::N;
-  T* mine = (T*)dynamic;
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), row = blockIdx.x / RANKS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
+  auto peer = [&](int k) { return RANKS == 1 ? &s : cluster.map_shared_rank(&s, k); };
+  const int rank = RANKS == 1 ? 0 : (int)cluster.block_rank(), row = blockIdx.x / RANKS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
   const T* src = logits + (int64_t)row * row_stride + base;
-  const int here = max(0, min(slice, vocab - base)), whole = vec ? here / N * N : 0;
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int i = tid * N; i < whole; i += kThreads * N) {
-    const uint4 u = *(const uint4*)(src + i);
-    *(uint4*)(mine + i) = u;
-    top = fmaxf(top, L::largest(u));
+  T* mine = keep ? (T*)(dynamic + sizeof(Shared)) : (T*)src;
+  const int here = max(0, min(slice, vocab - base));
+  float group[P::kGroups], top = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < P::kGroups; ++g) {
+    group[g] = -INFINITY;
+    uint4 u[P::kPer];
+#pragma unroll
+    for (int k = 0; k < P::kPer; ++k) {
+      const int i = (tid + (g * P::kPer + k) * kThreads) * N;
+      if (vec && i + N <= here) {
+        u[k] = *(const uint4*)(src + i);
+      } else {
+        Piece<T> x;
+#pragma unroll
+        for (int j = 0; j < N; ++j) x.e[j] = i + j < here ? src[i + j] : L::dead();
+        u[k] = *(const uint4*)&x;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < P::kPer; ++k) {
+      const int i = (tid + (g * P::kPer + k) * kThreads) * N;
+      if (keep && i < slice) *(uint4*)(mine + i) = u[k];
+      group[g] = fmaxf(group[g], L::largest(u[k]));
+    }
+    top = fmaxf(top, group[g]);
   }
-  for (int i = whole + tid; i < slice; i += kThreads) {
-    const T v = i < here ? src[i] : L::dead();
-    mine[i] = v;
-    top = fmaxf(top, L::widen(v));
-  }
+  if (tid < kTable * kCopies) s.table[tid / kCopies][tid % kCopies] = powers.of[tid / kCopies];
   const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
-  s.table[tid / kCopies][tid % kCopies] = exp2((double)(tid / kCopies) / kTable);   // (as many entries as threads)
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
   if (lane == 0) s.warp_top[warp] = top;
@@ -893,9 +926,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   if (tid < RANKS) {
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) top = fmaxf(top, s.warp_top[k]);
-    cluster.map_shared_rank(&s, tid)->tops[rank] = top;
+    peer(tid)->tops[rank] = top;
   }
-  cluster.sync();
+  if (RANKS == 1) __syncthreads(); else cluster.sync();
 #pragma unroll
   for (int k = 0; k < RANKS; ++k) top = fmaxf(top, s.tops[k]);
   top += 0.f;   // (of two zeros the positive one)
@@ -903,16 +936,31 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
     // nothing to choose from, or the lowest index of the largest logit
     if (top > -INFINITY) {
       int at = INT_MAX;
-      for (int i = tid; i < slice; i += kThreads)
-        if (L::widen(mine[i]) == top) { at = base + i; break; }
+#pragma unroll
+      for (int g = 0; g < P::kGroups; ++g)
+        if (group[g] == top && at == INT_MAX)
+          for (int i = 0; i < P::kPer * N; ++i) {
+            const int e = (tid + (g * P::kPer + i / N) * kThreads) * N + i % N;
+            if (e < here && L::widen(mine[e]) == top) { at = base + e; break; }
+          }
       at = __reduce_min_sync(~0u, at);
-      if (lane == 0 && at < INT_MAX) atomicMin(&cluster.map_shared_rank(&s, 0)->token, at);
-      cluster.sync();
+      if (lane == 0 && at < INT_MAX) atomicMin(&peer(0)->token, at);
+      if (RANKS == 1) __syncthreads(); else cluster.sync();
     }
     if (rank == 0 && tid == 0) tokens[row] = top > -INFINITY ? s.token : -1;
     return;
   }
-  Part<T, RANKS> part{s, cluster, mine, r, top, 46.166241308446828384 /* 32 / ln 2 */ / (double)r.temperature, vocab, slice, base, rank, row, tokens};
+  P part{s, cluster, mine, r, top, {}, 0.0, vocab, slice, keep ? slice : here, base, rank, row, tokens};
+#pragma unroll
+  for (int g = 0; g < P::kGroups; ++g) part.group[g] = group[g];
+  {
+    // 1 / temperature: the reciprocal in 32 bits and two steps of Newton's, each of which doubles its bits (a division takes several times as long)
+    const double t = (double)r.temperature;
+    double q = (double)__frcp_rn(r.temperature);
+    q = fma(fma(-t, q, 1.0), q, q);
+    q = fma(fma(-t, q, 1.0), q, q);
+    part.scale = 46.166241308446828384 * (r.temperature > 1e-4f && r.temperature < 1e4f ? q : 1.0 / t);   // 32 / ln 2
+  }
   if (!part.direct()) part.general();
 }
 
@@ -921,12 +969,18 @@ template <typename T> auto kernel_of(int ranks) { return ranks == 1 ? sample_ker
 template <typename T>
 int launch(int rows, int vocab, int64_t row, const void* logits, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens,
            cudaStream_t stream) {
+  // A slice goes to shared memory where it fits; it has to where a row is no number of aligned 16 bytes, because only the first pass reads
+  // single logits.
+  constexpr int kKeep = 160 * 1024;
+  const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
+  const bool must = !vec || vocab % (16 / (int)sizeof(T));
   int ranks = 1;
   auto slice_of = [&](int n) { return ((vocab + n - 1) / n + kThreads - 1) / kThreads * kThreads; };
-  while (ranks < kMaxCluster && (slice_of(ranks) * sizeof(T) > 64 * 1024 || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
+  while (ranks < kMaxCluster && (slice_of(ranks) > kSlice || (must && slice_of(ranks) * sizeof(T) > kKeep))) ranks *= 2;
   const int slice = slice_of(ranks);
-  const size_t smem = (size_t)slice * sizeof(T);
-  const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
+  const int keep = slice * sizeof(T) <= kKeep;
+  const size_t smem = sizeof(Shared) + (keep ? (size_t)slice * sizeof(T) : 0);
+  static const Powers powers = [] { Powers p; for (int j = 0; j < kTable; ++j) p.of[j] = std::exp2((double)j / kTable); return p; }();
   auto* fn = kernel_of<T>(ranks);
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
   cudaLaunchConfig_t cfg = {};
@@ -940,7 +994,7 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, (const T*)logits, row, vocab, slice, vec, temperature, top_k, top_p, min_p, uniform, tokens);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, (const T*)logits, row, vocab, slice, vec, keep, powers, temperature, top_k, top_p, min_p, uniform, tokens);
   if (e != cudaSuccess) { cudaGetLastError(); return -2; }
   return 0;
 }
