@@ -35,8 +35,10 @@ bool aligned16(std::initializer_list<const void*> ps) {
 
 // Turns per position in units of 2^-64, modulo one turn; frequencies of either sign.
 uint64_t turn_units(double radians) {
-  const long double two_pi = 6.283185307179586476925286766559005768L;
-  long double t = (long double)radians / two_pi;
+  const long double units = 18446744073709551616.0L / 6.283185307179586476925286766559005768L;
+  // up to half a turn, as nearly every frequency: one product
+  if (radians >= 0 && radians < 3.14) return (uint64_t)(int64_t)((long double)radians * units + 0.5L);
+  long double t = (long double)radians / 6.283185307179586476925286766559005768L;
   t -= floorl(t);
   const long double u = t * 18446744073709551616.0L;
   return u >= 18446744073709551615.0L ? 0 : (uint64_t)(u + 0.5L);

@@ -26,7 +26,8 @@ def freqs(pairs, base=10000.0):
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("batch,tokens,heads,channels,pairs,axes", [(1, 1, 1, 2, 1, 1), (2, 5, 3, 64, 32, 2), (1, 37, 12, 128, 64, 3), (3, 17, 2, 80, 24, 1), (1, 4, 1, 7, 3, 4),
-                                                                    (1, 300, 4, 256, 128, 3), (2, 3, 5, 16, 0, 1), (1, 1000, 1, 32, 16, 1)])
+                                                                    (1, 300, 4, 256, 128, 3), (2, 3, 5, 16, 0, 1), (1, 1000, 1, 32, 16, 1),
+                                                                    (1, 3, 2, 1023, 100, 1), (1, 2500, 7, 64, 32, 2)])
 def test_rotary(odla, gpu_lib, dtype, interleaved, batch, tokens, heads, channels, pairs, axes):
     g = gen(dtype, tokens, channels)
     x = randn(g, (batch, tokens, heads, channels), dtype)
