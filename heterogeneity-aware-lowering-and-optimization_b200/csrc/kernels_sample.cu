@@ -15,6 +15,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024, kWarps = kThreads / 32, kMaxCluster = 8;
 constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 256;
 constexpr int kSlice = 64 * kThreads;   // logits of a CTA at most: a thread names its own by the bits of one word
+constexpr float kNoUnits = 1000.f;   // weights from here on, below 2^-45, are no units
 constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
 
 // Logits as keys that compare like them: whole numbers, larger for larger logits, 0 for those that are never chosen (NaN, -inf).
@@ -99,9 +100,9 @@ struct alignas(16) Shared {
 // |r| <= ln 2 / 64 (P. T. P. Tang's table-driven method, 1989); the next term is below 1.3e-12, a fifth of that on average over r, and in sums
 // of many weights, of either size, less.  Eleven operations in 64 bits, two clocks of a scheduler each, are what a weight costs.  (A table of
 // 256 entries and two operations fewer were slower: 32 lanes at random places of it meet in the same banks.)
-__device__ __forceinline__ double exp_below(double d, double scale, const Shared& s) {
+template <bool NEAR> __device__ __forceinline__ double exp_below(double d, double scale, const Shared& s) {
   const double z = d * scale;
-  if (!(z > -32250.0)) return 0.0;                             // below exp(-698)
+  if (!NEAR && !(z > -32250.0)) return 0.0;                    // below exp(-698); NEAR: known to be above
   const double shift = 6755399441055744.0;                     // 1.5 * 2^52: adding it rounds to a whole number
   const double m = z + shift, g = z - (m - shift);
   const int n = __double2loint(m);
@@ -146,9 +147,8 @@ struct Row {
   int top_k;
 };
 
-// Sum over the block's threads before this one, and over all of them (whole numbers; the block has as many warps as a warp has lanes).
+// Sum over the block's threads before this one, and over all of them (whole numbers; a block has at most as many warps as a warp has lanes).
 template <typename V> __device__ __forceinline__ V block_scan(V mine, V* warps, V& total, int lane, int warp) {
-  static_assert(kWarps == 32, "a lane per warp");
   auto scan = [lane](V v) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -161,9 +161,9 @@ template <typename V> __device__ __forceinline__ V block_scan(V mine, V* warps, 
   __syncthreads();
   if (lane == 31) warps[warp] = upto;
   __syncthreads();
-  const V all = scan(warps[lane]);
+  const V all = scan(lane < kWarps ? warps[lane] : (V)0);
   total = __shfl_sync(~0u, all, 31);
-  const V before = __shfl_sync(~0u, all, (warp + 31) & 31);
+  const V before = __shfl_sync(~0u, all, (warp + kWarps - 1) % kWarps);
   return (warp ? before : 0) + upto - mine;
 }
 // Largest first; n2 a power of two, entries from n on are zeros.
@@ -198,7 +198,7 @@ template <typename T, int RANKS> struct Part {
   __device__ __forceinline__ Shared* peer(int k) { return RANKS == 1 ? &s : cluster.map_shared_rank(&s, k); }
   __device__ __forceinline__ void sync_row() { if (RANKS == 1) __syncthreads(); else cluster.sync(); }
   __device__ __forceinline__ T logit(int i) const { return i < limit ? logits[i] : L::dead(); }
-  __device__ __forceinline__ double weight(float v) const { return exp_below((double)v - (double)top, scale, s); }
+  __device__ __forceinline__ double weight(float v) const { return exp_below<false>((double)v - (double)top, scale, s); }
 
   // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them finds
   // the bin of the last kept token.
@@ -214,23 +214,150 @@ template <typename T, int RANKS> struct Part {
   // temperature, infinities).  All CTAs of a cluster take the same branches.
   __device__ __forceinline__ bool direct() {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int N = Piece<T>::N;
     const float per_unit = kBinsPerE / r.temperature;
     const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
     if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(top) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kTopK)) return false;
-    if (by_count) {
-      if (vocab / (kPer * Piece<T>::N) >= 2 * r.top_k) {
-        const int n = top_k<true>(per_unit);
-        if (n >= 0) return true;
-        if (n == -1) return false;
+    const double least = (double)r.min_p;
+    const int sub = slice / kWarps, warp_base = warp * sub;   // a warp's stretch
+    bool groups = by_count && vocab / (kPer * N) >= 2 * r.top_k;
+    int n = 0;
+    for (;;) {
+      int bin = kBins;
+      if (by_count || by_mass) {
+        bin = find_bin(by_count, groups, per_unit, by_count ? (double)r.top_k : (double)r.top_p);
+        // fewer than k tokens outside the last bin; a mark that rounding put between two bins; weights of no units
+        if (bin < 0 || (!by_count && bin == kBins - 1)) {
+          if (!groups) return false;
+          groups = false;
+          continue;
+        }
       }
-      return top_k<false>(per_unit) >= 0;
+      unsigned long long named = 0;
+      if (by_count) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          if (!groups || bin_of(place(group[g], per_unit)) <= bin) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+              const int i = tid + (g * kPer + k) * kThreads;
+              if (i < limit / N) {
+                const Piece<T> x = ((const Piece<T>*)logits)[i];
+                uint32_t mask = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
+                named |= (unsigned long long)mask << ((g * kPer + k) * N);
+              }
+            }
+          }
+      } else {
+        named = add_up(per_unit, by_mass, bin, sub, warp_base, lane, warp, tid);
+      }
+      if (by_count || by_mass) {
+        n = collect(by_count ? enlist(named, tid, kThreads) : enlist(named, warp_base / N + lane, 32));
+        if (n > kList) {
+          if (!groups) return false;
+          groups = false;
+          continue;
+        }
+      } else {
+        sync_row();
+      }
+      break;
     }
-    int bin = kBins;
-    if (by_mass) {
-      bin = find_bin<false, false>(per_unit, (double)r.top_p);
-      if (bin < 0 || bin == kBins - 1) return false;   // (a mark that rounding put between two bins; weights of no units)
+    if (by_count && rank) return true;
+    if (rank == 0) {
+      constexpr int kAll = RANKS * kWarps, kMine = kList / kThreads;
+      if (by_count && n <= kFew) { choose_from_few(n); return true; }
+      if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; s.pick = 0; }
+      unsigned long long sum_all = 0, sum_below = 0;
+      if (!by_count) {
+        // the sums of all warps, in index order
+#pragma unroll
+        for (int k = 0; k < RANKS; ++k) sum_all += s.all[k];
+        if (by_mass) block_scan(tid < kAll ? s.below[tid] : 0ull, s.warp_sum, sum_below, lane, warp);
+      }
+      if (n) {
+        sort(n, by_count, per_unit);
+        // exact weights of the list, largest first, kMine entries per thread; those kept are the first ones
+        const int count = by_count ? r.top_k : n;
+        unsigned long long unit[kMine], sum = 0, total;
+        double w[kMine];
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          const int i = tid * kMine + j;
+          w[j] = i < count ? weight(value_of(s.list[i])) : 0.0;
+          sum += unit[j] = i < count ? units(w[j]) : 0;
+        }
+        unsigned long long run = sum_below + block_scan(sum, s.warp_sum, total, lane, warp);
+        const double mark = (double)r.top_p * (double)(by_count ? total : sum_all);
+        int n_kept = 0;
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          const int i = tid * kMine + j;
+          const bool in_mass = i < count && (!by_mass || (double)run < mark || (i == 0 && sum_below == 0)), keep = in_mass && w[j] >= least;
+          if (by_count) {
+            if (keep) { n_kept = i + 1; sum += unit[j]; }
+            if (i < kTopK) s.weight[i] = keep ? unit[j] : 0;
+          } else if (in_mass) {
+            const unsigned long long entry = s.list[i];
+            if (!(i + 1 < n && (double)(run + unit[j]) < mark)) s.cut_entry = entry;   // the last of them ends the kept tokens
+            if (keep) atomicAdd(&s.taken[~(uint32_t)entry / (uint32_t)sub], unit[j]);
+          }
+          run += unit[j];
+        }
+        if (by_count) {
+          block_scan(sum, s.warp_sum, total, lane, warp);
+          if (n_kept) atomicMax(&s.pick, n_kept);
+          __syncthreads();
+          choose_by_digits(s.pick, (double)r.uniform * (double)total, lane, warp, tid);
+          return true;
+        }
+        if (tid == 0 && !((sum_below == 0 || (double)sum_below < mark) && mark <= (double)(sum_below + total))) s.ok = 0;
+      }
+      __syncthreads();
+      const unsigned long long taken = tid < kAll ? s.taken[tid] : 0;
+      unsigned long long sum_taken;
+      const unsigned long long before = block_scan(taken, s.warp_sum, sum_taken, lane, warp);
+      const double target = (double)r.uniform * (double)sum_taken;
+      if (!((double)before > target) && (double)(before + taken) > target)
+        for (int k = 0; k < RANKS; ++k) { Shared* o = peer(k); o->owner = tid; o->before = before; o->target = target; }
+      if (tid && tid < RANKS) { Shared* o = peer(tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
     }
-    return sum_and_choose(per_unit, by_mass, bin, lane, warp, tid);
+    sync_row();
+    if (!s.ok) return false;
+    if (s.owner / kWarps != rank) return true;
+    // the stretch of one warp, now by all warps of its CTA
+    const Key cut = (Key)(s.cut_entry >> 32);
+    const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
+    auto chosen = [&](int i) -> unsigned long long {
+      if (i >= sub) return 0;
+      const T x = logit(stretch + i);
+      const Key k = L::key(x);
+      if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
+      const double w = weight(L::widen(x));
+      return w >= least ? units(w) : 0;
+    };
+    unsigned long long mine = 0;
+    for (int i = warp * part + lane; i < (warp + 1) * part; i += 32) mine += chosen(i);
+    mine = warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) s.warp_sum[warp] = mine;
+    __syncthreads();
+    unsigned long long before = s.before;
+    for (int k = 0; k < warp; ++k) before += s.warp_sum[k];
+    if ((double)before > s.target || !((double)(before + mine) > s.target)) return true;
+    for (int i = warp * part; i < (warp + 1) * part; i += 32) {
+      const unsigned long long upto = before + warp_scan(chosen(i + lane), lane);
+      const uint32_t ballot = __ballot_sync(~0u, (double)upto > s.target);
+      if (ballot) {
+        if (lane == __ffs(ballot) - 1) tokens[row] = base + stretch + i + lane;
+        break;
+      }
+      before = __shfl_sync(~0u, upto, 31);
+    }
+    return true;
   }
 
   // The bin, as a float: nearest to (top - logit) * per_unit, which grows as logits fall; the last one for NaN and -inf.
@@ -238,12 +365,12 @@ template <typename T, int RANKS> struct Part {
   static __device__ __forceinline__ int bin_of(float at) { return (int)(__float_as_uint(at + 8388608.f) & 0x7fffffu); }
 
   // The bin in which the sum over bins passes `need` (a count, or a share of the mass), or -1.
-  template <bool COUNT, bool GROUPS> __device__ __forceinline__ int find_bin(float per_unit, double need) {
+  __device__ __forceinline__ int find_bin(bool count, bool groups, float per_unit, double need) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
     if (tid == 0) s.found = -1;
     __syncthreads();
-    if constexpr (GROUPS) {
+    if (groups) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int b = bin_of(place(group[g], per_unit));
@@ -258,7 +385,7 @@ template <typename T, int RANKS> struct Part {
           const float at = place(L::widen(x.e[j]), per_unit);
           const int b = bin_of(at);
           uint32_t add = 1;
-          if (!COUNT) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
+          if (!count) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
             const float d = ((float)b - at) * (1.f / kBinsPerE);
             add = __float_as_uint(fmaf(fmaf(fmaf(d, 1.f / 6, 0.5f), d, 1.f), d * 65536.f, 65536.f + 8388608.f)) & 0x7fffffu;
           }
@@ -280,7 +407,7 @@ template <typename T, int RANKS> struct Part {
         for (int k = 0; k < RANKS; ++k) n[k] = peer(k)->hist[b0 + j];
 #pragma unroll
         for (int k = 0; k < RANKS; ++k) v[j] += n[k];
-        if (!COUNT) v[j] = (unsigned long long)((float)v[j] * exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE) + 24.f));
+        if (!count) v[j] = (unsigned long long)((float)v[j] * exp2f((float)(b0 + j) * (-1.44269504f / kBinsPerE) + 24.f));
       }
       sum += v[j];
     }
@@ -294,7 +421,7 @@ template <typename T, int RANKS> struct Part {
       if (k == rank) offset = everything;
       everything += s.shares[k];
     }
-    const double mark = COUNT ? need : need * (double)everything;
+    const double mark = count ? need : need * (double)everything;
     unsigned long long run = offset + before;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
@@ -340,10 +467,24 @@ template <typename T, int RANKS> struct Part {
     sync_row();
     return all;
   }
-  // The first CTA's list, largest first: entries go to buckets by `place_of`, which never puts a smaller entry before a larger one; inside a bucket
-  // they are counted, or, where one is crowded, all are sorted by exchanges.
-  template <typename F> __device__ __forceinline__ void sort(int n, F place_of) {
+  // The first CTA's list, largest first.  Entries go to buckets, by their bins or, where they all share one, by key and, between equal keys, by
+  // index; inside a bucket they are counted, or, where one is crowded, all are sorted by exchanges.
+  __device__ __forceinline__ void sort(int n, bool by_bin, float per_unit) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    double spread = 0.0;
+    uint32_t high = 0;
+    if (!by_bin) {
+      if (tid == 0) { s.low_key = ~0u; s.high_key = 0; }
+      __syncthreads();
+      for (int i = tid; i < n; i += kThreads) { const uint32_t k = (uint32_t)(s.list[i] >> 32); atomicMin(&s.low_key, k); atomicMax(&s.high_key, k); }
+      __syncthreads();
+      high = s.high_key;
+      spread = (double)((float)kBins / ((float)(high - s.low_key) + 1.f));   // (any number will do that all entries share)
+    }
+    auto place_of = [&](unsigned long long e) {
+      if (by_bin) return bin_of(place(value_of(e), per_unit));
+      return min(kBins - 1, (int)(((double)(high - (uint32_t)(e >> 32)) + (double)(~(uint32_t)e) * (1.0 / kMaxVocab)) * spread));
+    };
     for (int i = tid; i < kBins; i += kThreads) s.bucket[i] = 0;
     if (tid == 0) s.crowded = 0;
     __syncthreads();
@@ -433,63 +574,9 @@ template <typename T, int RANKS> struct Part {
     if (tid == 0) tokens[row] = s.token;
   }
 
-  // Returns 0 when the token is written, -1 when the row has to go the general way, -2 when more tokens than fit lie in the groups' bin.
-  template <bool GROUPS> __device__ __forceinline__ int top_k(float per_unit) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int bin = find_bin<true, GROUPS>(per_unit, (double)r.top_k);
-    if (bin < 0) return GROUPS ? -2 : -1;   // (fewer than k of them outside the last bin)
-    unsigned long long named = 0;
-    if constexpr (GROUPS) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        if (bin_of(place(group[g], per_unit)) <= bin) {
-#pragma unroll
-          for (int k = 0; k < kPer; ++k) {
-            const int i = tid + (g * kPer + k) * kThreads;
-            if (i < limit / Piece<T>::N) {
-              const Piece<T> x = ((const Piece<T>*)logits)[i];
-              uint32_t mask = 0;
-#pragma unroll
-              for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
-              named |= (unsigned long long)mask << ((g * kPer + k) * Piece<T>::N);
-            }
-          }
-        }
-    } else {
-      int shift = 0;
-      for (int i = tid; i < limit / Piece<T>::N; i += kThreads, shift += Piece<T>::N) {
-        const Piece<T> x = ((const Piece<T>*)logits)[i];
-        uint32_t mask = 0;
-#pragma unroll
-        for (int j = 0; j < Piece<T>::N; ++j) mask |= (bin_of(place(L::widen(x.e[j]), per_unit)) <= bin ? 1u : 0u) << j;
-        named |= (unsigned long long)mask << shift;
-      }
-    }
-    const int n = collect(enlist(named, tid, kThreads));
-    if (n > kList) return GROUPS ? -2 : -1;
-    if (rank) return 0;
-    if (n <= kFew) { choose_from_few(n); return 0; }
-    sort(n, [&](unsigned long long e) { return bin_of(place(value_of(e), per_unit)); });
-    // the first top_k of the sorted list, an entry per thread
-    const bool by_mass = r.top_p < 1.f;
-    const double least = (double)r.min_p;
-    static_assert(kTopK <= kThreads, "an entry per thread");
-    const bool inside = tid < r.top_k;
-    const double w = inside ? weight(value_of(s.list[tid])) : 0.0;
-    const unsigned long long unit = inside ? units(w) : 0;
-    unsigned long long total;
-    const unsigned long long run = block_scan(unit, s.warp_sum, total, lane, warp);
-    const double mark = by_mass ? (double)r.top_p * (double)total : 0.0;
-    const bool keep = inside && (tid == 0 || ((!by_mass || (double)run < mark) && w >= least));
-    int n_kept = keep ? tid + 1 : 0;
-    if (tid < kTopK) s.weight[tid] = keep ? unit : 0;
-    if (tid == 0) s.pick = 0;
-    block_scan(keep ? unit : 0ull, s.warp_sum, total, lane, warp);
-    if (n_kept) atomicMax(&s.pick, n_kept);
-    __syncthreads();
-    n_kept = s.pick;
-    const double target = (double)r.uniform * (double)total;
-    // by index, six bits at a time: the digit at which the running sum passes the target
+  // From the list's first n_kept entries, with their weights beside them: by index, six bits at a time, the digit at which the running sum
+  // passes the target.
+  __device__ __forceinline__ void choose_by_digits(int n_kept, double target, int lane, int warp, int tid) {
     uint32_t prefix = 0;
     unsigned long long before = 0;
     for (int shift = 12; shift >= 0; shift -= 6) {
@@ -516,18 +603,17 @@ template <typename T, int RANKS> struct Part {
       before = s.above;
     }
     if (tid == 0) tokens[row] = (int)prefix;
-    return 0;
   }
 
-  __device__ __forceinline__ bool sum_and_choose(float per_unit, bool by_mass, int bin, int lane, int warp, int tid) {
+  // This CTA's exact sums, into the first CTA's memory; names the logits in the bin.
+  __device__ __forceinline__ unsigned long long add_up(float per_unit, bool by_mass, int bin, int sub, int warp_base, int lane, int warp, int tid) {
     constexpr int N = Piece<T>::N;
     Shared* first = peer(0);
-    const int sub = slice / kWarps, warp_base = warp * sub;   // a warp's stretch
     const double least = (double)r.min_p;
     unsigned long long named = 0;
     {
       // (where only min-p chooses, no weight past this place passes it, with room for the roundings of 32 bits)
-      const float last = by_mass || !(r.min_p > 0.f) ? (float)(kBins - 1) : fminf(-kBinsPerE * logf(r.min_p) + 1.f, (float)(kBins - 1));
+      const float last = by_mass || !(r.min_p > 0.f) ? kNoUnits : fminf(-kBinsPerE * logf(r.min_p) + 1.f, kNoUnits);
       const float floor = top - 70.f * r.temperature;   // no units; NaN and -inf become this
       const bool every = !(r.min_p > 0.f);              // min-p keeps all
       // a thread's sums of units are exact as doubles (64 logits at most); integer additions of two words would cost as much as the weights
@@ -542,7 +628,7 @@ template <typename T, int RANKS> struct Part {
           for (int j = 0; j < N; ++j) {
             const float v = fmaxf(L::widen(x.e[j]), floor);
             b[j] = (int)__float_as_uint(place(v, per_unit) + 8388608.f) - 0x4b000000;
-            w[j] = weight(v);
+            w[j] = exp_below<true>((double)v - (double)top, scale, s);
           }
           uint32_t mask = 0;
 #pragma unroll
@@ -562,114 +648,22 @@ template <typename T, int RANKS> struct Part {
       const unsigned long long sum_all = warp_sum((unsigned long long)all), sum_below = warp_sum((unsigned long long)below), sum_taken = warp_sum((unsigned long long)taken);
       if (lane == 0) { s.bucket[2 * warp] = (uint32_t)sum_all; s.bucket[2 * warp + 1] = (uint32_t)(sum_all >> 32); first->below[rank * kWarps + warp] = sum_below; first->taken[rank * kWarps + warp] = sum_taken; }
     }
-    int n = 0;
-    if (by_mass) n = enlist(named, warp_base / N + lane, 32);
     __syncthreads();
     if (tid == 0) {
       unsigned long long v = 0;
       for (int k = 0; k < kWarps; ++k) v += ((unsigned long long)s.bucket[2 * k + 1] << 32) + s.bucket[2 * k];
       first->all[rank] = v;
     }
-    if (by_mass) {
-      n = collect(n);
-      if (n > kList) return false;
-    } else {
-      sync_row();
-    }
-    if (rank == 0) {
-      // the sums of all warps, in index order
-      constexpr int kAll = RANKS * kWarps;
-      unsigned long long sum_all = 0, sum_below, total = 0;
-#pragma unroll
-      for (int k = 0; k < RANKS; ++k) sum_all += s.all[k];
-      if (tid == 0) { s.ok = 1; s.cut_entry = 0; s.owner = -1; }
-      if (by_mass) {
-        block_scan(tid < kAll ? s.below[tid] : 0ull, s.warp_sum, sum_below, lane, warp);
-        // one bin's tokens: buckets by key and, between equal keys, by index
-        if (tid == 0) { s.low_key = ~0u; s.high_key = 0; }
-        __syncthreads();
-        for (int i = tid; i < n; i += kThreads) { const uint32_t k = (uint32_t)(s.list[i] >> 32); atomicMin(&s.low_key, k); atomicMax(&s.high_key, k); }
-        __syncthreads();
-        const uint32_t high = s.high_key;
-        const double spread = (double)kBins / ((double)(high - s.low_key) + 1.0);
-        sort(n, [&](unsigned long long e) {
-          return min(kBins - 1, (int)(((double)(high - (uint32_t)(e >> 32)) + (double)(~(uint32_t)e) * (1.0 / kMaxVocab)) * spread));
-        });
-        constexpr int kMine = kList / kThreads;
-        unsigned long long unit[kMine], sum = 0;
-        double w[kMine];
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-          const int i = tid * kMine + j;
-          w[j] = i < n ? weight(value_of(s.list[i])) : 0.0;
-          sum += unit[j] = i < n ? units(w[j]) : 0;
-        }
-        unsigned long long run = sum_below + block_scan(sum, s.warp_sum, total, lane, warp);
-        const double mark = (double)r.top_p * (double)sum_all;
-        // (kept entries are the first ones; the last of them ends the kept tokens)
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-          const int i = tid * kMine + j;
-          const bool keep = i < n && ((double)run < mark || (i == 0 && sum_below == 0));
-          if (keep) {
-            const unsigned long long entry = s.list[i];
-            if (!(i + 1 < n && (double)(run + unit[j]) < mark)) s.cut_entry = entry;
-            if (w[j] >= least) atomicAdd(&s.taken[~(uint32_t)entry / (uint32_t)sub], unit[j]);
-          }
-          run += unit[j];
-        }
-        if (tid == 0 && !((sum_below == 0 || (double)sum_below < mark) && mark <= (double)(sum_below + total))) s.ok = 0;
-      }
-      __syncthreads();
-      const unsigned long long taken = tid < kAll ? s.taken[tid] : 0;
-      unsigned long long sum_taken;
-      const unsigned long long before = block_scan(taken, s.warp_sum, sum_taken, lane, warp);
-      const double target = (double)r.uniform * (double)sum_taken;
-      if (!((double)before > target) && (double)(before + taken) > target)
-        for (int k = 0; k < RANKS; ++k) { Shared* o = peer(k); o->owner = tid; o->before = before; o->target = target; }
-      if (tid && tid < RANKS) { Shared* o = peer(tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
-    }
-    sync_row();
-    if (!s.ok) return false;
-    if (s.owner / kWarps != rank) return true;
-    // the stretch of one warp, now by all warps of its CTA
-    const Key cut = (Key)(s.cut_entry >> 32);
-    const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
-    auto chosen = [&](int i) -> unsigned long long {
-      if (i >= sub) return 0;
-      const T x = logit(stretch + i);
-      const Key k = L::key(x);
-      if (!k || !(k > cut || (k == cut && base + stretch + i <= cut_index))) return 0;
-      const double w = weight(L::widen(x));
-      return w >= least ? units(w) : 0;
-    };
-    unsigned long long mine = 0;
-    for (int i = warp * part + lane; i < (warp + 1) * part; i += 32) mine += chosen(i);
-    mine = warp_sum(mine);
-    __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = mine;
-    __syncthreads();
-    unsigned long long before = s.before;
-    for (int k = 0; k < warp; ++k) before += s.warp_sum[k];
-    if ((double)before > s.target || !((double)(before + mine) > s.target)) return true;
-    for (int i = warp * part; i < (warp + 1) * part; i += 32) {
-      const unsigned long long upto = before + warp_scan(chosen(i + lane), lane);
-      const uint32_t ballot = __ballot_sync(~0u, (double)upto > s.target);
-      if (ballot) {
-        if (lane == __ffs(ballot) - 1) tokens[row] = base + stretch + i + lane;
-        break;
-      }
-      before = __shfl_sync(~0u, upto, 31);
-    }
-    return true;
+    return named;
   }
+
   // Any row: one search for top-k and one for top-p, each over 8 bits of the keys at a time from the top.
   __device__ __noinline__ void general() {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ranks = RANKS;
     const Key top_key = key_of_top();
     if (tid < 256) { s.lo[0][tid] = 0; s.hi[0][tid] = 0; }
     __syncthreads();
-    auto weight_of = [&](Key k) { return k == top_key ? 1.0 : exp_below((double)L::value(k) - (double)top, scale, s); };
+    auto weight_of = [&](Key k) { return k == top_key ? 1.0 : exp_below<false>((double)L::value(k) - (double)top, scale, s); };
     // Kept so far: key > t, or key == t and index <= c.
     Key t = 1;
     int c = INT_MAX, buffer = 0;
@@ -892,30 +886,34 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   T* mine = keep ? (T*)(dynamic + sizeof(Shared)) : (T*)src;
   const int here = max(0, min(slice, vocab - base));
   float group[P::kGroups], top = -INFINITY;
+  if (!vec) {   // (then the slice goes to shared memory)
+    for (int i = tid; i < slice; i += kThreads) mine[i] = i < here ? src[i] : L::dead();
+    __syncthreads();
+  }
+  const T* from = vec ? src : mine;
+  const int readable = vec ? here : slice;
 #pragma unroll
   for (int g = 0; g < P::kGroups; ++g) {
     group[g] = -INFINITY;
-    uint4 u[P::kPer];
 #pragma unroll
     for (int k = 0; k < P::kPer; ++k) {
       const int i = (tid + (g * P::kPer + k) * kThreads) * N;
-      if (vec && i + N <= here) {
-        u[k] = *(const uint4*)(src + i);
-      } else {
-        Piece<T> x;
-#pragma unroll
-        for (int j = 0; j < N; ++j) x.e[j] = i + j < here ? src[i + j] : L::dead();
-        u[k] = *(const uint4*)&x;
+      if (i + N <= readable) {
+        const uint4 u = *(const uint4*)(from + i);
+        if (vec && keep) *(uint4*)(mine + i) = u;
+        group[g] = fmaxf(group[g], L::largest(u));
+      } else if (vec && keep && i < slice) {   // past the row's last 16 bytes, and past the row
+#pragma unroll 1
+        for (int j = i; j < i + N; ++j) {
+          const T x = j < here ? src[j] : L::dead();
+          mine[j] = x;
+          group[g] = fmaxf(group[g], L::widen(x));
+        }
       }
     }
-#pragma unroll
-    for (int k = 0; k < P::kPer; ++k) {
-      const int i = (tid + (g * P::kPer + k) * kThreads) * N;
-      if (keep && i < slice) *(uint4*)(mine + i) = u[k];
-      group[g] = fmaxf(group[g], L::largest(u[k]));
-    }
-    top = fmaxf(top, group[g]);
   }
+#pragma unroll
+  for (int g = 0; g < P::kGroups; ++g) top = fmaxf(top, group[g]);
   if (tid < kTable * kCopies) s.table[tid / kCopies][tid % kCopies] = powers.of[tid / kCopies];
   const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
 #pragma unroll
@@ -961,7 +959,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
     q = fma(fma(-t, q, 1.0), q, q);
     part.scale = 46.166241308446828384 * (r.temperature > 1e-4f && r.temperature < 1e4f ? q : 1.0 / t);   // 32 / ln 2
   }
-  if (!part.direct()) part.general();
+  if (part.direct()) return;
+  P copy = part;   // (general() takes its address, which would put the registers of the other way in memory, too: 5000 clocks a row)
+  copy.general();
 }
 
 template <typename T> auto kernel_of(int ranks) { return ranks == 1 ? sample_kernel<T, 1> : ranks == 2 ? sample_kernel<T, 2> : ranks == 4 ? sample_kernel<T, 4> : sample_kernel<T, 8>; }
