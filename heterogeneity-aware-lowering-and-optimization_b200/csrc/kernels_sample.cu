@@ -12,8 +12,8 @@ namespace b200 {
 namespace {
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kMaxCluster = 8;
-constexpr int kBins = 2048, kList = 2048, kTopK = 1024, kBucket = 128, kFew = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 2048, kList = 1536, kTopK = 1024, kBucket = 128, kFew = kThreads / 4;
 constexpr int kSlice = 64 * kThreads;   // logits of a CTA at most: a thread names its own by the bits of one word
 constexpr float kNoUnits = 1000.f;   // weights from here on, below 2^-45, are no units
 constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
@@ -77,7 +77,7 @@ struct Powers { double of[kTable]; };   // 2^(j / 32)
 struct alignas(16) Shared {
   double table[kTable][kCopies];          // 2^(j / 32), a copy for each pair of banks
   // The direct way: a histogram (counts, or masses), then a list of (key, ~index); what every warp of the cluster has summed.
-  union { uint32_t hist[kBins]; unsigned long long list[kList]; };
+  union { uint32_t hist[kBins]; unsigned long long list[2048]; };   // (kList entries, room for a power of two when they are sorted by exchanges)
   union {
     unsigned long long spare[kList];      // while the list is sorted
     unsigned long long weight[kTopK];     // of the list's first, by rank (top-k)
@@ -205,7 +205,7 @@ template <typename T, int RANKS> struct Part {
   //   top-k up to 1024: a histogram of the largest logits of small groups, kept in registers (the k-th largest of those has at least k tokens above it, and rarely
   //   many more; of every logit where that did not hold, or the row is short).  All tokens down to that bin go to a list of the first CTA,
   //   which sorts it and does the rest alone.
-  //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 2^-16), for top-p; then every CTA sums exact weights,
+  //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 1e-4), for top-p; then every CTA sums exact weights,
   //   over all tokens, over those in higher bins, and of the latter, warp by warp, over those that min-p keeps; tokens in the bin itself
   //   go to the list.  The first CTA sorts it, finds the last token kept, and which warp's stretch of the row the choice lies in; that
   //   stretch's CTA finds it there.
@@ -384,11 +384,8 @@ template <typename T, int RANKS> struct Part {
         for (int j = 0; j < Piece<T>::N; ++j) {
           const float at = place(L::widen(x.e[j]), per_unit);
           const int b = bin_of(at);
-          uint32_t add = 1;
-          if (!count) {   // 2^16 e^(-(at - b) / 32), |at - b| <= 1/2, to 2^-22
-            const float d = ((float)b - at) * (1.f / kBinsPerE);
-            add = __float_as_uint(fmaf(fmaf(fmaf(d, 1.f / 6, 0.5f), d, 1.f), d * 65536.f, 65536.f + 8388608.f)) & 0x7fffffu;
-          }
+          // 2^16 (1 - (at - b) / 32) for 2^16 e^(-(at - b) / 32), |at - b| <= 1/2: at most 1.2e-4 off, and alike in all bins
+          const uint32_t add = count ? 1u : __float_as_uint(fmaf(((at + 8388608.f) - 8388608.f) - at, 65536.f / kBinsPerE, 65536.f + 8388608.f)) & 0x7fffffu;
           if (b < kBins - 1) atomicAdd(&s.hist[b], add);
         }
       }
@@ -622,24 +619,27 @@ template <typename T, int RANKS> struct Part {
       for (int i = warp_base / N + lane; i < min(warp_base + sub, limit) / N; i += 32, shift += N) {
         const Piece<T> x = ((const Piece<T>*)logits)[i];
         if (place(L::largest(*(const uint4*)&x), per_unit) < last) {
-          double w[N];
-          int b[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float v = fmaxf(L::widen(x.e[j]), floor);
-            b[j] = (int)__float_as_uint(place(v, per_unit) + 8388608.f) - 0x4b000000;
-            w[j] = exp_below<true>((double)v - (double)top, scale, s);
-          }
           uint32_t mask = 0;
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const double u = units_exact(w[j]);
-            all += u;
-            if (b[j] < bin) {
-              below += u;
-              if (!every && w[j] >= least) taken += u;
+          for (int j0 = 0; j0 < N; j0 += 4) {
+            double w[4];
+            int b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float v = fmaxf(L::widen(x.e[j0 + j]), floor);
+              b[j] = (int)__float_as_uint((top - v) * per_unit + 8388608.f) - 0x4b000000;
+              w[j] = exp_below<true>((double)v - (double)top, scale, s);
             }
-            mask |= (b[j] == bin ? 1u : 0u) << j;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const double u = units_exact(w[j]);
+              all += u;
+              if (b[j] < bin) {
+                below += u;
+                if (!every && w[j] >= least) taken += u;
+              }
+              mask |= (b[j] == bin ? 1u : 0u) << (j0 + j);
+            }
           }
           named |= (unsigned long long)mask << shift;
         }
@@ -792,10 +792,12 @@ template <typename T, int RANKS> struct Part {
       // (the mark is known to warp 0)
       const unsigned long long w = units(weight_of(found));
       if (tid == 0) {
+        // the fewest of them with which the sum reaches the mark: the quotient, which roundings can put off by one
+        const long long all = w ? (long long)(in_bin / w) : 1;
         long long j = w ? (long long)((mark - (double)above) / (double)w) : 1;
-        if (j < 1) j = 1;
-        while (j > 1 && (double)(above + (unsigned long long)(j - 1) * w) >= mark) --j;
-        while ((double)(above + (unsigned long long)j * w) < mark) ++j;
+        j = j < 1 ? 1 : j > all ? all : j;
+        for (int i = 0; i < 2 && j > 1 && (double)(above + (unsigned long long)(j - 1) * w) >= mark; ++i) --j;
+        for (int i = 0; i < 2 && j < all && (double)(above + (unsigned long long)j * w) < mark; ++i) ++j;
         s.pick = (int)j;
       }
       __syncthreads();
@@ -872,7 +874,7 @@ template <typename T, int RANKS> struct Part {
 // (`keep` is 0) the passes after the first read them from the caller's memory again, mostly from L2.  CTAs are few and large: what a row costs beside
 // its loads and weights is a chain of barriers, and a cluster's barrier costs several times a block's.
 template <typename T, int RANKS>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
                                                           const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
   using L = Logits<T>;
   using P = Part<T, RANKS>;
@@ -914,6 +916,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ 
   }
 #pragma unroll
   for (int g = 0; g < P::kGroups; ++g) top = fmaxf(top, group[g]);
+  static_assert(kTable * kCopies <= kThreads, "an entry per thread");
   if (tid < kTable * kCopies) s.table[tid / kCopies][tid % kCopies] = powers.of[tid / kCopies];
   const Row r{temperature ? temperature[row] : 1.f, top_p ? top_p[row] : 1.f, min_p ? fminf(min_p[row], 1.f) : 0.f, uniform[row], top_k ? top_k[row] : 0};
 #pragma unroll
@@ -971,14 +974,14 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
            cudaStream_t stream) {
   // A slice goes to shared memory where it fits; it has to where a row is no number of aligned 16 bytes, because only the first pass reads
   // single logits.
-  constexpr int kKeep = 160 * 1024;
+  constexpr size_t kKeep = 64 * 1024, kMost = 160 * 1024;   // two CTAs to an SM, or whatever fits
   const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
   const bool must = !vec || vocab % (16 / (int)sizeof(T));
   int ranks = 1;
   auto slice_of = [&](int n) { return ((vocab + n - 1) / n + kThreads - 1) / kThreads * kThreads; };
-  while (ranks < kMaxCluster && (slice_of(ranks) > kSlice || (must && slice_of(ranks) * sizeof(T) > kKeep))) ranks *= 2;
+  while (ranks < kMaxCluster && (slice_of(ranks) > kSlice || (must && slice_of(ranks) * sizeof(T) > kMost) || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
   const int slice = slice_of(ranks);
-  const int keep = slice * sizeof(T) <= kKeep;
+  const int keep = must || slice * sizeof(T) <= kKeep;
   const size_t smem = sizeof(Shared) + (keep ? (size_t)slice * sizeof(T) : 0);
   static const Powers powers = [] { Powers p; for (int j = 0; j < kTable; ++j) p.of[j] = std::exp2((double)j / kTable); return p; }();
   auto* fn = kernel_of<T>(ranks);
