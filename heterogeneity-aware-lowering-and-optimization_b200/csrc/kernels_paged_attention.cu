@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
 // row turns it into weights, which replace it there as the A operand of O += P V.  O stays in tensor memory over the whole chunk: a
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
 // rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
-// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks).
+// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3400.  Up to 128 rows leave the
+// second tile free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
 // Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values lie as
 // the products read them (rows of 64 channels, 128-byte swizzle); the ring alternates units of 128 keys and 128 values.  They arrive by
 // TMA in boxes of as many positions as divide both a page and a step, where those are at least the swizzle's eight; pages of other
@@ -345,7 +346,8 @@ constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
 struct True { static constexpr bool value = true; };
 struct False { static constexpr bool value = false; };
 struct WideShared {
-  uint64_t full[kWideRing], empty[kWideRing], q_full, s_full[2], p_full[2], o_done[2], drained;
+  float2 stat[128];         // split: reference and sum of the second tile's rows
+  uint64_t full[kWideRing], empty[kWideRing], q_full, s_full[2], p_half[2], p_full[2], o_done[2], handed, drained;
   uint32_t seen[4][4];   // which of a step's positions can be seen; a step's words are written at most two steps ahead
   uint32_t tmem;
   int abort;
@@ -373,6 +375,51 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Two floats in one register pair.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t x, uint32_t y) { return pair_of(__uint_as_float(x), __uint_as_float(y)); }
+__device__ __forceinline__ void unpack(uint64_t p, float (&e)[2]) { asm("mov.b64 {%0, %1}, %2;" : "=f"(e[0]), "=f"(e[1]) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x for two x <= 8 on the multiply-add pipes, for a quarter of all exponentials (256 rows behind 32768 positions: 92 -> 88.5 us; half of them: 94):
+// x = n + f with n whole, |f| <= 1/2; the series of 2^f up to the fifth power, whose rest is below 2.5e-6 (a two-hundredth of half a step
+// of fp16), times 2^n.  Below 2^-126 nothing is left of a weight; NaN stays NaN.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float (&e)[2]) {
+  float t[2];
+  unpack(x, t);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t[h]));   // -126
+  x = pair_of(t[0], t[1]);
+  // the sum's lowest bits are n + 127: shifted into place, 2^n
+  const uint64_t shift = pair_of(12582912.f + 127.f, 12582912.f + 127.f), back = pair_of(-12582912.f - 127.f, -12582912.f - 127.f), minus = pair_of(-1.f, -1.f);
+  const uint64_t n = add2(x, shift), f = fma2(add2(n, back), minus, x);
+  constexpr float l = 0.69314718056f;
+  uint64_t r = fma2(f, pair_of(l * l * l * l * l / 120, l * l * l * l * l / 120), pair_of(l * l * l * l / 24, l * l * l * l / 24));
+  r = fma2(r, f, pair_of(l * l * l / 6, l * l * l / 6));
+  r = fma2(r, f, pair_of(l * l / 2, l * l / 2));
+  r = fma2(r, f, pair_of(l, l));
+  r = fma2(r, f, pair_of(1.f, 1.f));
+  float m[2];
+  unpack(n, m);
+  unpack(mul2(r, pair_of(__float_as_uint(m[0]) << 23, __float_as_uint(m[1]) << 23)), e);
+}
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int channel, int position, int head, int page) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"((uint64_t)map),
                "r"(smem_u32(bar)), "r"(channel), "r"(position), "r"(head), "r"(page)
@@ -411,20 +458,22 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
     pages = p.page_table + (int64_t)b * p.a.table_width;
     slot = p.prefix_chunks + chunk;
   }
-  const int tiles = n_rows > 128 ? 2 : 1, steps = (end - begin + kWideStep - 1) / kWideStep;
-  const uint32_t columns = tiles == 2 ? 512u : 256u;
+  const int steps = (end - begin + kWideStep - 1) / kWideStep;
+  const bool split = n_rows <= 128;
+  constexpr uint32_t kColumns = 512;
   if (threadIdx.x == 0) {
     if (p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
     for (int i = 0; i < kWideRing; ++i) { mbar_init(&w.full[i], kLoaders * 33); mbar_init(&w.empty[i], 1); }
-    mbar_init(&w.q_full, 4 * tiles);
-    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
+    mbar_init(&w.q_full, split ? 4 : 8);
+    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_half[t], 4); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
+    mbar_init(&w.handed, 4);
     mbar_init(&w.drained, 1);
     w.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_proxy();
   }
   if (warp == 8 + kLoaders) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(columns) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -437,33 +486,37 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
 
   if (warp < 8) {
     // ------------------------------------------------------------------- softmax ----
-    const int tile = warp >> 2, quarter = warp & 3, r = tile * 128 + quarter * 32 + lane;
-    if (tile < tiles) {
+    const int tile = warp >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane, r = split ? in_tile : tile * 128 + in_tile;
+    {
       const bool live = r < n_rows;
       const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
-      const uint4* q = (const uint4*)((const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head);
       // (a negative scale becomes the sign of the queries: the largest score is then the largest product)
-      const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
-      const uint32_t s_row = s_q + tile * kUnit + (r & 127) * 128;
+      if (!(split && tile)) {
+        const uint4* q = (const uint4*)((const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head);
+        const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
+        const uint32_t s_row = s_q + tile * kUnit + in_tile * 128;
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        uint4 u = live ? q[c] : make_uint4(0, 0, 0, 0);
-        u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_row + (c >> 3) * kBox + (((c & 7) ^ (r & 7)) << 4)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+        for (int c = 0; c < kPieces; ++c) {
+          uint4 u = live ? q[c] : make_uint4(0, 0, 0, 0);
+          u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_row + (c >> 3) * kBox + (((c & 7) ^ (r & 7)) << 4)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w.q_full);
       }
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w.q_full);
       const float scale = fabsf(p.scale_log2e);
-      const uint32_t lanes = (uint32_t)(quarter * 32) << 16, t_s = tmem + tile * 128 + lanes, t_o = tmem + tiles * 128 + tile * D + lanes;
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16, t_s = tmem + tile * 128 + lanes, t_o = tmem + 256 + tile * D + lanes;
       float reference = -INFINITY, sum = 0.f;
       bool ok = true;
-      for (int i = 0; i < steps; ++i) {
+      const int own_steps = split ? (steps - tile + 1) / 2 : steps;
+      for (int i = 0; i < own_steps; ++i) {
+        const int step = split ? 2 * i + tile : i;
         if (!warp_wait(&w.s_full[tile], i & 1)) { ok = false; break; }
         tc_fence_after();
         uint32_t seen[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) seen[c] = *(volatile uint32_t*)&w.seen[i & 3][c];
+        for (int c = 0; c < 4; ++c) seen[c] = *(volatile uint32_t*)&w.seen[step & 3][c];
         const bool whole = (seen[0] & seen[1] & seen[2] & seen[3]) == ~0u;
         float mx = -INFINITY;
         auto largest = [&](auto all) {
@@ -505,9 +558,10 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
           }
         }
         const float base = reference == -INFINITY ? 0.f : reference;
+        const uint64_t scale2 = pair_of(scale, scale), base2 = pair_of(-base, -base);
         auto weights = [&](auto all) {
           uint32_t v[2][32], u[16];
-          float part[2] = {0.f, 0.f};
+          uint64_t part = 0;   // two zeros
           tmem_ld32(t_s, v[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -516,17 +570,25 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               float e[2];
+              const uint64_t x = fma2(pair_of(v[c & 1][2 * k], v[c & 1][2 * k + 1]), scale2, base2);
+              if (k % 4 == 3) exp2_pair(x, e); else { unpack(x, e); e[0] = exp2_fast(e[0]); e[1] = exp2_fast(e[1]); }
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                e[h] = exp2_fast(fmaf(__uint_as_float(v[c & 1][2 * k + h]), scale, -base));
+              for (int h = 0; h < 2; ++h)
                 if (!decltype(all)::value && !(seen[c] >> (2 * k + h) & 1)) e[h] = 0.f;
-                part[h] += e[h];
-              }
+              part = add2(part, pair_of(e[0], e[1]));
               u[k] = Mma<T>::pack(e[0], e[1]);
             }
             tmem_st16(t_s + c * 16, u);   // (over scores that have been read)
+            if (c == 1) {   // the first half of the weights can be multiplied
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&w.p_half[tile]);
+            }
           }
-          sum += part[0] + part[1];
+          float e[2];
+          unpack(part, e);
+          sum += e[0] + e[1];
         };
         if (whole) weights(True()); else weights(False());
         tmem_st_wait();
@@ -534,22 +596,58 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
         __syncwarp();
         if (lane == 0) mbar_arrive(&w.p_full[tile]);
       }
-      if (ok) ok = warp_wait(&w.o_done[tile], 0);
+      // All products done, queries and ring are free: the rows of the result go there (16 bytes apart from each other's banks), and each on as one
+      // copy (a thread's own stores, 16 bytes of 32 rows at a time, took 3.6 us).
+      if (ok) ok = warp_wait(&w.o_done[0], 0);
+      if (ok && (!split || steps > 1)) ok = warp_wait(&w.o_done[1], 0);
       tc_fence_after();
-      const int64_t at = ((int64_t)head * p.rows + row) * p.slots + slot;
-      if (live) p.stat[at] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
-      if (ok) {
+      constexpr uint32_t kRow = D * 4 + 16;
+      const uint32_t row_at = smem + (uint32_t)r * kRow;
+      const bool hands = split && tile, takes = split && !tile && steps > 1;
+      if (hands) w.stat[in_tile] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
+      float mine = 1.f, theirs = 0.f;
+      if (takes) {
+        if (ok) ok = warp_wait(&w.handed, 0);
+        if (ok) {
+          const float2 st = w.stat[in_tile];
+          const float top = fmaxf(reference, st.x), base = top == -INFINITY ? 0.f : top;
+          mine = exp2_fast(reference - base);
+          theirs = exp2_fast(st.x - base);
+          sum = sum * mine + st.y * theirs;
+          reference = top;
+        }
+      }
+      if (ok && own_steps) {
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
           tmem_ld32(t_o + c * 32, v);
           tmem_ld_wait32(v);
-          if (live) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              *(float4*)(p.part + at * D + c * 32 + k * 4) =
-                  make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t to = row_at + c * 128 + k * 16;
+            float x[4] = {__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])};
+            if (takes) {
+              float y[4];
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(to) : "memory");
+#pragma unroll
+              for (int h = 0; h < 4; ++h) x[h] = x[h] * mine + y[h] * theirs;
+            }
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]) : "memory");
           }
+        }
+      }
+      if (hands) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w.handed);
+      } else if (live) {
+        const int64_t at = ((int64_t)head * p.rows + row) * p.slots + slot;
+        p.stat[at] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
+        if (ok) {
+          fence_async_proxy();
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.part + at * D), "r"(row_at), "n"(D * 4) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
       }
       tc_fence_before();
@@ -647,37 +745,44 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
     };
     bool ok = wait(&w.q_full, 0);
     auto scores = [&](int i, int t) {   // S_t = Q_t K_i^T
-      const uint32_t k = s_ring + (2 * i % kWideRing) * kUnit, q = s_q + t * kUnit;
+      const uint32_t k = s_ring + (2 * i % kWideRing) * kUnit, q = s_q + (split ? 0u : t * kUnit);
 #pragma unroll
       for (int n = 0; n < D / 16; ++n)
         umma_f16(tmem + t * 128, desc(q + (n >> 2) * kBox + (n & 3) * 32, 1), desc(k + (n >> 2) * kBox + (n & 3) * 32, 1), idesc_s, n ? 1u : 0u);
       umma_commit(&w.s_full[t]);
     };
-    if (ok) ok = landed(0);
-    if (ok) {
+    // Every tile takes every step; split, step i belongs to tile i & 1, whose next one is i + 2.
+    const int ahead = split ? 2 : 1;
+    for (int i = 0; i < min(ahead, steps) && ok; ++i) {
+      ok = landed(2 * i);
+      if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) scores(0, t);
-      umma_commit(&w.empty[0]);
+      if (split) scores(i, i); else for (int t = 0; t < 2; ++t) scores(i, t);
+      umma_commit(&w.empty[2 * i % kWideRing]);
     }
     for (int i = 0; i < steps && ok; ++i) {
-      const int vu = 2 * i + 1, ku = 2 * i + 2;
-      const bool more = i + 1 < steps;
-      for (int t = 0; t < tiles && ok; ++t) {
-        if (t == 0) ok = landed(vu);
-        ok = ok && wait(&w.p_full[t], i & 1);
-        if (!ok) break;
-        tc_fence_after();
+      const int vu = 2 * i + 1, ku = 2 * (i + ahead), t0 = split ? i & 1 : 0, t1 = split ? t0 : 1, turn = split ? i >> 1 : i;
+      const bool more = i + ahead < steps;
+      for (int t = t0; t <= t1 && ok; ++t) {
+        if (t == t0) ok = landed(vu);
         const uint32_t v = s_ring + (vu % kWideRing) * kUnit;
 #pragma unroll
-        for (int n = 0; n < kWideStep / 16; ++n)
-          umma_tmem_a(tmem + tiles * 128 + t * D, tmem + t * 128 + n * 8, desc(v + n * 2048, kBox >> 4), idesc_o, (i || n) ? 1u : 0u);
-        if (t == tiles - 1) umma_commit(&w.empty[vu % kWideRing]);
+        for (int h = 0; h < 2; ++h) {   // half of the weights while the other half is worked out
+          ok = ok && wait(h ? &w.p_full[t] : &w.p_half[t], turn & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int n = h * 4; n < h * 4 + 4; ++n)
+            umma_tmem_a(tmem + 256 + t * D, tmem + t * 128 + n * 8, desc(v + n * 2048, kBox >> 4), idesc_o, (turn || n) ? 1u : 0u);
+        }
+        if (!ok) break;
+        if (t == t1) umma_commit(&w.empty[vu % kWideRing]);
         if (!more) { umma_commit(&w.o_done[t]); continue; }
-        if (t == 0) ok = landed(ku);
+        if (t == t0) ok = landed(ku);
         if (!ok) break;
         tc_fence_after();
-        scores(i + 1, t);
-        if (t == tiles - 1) umma_commit(&w.empty[ku % kWideRing]);
+        scores(i + ahead, t);
+        if (t == t1) umma_commit(&w.empty[ku % kWideRing]);
       }
     }
     if (!ok) { umma_commit(&w.drained); await_landing(&w.drained, 0); }   // products in flight end before their memory goes
@@ -686,7 +791,7 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
   __syncthreads();
   if (warp == 8 + kLoaders) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
   }
   grid_dependency_wait();   // the end of this grid is the end of tile_kernel's, which it may have started under
 }
@@ -768,14 +873,14 @@ Params plan(const PagedAttention& a) {
     return (int)chunk;
   };
   if (a.prefix_length && p.rows > kRows) {
-    // Blocks of equal work on 148 SMs: the number of chunks with the shortest estimate of waves of steps (1.4 us each, 3 us at both ends) and of
+    // Blocks of equal work on 148 SMs: the number of chunks with the shortest estimate of waves of steps (1.9 us each, 1.1 us split; 5 us at both ends) and of
     // the partial results' way to memory and back.
     p.wide_tiles = (p.rows + kWideRows - 1) / kWideRows;
     const int tiles = p.wide_tiles * a.kv_heads, all = (a.prefix_length + kWideStep - 1) / kWideStep;
     double best = 1e30;
     for (int c = 1; c <= all && c <= 64; ++c) {
       const int steps = (all + c - 1) / c;
-      const double us = (double)((tiles * (int64_t)c + 147) / 148) * (steps * 1.4 + 3.0) + (double)c * p.rows * a.kv_heads * a.channels * 8 / 5e6;
+      const double us = (double)((tiles * (int64_t)c + 147) / 148) * (steps * (p.rows > 128 ? 1.9 : 1.1) + 5.0) + (double)c * p.rows * a.kv_heads * a.channels * 8 / 5e6;
       if (us < best) { best = us; p.prefix_chunk = steps * kWideStep; }
     }
     p.prefix_tiles = 0;
