@@ -2,6 +2,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <climits>
 #include <cstdlib>
 
 #include "kernels.h"
@@ -85,11 +86,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
   return x;
 }
-__device__ __forceinline__ int own_length(const Params& p, int b) {
+__device__ __forceinline__ int capped(const Params& p, int n) {
   const long long cap = (long long)p.a.table_width * p.a.page_size;
-  const int n = p.lengths[b];
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
+__device__ __forceinline__ int own_length(const Params& p, int b) { return capped(p, p.lengths[b]); }
 
 // Own positions that every query of the sequence sees.
 __device__ __forceinline__ int common_length(const Params& p, int length) { return max(0, length - p.a.queries + 1); }
@@ -102,7 +103,7 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 // Softmax runs over positions with maximum and sum per row; the weights are rounded to the cache's type for the second product, and the
 // sum is taken of the rounded ones, so that the result is an average of values with weights that add up to one.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kPieces = D / 8, kUnit = kStep * D * 2;   // 16-byte pieces of a row; bytes of a unit
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
   const int prefix_items = p.prefix_tiles * p.prefix_chunks;
   const bool own = item >= prefix_items;
   const int* pages;
-  int row0, n_rows, begin, end, slot, length = 0;
+  int row0, n_rows, begin, end, slot, length = 0, b_own = 0;
   if (!own) {
     const int chunk = item / p.prefix_tiles, tile = item - chunk * p.prefix_tiles;
     row0 = tile * kRows;
@@ -123,35 +124,47 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     slot = chunk;
   } else {
     item -= prefix_items;
-    const int b = item % p.a.batch, rest = item / p.a.batch, chunk = rest / p.own_tiles, tile = rest - chunk * p.own_tiles;
+    b_own = item % p.a.batch;
+    const int rest = item / p.a.batch, chunk = rest / p.own_tiles, tile = rest - chunk * p.own_tiles;
     const int per = p.a.queries * p.group;
-    row0 = b * per + tile * kRows;
+    row0 = b_own * per + tile * kRows;
     n_rows = min(kRows, per - tile * kRows);
-    length = own_length(p, b);
-    begin = chunk * p.own_chunk + (p.own_wide_tiles ? common_length(p, length) : 0);
-    end = min(begin + p.own_chunk, length);
-    if (begin >= end) return;   // (the sum over slots knows)
-    pages = p.page_table + (int64_t)b * p.a.table_width;
+    begin = chunk * p.own_chunk;
+    if (p.own_wide_tiles) begin += common_length(p, own_length(p, b_own));
+    end = (int)min((int64_t)begin + p.own_chunk, (int64_t)p.a.table_width * p.a.page_size);   // (until the length is there)
+    pages = p.page_table + (int64_t)b_own * p.a.table_width;
     slot = p.prefix_chunks + p.own_wide_chunks + chunk;
   }
+  // The length, the first page numbers and the queries are asked for at once; page numbers after that a step early.
+  if (own) length = p.lengths[b_own];
+  auto ask = [&](int step) {
+    const int pos = begin + step * kStep + lane;
+    return lane < kStep && pos < end ? pages[pos / p.a.page_size] : -1;
+  };
+  int page = ask(warp);
   // the rows this lane has a share of: row0 + lane / 4 and + 8
   int limit[2];
   uint32_t qa[D / 16][4];
-  {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (lane >> 2) + 8 * h;
-      const bool live = r < n_rows;
-      const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
-      limit[h] = !live ? 0 : own ? length - p.a.queries + j + 1 : p.a.prefix_length;
-      const T* q = (const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head;
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+    const bool live = r < n_rows;
+    const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
+    limit[h] = !live ? INT_MIN : j;
+    const T* q = (const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qa[k][h] = live ? *(const uint32_t*)(q + k * 16 + (lane & 3) * 2) : 0u;
-        qa[k][h + 2] = live ? *(const uint32_t*)(q + k * 16 + 8 + (lane & 3) * 2) : 0u;
-      }
+    for (int k = 0; k < D / 16; ++k) {
+      qa[k][h] = live ? *(const uint32_t*)(q + k * 16 + (lane & 3) * 2) : 0u;
+      qa[k][h + 2] = live ? *(const uint32_t*)(q + k * 16 + 8 + (lane & 3) * 2) : 0u;
     }
   }
+  if (own) {
+    length = capped(p, length);
+    end = min(end, length);
+    if (begin >= end) return;   // (the sum over slots knows)
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) limit[h] = limit[h] == INT_MIN ? 0 : own ? length - p.a.queries + limit[h] + 1 : p.a.prefix_length;
   // positions below `all` are seen by every row of the tile
   int all = own ? length - p.a.queries + row0 / p.group % p.a.queries + 1 : p.a.prefix_length;
   const int n_steps = (end - begin + kStep - 1) / kStep;
@@ -167,16 +180,14 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
       if (!(u & 1)) {
         const int pos = begin + step * kStep + lane;
         off = -1;
-        if (pos < end) {
-          const int n = pos / p.a.page_size, page = pages[n];
-          if (page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos - n * p.a.page_size) * p.a.c_token;
-        }
+        if (lane < kStep && pos < end && page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos % p.a.page_size) * p.a.c_token;
         seen = __ballot_sync(~0u, off >= 0);
+        page = ask(step + kWarps);
       }
       const T* base = (u & 1) ? vc : kc;
       const uint32_t dst = ring + (u % kRing) * kUnit;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
+      for (int i = 0; i < kPieces * kStep / 32; ++i) {
         const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
         const int64_t o = __shfl_sync(~0u, off, r);
         copy16(dst + r * (D * 2) + ((c ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
@@ -217,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) tile_kernel(const __grid_constant__ 
     __syncwarp();
     issue(2 * i + 3);
     // scores in powers of two; a position that is not seen has none
-    const bool masked = seen != ~0u || at + kStep > all;
+    const bool masked = seen != ~0u >> (32 - kStep) || at + kStep > all;
     float mx[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < kStep / 8; ++n)
@@ -796,8 +807,8 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
   grid_dependency_wait();   // the end of this grid is the end of tile_kernel's, which it may have started under
 }
 
-// The sum over a row's slots; a warp per row.  Lanes read the statistics of 32 slots at once, and the partial results in groups of eight
-// independent loads.
+// The sum over a row's slots; a warp per row.  The statistics of 32 slots and the partial results of the first eight are asked for at once, before
+// it is known which of them were written: the kernel is a chain of latencies.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
   const int lane = threadIdx.x & 31;
@@ -808,46 +819,54 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   const int length = live ? own_length(p, b) : 0;   // (an input: nothing before this kernel writes it)
   grid_dependency_wait();
   if (!live) return;
-  // slots that were written: all of the prefix's, as many of the sequence's as it has positions for, and that of the last positions
-  const int span = p.own_wide_tiles ? common_length(p, length) : length, chunk = p.own_wide_tiles ? p.own_wide_chunk : p.own_chunk;
-  const int first = p.prefix_chunks + (span > 0 ? (span + chunk - 1) / chunk : 0);
-  const bool tail = p.own_wide_tiles && p.own_chunks && length > span;
-  const int used = first + (tail ? 1 : 0);
-  auto slot_of = [&](int i) { return i < first ? i : p.prefix_chunks + p.own_wide_chunks; };
-  const float2* stat = p.stat + id * p.slots;
-  const float* part = p.part + id * p.slots * D + lane * (D / 32);
   constexpr int N = D / 32;
+  const float2* stat = p.stat + id * p.slots;
+  const float* part = p.part + id * p.slots * D + lane * N;
+  float x[8][N];
+  auto fetch = [&](int from) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float* src = part + (int64_t)min(from + e, p.slots - 1) * D;
+      if constexpr (N == 4) { const float4 v = *(const float4*)src; x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w; }
+      else { const float2 v = *(const float2*)src; x[e][0] = v.x; x[e][1] = v.y; }
+    }
+  };
   float top = -INFINITY, sum = 0.f, acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  for (int i0 = 0; i0 < used; i0 += 32) {
-    const int i = i0 + lane, n = min(32, used - i0);
-    const float2 st = i < used ? stat[slot_of(i)] : make_float2(-INFINITY, 0.f);
-    float mx = fmaxf(top, st.x);
+  if (p.slots) {
+    float2 st = stat[min(lane, p.slots - 1)];
+    fetch(0);
+    // slots that were written: all of the prefix's, as many of the sequence's as it has positions for, and that of the last positions
+    const int span = p.own_wide_tiles ? common_length(p, length) : length, chunk = p.own_wide_tiles ? p.own_wide_chunk : p.own_chunk;
+    const int first = p.prefix_chunks + (span > 0 ? (span + chunk - 1) / chunk : 0);
+    const bool tail = p.own_wide_tiles && p.own_chunks && length > span;
+    const int last = p.prefix_chunks + p.own_wide_chunks, all = tail ? last + 1 : first;
+    for (int i0 = 0; i0 < all; i0 += 32) {
+      const int i = i0 + lane;
+      const bool written = i < first || (tail && i == last);
+      if (i0) st = stat[min(i, p.slots - 1)];
+      float mx = written ? fmaxf(top, st.x) : top;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-    const float base = mx == -INFINITY ? 0.f : mx, f = i < used ? exp2_fast(st.x - base) : 0.f, corr = exp2_fast(top - base);
-    top = mx;
-    float s = f * st.y;
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+      const float base = mx == -INFINITY ? 0.f : mx, f = written ? exp2_fast(st.x - base) : 0.f, corr = exp2_fast(top - base);
+      top = mx;
+      float s = written ? f * st.y : 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    sum = sum * corr + s;
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+      sum = sum * corr + s;
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] *= corr;
-    for (int m = 0; m < n; m += 8) {
-      float x[8][N];
+      for (int k = 0; k < N; ++k) acc[k] *= corr;
+      const uint32_t there = __ballot_sync(~0u, written);
+      for (int m = 0; m < min(32, all - i0); m += 8) {
+        if (i0 + m) fetch(i0 + m);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float* src = part + (int64_t)slot_of(i0 + min(m + e, n - 1)) * D;
-        if constexpr (N == 4) { const float4 v = *(const float4*)src; x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w; }
-        else { const float2 v = *(const float2*)src; x[e][0] = v.x; x[e][1] = v.y; }
-      }
+        for (int e = 0; e < 8; ++e) {
+          const float w = __shfl_sync(~0u, f, m + e);
+          if (there >> (m + e) & 1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = __shfl_sync(~0u, f, (m + e) & 31);
-        if (m + e < n) {
-#pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] += w * x[e][k];
+            for (int k = 0; k < N; ++k) acc[k] += w * x[e][k];
+          }
         }
       }
     }
@@ -867,9 +886,11 @@ Params plan(const PagedAttention& a) {
   p.prefix_tiles = (p.rows + kRows - 1) / kRows;
   p.own_tiles = (a.queries * p.group + kRows - 1) / kRows;
   const int64_t own_max = (int64_t)a.table_width * a.page_size;
+  // Chunks for tile_kernel: two and a half blocks for each of the 296 that run at once even out ragged lengths (16 sequences of up to 2500
+  // positions, 35 rows: 512 positions 34 us, 256 41, 2048 45; 128 sequences of up to 900: whole 55.9 us, 512 57.7).
   auto chunk_of = [&](int64_t positions, int64_t tiles) {
     int64_t chunk = 4096;
-    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < 2 * 148) chunk /= 2;
+    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < 5 * 148) chunk /= 2;
     return (int)chunk;
   };
   if (a.prefix_length && p.rows > kRows) {
@@ -889,7 +910,9 @@ Params plan(const PagedAttention& a) {
   }
   p.prefix_chunks = (a.prefix_length + p.prefix_chunk - 1) / p.prefix_chunk;
   const int64_t per = (int64_t)a.queries * p.group;
-  if (per > kRows && own_max > kWideStep) {
+  // (up to four tiles of 16 rows read the cache again from L2 in less time than the wide kernel's blocks need to begin and end: 35 rows as
+  // above 34 us and 47; 64 to 256 rows fill its tiles)
+  if (per > 4 * kRows && own_max > kWideStep) {
     p.own_wide_tiles = (int)((per + kWideRows - 1) / kWideRows);
     const int64_t all = (own_max + kWideStep - 1) / kWideStep, tiles = (int64_t)p.own_wide_tiles * a.batch * a.kv_heads;
     int64_t steps = 32;

@@ -186,6 +186,10 @@ SHAPES = [  # batch, queries, heads, kv heads, channels, page, prefix, own lengt
     (34, 1, 8, 1, 128, 24, 1500, [i % 7 for i in range(34)]),
     (70, 2, 4, 1, 128, 16, 129, [2 + i % 9 for i in range(70)]),
     (24, 1, 6, 1, 64, 100, 2049, [0] * 24),
+    (2, 9, 8, 1, 128, 24, 70, [400, 35]),
+    (3, 20, 8, 1, 64, 16, 0, [300, 20, 7]),
+    (1, 40, 8, 1, 128, 48, 200, [290]),
+    (2, 70, 4, 1, 128, 7, 5, [200, 66]),
 ]
 
 
