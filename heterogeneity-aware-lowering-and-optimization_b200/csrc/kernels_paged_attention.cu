@@ -30,6 +30,8 @@ struct Params {
   // its queries see (the last queries - 1 positions remain for tile_kernel, in the last slot).  0: tile_kernel takes them all.
   int wide_tiles, own_wide_tiles, own_wide_chunks, own_wide_chunk;
   float scale_log2e;
+  int join_warps;                    // 4 or 1: warps that share a row's slots
+  int wide_first;                    // no tile_kernel in front
   int box_shift;                     // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
   uint32_t spin_limit;
   int test_skip_stage;               // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
@@ -107,6 +109,8 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kPieces = D / 8, kUnit = kStep * D * 2;   // 16-byte pieces of a row; bytes of a unit
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+  // The kernel in front may still be writing the cache; the wide kernel may start once every block here knows that it is not.
+  grid_dependency_wait();
   launch_dependents();
   // what this block works on
   int item = blockIdx.x;
@@ -447,6 +451,7 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
   constexpr uint32_t kUnit = kBoxes * kBox;
   const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem, s_ring = smem + 2 * kUnit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y;
+  if (p.wide_first) grid_dependency_wait();
   launch_dependents();
   int row0, n_rows, begin, end, slot;
   const int* pages;
@@ -807,26 +812,29 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
   grid_dependency_wait();   // the end of this grid is the end of tile_kernel's, which it may have started under
 }
 
-// The sum over a row's slots; a warp per row.  The statistics of 32 slots and the partial results of the first eight are asked for at once, before
-// it is known which of them were written: the kernel is a chain of latencies.
+// The sum over a row's slots, by a warp or, for more than eight slots, by the four of a block.  Statistics and partial results are asked for at
+// once, before it is known which slots were written: the kernel is a chain of latencies.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);   // head * rows + row
+  constexpr int N = D / 32;
+  __shared__ float shared_acc[kWarps][D];
+  __shared__ float2 shared_stat[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = p.join_warps, part_of = share == 1 ? 0 : warp;
+  const int64_t id = share == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x;   // head * rows + row
   const bool live = id < (int64_t)p.rows * p.a.kv_heads;
   const int head = live ? (int)(id / p.rows) : 0, row = live ? (int)(id - (int64_t)head * p.rows) : 0;
   const int g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
-  const int length = live ? own_length(p, b) : 0;   // (an input: nothing before this kernel writes it)
   grid_dependency_wait();
-  if (!live) return;
-  constexpr int N = D / 32;
+  if (!live) return;   // (whole blocks where a block shares a row)
+  const int length = own_length(p, b);
+  // slots part_of, part_of + share, ...
   const float2* stat = p.stat + id * p.slots;
   const float* part = p.part + id * p.slots * D + lane * N;
   float x[8][N];
   auto fetch = [&](int from) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float* src = part + (int64_t)min(from + e, p.slots - 1) * D;
+      const float* src = part + (int64_t)min((from + e) * share + part_of, p.slots - 1) * D;
       if constexpr (N == 4) { const float4 v = *(const float4*)src; x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w; }
       else { const float2 v = *(const float2*)src; x[e][0] = v.x; x[e][1] = v.y; }
     }
@@ -835,15 +843,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
   if (p.slots) {
-    float2 st = stat[min(lane, p.slots - 1)];
+    float2 st = stat[min(lane * share + part_of, p.slots - 1)];
     fetch(0);
     // slots that were written: all of the prefix's, as many of the sequence's as it has positions for, and that of the last positions
     const int span = p.own_wide_tiles ? common_length(p, length) : length, chunk = p.own_wide_tiles ? p.own_wide_chunk : p.own_chunk;
     const int first = p.prefix_chunks + (span > 0 ? (span + chunk - 1) / chunk : 0);
     const bool tail = p.own_wide_tiles && p.own_chunks && length > span;
-    const int last = p.prefix_chunks + p.own_wide_chunks, all = tail ? last + 1 : first;
+    const int last = p.prefix_chunks + p.own_wide_chunks, all = ((tail ? last + 1 : first) + share - 1) / share;
     for (int i0 = 0; i0 < all; i0 += 32) {
-      const int i = i0 + lane;
+      const int i = (i0 + lane) * share + part_of;
       const bool written = i < first || (tail && i == last);
       if (i0) st = stat[min(i, p.slots - 1)];
       float mx = written ? fmaxf(top, st.x) : top;
@@ -869,6 +877,28 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
           }
         }
       }
+    }
+  }
+  if (share > 1) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) shared_acc[warp][lane * N + k] = acc[k];
+    if (lane == 0) shared_stat[warp] = make_float2(top, sum);
+    __syncthreads();
+    if (warp) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, shared_stat[w].x);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 st = shared_stat[w];
+      const float f = exp2_fast(st.x - base);
+      sum += f * st.y;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += f * shared_acc[w][lane * N + k];
     }
   }
   T* y = (T*)p.y + b * p.a.y_batch + j * p.a.y_token + (int64_t)(head * p.group + g) * p.a.y_head + lane * N;
@@ -926,10 +956,11 @@ Params plan(const PagedAttention& a) {
     p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
   }
   p.slots = p.prefix_chunks + p.own_wide_chunks + p.own_chunks;
+  p.join_warps = p.slots > 8 ? kWarps : 1;
   return p;
 }
 
-template <typename F, typename... Args> bool start(F* fn, dim3 grid, int threads, size_t smem, bool overlap, cudaStream_t stream, const Args&... args) {
+template <typename F, typename... Args> bool start(F* fn, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
   if (smem > 48 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return false; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -940,7 +971,7 @@ template <typename F, typename... Args> bool start(F* fn, dim3 grid, int threads
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = overlap ? 1 : 0;
+  cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, fn, args...) == cudaSuccess) return true;
   cudaGetLastError();
   return false;
@@ -959,8 +990,9 @@ bool box_map(CUtensorMap* m, const Params& p, const void* base, int positions) {
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Up to three launches: tiles of 16 rows, wide tiles, the sum.  The wide kernel starts while the last blocks of the first still run (neither
-// reads what the other writes) and ends no earlier; the sum waits for the kernel in front of it.
+// Up to three launches: tiles of 16 rows, wide tiles, the sum.  All may start while the kernel in front still runs, and wait where they need its
+// results: the first at its start; the wide kernel, which reads nothing that the first writes, only before it ends (a grid that waited has
+// ended after all in front of it); the sum at its start.
 template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
   const int64_t wide_items = (int64_t)p.wide_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_wide_tiles * p.own_wide_chunks;
@@ -968,17 +1000,18 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
   constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
   const unsigned heads = (unsigned)p.a.kv_heads;
-  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, false, stream, p)) return -2;
+  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, stream, p)) return -2;
   if (wide_items) {
+    p.wide_first = items == 0;
     CUtensorMap keys{}, values{};
     p.box_shift = 0;
     int shift = 0;
     while (shift < 7 && p.a.page_size % (2 << shift) == 0) ++shift;
     if (shift >= 3 && box_map(&keys, p, p.k, 1 << shift) && box_map(&values, p, p.v, 1 << shift)) p.box_shift = shift;
-    if (!start(wide_kernel<T, D>, dim3((unsigned)wide_items, heads), kWideThreads, wide, items > 0, stream, p, keys, values)) return -2;
+    if (!start(wide_kernel<T, D>, dim3((unsigned)wide_items, heads), kWideThreads, wide, stream, p, keys, values)) return -2;
   }
   const int64_t ids = (int64_t)p.rows * p.a.kv_heads;
-  return start(join_kernel<T, D>, dim3((unsigned)((ids + kWarps - 1) / kWarps)), kThreads, 0, items + wide_items > 0, stream, p) ? 0 : -2;
+  return start(join_kernel<T, D>, dim3((unsigned)(p.join_warps == 1 ? (ids + kWarps - 1) / kWarps : ids)), kThreads, 0, stream, p) ? 0 : -2;
 }
 
 }  // namespace

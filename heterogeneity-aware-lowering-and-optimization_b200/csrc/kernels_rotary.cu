@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(VEC == 1 ? 2 * kThreads : kThreads, VEC == 1 ?
     if (w.second) store<T, VEC>(w.dst + w.at + w.step, w.x[1]);
   };
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // (launched while the kernel in front may still be writing what this one reads)
   Row now;
   fetch(now);
   if (g.pairs > 0) {
@@ -174,8 +175,19 @@ template <typename T> int launch(const TurnGeom& g, cudaStream_t stream) {
   const int64_t blocks = (total + block_tokens - 1) / block_tokens;
   const size_t smem = 2 * sizeof(float) * (size_t)block_tokens * (size_t)g.pairs;
   auto* fn = wide ? (g.interleaved ? turn_kernel<T, VEC, true> : turn_kernel<T, VEC, false>) : (g.interleaved ? turn_kernel<T, 1, true> : turn_kernel<T, 1, false>);
-  fn<<<(unsigned)blocks, threads, smem, stream>>>(g, block_tokens, per_row);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, g, block_tokens, per_row) == cudaSuccess) return 0;
+  cudaGetLastError();
+  return -2;
 }
 
 }  // namespace

@@ -887,6 +887,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict
   const T* src = logits + (int64_t)row * row_stride + base;
   T* mine = keep ? (T*)(dynamic + sizeof(Shared)) : (T*)src;
   const int here = max(0, min(slice, vocab - base));
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // (launched while the kernel in front may still be writing the logits)
   float group[P::kGroups], top = -INFINITY;
   if (!vec) {   // (then the slice goes to shared memory)
     for (int i = tid; i < slice; i += kThreads) mine[i] = i < here ? src[i] : L::dead();
@@ -991,12 +992,14 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, (const T*)logits, row, vocab, slice, vec, keep, powers, temperature, top_k, top_p, min_p, uniform, tokens);
   if (e != cudaSuccess) { cudaGetLastError(); return -2; }
   return 0;
