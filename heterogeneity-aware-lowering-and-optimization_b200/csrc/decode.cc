@@ -129,7 +129,7 @@ extern "C" int odla_b200_paged_attention(const odla_b200_paged_cache* c, const v
   if (!key_cache || !value_cache || !q || !y || !lengths || (d->prefix_length && !prefix_pages) || (d->table_width && !page_table)) return -1;
   if (!aligned16({key_cache, value_cache, q, y, workspace}) || (uintptr_t)prefix_pages % 4 || (uintptr_t)page_table % 4 || (uintptr_t)lengths % 4) return -1;
   const long long need = paged_attention_workspace(a);
-  if (workspace_bytes < need || (need && !workspace)) return -1;
+  if (need < 0 || workspace_bytes < need || (need && !workspace)) return -1;
   if (!have_device("odla_b200_paged_attention")) return -2;
   return paged_attention(a, key_cache, value_cache, q, prefix_pages, page_table, lengths, y, workspace, (cudaStream_t)stream);
 }

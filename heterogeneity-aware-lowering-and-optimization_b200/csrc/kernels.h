@@ -295,7 +295,7 @@ struct PagedAttention {
   float scale;
   int64_t c_page, c_head, c_token, q_batch, q_token, q_head, y_batch, y_token, y_head;
 };
-int64_t paged_attention_workspace(const PagedAttention& a);
+int64_t paged_attention_workspace(const PagedAttention& a);   // bytes, -1: too many blocks
 int paged_attention(const PagedAttention& a, const void* key_cache, const void* value_cache, const void* q, const int* prefix_pages, const int* page_table,
                     const int* lengths, void* y, void* workspace, cudaStream_t stream);
 

@@ -812,7 +812,7 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
   grid_dependency_wait();   // the end of this grid is the end of tile_kernel's, which it may have started under
 }
 
-// The sum over a row's slots, by a warp or, for more than eight slots, by the four of a block.  Statistics and partial results are asked for at
+// The sum over a row's slots, by a warp or, for more than sixteen slots, by the four of a block.  Statistics and partial results are asked for at
 // once, before it is known which slots were written: the kernel is a chain of latencies.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
@@ -956,9 +956,12 @@ Params plan(const PagedAttention& a) {
     p.own_chunks = (int)((own_max + p.own_chunk - 1) / p.own_chunk);
   }
   p.slots = p.prefix_chunks + p.own_wide_chunks + p.own_chunks;
-  p.join_warps = p.slots > 8 ? kWarps : 1;
+  p.join_warps = p.slots > 16 ? kWarps : 1;   // (10 slots of 4096 rows: one warp 118 us for the whole call, four 124.6)
   return p;
 }
+
+int64_t tile_items(const Params& p) { return (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks; }
+int64_t wide_tile_items(const Params& p) { return (int64_t)p.wide_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_wide_tiles * p.own_wide_chunks; }
 
 template <typename F, typename... Args> bool start(F* fn, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
   if (smem > 48 * 1024 && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return false; }
@@ -994,9 +997,7 @@ bool box_map(CUtensorMap* m, const Params& p, const void* base, int positions) {
 // results: the first at its start; the wide kernel, which reads nothing that the first writes, only before it ends (a grid that waited has
 // ended after all in front of it); the sum at its start.
 template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
-  const int64_t items = (int64_t)p.prefix_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_tiles * p.own_chunks;
-  const int64_t wide_items = (int64_t)p.wide_tiles * p.prefix_chunks + (int64_t)p.a.batch * p.own_wide_tiles * p.own_wide_chunks;
-  if (items >= (1ll << 31) || wide_items >= (1ll << 31)) return -1;
+  const int64_t items = tile_items(p), wide_items = wide_tile_items(p);
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
   constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
   const unsigned heads = (unsigned)p.a.kv_heads;
@@ -1019,6 +1020,7 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
 int64_t paged_attention_workspace(const PagedAttention& a) {
   if (a.batch == 0) return 0;
   const Params p = plan(a);
+  if (tile_items(p) >= (1ll << 31) || wide_tile_items(p) >= (1ll << 31)) return -1;   // more blocks than a grid has
   return (int64_t)p.rows * a.kv_heads * p.slots * ((int64_t)a.channels * 4 + 8);
 }
 

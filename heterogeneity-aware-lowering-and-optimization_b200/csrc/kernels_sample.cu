@@ -323,6 +323,9 @@ template <typename T, int RANKS> struct Part {
       const double target = (double)r.uniform * (double)sum_taken;
       if (!((double)before > target) && (double)(before + taken) > target)
         for (int k = 0; k < RANKS; ++k) { Shared* o = peer(k); o->owner = tid; o->before = before; o->target = target; }
+      __syncthreads();
+      if (tid == 0 && s.owner < 0) s.ok = 0;
+      __syncthreads();
       if (tid && tid < RANKS) { Shared* o = peer(tid); o->cut_entry = s.cut_entry; o->ok = s.ok; }
     }
     sync_row();

@@ -378,3 +378,172 @@ def test_sample_leaves_the_rest_and_strides(odla, gpu_lib):
     assert (out[:2] == -3).all() and (out[6:] == -3).all() and (out[2:6] >= 0).all()
     same = R.call_sample(odla, gpu_lib, logits[:1].expand(4, 700), None, None, None, None, u, 0, row=0)
     assert (same.cpu().numpy() == R.sample(logits[:1].expand(4, 700).double().cpu().numpy(), None, None, None, None, u.cpu().numpy())).all()
+
+
+# ------------------------------------------------------------ far offsets, replays ----
+def test_offsets_beyond_32_bits(odla, gpu_lib):
+    """Pages, tokens and rows more than 2^32 elements apart (16 GB of which a few rows are touched)."""
+    g = gen(64)
+    far = (1 << 32) + 64
+    big = torch.empty(2 * far + 4096, dtype=torch.float16, device="cuda")
+    kc = torch.as_strided(big, (2, 1, 16, 64), (far, 1024, 64, 1))
+    vc = torch.as_strided(big, (2, 1, 16, 64), (far, 1024, 64, 1), 2048)
+    kc.copy_(randn(g, (2, 1, 16, 64), 1)), vc.copy_(randn(g, (2, 1, 16, 64), 1))
+    # append to the far page
+    row = randn(g, (2, 3, 64), 1)
+    slots = torch.tensor([16 + 15, 16 + 14], device="cuda")
+    pos = torch.tensor([[3, 4]], dtype=torch.int32, device="cuda")
+    f = freqs(32)
+    spec, cache = odla.rotary_spec(f), R.cache_of(odla, kc, 1)
+    out = torch.empty((2, 1, 64), dtype=torch.float16, device="cuda")
+    d = odla.AppendDesc(tokens=2, heads=1, q_token=192, q_head=64, k_token=192, k_head=64, v_token=192, v_head=64, y_token=64, y_head=64)
+    assert gpu_lib.b200_paged_append(C.byref(cache), kc.data_ptr(), vc.data_ptr(), C.byref(d), C.byref(spec), row.data_ptr(), row.data_ptr() + 128, row.data_ptr() + 256, out.data_ptr(),
+                                     pos.data_ptr(), slots.data_ptr(), R.stream()) == 0
+    want, size = R.turned(row, pos, f, [0] * 32, False)
+    R.close(kc[1, 0, [15, 14]], want[:, 1], R.turn_tolerance(want, size, 1)[:, 1])
+    assert torch.equal(vc[1, 0, [15, 14]], row[:, 2])
+    # attention over both pages, by small tiles and by wide ones
+    for batch in (1, 20):
+        q = randn(g, (batch, 1, 1, 64), 1)
+        table = torch.tensor([[1, 0]] * batch, dtype=torch.int32, device="cuda")
+        pages = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+        check_attention(odla, gpu_lib, (q, kc, vc, pages, table, torch.full((batch,), 20, dtype=torch.int32, device="cuda")), 32)
+    # rotary and sampling from rows far apart
+    x = torch.as_strided(big, (1, 2, 1, 64), (0, far, 64, 1), 8192 - 4096)
+    x.copy_(randn(g, (1, 2, 1, 64), 1))
+    y = torch.empty((1, 2, 1, 64), dtype=torch.float16, device="cuda")
+    p = torch.tensor([[[5, 6]]], dtype=torch.int32, device="cuda")
+    rd = odla.RotaryDesc(dtype=1, batch=1, tokens=2, heads=1, channels=64, x_batch=0, x_token=far, x_head=64, y_batch=0, y_token=64, y_head=64)
+    assert gpu_lib.b200_rotary(C.byref(spec), C.byref(rd), x.data_ptr(), y.data_ptr(), p.data_ptr(), R.stream()) == 0
+    want, size = R.turned(x, p, f, [0] * 32, False)
+    R.close(y, want, R.turn_tolerance(want, size, 1))
+    logits = torch.as_strided(big, (2, 1000), (far, 1))
+    logits.copy_(randn(g, (2, 1000), 1))
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    check_sample(odla, gpu_lib, logits, (None, None, None, None), u, 1)
+
+
+def captured(call):
+    """`call` as a graph on a stream of its own."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    return graph
+
+
+def test_captured_rotary_append_and_sample_follow_their_inputs(odla, gpu_lib):
+    g = gen(65)
+    x, y = randn(g, (1, 9, 4, 64), 2), torch.empty((1, 9, 4, 64), dtype=torch.bfloat16, device="cuda")
+    pos = torch.arange(9, dtype=torch.int32, device="cuda").view(1, 1, 9)
+    f = freqs(32)
+    spec = odla.rotary_spec(f)
+    rd = odla.RotaryDesc(dtype=2, batch=1, tokens=9, heads=4, channels=64, x_batch=2304, x_token=256, x_head=64, y_batch=2304, y_token=256, y_head=64)
+    kc, vc = (torch.zeros((4, 2, 8, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = R.cache_of(odla, kc, 2)
+    ad = odla.AppendDesc(tokens=9, heads=0, k_token=256, k_head=64, v_token=256, v_head=64)
+    slots = torch.arange(9, device="cuda")
+    logits, u = randn(g, (5, 3000), 2), torch.rand(5, generator=g, device="cuda")
+    k = torch.full((5,), 40, dtype=torch.int32, device="cuda")
+    tokens = torch.empty(5, dtype=torch.int32, device="cuda")
+
+    def calls():
+        assert gpu_lib.b200_rotary(C.byref(spec), C.byref(rd), x.data_ptr(), y.data_ptr(), pos.data_ptr(), R.stream()) == 0
+        assert gpu_lib.b200_paged_append(C.byref(cache), kc.data_ptr(), vc.data_ptr(), C.byref(ad), None, None, y.data_ptr(), y.data_ptr() + 256, None, None, slots.data_ptr(),
+                                         R.stream()) == 0
+        R.call_sample(odla, gpu_lib, logits, None, k, None, None, u, 2, tokens=tokens)
+    calls()
+    graph = captured(calls)
+    spec.frequency[0] = 77.0                 # descriptors are read during the call, not when the graph runs
+    rd.tokens, ad.tokens = 1, 0
+    for i in range(3):
+        x.copy_(randn(g, tuple(x.shape), 2)), pos.add_(1000), slots.add_(3), logits.copy_(randn(g, (5, 3000), 2)), u.copy_(torch.rand(5, generator=g, device="cuda"))
+        graph.replay()
+        want, size = R.turned(x, pos, f, [0] * 32, False)
+        R.close(y, want, R.turn_tolerance(want, size, 2))
+        at = slots.tolist()
+        assert torch.equal(kc.transpose(1, 2).reshape(32, 2, 64)[at], y[0, :, :2]) and torch.equal(vc.transpose(1, 2).reshape(32, 2, 64)[at], y[0, :, 2:])
+        assert (tokens.cpu().numpy() == R.sample(logits.double().cpu().numpy(), None, k.cpu().numpy(), None, None, u.cpu().numpy())).all()
+
+
+def test_calls_on_two_streams_at_once(odla, gpu_lib):
+    cases = [attention_case(2, 24, 1, 8, 2, 128, 16, 500 + 100 * i, [80] * 24, seed=i) for i in range(2)]
+    logits = [3 * randn(gen(70 + i), (30, 20000), 0) for i in range(2)]
+    us = [torch.rand(30, generator=gen(80 + i), device="cuda") for i in range(2)]
+    alone = [R.call_attention(odla, gpu_lib, *c[:4], 500 + 100 * i, *c[4:], 0.088) for i, c in enumerate(cases)]
+    tokens = [R.call_sample(odla, gpu_lib, l, None, None, None, None, u, 0) for l, u in zip(logits, us)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((R.call_attention(odla, gpu_lib, *cases[i][:4], 500 + 100 * i, *cases[i][4:], 0.088),
+                               R.call_sample(odla, gpu_lib, logits[i], None, None, None, None, us[i], 0)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y, t in got[i]:
+            assert torch.equal(y, alone[i]) and torch.equal(t, tokens[i])
+
+
+# --------------------------------------------------------------------- a whole step ----
+def test_a_decoding_loop_next_to_planned_graphs(odla, gpu_lib):
+    """What a program does for each new token: the projection as a planned graph, append, attention, the output layer as a planned
+    graph, sampling.  Every stage against its 64-bit form on what it was given; three sequences behind one prompt, one slot of the batch unused."""
+    g = gen(90)
+    B, H, KH, D, V, PS, P, steps = 4, 4, 2, 64, 700, 8, 21, 6
+    hidden, width = H * D, (H + 2 * KH) * D
+    rng = np.random.default_rng(3)
+    w_in, w_out = ((rng.standard_normal((hidden, n)) / np.sqrt(hidden)).astype(np.float32) for n in (width, V))
+    table_emb = randn(g, (V, hidden), 1)
+    project, answer = odla.Graph(gpu_lib, "project", fp16=True, n_gpus=1), None
+    project.Output(project.Gemm(project.Argument("x", (B, hidden), odla.FLOAT16), False, project.Constant("w", w_in), False, 1.0, 0.0, None, (B, width), "qkv"))
+    project.context()
+    answer = odla.Graph(gpu_lib, "answer", fp16=True, n_gpus=1)
+    answer.Output(answer.Gemm(answer.Argument("c", (B, hidden), odla.FLOAT16), False, answer.Constant("w", w_out), False, 1.0, 0.0, None, (B, V), "logits"))
+    answer.context()
+    pages = 16
+    kc, vc = (randn(g, (pages, KH, PS, D), 1) for _ in range(2))
+    prefix_pages = torch.tensor([5, 2, 9], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0], [1], [3], [-1]], dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
+    x = randn(g, (B, hidden), 1)
+    qkv, turned, ctx = (torch.empty((B, n), dtype=torch.float16, device="cuda") for n in (width, hidden, hidden))
+    logits, tokens = torch.empty((B, V), dtype=torch.float16, device="cuda"), torch.empty(B, dtype=torch.int32, device="cuda")
+    f = freqs(D // 2)
+    spec, cache = odla.rotary_spec(f), R.cache_of(odla, kc, 1)
+    ad = odla.AppendDesc(tokens=B, heads=H, q_token=width, q_head=D, k_token=width, k_head=D, v_token=width, v_head=D, y_token=hidden, y_head=D)
+    for step in range(steps):
+        torch.cuda.synchronize()
+        project.bind_input("x", x.data_ptr()), project.bind_output("qkv", qkv.data_ptr())
+        assert project.execute() == odla.SUCCESS
+        want = x.double() @ torch.tensor(w_in, device="cuda").half().double()
+        # 256 products summed in fp32, rounded once
+        bound = x.double().abs() @ torch.tensor(w_in, device="cuda").half().double().abs()
+        R.close(qkv, want, bound * 260 * 2.0 ** -24 + want.abs() * 2.0 ** -11 + 2.0 ** -25, "projection")
+        positions = torch.full((1, B), P + step, dtype=torch.int32, device="cuda")
+        slots = torch.where(table[:, 0] >= 0, table[:, 0].long() * PS + step, -1)
+        lengths.copy_(torch.where(table[:, 0] >= 0, step + 1, 0))
+        es = 2 * D
+        assert gpu_lib.b200_paged_append(C.byref(cache), kc.data_ptr(), vc.data_ptr(), C.byref(ad), C.byref(spec), qkv.data_ptr(), qkv.data_ptr() + H * es, qkv.data_ptr() + (H + KH) * es,
+                                         turned.data_ptr(), positions.data_ptr(), slots.data_ptr(), R.stream()) == 0
+        rows, size = R.turned(qkv.view(B, H + 2 * KH, D), positions, f, [0] * (D // 2), False)
+        tol = R.turn_tolerance(rows, size, 1)
+        R.close(turned.view(B, H, D), rows[:, :H], tol[:, :H], "queries")
+        for b in range(3):
+            R.close(kc[int(table[b, 0]), :, step], rows[b, H:H + KH], tol[b, H:H + KH], "keys")
+            assert torch.equal(vc[int(table[b, 0]), :, step], qkv.view(B, -1, D)[b, H + KH:])
+        y = R.call_attention(odla, gpu_lib, turned.view(B, 1, H, D), kc, vc, prefix_pages, P, table, lengths, 0.125, y=ctx.view(B, 1, H, D))
+        want, tol = R.attention(turned.view(B, 1, H, D).cpu(), kc.cpu(), vc.cpu(), prefix_pages.cpu(), P, table.cpu(), lengths.cpu(), 0.125)
+        R.close(y, want, tol, "attention")
+        torch.cuda.synchronize()
+        answer.bind_input("c", ctx.data_ptr()), answer.bind_output("logits", logits.data_ptr())
+        assert answer.execute() == odla.SUCCESS
+        T, k, p = torch.tensor([0.7, 1.0, 0.0, 1.0], device="cuda"), torch.tensor([0, 30, 0, 0], dtype=torch.int32, device="cuda"), torch.tensor([0.9, 1.0, 1.0, 0.5], device="cuda")
+        u = torch.rand(B, generator=g, device="cuda")
+        R.call_sample(odla, gpu_lib, logits, T, k, p, None, u, 1, tokens=tokens)
+        assert (tokens.cpu().numpy() == R.sample(logits.double().cpu().numpy(), T.cpu().numpy(), k.cpu().numpy(), p.cpu().numpy(), None, u.cpu().numpy())).all()
+        x.copy_(table_emb[tokens.long()])
+    project.close()
+    answer.close()
