@@ -15,8 +15,8 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
 constexpr int kBins = 2048, kList = 1536, kTopK = 1024, kBucket = 128, kFew = kThreads / 4;
 constexpr int kSlice = 64 * kThreads;   // logits of a CTA at most: a thread names its own by the bits of one word
-constexpr float kNoUnits = 1000.f;   // weights from here on, below 2^-45, are no units
-constexpr float kBinsPerE = 32.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-92, which are no units
+constexpr float kNoUnits = 2000.f;   // weights from here on, below 2^-45, are no units
+constexpr float kBinsPerE = 64.f;   // bins per factor e of the weight: bin 2047 holds weights below 2^-46, which are no units
 
 // Logits as keys that compare like them: whole numbers, larger for larger logits, 0 for those that are never chosen (NaN, -inf).
 // -0 becomes +0: equal logits must have equal keys.
@@ -200,16 +200,18 @@ template <typename T, int RANKS> struct Part {
   __device__ __forceinline__ T logit(int i) const { return i < limit ? logits[i] : L::dead(); }
   __device__ __forceinline__ double weight(float v) const { return exp_below<false>((double)v - (double)top, scale, s); }
 
-  // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/32): one histogram over 2048 of them finds
+  // What nearly every row takes.  A bin is a range of logits whose weights differ by a factor of e^(1/64): one histogram over 2048 of them finds
   // the bin of the last kept token.
   //   top-k up to 1024: a histogram of the largest logits of small groups, kept in registers (the k-th largest of those has at least k tokens above it, and rarely
   //   many more; of every logit where that did not hold, or the row is short).  All tokens down to that bin go to a list of the first CTA,
   //   which sorts it and does the rest alone.
-  //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 1e-4), for top-p; then every CTA sums exact weights,
+  //   otherwise: a histogram of masses, 32-bit and relative to the bin's middle (good to 2^-16 each), for top-p; then every CTA sums exact weights,
   //   over all tokens, over those in higher bins, and of the latter, warp by warp, over those that min-p keeps; tokens in the bin itself
   //   go to the list.  The first CTA sorts it, finds the last token kept, and which warp's stretch of the row the choice lies in; that
   //   stretch's CTA finds it there.
-  // The histogram of masses only proposes the bin: the exact sums have to confirm it.  Returns false, with nothing written, where that fails,
+  // The histogram of masses only proposes the bin: the exact sums have to confirm it.  Returns false, with nothing written, where that fails
+  // (a mark so near the edge of a bin that the proposal fell on the wrong side: one of 5000 rows with top-p, and the call then takes 140 us longer at
+  // 128000 tokens; listing the neighbour, too, where the mark is near an edge cost every call 1 %),
   // the list is full (many equal logits), or a parameter is out of this way's range (top-k above 1024, uniform outside (0, 1),
   // temperature, infinities).  All CTAs of a cluster take the same branches.
   __device__ __forceinline__ bool direct() {
@@ -228,9 +230,12 @@ template <typename T, int RANKS> struct Part {
         bin = find_bin(by_count, groups, per_unit, by_count ? (double)r.top_k : (double)r.top_p);
         // fewer than k tokens outside the last bin; a mark that rounding put between two bins; weights of no units
         if (bin < 0 || (!by_count && bin == kBins - 1)) {
-          if (!groups) return false;
-          groups = false;
-          continue;
+          if (!by_count) return false;
+          if (groups) {
+            groups = false;
+            continue;
+          }
+          bin = kBins - 2;   // all there are: what lies in the last bin has no units
         }
       }
       unsigned long long named = 0;
@@ -280,7 +285,7 @@ template <typename T, int RANKS> struct Part {
       if (n) {
         sort(n, by_count, per_unit);
         // exact weights of the list, largest first, kMine entries per thread; those kept are the first ones
-        const int count = by_count ? r.top_k : n;
+        const int count = by_count ? min(r.top_k, n) : n;
         unsigned long long unit[kMine], sum = 0, total;
         double w[kMine];
 #pragma unroll
@@ -387,8 +392,10 @@ template <typename T, int RANKS> struct Part {
         for (int j = 0; j < Piece<T>::N; ++j) {
           const float at = place(L::widen(x.e[j]), per_unit);
           const int b = bin_of(at);
-          // 2^16 (1 - (at - b) / 32) for 2^16 e^(-(at - b) / 32), |at - b| <= 1/2: at most 1.2e-4 off, and alike in all bins
-          const uint32_t add = count ? 1u : __float_as_uint(fmaf(((at + 8388608.f) - 8388608.f) - at, 65536.f / kBinsPerE, 65536.f + 8388608.f)) & 0x7fffffu;
+          // 2^16 e^(-(at - b) / 64), |at - b| <= 1/2, to 8e-8 and a whole number.
+          const float d = ((at + 8388608.f) - 8388608.f) - at;
+          constexpr float c = 1.f / kBinsPerE;
+          const uint32_t add = count ? 1u : __float_as_uint(fmaf(fmaf(d, 32768.f * c * c, 65536.f * c), d, 65536.f + 8388608.f)) & 0x7fffffu;
           if (b < kBins - 1) atomicAdd(&s.hist[b], add);
         }
       }
@@ -630,7 +637,7 @@ template <typename T, int RANKS> struct Part {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float v = fmaxf(L::widen(x.e[j0 + j]), floor);
-              b[j] = (int)__float_as_uint((top - v) * per_unit + 8388608.f) - 0x4b000000;
+              b[j] = (int)__float_as_uint(__fmul_rn(top - v, per_unit) + 8388608.f) - 0x4b000000;   // (two roundings, as in the histogram)
               w[j] = exp_below<true>((double)v - (double)top, scale, s);
             }
 #pragma unroll
@@ -874,8 +881,8 @@ template <typename T, int RANKS> struct Part {
 };
 
 // One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps in shared memory; where they do not fit
-// (`keep` is 0) the passes after the first read them from the caller's memory again, mostly from L2.  CTAs are few and large: what a row costs beside
-// its loads and weights is a chain of barriers, and a cluster's barrier costs several times a block's.
+// (`keep` is 0) the passes after the first read them from the caller's memory again, mostly from L2.  Two CTAs share an SM, so that one
+// computes while the other waits: what a row costs beside its loads and weights is a chain of barriers.
 template <typename T, int RANKS>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
                                                           const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
@@ -885,6 +892,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict
   Shared& s = *(Shared*)dynamic;
   constexpr int N = Piece<T>::N;
   cg::cluster_group cluster = cg::this_cluster();
+  if (RANKS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (its other half stands before the first access to a peer's memory)
   auto peer = [&](int k) { return RANKS == 1 ? &s : cluster.map_shared_rank(&s, k); };
   const int rank = RANKS == 1 ? 0 : (int)cluster.block_rank(), row = blockIdx.x / RANKS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, base = rank * slice;
   const T* src = logits + (int64_t)row * row_stride + base;
@@ -927,6 +935,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
   if (lane == 0) s.warp_top[warp] = top;
   if (tid == 0) s.token = INT_MAX;
+  if (RANKS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // all CTAs of the cluster have begun
   __syncthreads();
   if (tid < RANKS) {
 #pragma unroll
@@ -958,14 +967,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict
   P part{s, cluster, mine, r, top, {}, 0.0, vocab, slice, keep ? slice : here, base, rank, row, tokens};
 #pragma unroll
   for (int g = 0; g < P::kGroups; ++g) part.group[g] = group[g];
-  {
-    // 1 / temperature: the reciprocal in 32 bits and two steps of Newton's, each of which doubles its bits (a division takes several times as long)
-    const double t = (double)r.temperature;
-    double q = (double)__frcp_rn(r.temperature);
-    q = fma(fma(-t, q, 1.0), q, q);
-    q = fma(fma(-t, q, 1.0), q, q);
-    part.scale = 46.166241308446828384 * (r.temperature > 1e-4f && r.temperature < 1e4f ? q : 1.0 / t);   // 32 / ln 2
-  }
+  part.scale = 46.166241308446828384 / (double)r.temperature;   // 32 / ln 2
   if (part.direct()) return;
   P copy = part;   // (general() takes its address, which would put the registers of the other way in memory, too: 5000 clocks a row)
   copy.general();

@@ -369,6 +369,31 @@ def test_sample_masks_infinities_and_nan(odla, gpu_lib, dtype, vocab):
         check_sample(odla, gpu_lib, x, tuple(torch.full((14,), v, device="cuda", dtype=torch.int32 if i == 1 else torch.float32) for i, v in enumerate((T, k, p, m))), u, dtype)
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_sample_masks_that_leave_parts_of_a_row(odla, gpu_lib, dtype):
+    """Whole stretches of a long row allow nothing, or less than k; the largest logits lie all in one place, or in order."""
+    g = gen(77, dtype)
+    rows, vocab = 40, 90000
+    x = 2 * torch.randn((rows, vocab), generator=g, device="cuda")
+    inf = float("inf")
+    x[0:4, 20000:] = -inf
+    x[4:8, :85000] = -inf
+    x[8:12, 17:] = -inf
+    x[12:16] = x[12:16].sort(dim=-1, descending=True).values
+    x[16:20] = x[16:20].sort(dim=-1).values
+    x[20:24, 30000:30500] += 30
+    x[24:28, ::3] = float("nan")
+    x[28:32] = -inf
+    x[28:30, 89999] = 1.0
+    x[32:34, 70000] = inf
+    x[34:36, 5] = torch.finfo(R.TORCH[dtype]).min
+    x[36:38] = x[36:38].round()
+    u = torch.rand(rows, generator=g, device="cuda")
+    x = x.to(R.TORCH[dtype])
+    for k, p in ((3, 1.0), (40, 0.9), (300, 0.99), (1000, 0.5), (0, 0.8)):
+        check_sample(odla, gpu_lib, x, (torch.full((rows,), 0.9, device="cuda"), torch.full((rows,), k, dtype=torch.int32, device="cuda"), torch.full((rows,), p, device="cuda"), None), u, dtype)
+
+
 def test_sample_leaves_the_rest_and_strides(odla, gpu_lib):
     g = gen(8)
     logits = torch.randn((4, 700), generator=g, device="cuda")
