@@ -415,12 +415,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 // 2^x for two x <= 8 on the multiply-add pipes, for a quarter of all exponentials (256 rows behind 32768 positions: 92 -> 88.5 us; half of them: 94):
 // x = n + f with n whole, |f| <= 1/2; the series of 2^f up to the fifth power, whose rest is below 2.5e-6 (a two-hundredth of half a step
-// of fp16), times 2^n.  Below 2^-126 nothing is left of a weight; NaN stays NaN.
+// of fp16), times 2^n.  Below 2^-126.5, where 2^n has no exponent left, a weight is zero; NaN stays NaN.
 __device__ __forceinline__ void exp2_pair(uint64_t x, float (&e)[2]) {
   float t[2];
   unpack(x, t);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(t[h]));   // -126
+  for (int h = 0; h < 2; ++h) asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t[h]));   // -127
   x = pair_of(t[0], t[1]);
   // the sum's lowest bits are n + 127: shifted into place, 2^n
   const uint64_t shift = pair_of(12582912.f + 127.f, 12582912.f + 127.f), back = pair_of(-12582912.f - 127.f, -12582912.f - 127.f), minus = pair_of(-1.f, -1.f);

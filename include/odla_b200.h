@@ -570,7 +570,7 @@ typedef struct {
 
 /* y = softmax(scale * q k^T) v over what each query sees, the prefix read once for the whole batch.  dtype fp16 or bf16,
  * channels 64 or 128, q, y, caches 16-byte aligned with strides that are multiples of 8 elements, heads a multiple of
- * cache->heads.  A query that sees nothing gets zeros (lengths[b] <= 0 and no prefix: a padded batch).  Own lengths beyond
+ * cache->heads.  A query that sees nothing gets zeros (lengths[b] <= 0 and no prefix: a padded batch), and so does one whose scores are all minus infinity.  Own lengths beyond
  * table_width pages count as table_width pages; positions on a page that the cache does not have (a negative entry) are
  * not seen.  What the cache holds in slots that no query sees may be anything, NaN included.
  * lengths, page_table and prefix_pages are device memory and read when the kernels run, so a captured call follows them.

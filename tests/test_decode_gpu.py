@@ -247,6 +247,29 @@ def test_attention_extreme_scores(odla, gpu_lib, prefix):
     check_attention(odla, gpu_lib, case, prefix, scale=-0.2)
 
 
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("prefix,batch,channels", [(0, 3, 64), (600, 24, 128), (600, 80, 64)])
+def test_attention_scores_of_minus_infinity_weigh_nothing(odla, gpu_lib, dtype, prefix, batch, channels):
+    """All scores minus infinity: zeros.  All but one: that position's value, to the rounding of one weight over itself."""
+    case = attention_case(dtype, batch, 1, 4, 1, channels, 16, prefix, [70] * batch, poison=False)
+    q, kc, vc, pp, table, lengths = case
+    q[..., 0] = 1.0
+    kc[..., 0] = float("-inf")
+    y = R.call_attention(odla, gpu_lib, q, kc, vc, pp, prefix, table, lengths, 0.125)
+    assert (y == 0).all()
+    if prefix:
+        kc[int(pp[20]), 0, 7, 0] = 0.0
+        want = vc[int(pp[20]), 0, 7].expand(batch, 4, channels)
+    else:
+        want = torch.zeros((batch, 4, channels), dtype=q.dtype, device="cuda")
+        for b in range(batch):
+            kc[int(table[b, 2]), 0, 3, 0] = 0.0
+            want[b] = vc[int(table[b, 2]), 0, 3]
+    y = R.call_attention(odla, gpu_lib, q, kc, vc, pp, prefix, table, lengths, 0.125)
+    # (w v) / w: two roundings in 32 bits, which may move a value of the type by a step only where they cross its rounding border; v itself is no border
+    assert torch.equal(y[:, 0], want)
+
+
 def test_attention_strides_and_neighbours(odla, gpu_lib):
     """Queries inside a projection's rows, results inside a wider buffer: what lies between stays as it was."""
     q, kc, vc, pp, table, lengths = attention_case(1, 3, 2, 6, 2, 64, 16, 50, [33, 64, 2])
