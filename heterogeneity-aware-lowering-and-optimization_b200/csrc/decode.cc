@@ -2,6 +2,8 @@
 // before anything is enqueued; the kernels check what only they can see (slots, page numbers, lengths).
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
+#include <utility>
 
 #include "common.h"
 
@@ -20,6 +22,12 @@ bool have_device(const char* what) {
 bool strides_ok(std::initializer_list<long long> s) {
   for (long long v : s)
     if (v < 0 || v > kMaxElements) return false;
+  return true;
+}
+// Rows that are written must not lie on one another: no stride below a row's channels where there is more than one.
+bool apart(int channels, std::initializer_list<std::pair<long long, long long>> extents) {
+  for (const auto& e : extents)
+    if (e.first > 1 && e.second < channels) return false;
   return true;
 }
 bool element_aligned(int dtype, std::initializer_list<const void*> ps) {
@@ -63,6 +71,7 @@ bool attention_args(const odla_b200_paged_cache* c, const odla_b200_paged_attent
   if (!cache_ok(c) || !d || c->dtype == 0 || (c->channels != 64 && c->channels != 128)) return false;
   if (d->batch < 0 || d->queries < 1 || d->heads < 1 || d->heads > 1024 || d->heads % c->heads || d->prefix_length < 0 || d->table_width < 0 || !std::isfinite(d->scale)) return false;
   if (!strides_ok({d->q_batch, d->q_token, d->q_head, d->y_batch, d->y_token, d->y_head})) return false;
+  if (!apart(c->channels, {{d->batch, d->y_batch}, {d->queries, d->y_token}, {d->heads, d->y_head}})) return false;
   for (long long s : {c->page, c->head, c->token, d->q_batch, d->q_token, d->q_head, d->y_batch, d->y_token, d->y_head})
     if (s % 8) return false;
   // positions are counted in 32 bits, rows of the workspace too
@@ -80,6 +89,7 @@ extern "C" int odla_b200_rotary(const odla_b200_rotary_spec* spec, const odla_b2
   if (!spec_ok(spec, d->channels) || (long long)d->batch * d->tokens >= (1ll << 31)) return -1;
   if (!strides_ok({d->x_batch, d->x_token, d->x_head, d->y_batch, d->y_token, d->y_head})) return -1;
   if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return 0;
+  if (!apart(d->channels, {{d->batch, d->y_batch}, {d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
   if (!x || !y || (spec->pairs && !positions) || !element_aligned(d->dtype, {x, y}) || (uintptr_t)positions % 4) return -1;
   if (x == y && (d->x_batch != d->y_batch || d->x_token != d->y_token || d->x_head != d->y_head)) return -1;
   if (!have_device("odla_b200_rotary")) return -2;
@@ -99,6 +109,8 @@ extern "C" int odla_b200_paged_append(const odla_b200_paged_cache* c, void* key_
   if (!cache_ok(c) || !d || d->tokens < 0 || d->heads < 0 || d->heads > 1024 || (spec && !spec_ok(spec, c->channels))) return -1;
   if (!strides_ok({d->q_token, d->q_head, d->k_token, d->k_head, d->v_token, d->v_head, d->y_token, d->y_head})) return -1;
   if (d->tokens == 0) return 0;
+  if (!apart(c->channels, {{c->pages, c->page}, {c->page_size, c->token}, {c->heads, c->head}, {d->heads, d->y_head}})) return -1;
+  if (d->heads && !apart(c->channels, {{d->tokens, d->y_token}})) return -1;
   if (!key_cache || !value_cache || !k || !v || !slots || (d->heads && (!q || !q_out)) || (spec && spec->pairs && !positions)) return -1;
   if (!element_aligned(c->dtype, {key_cache, value_cache, q, k, v, q_out}) || (uintptr_t)positions % 4 || (uintptr_t)slots % 8) return -1;
   if (d->heads && q == q_out && (d->q_token != d->y_token || d->q_head != d->y_head)) return -1;

@@ -57,6 +57,22 @@ def test_rotary_refuses_pointers_and_specs(odla, lib):
         odla.rotary_spec([1.0], axis=[4])
 
 
+def test_rows_that_would_be_written_over_one_another_are_refused(odla, lib):
+    s = spec(odla)
+    for kw in (dict(y_batch=0), dict(y_token=0), dict(y_head=63), dict(y_head=1)):
+        assert call_rotary(lib, s, rotary_desc(odla, **kw)) == -1, kw
+    for kw in (dict(page=0), dict(head=0), dict(token=63)):
+        assert call_append(lib, cache(odla, **kw), append_desc(odla), s) == -1, kw
+    for kw in (dict(y_token=0), dict(y_head=32)):
+        assert call_append(lib, cache(odla), append_desc(odla, **kw), s) == -1, kw
+    for kw in (dict(y_batch=0), dict(y_head=56), dict(queries=2, y_token=0)):
+        d = attention_desc(odla, **kw)
+        assert call_attention(lib, cache(odla), d) == -1 and lib.b200_paged_attention_workspace(C.byref(cache(odla)), C.byref(d)) == -1, kw
+    # a stride of an extent of one is never used, and rows that are only read may lie anywhere
+    d = attention_desc(odla, batch=1, y_batch=0, y_token=0, q_head=0)
+    assert lib.b200_paged_attention_workspace(C.byref(cache(odla, page=0)), C.byref(d)) > 0
+
+
 def cache(odla, **kw):
     return odla.PagedCache(**dict(dict(dtype=1, pages=8, page_size=16, heads=2, channels=64, page=2048, head=1024, token=64), **kw))
 
