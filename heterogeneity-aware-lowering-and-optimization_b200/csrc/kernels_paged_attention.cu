@@ -13,7 +13,7 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 16, kStep = 32;   // rows of a tile; positions a warp takes at a time
-constexpr int kRing = 3;                                                    // units of kStep rows of keys or of values, per warp
+constexpr int kRing = 3;                                                    // units of kStep rows of keys or of values, for each warp
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -25,11 +25,13 @@ struct Params {
   float2* stat;
   int group, rows;                   // query heads of a cache head; rows of one cache head = batch * queries * group
   int prefix_chunk, prefix_chunks, own_chunk, own_chunks, slots;
-  int prefix_tiles, own_tiles;       // tiles of 16 rows: over all rows, and over those of one sequence
+  int team;                          // 1, 2 or 4 tiles of 16 rows that a block of tile_kernel takes
+  int prefix_tiles, own_tiles;       // its blocks of rows: over all rows, and over those of one sequence
   // The tensor-core kernel's tiles of 256 rows: over all rows, for the prefix, and over those of one sequence, for the own positions that all
   // its queries see (the last queries - 1 positions remain for tile_kernel, in the last slot).  0: tile_kernel takes them all.
   int wide_tiles, own_wide_tiles, own_wide_chunks, own_wide_chunk;
   float scale_log2e;
+  uint32_t page_factor, page_shift;  // n / page_size = n * page_factor >> page_shift for n < 2^30
   int join_warps;                    // 4 or 1: warps that share a row's slots
   int wide_first;                    // no tile_kernel in front
   int box_shift;                     // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
@@ -41,7 +43,7 @@ template <typename T> struct Mma;
 template <> struct Mma<__half> {
   static constexpr bool kBf16 = false;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -58,7 +60,7 @@ template <> struct Mma<__half> {
 template <> struct Mma<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -94,21 +96,29 @@ __device__ __forceinline__ int capped(const Params& p, int n) {
 }
 __device__ __forceinline__ int own_length(const Params& p, int b) { return capped(p, p.lengths[b]); }
 
+__device__ __forceinline__ int page_of(const Params& p, int n) { return (int)((uint64_t)(uint32_t)n * p.page_factor >> p.page_shift); }
+
 // Own positions that every query of the sequence sees.
 __device__ __forceinline__ int common_length(const Params& p, int length) { return max(0, length - p.a.queries + 1); }
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A tile of up to 16 rows (query, query head) of one cache head against one chunk of positions, of the prefix or of one sequence.
-// Bound by the cache's bytes: 16 rows do 16 products for each two bytes read, far below what the tensor cores could do, so that the
-// kernel's work is to keep loads in flight.  Each warp has positions and a ring of its own: no warp waits for another until
-// the end.  The ring's units alternate keys and values of 32 positions; two of the three are always in flight.
+// Up to TEAM tiles of 16 rows (query, query head) of one cache head against one chunk of positions, of the prefix or of one sequence.
+// The cache's bytes are the least it has to do: 16 rows do 16 products for each two bytes read, far below what the tensor cores could do.  What
+// bounds it is a warp's chain of latencies, about 2000 clocks for a step of 32 positions of 128 channels (loads asked for 500, Q K^T 400, softmax 450,
+// P V 420), with the two warps per scheduler that 250 registers allow: 128 sequences of up to 900 positions, 236 MB, take 53 us, 4.5 TB/s.
+// With one tile each warp has positions and a ring of its own: no warp waits for another until
+// the end.  The ring's units alternate keys and values of 32 positions; two of the three are always in flight.  With more tiles the warps that take
+// them over the same positions are a team, which shares its warps' rings, loads and a barrier for each unit, so that a sequence's
+// cache is read once (64 rows of 8 sequences of up to 2500 positions: 35.6 us, a tile for each block 43.9; 24 of 32 of up to 1500: 26.8 and 30).
+// Copies of 16 bytes by all lanes, not one bulk copy for each position: of those an SM starts one in some 25 clocks (53 -> 73 us).
 // Softmax runs over positions with maximum and sum per row; the weights are rounded to the cache's type for the second product, and the
 // sum is taken of the rounded ones, so that the result is an average of values with weights that add up to one.
-template <typename T, int D>
+template <typename T, int D, int TEAM>
 __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int kPieces = D / 8, kUnit = kStep * D * 2;   // 16-byte pieces of a row; bytes of a unit
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = blockIdx.y;
+  constexpr int kTeams = kWarps / TEAM, kSlots = kRing * TEAM;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM, head = blockIdx.y;
   // The kernel in front may still be writing the cache; the wide kernel may start once every block here knows that it is not.
   grid_dependency_wait();
   launch_dependents();
@@ -120,8 +130,8 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   int row0, n_rows, begin, end, slot, length = 0, b_own = 0;
   if (!own) {
     const int chunk = item / p.prefix_tiles, tile = item - chunk * p.prefix_tiles;
-    row0 = tile * kRows;
-    n_rows = min(kRows, p.rows - row0);
+    row0 = tile * (kRows * TEAM);
+    n_rows = min(kRows * TEAM, p.rows - row0);
     begin = chunk * p.prefix_chunk;
     end = min(begin + p.prefix_chunk, p.a.prefix_length);
     pages = p.prefix_pages;
@@ -131,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
     b_own = item % p.a.batch;
     const int rest = item / p.a.batch, chunk = rest / p.own_tiles, tile = rest - chunk * p.own_tiles;
     const int per = p.a.queries * p.group;
-    row0 = b_own * per + tile * kRows;
-    n_rows = min(kRows, per - tile * kRows);
+    row0 = b_own * per + tile * (kRows * TEAM);
+    n_rows = min(kRows * TEAM, per - tile * (kRows * TEAM));
     begin = chunk * p.own_chunk;
     if (p.own_wide_tiles) begin += common_length(p, own_length(p, b_own));
     end = (int)min((int64_t)begin + p.own_chunk, (int64_t)p.a.table_width * p.a.page_size);   // (until the length is there)
@@ -143,23 +153,27 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   if (own) length = p.lengths[b_own];
   auto ask = [&](int step) {
     const int pos = begin + step * kStep + lane;
-    return lane < kStep && pos < end ? pages[pos / p.a.page_size] : -1;
+    return lane < kStep && pos < end ? pages[page_of(p, pos)] : -1;
   };
-  int page = ask(warp);
-  // the rows this lane has a share of: row0 + lane / 4 and + 8
+  int page = ask(team);
+  // this warp's rows, and those of them that this lane has a share of: row + lane / 4 and + 8
+  const int row_w = row0 + member * kRows, rows_w = min(kRows, n_rows - member * kRows);   // (none or less: it loads with the others, no more)
   int limit[2];
   uint32_t qa[D / 16][4];
+  // (the scale's sign becomes that of the queries: the largest score is then the largest product; without a scale all products are zero)
+  const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u, any = p.scale_log2e == 0.f ? 0u : ~0u;
+  const float scale = p.scale_log2e == 0.f ? 1.f : fabsf(p.scale_log2e);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = (lane >> 2) + 8 * h;
-    const bool live = r < n_rows;
-    const int row = row0 + (live ? r : 0), g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
+    const bool live = r < rows_w;
+    const int row = live ? row_w + r : row0, g = row % p.group, j = row / p.group % p.a.queries, b = row / (p.group * p.a.queries);
     limit[h] = !live ? INT_MIN : j;
     const T* q = (const T*)p.q + b * p.a.q_batch + j * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      qa[k][h] = live ? *(const uint32_t*)(q + k * 16 + (lane & 3) * 2) : 0u;
-      qa[k][h + 2] = live ? *(const uint32_t*)(q + k * 16 + 8 + (lane & 3) * 2) : 0u;
+      qa[k][h] = live ? (*(const uint32_t*)(q + k * 16 + (lane & 3) * 2) ^ sign) & any : 0u;
+      qa[k][h + 2] = live ? (*(const uint32_t*)(q + k * 16 + 8 + (lane & 3) * 2) ^ sign) & any : 0u;
     }
   }
   if (own) {
@@ -170,29 +184,30 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
 #pragma unroll
   for (int h = 0; h < 2; ++h) limit[h] = limit[h] == INT_MIN ? 0 : own ? length - p.a.queries + limit[h] + 1 : p.a.prefix_length;
   // positions below `all` are seen by every row of the tile
-  int all = own ? length - p.a.queries + row0 / p.group % p.a.queries + 1 : p.a.prefix_length;
+  const int all = own ? length - p.a.queries + row_w / p.group % p.a.queries + 1 : p.a.prefix_length;
   const int n_steps = (end - begin + kStep - 1) / kStep;
-  const uint32_t ring = shared_address(smem) + warp * (kRing * kUnit);
+  const uint32_t ring = shared_address(smem) + team * (kSlots * kUnit);
 
   const T *kc = (const T*)p.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.v + (int64_t)head * p.a.c_head;
   int64_t off = -1;
-  // unit u: keys (u even) or values (u odd) of this warp's step u / 2; returns which of the 32 positions can be seen at all
+  // unit u: keys (u even) or values (u odd) of this team's step u / 2, of which each of its warps brings a part; returns which of the 32 positions can
+  // be seen at all
   auto issue = [&](int u) -> uint32_t {
     uint32_t seen = 0;
-    const int step = warp + (u >> 1) * kWarps;
+    const int step = team + (u >> 1) * kTeams;
     if (step < n_steps) {
       if (!(u & 1)) {
         const int pos = begin + step * kStep + lane;
         off = -1;
-        if (lane < kStep && pos < end && page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos % p.a.page_size) * p.a.c_token;
+        if (lane < kStep && pos < end && page >= 0 && page < p.a.pages) off = page * p.a.c_page + (int64_t)(pos - page_of(p, pos) * p.a.page_size) * p.a.c_token;
         seen = __ballot_sync(~0u, off >= 0);
-        page = ask(step + kWarps);
+        page = ask(step + kTeams);
       }
       const T* base = (u & 1) ? vc : kc;
-      const uint32_t dst = ring + (u % kRing) * kUnit;
+      const uint32_t dst = ring + (u % kSlots) * kUnit;
 #pragma unroll
-      for (int i = 0; i < kPieces * kStep / 32; ++i) {
-        const int n = i * 32 + lane, r = n / kPieces, c = n % kPieces;
+      for (int i = 0; i < kPieces * kStep / 32 / TEAM; ++i) {
+        const int n = (member * (kPieces * kStep / 32 / TEAM) + i) * 32 + lane, r = n / kPieces, c = n % kPieces;
         const int64_t o = __shfl_sync(~0u, off, r);
         copy16(dst + r * (D * 2) + ((c ^ (r & 7)) << 4), base + (o < 0 ? 0 : o) + c * 8, o >= 0);
       }
@@ -206,63 +221,94 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
   for (int i = 0; i < D / 8; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-  uint32_t seen = issue(0);
-  issue(1);
-  uint32_t next = issue(2);
-  for (int i = 0, step = warp; step < n_steps; ++i, step += kWarps) {
+  // Masks of the steps whose keys are on their way, the next one first.  A warp of its own refills a unit as soon as it has read it; a team
+  // behind the barrier that tells that the next one is there, which is also where all have read it.
+  constexpr int kAhead = TEAM == 1 ? 2 : kSlots / 2;
+  uint32_t ahead[kAhead];
+#pragma unroll
+  for (int u = 0; u < (TEAM == 1 ? kSlots : kSlots - 1); ++u) {
+    const uint32_t seen = issue(u);
+    if (!(u & 1)) ahead[u / 2] = seen;
+  }
+  auto await = [&]() {
+    copies_wait<TEAM == 1 ? 2 : kSlots - 2>();
+    if (TEAM == 1) __syncwarp(); else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
+  };
+  auto push = [&](uint32_t seen) {
+#pragma unroll
+    for (int k = 0; k + 1 < kAhead; ++k) ahead[k] = ahead[k + 1];
+    ahead[kAhead - 1] = seen;
+  };
+  for (int i = 0, step = team; step < n_steps; ++i, step += kTeams) {
     const int at = begin + step * kStep;
-    copies_wait<2>();
-    __syncwarp();
-    const uint32_t ku = ring + (2 * i % kRing) * kUnit, vu = ring + ((2 * i + 1) % kRing) * kUnit;
+    const uint32_t seen = ahead[0];
+    await();
+    if (TEAM > 1) issue(2 * i + kSlots - 1);
+    const uint32_t ku = ring + (2 * i % kSlots) * kUnit, vu = ring + ((2 * i + 1) % kSlots) * kUnit;
+    uint32_t pa[kStep / 16][4];
+    if (TEAM == 1 || rows_w > 0) {
     float s[kStep / 8][4];
 #pragma unroll
     for (int n = 0; n < kStep / 8; ++n)
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[n][k] = 0.f;
+    // (four sums side by side: each of a sum's products waits for the one before it)
 #pragma unroll
-    for (int n = 0; n < kStep / 8; ++n)
+    for (int k = 0; k < D / 32; ++k) {
+      uint32_t b[kStep / 8][4];
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {   // 8 positions x 32 channels
-        uint32_t b[4];
+      for (int n = 0; n < kStep / 8; ++n) {   // 8 positions x 32 channels
         const int r = n * 8 + (lane & 7), c = k * 4 + (lane >> 3);
-        ldmatrix4<false>(b, ku + r * (D * 2) + ((c ^ (r & 7)) << 4));
-        Mma<T>::run(s[n], qa[2 * k], b[0], b[1]);
-        Mma<T>::run(s[n], qa[2 * k + 1], b[2], b[3]);
+        ldmatrix4<false>(b[n], ku + r * (D * 2) + ((c ^ (r & 7)) << 4));
       }
-    __syncwarp();
-    issue(2 * i + 3);
-    // scores in powers of two; a position that is not seen has none
-    const bool masked = seen != ~0u >> (32 - kStep) || at + kStep > all;
-    float mx[2] = {m[0], m[1]};
 #pragma unroll
-    for (int n = 0; n < kStep / 8; ++n)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int pos = n * 8 + (lane & 3) * 2 + (k & 1);
-        s[n][k] *= p.scale_log2e;
-        if (masked && (!(seen >> pos & 1) || at + pos >= limit[k >> 1])) s[n][k] = -INFINITY;
-        mx[k >> 1] = fmaxf(mx[k >> 1], s[n][k]);
-      }
-    float base[2];
+        for (int n = 0; n < kStep / 8; ++n) Mma<T>::run(s[n], qa[2 * k + h], b[n][2 * h], b[n][2 * h + 1]);
+    }
+    if (TEAM == 1) {
+      __syncwarp();
+      issue(2 * i + 3);
+    }
+    // a position that is not seen has no score
+    if (seen != ~0u >> (32 - kStep) || at + kStep > all) {
+#pragma unroll
+      for (int n = 0; n < kStep / 8; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int pos = n * 8 + (lane & 3) * 2 + (k & 1);
+          if (!(seen >> pos & 1) || at + pos >= limit[k >> 1]) s[n][k] = -INFINITY;
+        }
+    }
+    float base[2], mx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      mx[h] = m[h];
+#pragma unroll
+      for (int n = 0; n < kStep / 8; ++n) mx[h] = fmaxf(mx[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 1));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(~0u, mx[h], 2));
-      base[h] = mx[h] == -INFINITY ? 0.f : mx[h];
-      const float corr = exp2_fast(m[h] - base[h]);   // 0 at first
-      m[h] = mx[h];
-      l[h] *= corr;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= corr; o[n][2 * h + 1] *= corr; }
+      base[h] = mx[h] == -INFINITY ? 0.f : mx[h] * scale;
     }
-    uint32_t pa[kStep / 16][4];
+    if (__any_sync(~0u, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float corr = exp2_fast(m[h] * scale - base[h]);   // 0 at first
+        m[h] = mx[h];
+        l[h] *= corr;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= corr; o[n][2 * h + 1] *= corr; }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < kStep / 8; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        pa[n >> 1][(n & 1) * 2 + h] = Mma<T>::pack(exp2_fast(s[n][2 * h] - base[h]), exp2_fast(s[n][2 * h + 1] - base[h]), l[h]);
-    copies_wait<2>();
-    __syncwarp();
+        pa[n >> 1][(n & 1) * 2 + h] = Mma<T>::pack(exp2_fast(s[n][2 * h] * scale - base[h]), exp2_fast(s[n][2 * h + 1] * scale - base[h]), l[h]);
+    }
+    await();
+    if (TEAM > 1) push(issue(2 * i + kSlots));
+    if (TEAM > 1 && rows_w <= 0) continue;
     if (at + kStep <= all || !own) {
 #pragma unroll
       for (int k = 0; k < kStep / 16; ++k)
@@ -277,10 +323,10 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
     } else {
       // Positions that later queries of the tile see and earlier ones do not: a weight of zero does not hide an infinity there, so each
       // query has its product with the values that it sees, and the other rows take nothing of it.
-      const int q0 = row0 / p.group, q1 = (row0 + n_rows - 1) / p.group;
+      const int q0 = row_w / p.group, q1 = (row_w + rows_w - 1) / p.group;
       for (int qi = q0; qi <= q1; ++qi) {
         const int lim = length - p.a.queries + qi % p.a.queries + 1 - at;
-        const bool mine[2] = {(row0 + (lane >> 2)) / p.group == qi, (row0 + (lane >> 2) + 8) / p.group == qi};
+        const bool mine[2] = {(row_w + (lane >> 2)) / p.group == qi, (row_w + (lane >> 2) + 8) / p.group == qi};
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k) {
           const int pos = k * 16 + (lane & 3) * 2;
@@ -300,9 +346,10 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
         }
       }
     }
-    __syncwarp();
-    seen = next;
-    next = issue(2 * i + 4);
+    if (TEAM == 1) {
+      __syncwarp();
+      push(issue(2 * i + 4));
+    }
   }
   copies_wait<0>();
 #pragma unroll
@@ -310,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
     l[h] += __shfl_xor_sync(~0u, l[h], 1);
     l[h] += __shfl_xor_sync(~0u, l[h], 2);
   }
-  // ---- the four warps' results become one ----
+  // ---- the teams' results become one ----
   __syncthreads();
   float* so = (float*)smem;                                 // [warp][16 rows][D + 4]: the padding spreads rows over the banks
   float2* sm = (float2*)(so + kWarps * kRows * (D + 4));    // [warp][16]
@@ -319,19 +366,19 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
     const int r = (lane >> 2) + 8 * h;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) *(float2*)&so[(warp * kRows + r) * (D + 4) + n * 8 + (lane & 3) * 2] = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-    if ((lane & 3) == 0) sm[warp * kRows + r] = make_float2(m[h], l[h]);
+    if ((lane & 3) == 0) sm[warp * kRows + r] = make_float2(m[h] * scale, l[h]);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n_rows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    const int r = i / (D / 4), c = i % (D / 4) * 4;   // (rows lie [team][member][16])
     float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kRows + r].x);
+    for (int w = 0; w < kTeams; ++w) top = fmaxf(top, sm[w * (TEAM * kRows) + r].x);
     const float base = top == -INFINITY ? 0.f : top;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 st = sm[w * kRows + r];
+    for (int w = 0; w < kTeams; ++w) {
+      const float2 st = sm[w * (TEAM * kRows) + r];
       const float f = exp2_fast(st.x - base);
-      const float4 x = *(const float4*)&so[(w * kRows + r) * (D + 4) + c];
+      const float4 x = *(const float4*)&so[(w * (TEAM * kRows) + r) * (D + 4) + c];
       sum += f * st.y;
       acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
     }
@@ -913,14 +960,20 @@ Params plan(const PagedAttention& a) {
   p.group = a.heads / a.kv_heads;
   p.rows = a.batch * a.queries * p.group;
   p.scale_log2e = a.scale * kLog2e;
+  while ((1ll << p.page_shift) < a.page_size) ++p.page_shift;
+  p.page_shift += 30;
+  p.page_factor = (uint32_t)((1ull << p.page_shift) / a.page_size + 1);   // factor * page_size exceeds 2^shift by at most page_size <= 2^(shift - 30)
   p.prefix_tiles = (p.rows + kRows - 1) / kRows;
-  p.own_tiles = (a.queries * p.group + kRows - 1) / kRows;
+  const int64_t per = (int64_t)a.queries * p.group;
+  p.team = per <= kRows ? 1 : per <= 2 * kRows ? 2 : 4;
+  p.own_tiles = (int)((per + kRows * p.team - 1) / (kRows * p.team));
   const int64_t own_max = (int64_t)a.table_width * a.page_size;
-  // Chunks for tile_kernel: two and a half blocks for each of the 296 that run at once even out ragged lengths (16 sequences of up to 2500
-  // positions, 35 rows: 512 positions 34 us, 256 41, 2048 45; 128 sequences of up to 900: whole 55.9 us, 512 57.7).
+  // Chunks for tile_kernel: two and a half blocks for each of the 296 that run at once even out ragged lengths (128 sequences of up to 900
+  // positions, 4 rows: whole 55.9 us, 512 57.7); of teams, whose block takes four times as long over a chunk, one (16 sequences of up to 2500
+  // positions, 35 rows: 512 positions 32 us, 256 35; 40 rows of one: 128 14.9, 512 25).
   auto chunk_of = [&](int64_t positions, int64_t tiles) {
     int64_t chunk = 4096;
-    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < 5 * 148) chunk /= 2;
+    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < (p.team == 1 ? 5 : 2) * 148) chunk /= 2;
     return (int)chunk;
   };
   if (a.prefix_length && p.rows > kRows) {
@@ -939,9 +992,8 @@ Params plan(const PagedAttention& a) {
     p.prefix_chunk = chunk_of(a.prefix_length, p.prefix_tiles);
   }
   p.prefix_chunks = (a.prefix_length + p.prefix_chunk - 1) / p.prefix_chunk;
-  const int64_t per = (int64_t)a.queries * p.group;
-  // (up to four tiles of 16 rows read the cache again from L2 in less time than the wide kernel's blocks need to begin and end: 35 rows as
-  // above 34 us and 47; 64 to 256 rows fill its tiles)
+  // (up to four tiles of 16 rows take a team less time than the wide kernel's blocks need to begin and end: 35 rows as above 32 us and 47; 64 to
+  // 256 rows fill its tiles)
   if (per > 4 * kRows && own_max > kWideStep) {
     p.own_wide_tiles = (int)((per + kWideRows - 1) / kWideRows);
     const int64_t all = (own_max + kWideStep - 1) / kWideStep, tiles = (int64_t)p.own_wide_tiles * a.batch * a.kv_heads;
@@ -1001,7 +1053,8 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   constexpr size_t ring = (size_t)kWarps * kRing * kStep * D * 2, merge = (size_t)kWarps * kRows * (D + 4) * 4 + kWarps * kRows * 8, smem = ring > merge ? ring : merge;
   constexpr size_t wide = (size_t)(2 + kWideRing) * (D / 64) * kBox + 1024;
   const unsigned heads = (unsigned)p.a.kv_heads;
-  if (items && !start(tile_kernel<T, D>, dim3((unsigned)items, heads), kThreads, smem, stream, p)) return -2;
+  auto* tiles = p.team == 1 ? tile_kernel<T, D, 1> : p.team == 2 ? tile_kernel<T, D, 2> : tile_kernel<T, D, 4>;
+  if (items && !start(tiles, dim3((unsigned)items, heads), kThreads, smem, stream, p)) return -2;
   if (wide_items) {
     p.wide_first = items == 0;
     CUtensorMap keys{}, values{};

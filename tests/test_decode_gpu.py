@@ -200,6 +200,23 @@ def test_attention(odla, gpu_lib, dtype, token_major, shape):
     check_attention(odla, gpu_lib, attention_case(dtype, *shape, token_major=token_major), shape[6])
 
 
+@pytest.mark.parametrize("shape", [(3, 3, 12, 2, 64, 16, 0, [700, 33, 5]), (2, 8, 8, 1, 64, 24, 100, [1300, 40]), (5, 2, 20, 2, 128, 16, 0, [2, 1, 513, 128, 90]),
+                                   (1, 8, 40, 8, 128, 100, 0, [2100]), (4, 4, 16, 1, 128, 7, 40, [0, 4, 31, 1025]), (40, 2, 24, 1, 64, 64, 0, [i * 29 % 300 for i in range(40)])])
+def test_attention_teams_of_tiles(odla, gpu_lib, shape):
+    """17 to 64 rows of a sequence: two or four tiles of 16, the last of them partly or wholly empty, over the same positions."""
+    check_attention(odla, gpu_lib, attention_case(1, *shape), shape[6])
+    check_attention(odla, gpu_lib, attention_case(2, *shape, token_major=True, seed=1), shape[6], scale=-0.1)
+
+
+@pytest.mark.parametrize("queries,heads", [(3, 6), (5, 28)])
+def test_attention_a_later_querys_infinity_in_teams(odla, gpu_lib, queries, heads):
+    q, kc, vc, pp, table, lengths = attention_case(1, 2, queries, heads, heads // 6 if heads == 6 else 4, 64, 16, 0, [70, queries])
+    for i, n in enumerate((70, queries)):
+        vc[int(table[i, (n - 1) // 16]), :, (n - 1) % 16] = float("inf")      # only the last query sees it
+    y = R.call_attention(odla, gpu_lib, q, kc, vc, None, 0, table, lengths, 0.125)
+    assert torch.isfinite(y[:, :-1]).all() and not torch.isfinite(y[:, -1]).any()
+
+
 def test_attention_sees_nothing(odla, gpu_lib):
     q, kc, vc, pp, table, lengths = attention_case(1, 4, 2, 4, 2, 64, 16, 0, [0, 1, 40, 0])
     lengths[3] = -5
