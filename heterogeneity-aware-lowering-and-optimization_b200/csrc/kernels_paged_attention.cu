@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
 // row turns it into weights, which replace it there as the A operand of O += P V.  O stays in tensor memory over the whole chunk: a
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
 // rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
-// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3400.  Up to 128 rows leave the
+// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3100 to 3200: a softmax warp works for 2000 and waits 1100 for the next scores, behind the last
+// products with its weights.  Up to 128 rows leave the
 // second tile free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
 // Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values lie as
 // the products read them (rows of 64 channels, 128-byte swizzle); the ring alternates units of 128 keys and 128 values.  They arrive by
@@ -589,11 +590,15 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
           for (int c = 0; c < 4; ++c) {
             tmem_ld_wait32(v[c & 1]);
             if (c < 3) tmem_ld32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
-            float m2[2] = {mx, mx};
+            float m4[4] = {mx, mx, mx, mx};
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (decltype(all)::value || (seen[c] >> k & 1)) m2[k & 1] = fmaxf(m2[k & 1], __uint_as_float(v[c & 1][k]));
-            mx = fmaxf(m2[0], m2[1]);
+            for (int k = 0; k < 32; k += 2) {
+              float x[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) x[h] = decltype(all)::value || (seen[c] >> (k + h) & 1) ? __uint_as_float(v[c & 1][k + h]) : -INFINITY;
+              m4[k >> 1 & 3] = fmaxf(m4[k >> 1 & 3], fmaxf(x[0], x[1]));
+            }
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           }
         };
         if (whole) largest(True()); else largest(False());
