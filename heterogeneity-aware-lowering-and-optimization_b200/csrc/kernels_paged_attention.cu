@@ -395,9 +395,10 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
 // row turns it into weights, which replace it there as the A operand of O += P V.  O stays in tensor memory over the whole chunk: a
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
 // rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
-// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3100 to 3200: a softmax warp works for 2000 and waits 1100 for the next scores, behind the last
-// products with its weights.  Up to 128 rows leave the
-// second tile free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
+// is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3100 to 3200: a softmax warp
+// works for 2000 and waits 1100 for the next scores, which stand behind the last products with its weights (512 rows behind 32768 positions, 8 cache
+// heads: 73 us, 940 TFLOP/s).  Up to 128 rows leave the second tile free: it takes the same rows against every other step (`split`), and hands its
+// sums to the first at the end.
 // Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products (twelve warps leave a thread 168 registers).  Keys and values lie as
 // the products read them (rows of 64 channels, 128-byte swizzle); the ring alternates units of 128 keys and 128 values.  They arrive by
 // TMA in boxes of as many positions as divide both a page and a step, where those are at least the swizzle's eight; pages of other
