@@ -213,13 +213,17 @@ template <typename T, int RANKS> struct Part {
   // (a mark so near the edge of a bin that the proposal fell on the wrong side: one of 5000 rows with top-p, and the call then takes 140 us longer at
   // 128000 tokens; listing the neighbour, too, where the mark is near an edge cost every call 1 %),
   // the list is full (many equal logits), or a parameter is out of this way's range (top-k above 1024, uniform outside (0, 1),
-  // temperature, infinities).  All CTAs of a cluster take the same branches.
+  // temperature, infinities, logits beside which 70 temperatures vanish).  All CTAs of a cluster take the same branches.
   __device__ __forceinline__ bool direct() {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int N = Piece<T>::N;
     const float per_unit = kBinsPerE / r.temperature;
     const bool by_count = r.top_k > 0 && r.top_k < vocab, by_mass = r.top_p < 1.f;
     if (!(r.uniform > 0.f && r.uniform < 1.f) || !(fabsf(top) < 1e30f) || !(r.temperature > 1e-4f && r.temperature < 1e4f) || (by_count && r.top_k > kTopK)) return false;
+    // The logit that dead and far ones count as, 70 temperatures below the largest.  Where 32 bits round the difference to at least one step, it is
+    // more than 46 temperatures (two thirds), a weight of no units; where they round it to none, this would be the largest logit itself.
+    const float floor = top - 70.f * r.temperature;
+    if (!by_count && !(floor < top)) return false;
     const double least = (double)r.min_p;
     const int sub = slice / kWarps, warp_base = warp * sub;   // a warp's stretch
     bool groups = by_count && vocab / (kPer * N) >= 2 * r.top_k;
@@ -256,7 +260,7 @@ template <typename T, int RANKS> struct Part {
             }
           }
       } else {
-        named = add_up(per_unit, by_mass, bin, sub, warp_base, lane, warp, tid);
+        named = add_up(per_unit, floor, by_mass, bin, sub, warp_base, lane, warp, tid);
       }
       if (by_count || by_mass) {
         n = collect(by_count ? enlist(named, tid, kThreads) : enlist(named, warp_base / N + lane, 32));
@@ -336,7 +340,8 @@ template <typename T, int RANKS> struct Part {
     sync_row();
     if (!s.ok) return false;
     if (s.owner / kWarps != rank) return true;
-    // the stretch of one warp, now by all warps of its CTA
+    // The stretch of one warp, now by all warps of its CTA.  Its tokens and their units are those that were summed (a logit's bin follows from
+    // its value, falls as it grows, and every weight of no units counts for nothing in both), so that one of the warps passes the target.
     const Key cut = (Key)(s.cut_entry >> 32);
     const int cut_index = by_mass ? (int)~(uint32_t)s.cut_entry : INT_MAX, stretch = (s.owner - rank * kWarps) * sub, part = (sub / kWarps + 31) & ~31;
     auto chosen = [&](int i) -> unsigned long long {
@@ -612,8 +617,8 @@ template <typename T, int RANKS> struct Part {
     if (tid == 0) tokens[row] = (int)prefix;
   }
 
-  // This CTA's exact sums, into the first CTA's memory; names the logits in the bin.
-  __device__ __forceinline__ unsigned long long add_up(float per_unit, bool by_mass, int bin, int sub, int warp_base, int lane, int warp, int tid) {
+  // This CTA's exact sums, into the first CTA's memory; names the logits in the bin.  Logits below `floor`, NaN and -inf among them, become it.
+  __device__ __forceinline__ unsigned long long add_up(float per_unit, float floor, bool by_mass, int bin, int sub, int warp_base, int lane, int warp, int tid) {
     constexpr int N = Piece<T>::N;
     Shared* first = peer(0);
     const double least = (double)r.min_p;
@@ -621,7 +626,6 @@ template <typename T, int RANKS> struct Part {
     {
       // (where only min-p chooses, no weight past this place passes it, with room for the roundings of 32 bits)
       const float last = by_mass || !(r.min_p > 0.f) ? kNoUnits : fminf(-kBinsPerE * logf(r.min_p) + 1.f, kNoUnits);
-      const float floor = top - 70.f * r.temperature;   // no units; NaN and -inf become this
       const bool every = !(r.min_p > 0.f);              // min-p keeps all
       // a thread's sums of units are exact as doubles (64 logits at most); integer additions of two words would cost as much as the weights
       double all = 0, below = 0, taken = 0;

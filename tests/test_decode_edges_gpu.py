@@ -1,0 +1,53 @@
+"""Calls at the edges of what a decoder's entry points allow, against plain 64-bit forms."""
+import ctypes as C
+
+import pytest
+import torch
+
+import decode_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def check_sample(odla, lib, logits, p, u, dtype):
+    """Every row gets a token (call_sample fills them with -7 first), and the rule's."""
+    got = R.call_sample(odla, lib, logits, *p, u, dtype).cpu().numpy()
+    want = R.sample(logits.double().cpu().numpy(), *[None if x is None else x.cpu().numpy() for x in p], u.cpu().numpy())
+    bad = [(i, int(got[i]), int(want[i])) for i in range(len(want)) if got[i] != want[i]]
+    assert not bad, bad[:8]
+
+
+# --------------------------------------------------------------------- sampling ----
+@pytest.mark.parametrize("dtype,top", [(0, 1e5), (0, 1e6), (0, 1e9), (0, 1e10), (0, 1e20), (1, 6e4), (2, 1e6), (2, 1e9), (2, 1e10), (2, 1e20)])
+@pytest.mark.parametrize("vocab", [1000, 12000])
+def test_sample_a_maximum_beside_which_a_temperature_vanishes(odla, gpu_lib, dtype, top, vocab):
+    """One token forced far above the others, two equal ones, and one a step of the type below: next to masked logits and NaN in the same 16
+    bytes and to ordinary ones.  70 temperatures are less than half a step of 32 bits of the largest logit, or about as much, or more."""
+    g = torch.Generator(device="cuda").manual_seed(vocab + dtype)
+    us = [2.0 ** -20, 0.1, 0.24, 0.25, 0.3, 0.49, 0.5, 0.7, 0.76, 0.9, 1 - 2.0 ** -24]
+    kinds, rows = 4, 4 * len(us)
+    x = 3 * torch.randn((rows, vocab), generator=g, device="cuda")
+    inf, step = float("inf"), top * torch.finfo(R.TORCH[dtype]).eps
+    at = 8 * 37
+    for r in range(rows):
+        kind = r % kinds
+        x[r, at + 3] = top
+        x[r, at] = -inf
+        x[r, at + 1] = float("nan")
+        if kind == 1:
+            x[r, vocab - 9] = top
+        if kind == 2:
+            x[r, at + 2] = top - step
+        if kind == 3:
+            x[r, :at + 3] = -inf
+            x[r, at + 4:] = float("nan")
+    u = torch.tensor(us, device="cuda").repeat_interleave(kinds)
+    x = x.to(R.TORCH[dtype])
+
+    def full(v, t=torch.float32):
+        return torch.full((rows,), v, device="cuda", dtype=t)
+    for T in (2e-4, 0.45, 1.0, step / 140, step / 3):
+        for p in ((full(T), None, None, None), (full(T), None, None, full(0.05)), (full(T), None, full(0.9), None), (full(T), full(20, torch.int32), None, None),
+                  (full(T), full(20, torch.int32), full(0.7), full(0.01))):
+            check_sample(odla, gpu_lib, x, p, u, dtype)
+    check_sample(odla, gpu_lib, x, (None, None, None, None), u, dtype)
