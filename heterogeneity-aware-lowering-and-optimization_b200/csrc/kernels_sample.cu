@@ -984,18 +984,21 @@ int launch(int rows, int vocab, int64_t row, const void* logits, const float* te
            cudaStream_t stream) {
   // A slice goes to shared memory where it fits; it has to where a row is no number of aligned 16 bytes, because only the first pass reads
   // single logits.
-  constexpr size_t kKeep = 64 * 1024, kMost = 160 * 1024;   // two CTAs to an SM, or whatever fits
+  constexpr size_t kKeep = 64 * 1024;   // two CTAs to an SM
   const int vec = (uintptr_t)logits % 16 == 0 && row * sizeof(T) % 16 == 0;
   const bool must = !vec || vocab % (16 / (int)sizeof(T));
   int ranks = 1;
   auto slice_of = [&](int n) { return ((vocab + n - 1) / n + kThreads - 1) / kThreads * kThreads; };
-  while (ranks < kMaxCluster && (slice_of(ranks) > kSlice || (must && slice_of(ranks) * sizeof(T) > kMost) || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
+  while (ranks < kMaxCluster && (slice_of(ranks) > kSlice || (rows * ranks < 148 && slice_of(ranks) > 2048))) ranks *= 2;
   const int slice = slice_of(ranks);
   const int keep = must || slice * sizeof(T) <= kKeep;
   const size_t smem = sizeof(Shared) + (keep ? (size_t)slice * sizeof(T) : 0);
   static const Powers powers = [] { Powers p; for (int j = 0; j < kTable; ++j) p.of[j] = std::exp2((double)j / kTable); return p; }();
   auto* fn = kernel_of<T>(ranks);
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
+  // The kernel's limit is one for all host threads: always that of the longest slice, so that no call lowers it under another's launch.
+  constexpr size_t kMost = sizeof(Shared) + kSlice * sizeof(T);
+  static_assert(kMost <= 227 * 1024 && kMaxVocab <= kSlice * kMaxCluster, "any slice fits");
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost) != cudaSuccess) { cudaGetLastError(); return -2; }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * (unsigned)ranks);
   cfg.blockDim = dim3(kThreads);

@@ -51,3 +51,35 @@ def test_sample_a_maximum_beside_which_a_temperature_vanishes(odla, gpu_lib, dty
                   (full(T), full(20, torch.int32), full(0.7), full(0.01))):
             check_sample(odla, gpu_lib, x, p, u, dtype)
     check_sample(odla, gpu_lib, x, (None, None, None, None), u, dtype)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_sample_from_two_host_threads(odla, gpu_lib, dtype):
+    """Rows of different lengths ask the same kernel for different amounts of shared memory; no thread's call may be refused for the other's."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(dtype)
+    jobs = []
+    for vocab in (30522, 1000):
+        logits = (3 * torch.randn((256, vocab), generator=g, device="cuda")).to(R.TORCH[dtype])
+        u = torch.rand(256, generator=g, device="cuda")
+        jobs.append((logits, u, R.call_sample(odla, gpu_lib, logits, None, None, None, None, u, dtype), torch.empty(256, dtype=torch.int32, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    refused = [0, 0]
+
+    def work(i):
+        logits, u, _, out, stream = jobs[i]
+        d = odla.SampleDesc(dtype=dtype, rows=256, vocab=logits.shape[1], row=logits.shape[1])
+        args = (C.byref(d), logits.data_ptr(), None, None, None, None, u.data_ptr(), out.data_ptr(), stream.cuda_stream)
+        for n in range(1500):
+            refused[i] += gpu_lib.b200_sample(*args) != 0
+            if n % 100 == 99:
+                stream.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert refused == [0, 0]
+    for _, _, alone, out, _ in jobs:
+        assert torch.equal(out, alone)
