@@ -76,7 +76,8 @@ bool attention_args(const odla_b200_paged_cache* c, const odla_b200_paged_attent
     if (s % 8) return false;
   // positions are counted in 32 bits, rows of the workspace too
   if ((long long)d->table_width * c->page_size + d->prefix_length >= (1ll << 30)) return false;
-  if ((long long)d->batch * d->queries * d->heads >= (1ll << 24)) return false;
+  // (two factors first: three ints may pass 64 bits)
+  if ((long long)d->batch * d->queries >= (1ll << 24) || (long long)d->batch * d->queries * d->heads >= (1ll << 24)) return false;
   a = PagedAttention{kStorage[c->dtype], d->batch, d->queries, d->heads, c->heads, c->channels, c->pages, c->page_size, d->prefix_length, d->table_width, d->scale,
                      c->page, c->head, c->token, d->q_batch, d->q_token, d->q_head, d->y_batch, d->y_token, d->y_head};
   return true;
