@@ -2,6 +2,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdlib>
 
@@ -960,6 +961,28 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   for (int k = 0; k < N; k += 2) *(uint32_t*)(y + k) = Mma<T>::pack(acc[k] * inverse, acc[k + 1] * inverse);
 }
 
+constexpr int kChunkLeast = 128, kChunkMost = 4096;                // positions of a chunk
+constexpr int kEnoughTiles = 5 * 148, kEnoughTeams = 2 * 148;      // blocks from which on chunks are not cut further
+constexpr int64_t kPrefixSlots = 1 << 17, kPrefixChunks = 16;      // the wide kernel's partial results of the prefix: as many in all, or for each row
+int64_t pieces(int64_t n, int64_t of) { return (n + of - 1) / of; }
+
+// Partial results (of one row of one head each) that the workspace has room for: at least as many as plan() chooses, and no fewer for a larger
+// batch, table or prefix or for more queries or heads.  What plan() chooses does not grow like that, because fewer sequences are cut into more chunks;
+// but where it halves chunks it had less than `enough` blocks before, and has less than twice as many then.
+int64_t room_for(const PagedAttention& a) {
+  const int64_t per = (int64_t)a.queries * (a.heads / a.kv_heads), rows = a.batch * per, all = rows * a.kv_heads, own = (int64_t)a.table_width * a.page_size;
+  int64_t prefix = 0;
+  if (a.prefix_length) {
+    const int64_t least = pieces(a.prefix_length, kChunkLeast), most = pieces(a.prefix_length, kChunkMost), few = std::min<int64_t>(rows, kRows);
+    prefix = std::min(few * a.kv_heads * least, std::max(few * a.kv_heads * most, few * 2 * kEnoughTiles));
+    if (rows > kRows) prefix = std::max(prefix, std::min(all * std::min<int64_t>(least, 64), std::max(kPrefixSlots, kPrefixChunks * all)));
+  }
+  // a block has up to 16 rows of a sequence, a team's up to 64, the wide kernel's up to 256
+  const int64_t cut = std::max(std::min<int64_t>(per, kRows) * 2 * kEnoughTiles, std::min<int64_t>(per, kWideRows) * 2 * kEnoughTeams);
+  const int64_t tail = a.queries > 1 && per > 4 * kRows && own > kWideStep ? all : 0;
+  return prefix + std::min(all * pieces(own, kChunkLeast), std::max(all * pieces(own, kChunkMost), cut)) + tail;
+}
+
 Params plan(const PagedAttention& a) {
   Params p{};
   p.a = a;
@@ -978,17 +1001,19 @@ Params plan(const PagedAttention& a) {
   // positions, 4 rows: whole 55.9 us, 512 57.7); of teams, whose block takes four times as long over a chunk, one (16 sequences of up to 2500
   // positions, 35 rows: 512 positions 32 us, 256 35; 40 rows of one: 128 14.9, 512 25).
   auto chunk_of = [&](int64_t positions, int64_t tiles) {
-    int64_t chunk = 4096;
-    while (chunk > 128 && tiles * a.kv_heads * ((positions + chunk - 1) / chunk) < (p.team == 1 ? 5 : 2) * 148) chunk /= 2;
+    int64_t chunk = kChunkMost;
+    while (chunk > kChunkLeast && tiles * a.kv_heads * pieces(positions, chunk) < (p.team == 1 ? kEnoughTiles : kEnoughTeams)) chunk /= 2;
     return (int)chunk;
   };
   if (a.prefix_length && p.rows > kRows) {
     // Blocks of equal work on 148 SMs: the number of chunks with the shortest estimate of waves of steps (1.9 us each, 1.1 us split; 5 us at both ends) and of
-    // the partial results' way to memory and back.
+    // the partial results' way to memory and back; up to 64, for many rows less, to bound the workspace (by the estimate that costs at most 5 %, and
+    // only from 3000 rows of all heads and 97000 positions on).
     p.wide_tiles = (p.rows + kWideRows - 1) / kWideRows;
     const int tiles = p.wide_tiles * a.kv_heads, all = (a.prefix_length + kWideStep - 1) / kWideStep;
+    const int64_t most = std::min<int64_t>(64, std::max(kPrefixChunks, kPrefixSlots / ((int64_t)p.rows * a.kv_heads)));
     double best = 1e30;
-    for (int c = 1; c <= all && c <= 64; ++c) {
+    for (int c = 1; c <= all && c <= most; ++c) {
       const int steps = (all + c - 1) / c;
       const double us = (double)((tiles * (int64_t)c + 147) / 148) * (steps * (p.rows > 128 ? 1.9 : 1.1) + 5.0) + (double)c * p.rows * a.kv_heads * a.channels * 8 / 5e6;
       if (us < best) { best = us; p.prefix_chunk = steps * kWideStep; }
@@ -1003,8 +1028,8 @@ Params plan(const PagedAttention& a) {
   if (per > 4 * kRows && own_max > kWideStep) {
     p.own_wide_tiles = (int)((per + kWideRows - 1) / kWideRows);
     const int64_t all = (own_max + kWideStep - 1) / kWideStep, tiles = (int64_t)p.own_wide_tiles * a.batch * a.kv_heads;
-    int64_t steps = 32;
-    while (steps > 4 && tiles * ((all + steps - 1) / steps) < 2 * 148) steps /= 2;
+    int64_t steps = kChunkMost / kWideStep;
+    while (steps > 4 && tiles * pieces(all, steps) < kEnoughTeams) steps /= 2;
     p.own_wide_chunk = (int)steps * kWideStep;
     p.own_wide_chunks = (int)((all + steps - 1) / steps);
     p.own_chunk = (a.queries - 1 + kStep - 1) / kStep * kStep;
@@ -1080,7 +1105,7 @@ int64_t paged_attention_workspace(const PagedAttention& a) {
   if (a.batch == 0) return 0;
   const Params p = plan(a);
   if (tile_items(p) >= (1ll << 31) || wide_tile_items(p) >= (1ll << 31)) return -1;   // more blocks than a grid has
-  return (int64_t)p.rows * a.kv_heads * p.slots * ((int64_t)a.channels * 4 + 8);
+  return room_for(a) * ((int64_t)a.channels * 4 + 8);
 }
 
 int paged_attention(const PagedAttention& a, const void* key_cache, const void* value_cache, const void* q, const int* prefix_pages, const int* page_table, const int* lengths,

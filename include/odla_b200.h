@@ -576,7 +576,8 @@ typedef struct {
  * not seen.  What the cache holds in slots that no query sees may be anything, NaN included.
  * lengths, page_table and prefix_pages are device memory and read when the kernels run, so a captured call follows them.
  * workspace: odla_b200_paged_attention_workspace(cache, desc) bytes (16-byte aligned; -1 for arguments that the call refuses), which need not
- * be cleared; calls that may run at the same time need one each.  A bounded wait inside the kernel that expires gives rows of NaN. */
+ * be cleared; they suffice for every call over that cache whose batch, queries, heads, prefix_length and table_width are no larger.  Calls that may
+ * run at the same time need one each.  A bounded wait inside the kernel that expires gives rows of NaN. */
 long long odla_b200_paged_attention_workspace(const odla_b200_paged_cache* cache, const odla_b200_paged_attention_desc* desc);
 int odla_b200_paged_attention(const odla_b200_paged_cache* cache, const void* key_cache, const void* value_cache,
                               const odla_b200_paged_attention_desc* desc, const void* q, const int* prefix_pages,

@@ -27,3 +27,35 @@ def test_attention_refuses_more_rows_than_it_counts(odla, lib, batch, queries, h
                            q_token=64 * heads, q_batch=64 * heads, y_token=64 * heads, y_batch=64 * heads * queries)
         assert lib.b200_paged_attention_workspace(C.byref(cache(odla)), C.byref(d)) == -1
         assert call_attention(lib, cache(odla), d) == -1
+
+
+def workspace(odla, lib, heads, channels, page, **kw):
+    c = cache(odla, heads=heads[1], channels=channels, page_size=page, page=heads[1] * page * channels, head=page * channels, token=channels)
+    row = heads[0] * channels
+    q = kw.get("queries", 1)
+    d = attention_desc(odla, **dict(dict(heads=heads[0], q_batch=q * row, q_token=row, q_head=channels, y_batch=q * row, y_token=row, y_head=channels), **kw))
+    return lib.b200_paged_attention_workspace(C.byref(c), C.byref(d))
+
+
+@pytest.mark.parametrize("heads,channels,page", [((32, 8), 128, 16), ((12, 12), 64, 16), ((64, 8), 128, 64), ((28, 4), 128, 24), ((8, 1), 128, 1), ((16, 2), 64, 100)])
+def test_a_workspace_for_the_largest_call_serves_every_smaller_one(odla, lib, heads, channels, page):
+    """Sizes never fall as batch, queries, heads, prefix or table grow: along each of them, and from any shape to any larger one."""
+    import random
+    batches, prefixes, widths, queries = (range(1, 200), (0, 1, 100, 129, 1999, 8192, 32768, 131072, 10 ** 6), (0, 1, 2, 5, 44, 60, 256, 1000, 8192), (1, 2, 3, 4, 5, 8, 9, 16, 17, 33, 64, 65, 70, 300))
+    for prefix in prefixes:
+        for width in widths:
+            sizes = [workspace(odla, lib, heads, channels, page, batch=b, prefix_length=prefix, table_width=width) for b in batches]
+            assert all(0 <= x <= y for x, y in zip(sizes, sizes[1:])), (prefix, width)
+    rng = random.Random(heads[0] * channels + page)
+    for _ in range(3000):
+        large = dict(batch=rng.choice(batches), prefix_length=rng.choice(prefixes), table_width=rng.choice(widths), queries=rng.choice(queries))
+        small = {k: rng.choice([v, max(v - 1, 0), v // 2, rng.randint(0, v)]) for k, v in large.items()}
+        small["batch"], small["queries"] = max(small["batch"], 1), max(small["queries"], 1)
+        fewer = (rng.choice([heads[0], heads[1]]), heads[1])
+        assert 0 <= workspace(odla, lib, fewer, channels, page, **small) <= workspace(odla, lib, heads, channels, page, **large), (fewer, small, large)
+
+
+def test_a_workspace_of_shapes_that_are_cut_finely_when_they_are_few(odla, lib):
+    for prefix, own, large, small in ((0, 4096, 48, 23), (32768, 960, 100, 64), (8192, 704, 32, 30), (8192, 0, 127, 64)):
+        sizes = [workspace(odla, lib, (32, 8), 128, 16, batch=b, prefix_length=prefix, table_width=own // 16) for b in (small, large)]
+        assert 0 < sizes[0] <= sizes[1]

@@ -83,3 +83,30 @@ def test_sample_from_two_host_threads(odla, gpu_lib, dtype):
     assert refused == [0, 0]
     for _, _, alone, out, _ in jobs:
         assert torch.equal(out, alone)
+
+
+# -------------------------------------------------------------------- attention ----
+@pytest.mark.parametrize("heads,kv,channels,queries", [(32, 8, 128, 1), (8, 1, 64, 5), (8, 8, 64, 3), (16, 1, 64, 8)])
+def test_attention_one_workspace_for_the_largest_call_and_all_smaller_ones(odla, gpu_lib, heads, kv, channels, queries):
+    """Sized once, for the largest batch and table; every smaller call has the same bits as with a workspace of its own, and writes nothing behind it."""
+    g = torch.Generator(device="cuda").manual_seed(heads + channels)
+    page, batch, prefix, width = 16, 48, 700, 40
+    pages = 44 + batch * width
+    kc, vc = (torch.randn((pages, kv, page, channels), generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn((batch, queries, heads, channels), generator=g, device="cuda").half()
+    table = (44 + torch.arange(batch * width, device="cuda").view(batch, width)).to(torch.int32)
+    pp = torch.arange(44, dtype=torch.int32, device="cuda")
+    lengths = torch.randint(0, width * page + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    cache = R.cache_of(odla, kc, 1)
+    n = heads * channels
+    d = odla.PagedAttentionDesc(batch=batch, queries=queries, heads=heads, prefix_length=prefix, table_width=width, scale=0.1, q_batch=queries * n, q_token=n, q_head=channels,
+                                y_batch=queries * n, y_token=n, y_head=channels)
+    size = gpu_lib.b200_paged_attention_workspace(C.byref(cache), C.byref(d))
+    room = torch.full((size + (1 << 26),), 85, dtype=torch.uint8, device="cuda")
+    for b in (48, 47, 24, 23, 11, 5, 2, 1):
+        for w, shared in ((40, 700), (40, 0), (7, 700), (1, 129), (0, 700)):
+            args = (q[:b], kc, vc, pp, shared, table[:b, :w].contiguous(), lengths[:b], 0.1)
+            own = R.call_attention(odla, gpu_lib, *args)
+            y = R.call_attention(odla, gpu_lib, *args, workspace=room[:size])
+            assert torch.equal(y, own), (b, w, shared)
+    assert (room[size:] == 85).all()
