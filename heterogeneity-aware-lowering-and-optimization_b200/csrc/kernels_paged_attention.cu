@@ -43,6 +43,7 @@ struct Params {
 template <typename T> struct Mma;
 template <> struct Mma<__half> {
   static constexpr bool kBf16 = false;
+  static constexpr float kLift = 7.f;   // (see wide_kernel)
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -60,6 +61,7 @@ template <> struct Mma<__half> {
 };
 template <> struct Mma<__nv_bfloat16> {
   static constexpr bool kBf16 = true;
+  static constexpr float kLift = 0.f;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -395,7 +397,9 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(const __grid_constant
 // 128 rows, so that the products of one tile run under the softmax of the other.  S = Q K^T goes to tensor memory; a thread per
 // row turns it into weights, which replace it there as the A operand of O += P V.  O stays in tensor memory over the whole chunk: a
 // row's reference is not its running maximum but one that follows it only when it has been passed by more than 2^8, so that O is rarely
-// rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  At 256 rows a step of 128 positions
+// rescaled; weights up to 2^8 have the same relative rounding, and the sums are fp32.  fp16 has no numbers below 2^-24, and
+// the thousands of positions of the largest one's chunk count together although each weighs less: there the reference lies 2^7 below, and the largest
+// weights are 2^7 to 2^15.  At 256 rows a step of 128 positions
 // is 4 products of 128 x 128 x D (about 2000 clocks for D = 128) and 32768 exponentials (2048 clocks); it takes 3100 to 3200: a softmax warp
 // works for 2000 and waits 1100 for the next scores, which stand behind the last products with its weights (512 rows behind 32768 positions, 8 cache
 // heads: 73 us, 940 TFLOP/s).  Up to 128 rows leave the second tile free: it takes the same rows against every other step (`split`), and hands its
@@ -463,7 +467,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x for two x <= 8 on the multiply-add pipes, for a quarter of all exponentials (256 rows behind 32768 positions: 92 -> 88.5 us; half of them: 94):
+// 2^x for two x <= 15 on the multiply-add pipes, for a quarter of all exponentials (256 rows behind 32768 positions: 92 -> 88.5 us; half of them: 94):
 // x = n + f with n whole, |f| <= 1/2; the series of 2^f up to the fifth power, whose rest is below 2.5e-6 (a two-hundredth of half a step
 // of fp16), times 2^n.  Below 2^-126.5, where 2^n has no exponent left, a weight is zero; NaN stays NaN.
 __device__ __forceinline__ void exp2_pair(uint64_t x, float (&e)[2]) {
@@ -604,7 +608,7 @@ wide_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMa
           }
         };
         if (whole) largest(True()); else largest(False());
-        mx = mx == -INFINITY ? mx : mx * scale;   // (a scale of zero keeps it a number)
+        mx = mx == -INFINITY ? mx : mx * scale - Mma<T>::kLift;   // (a scale of zero keeps it a number)
         const bool passed = mx > (i ? reference + 8.f : -INFINITY);
         if (__any_sync(~0u, passed)) {
           const float next = passed ? mx : reference, corr = passed ? exp2_fast(reference - mx) : 1.f;

@@ -110,3 +110,36 @@ def test_attention_one_workspace_for_the_largest_call_and_all_smaller_ones(odla,
             y = R.call_attention(odla, gpu_lib, *args, workspace=room[:size])
             assert torch.equal(y, own), (b, w, shared)
     assert (room[size:] == 85).all()
+
+
+@pytest.mark.parametrize("batch,queries", [(1, 1), (1, 5), (3, 8), (70, 1)])
+def test_attention_thousands_of_small_fp16_weights_are_not_lost(odla, gpu_lib, batch, queries):
+    """One position in front of 32000 others that weigh 2^-25.02 of it each, below half of the smallest fp16 number; together 2^-10.  Where all
+    values are one, so is the average.  Where only the many have a value, 1024, the average is 1024 n w / (1 + n w).
+
+    Bound: a weight may be off by a half step of fp16 relative to it (2^-11), or, where it is held as a subnormal, by 2^-25 of a scale that lies
+    2^7 above the largest weight at least: together less than n (w 2^-11 + 2^-32) of the whole, 2^-16.6, far below half a step of fp16 at one."""
+    prefix, own, page, D = 32000, 40, 16, 64
+    shared, width = prefix // page, -(-own // page)
+    pages = shared + batch * width
+    q = torch.zeros((batch, queries, 4, D), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    kc = torch.zeros((pages, 2, page, D), dtype=torch.float16, device="cuda")
+    vc = torch.ones_like(kc)
+    scale = 25.02 / 32.0 * 0.6931471805599453       # a score of 32 is 25.02 powers of two
+    kc[5, :, 3, 0] = 32.0                           # one position of the prefix
+    pp = torch.arange(shared, dtype=torch.int32, device="cuda")
+    table = (shared + torch.arange(batch * width, device="cuda").view(batch, width)).to(torch.int32)
+    lengths = torch.full((batch,), own, dtype=torch.int32, device="cuda")
+    y = R.call_attention(odla, gpu_lib, q, kc, vc, pp, prefix, table, lengths, scale)
+    assert (y == 1).all(), y.float().aminmax()
+    vc.fill_(1024.0)
+    vc[5, :, 3] = 0.0
+    y = R.call_attention(odla, gpu_lib, q, kc, vc, pp, prefix, table, lengths, scale)
+    for j in range(queries):
+        n = prefix - 1 + own - queries + j + 1
+        w = 2.0 ** -25.02
+        want = 1024 * n * w / (1 + n * w)
+        # (the scale itself is 32 bits: the exponent of 25 is good to 25 x 2^-23 of a power of two)
+        bound = 1024 * n * (w * (2.0 ** -11 + 2.0 ** -17) + 2.0 ** -32) + want * 2.0 ** -11
+        assert (y[:, j].double() - want).abs().max() <= bound, (float(y[:, j].min()), want, bound)
