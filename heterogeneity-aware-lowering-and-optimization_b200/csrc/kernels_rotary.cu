@@ -34,8 +34,9 @@ template <typename T, int VEC> __device__ __forceinline__ void store(T* p, const
 //
 // Angles.  A frequency arrives as turns per position in units of 2^-64 (host: turn_units), so that position * frequency modulo 2^64
 // is the angle modulo one turn, exactly, however far the position: no reduction in floating point, whose error grows with
-// it.  The nearest quarter turn is taken off as whole numbers; what is left, at most an eighth, becomes fp32 with a relative error
-// of 2^-24.
+// it.  The nearest quarter turn is taken off as whole numbers of 64 bits; what is left, at most an eighth, becomes fp32 with a relative error
+// of 2^-24, beside that of the frequency's own rounding, |position| * 2^-65 turns.  (Its upper 32 bits alone, 2^-32 of a turn, would leave the sine of
+// 1e-4 sixteen bits.)
 //
 // A block takes a few tokens and works out their cosines and sines once, for all heads, into shared memory (in planes of four values, so that
 // the pieces of a row read them without bank conflicts); the first rows are already on their way then.  A thread has one
@@ -138,9 +139,10 @@ __global__ void __launch_bounds__(VEC == 1 ? 2 * kThreads : kThreads, VEC == 1 ?
       const int* pos = g.positions + (int64_t)g.axis[p] * total + first;
       float* to = (float*)planes + (p % VEC / kEach * plane + p / VEC) * kEach + p % kEach;
       for (int t = threadIdx.x / g.pairs; t < n_tok; t += groups) {
-        const uint32_t phase = (uint32_t)(((uint64_t)(int64_t)pos[t] * f) >> 32), quarter = (phase + 0x20000000u) >> 30;
+        const uint64_t phase = (uint64_t)(int64_t)pos[t] * f;
+        const uint32_t quarter = ((uint32_t)(phase >> 32) + 0x20000000u) >> 30;
         float sine, cosine;
-        sincospif((float)(int)(phase - (quarter << 30)) * (1.0f / 2147483648.0f), &sine, &cosine);
+        sincospif((float)(int64_t)(phase - ((uint64_t)quarter << 62)) * 0x1p-63f, &sine, &cosine);
         const float x = (quarter & 1) ? sine : cosine, y = (quarter & 1) ? cosine : sine;
         to[t * pieces * kEach] = quarter == 1 || quarter == 2 ? -x : x;
         to[(kPlanes * plane + t * pieces) * kEach] = quarter >= 2 ? -y : y;

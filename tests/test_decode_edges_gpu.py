@@ -143,3 +143,63 @@ def test_attention_thousands_of_small_fp16_weights_are_not_lost(odla, gpu_lib, b
         # (the scale itself is 32 bits: the exponent of 25 is good to 25 x 2^-23 of a power of two)
         bound = 1024 * n * (w * (2.0 ** -11 + 2.0 ** -17) + 2.0 ** -32) + want * 2.0 ** -11
         assert (y[:, j].double() - want).abs().max() <= bound, (float(y[:, j].min()), want, bound)
+
+
+# ---------------------------------------------------------------------- turning ----
+def pi_digits(digits):
+    """pi by Machin's formula, in whole numbers."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = digits + 20
+    one = 10 ** (digits + 10)
+
+    def arctan_inverse(n):
+        total = term = one // n
+        k, sign = 3, -1
+        while term:
+            term //= n * n
+            total += sign * (term // k)
+            k, sign = k + 2, -sign
+        return total
+    return Decimal(4 * (4 * arctan_inverse(5) - arctan_inverse(239))) / Decimal(one)
+
+
+def exact_angles(positions, frequencies):
+    """position * frequency modulo a turn, in (-pi, pi], as float64 that is good to 2^-53 of itself."""
+    from decimal import Decimal
+    two_pi = 2 * pi_digits(420)
+    out = []
+    for p in positions:
+        row = []
+        for f in frequencies:
+            a = (Decimal(int(p)) * Decimal(f)) % two_pi      # (keeps the sign of the product)
+            a = a - two_pi if a > two_pi / 2 else a + two_pi if a < -two_pi / 2 else a
+            row.append(float(a))
+        out.append(row)
+    return torch.tensor(out, dtype=torch.float64, device="cuda")
+
+
+def turn(odla, lib, x, positions, frequency, interleaved=False):
+    """x [tokens, 1, channels] in fp32."""
+    tokens, _, ch = x.shape
+    d = odla.RotaryDesc(dtype=0, batch=1, tokens=tokens, heads=1, channels=ch, x_batch=tokens * ch, x_token=ch, x_head=ch, y_batch=tokens * ch, y_token=ch, y_head=ch)
+    y, spec = torch.empty_like(x), odla.rotary_spec(frequency, interleaved=interleaved)
+    assert lib.b200_rotary(C.byref(spec), C.byref(d), x.data_ptr(), y.data_ptr(), positions.data_ptr(), R.stream()) == 0
+    return y
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_small_angles_keep_their_bits(odla, gpu_lib, interleaved):
+    """(0, b) -> (-b sin t, b cos t): the sine of a small angle shows by itself, relative to its own size.
+
+    The angle is good to |position| 2^-65 turns (the frequency's rounding) and 2^-24 of itself, sincospif to a step (2^-23 relative at most), the product to 2^-24."""
+    frequency = [10.0 ** -e * s for e in (9, 8, 7, 6, 5, 4, 3, 2) for s in (1, -1)]
+    pos = [1, -1, 3, 77, 1000, -4096]
+    n = len(frequency)
+    b = 1 + torch.rand((len(pos), 1, n), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    x = torch.stack([torch.zeros_like(b), b], -1).flatten(-2) if interleaved else torch.cat([torch.zeros_like(b), b], -1)
+    y = turn(odla, gpu_lib, x, torch.tensor(pos, dtype=torch.int32, device="cuda"), frequency, interleaved)
+    got = y[..., 0::2] if interleaved else y[..., :n]
+    ang = exact_angles(pos, frequency).unsqueeze(1)
+    want = -b.double() * ang.sin()
+    p = torch.tensor(pos, dtype=torch.float64, device="cuda").abs().view(-1, 1, 1)
+    R.close(got, want, want.abs() * 2.0 ** -22 + b.double() * p * 2.0 ** -65 * 6.2832)
