@@ -2,6 +2,7 @@
 // before anything is enqueued; the kernels check what only they can see (slots, page numbers, lengths).
 #include <cmath>
 #include <cstdio>
+#include <cstring>
 #include <initializer_list>
 #include <utility>
 
@@ -41,15 +42,29 @@ bool aligned16(std::initializer_list<const void*> ps) {
   return true;
 }
 
-// Turns per position in units of 2^-64, modulo one turn; frequencies of either sign.
+// 1 / (2 pi) as a binary fraction, the first bits first.
+constexpr uint64_t kTurnsOfRadian[20] = {
+  0x28BE60DB9391054A, 0x7F09D5F47D4D3770, 0x36D8A5664F10E410, 0x7F9458EAF7AEF158, 0x6DC91B8E909374B8,
+  0x01924BBA82746487, 0x3F877AC72C4A69CF, 0xBA208D7D4BAED121, 0x3A671C09AD17DF90, 0x4E64758E60D4CE7D,
+  0x272117E2EF7E4A0E, 0xC7FE25FFF7816603, 0xFBCBC462D6829B47, 0xDB4D9FB3C9F2C26D, 0xD3D18FD9A797FA8B,
+  0x5D49EEB1FAF97C5E, 0xCF41CE7DE294A4BA, 0x9AFED7EC47E35742, 0x1580CC11BF1EDAEA, 0xFC33EF0826BD0D87};
+// Turns per position in units of 2^-64, modulo one turn, to the nearest; any finite frequency, of either sign.  The frequency is a whole number of 53
+// bits times 2^e, and of 2^e / (2 pi) only the bits behind the point matter: 192 of them are multiplied (M. H. Payne and R. N. Hanek, "Radian reduction
+// for trigonometric functions", 1983).
 uint64_t turn_units(double radians) {
-  const long double units = 18446744073709551616.0L / 6.283185307179586476925286766559005768L;
-  // up to half a turn, as nearly every frequency: one product
-  if (radians >= 0 && radians < 3.14) return (uint64_t)(int64_t)((long double)radians * units + 0.5L);
-  long double t = (long double)radians / 6.283185307179586476925286766559005768L;
-  t -= floorl(t);
-  const long double u = t * 18446744073709551616.0L;
-  return u >= 18446744073709551615.0L ? 0 : (uint64_t)(u + 0.5L);
+  uint64_t bits;
+  memcpy(&bits, &radians, 8);
+  const int field = (int)(bits >> 52 & 0x7ff), e = (field ? field : 1) - 1075;
+  const uint64_t m = (bits & ((1ull << 52) - 1)) | (field ? 1ull << 52 : 0);
+  auto word = [](int at) -> uint64_t {   // 64 bits from place `at` on; there is nothing in front of the point
+    if (at < 0) return at > -64 ? kTurnsOfRadian[0] >> -at : 0;
+    const int i = at / 64, s = at % 64;
+    return s ? kTurnsOfRadian[i] << s | kTurnsOfRadian[i + 1] >> (64 - s) : kTurnsOfRadian[i];
+  };
+  typedef unsigned __int128 Wide;
+  const Wide low = (Wide)m * word(e + 64) + (uint64_t)((Wide)m * word(e + 128) >> 64);
+  const uint64_t u = m * word(e) + (uint64_t)(low >> 64) + (uint64_t)((uint64_t)low >> 63);
+  return bits >> 63 ? 0 - u : u;
 }
 bool spec_ok(const odla_b200_rotary_spec* s, int channels) {
   if (s->pairs < 0 || s->pairs > ODLA_B200_MAX_ROTARY_PAIRS || 2 * s->pairs > channels || s->axes < 1 || s->axes > 4) return false;

@@ -509,8 +509,10 @@ int odla_b200_reduce_mean_noalloc(const void* x, void* y, int dtype, const long 
 
 /* Which channels turn, and how fast.  Pair i is channels (2i, 2i + 1) of a head when `interleaved`, else (i, i + pairs); channels
  * from 2 * pairs on stay as they are.  It turns by position[axis[i]] * frequency[i] radians (any finite frequency; positions
- * are int32 and may be negative), reduced exactly, so that far positions are as accurate as near ones:
+ * are int32 and may be negative):
  *   (a, b) -> (a cos - b sin, a sin + b cos).
+ * The frequency is rounded to a multiple of 2^-64 turns and all else is reduced exactly: the angle of position p is good to |p| * 2^-65 turns, then
+ * to 2^-24 of what is left beyond the nearest quarter turn.
  * Opposite frequencies turn back. */
 #define ODLA_B200_MAX_ROTARY_PAIRS 128
 typedef struct {

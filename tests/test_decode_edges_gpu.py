@@ -203,3 +203,21 @@ def test_rotary_small_angles_keep_their_bits(odla, gpu_lib, interleaved):
     want = -b.double() * ang.sin()
     p = torch.tensor(pos, dtype=torch.float64, device="cuda").abs().view(-1, 1, 1)
     R.close(got, want, want.abs() * 2.0 ** -22 + b.double() * p * 2.0 ** -65 * 6.2832)
+
+
+def test_rotary_any_finite_frequency(odla, gpu_lib):
+    """Frequencies of many turns per position, up to the largest double, at near and far positions: the angle is good to |position| 2^-65 turns."""
+    frequency = [0.7, 6.5, 7.3e3, 1e8 + 0.1, 3.7e15, 2.0 ** 53 + 2, 1.3 * 2.0 ** 64, 1e30, 1.2345e100, 8.5e299, 1.7e308, 2.0 ** 1023, 5e-324, 2.0 ** -60]
+    frequency += [-f for f in frequency]
+    pos = [1, 2, 3, -7, 4097, 2 ** 31 - 1, -2 ** 31]
+    n = len(frequency)
+    x = torch.randn((len(pos), 1, 2 * n), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    y = turn(odla, gpu_lib, x, torch.tensor(pos, dtype=torch.int32, device="cuda"), frequency)
+    ang = exact_angles(pos, frequency).unsqueeze(1)
+    a, b, c, s = x[..., :n].double(), x[..., n:].double(), ang.cos(), ang.sin()
+    want, size = torch.cat([a * c - b * s, a * s + b * c], -1), (a.abs() + b.abs()).repeat(1, 1, 2)
+    p = torch.tensor(pos, dtype=torch.float64, device="cuda").abs().view(-1, 1, 1)
+    R.close(y, want, R.turn_tolerance(want, size, 0) + size * p * 2.0 ** -65 * 6.2832)
+    # opposite frequencies turn back
+    back = turn(odla, gpu_lib, y, torch.tensor(pos, dtype=torch.int32, device="cuda"), [-f for f in frequency])
+    R.close(back, x.double(), 4 * R.turn_tolerance(x.double(), size, 0))
