@@ -1,5 +1,6 @@
 // The entry points of a decoder's serving step (declared in include/odla_b200.h): their arguments are checked here, completely,
 // before anything is enqueued; the kernels check what only they can see (slots, page numbers, lengths).
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -25,10 +26,19 @@ bool strides_ok(std::initializer_list<long long> s) {
     if (v < 0 || v > kMaxElements) return false;
   return true;
 }
-// Rows that are written must not lie on one another: no stride below a row's channels where there is more than one.
+// Rows that are written must not lie on one another: sorted by stride, each extent above 1 steps over all that the smaller strides reach.  Every dense
+// tensor, in any order of its extents, and every slice of one is laid out like that.
 bool apart(int channels, std::initializer_list<std::pair<long long, long long>> extents) {
+  std::pair<long long, long long> by_stride[3];   // (stride, extent)
+  int n = 0;
   for (const auto& e : extents)
-    if (e.first > 1 && e.second < channels) return false;
+    if (e.first > 1) by_stride[n++] = {e.second, e.first};
+  std::sort(by_stride, by_stride + n);
+  __int128 reach = channels;
+  for (int i = 0; i < n; ++i) {
+    if (by_stride[i].first < reach) return false;
+    reach += (__int128)by_stride[i].first * (by_stride[i].second - 1);
+  }
   return true;
 }
 bool element_aligned(int dtype, std::initializer_list<const void*> ps) {
@@ -125,8 +135,8 @@ extern "C" int odla_b200_paged_append(const odla_b200_paged_cache* c, void* key_
   if (!cache_ok(c) || !d || d->tokens < 0 || d->heads < 0 || d->heads > 1024 || (spec && !spec_ok(spec, c->channels))) return -1;
   if (!strides_ok({d->q_token, d->q_head, d->k_token, d->k_head, d->v_token, d->v_head, d->y_token, d->y_head})) return -1;
   if (d->tokens == 0) return 0;
-  if (!apart(c->channels, {{c->pages, c->page}, {c->page_size, c->token}, {c->heads, c->head}, {d->heads, d->y_head}})) return -1;
-  if (d->heads && !apart(c->channels, {{d->tokens, d->y_token}})) return -1;
+  if (!apart(c->channels, {{c->pages, c->page}, {c->page_size, c->token}, {c->heads, c->head}})) return -1;
+  if (d->heads && !apart(c->channels, {{d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
   if (!key_cache || !value_cache || !k || !v || !slots || (d->heads && (!q || !q_out)) || (spec && spec->pairs && !positions)) return -1;
   if (!element_aligned(c->dtype, {key_cache, value_cache, q, k, v, q_out}) || (uintptr_t)positions % 4 || (uintptr_t)slots % 8) return -1;
   if (d->heads && q == q_out && (d->q_token != d->y_token || d->q_head != d->y_head)) return -1;

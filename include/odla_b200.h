@@ -502,7 +502,8 @@ int odla_b200_reduce_mean_noalloc(const void* x, void* y, int dtype, const long 
  * They take DEVICE pointers on the current device, only enqueue kernels on `stream` (a cudaStream_t as void*, NULL = the default
  * stream, of the same device) and allocate nothing, so they can be captured into a CUDA graph; descriptors are host memory
  * and are read during the call.  dtype: 0 = fp32, 1 = fp16, 2 = bf16.  Strides count elements and are not negative; channels are
- * contiguous, and rows that are written must not overlap (a stride below the channels, of an extent above 1, is refused).  Any
+ * contiguous, and rows that are written must not overlap: of the extents above 1 each stride has to step over all that the smaller strides
+ * reach, as in a dense tensor with its extents in any order, or a slice of one; others are refused.  Any
  * other strides and any pointers aligned to the element are served; 16-byte alignment of pointers and
  * strides is faster (odla_b200_paged_attention asks for it).  They return 0, -1 (bad argument, nothing enqueued) or -2 (CUDA
  * error).  Zero tokens, sequences or rows are a valid call that does nothing. */

@@ -59,3 +59,49 @@ def test_a_workspace_of_shapes_that_are_cut_finely_when_they_are_few(odla, lib):
     for prefix, own, large, small in ((0, 4096, 48, 23), (32768, 960, 100, 64), (8192, 704, 32, 30), (8192, 0, 127, 64)):
         sizes = [workspace(odla, lib, (32, 8), 128, 16, batch=b, prefix_length=prefix, table_width=own // 16) for b in (small, large)]
         assert 0 < sizes[0] <= sizes[1]
+
+
+def rotary_desc(odla, **kw):
+    base = dict(dtype=1, batch=2, tokens=3, heads=4, channels=64, x_batch=768, x_token=256, x_head=64, y_batch=768, y_token=256, y_head=64)
+    return odla.RotaryDesc(**dict(base, **kw))
+
+
+def call_rotary(odla, lib, d):
+    return lib.b200_rotary(C.byref(odla.rotary_spec([0.1] * 32)), C.byref(d), A, A + 4096, A, None)
+
+
+@pytest.mark.parametrize("kw", [dict(y_token=64), dict(y_token=128), dict(y_token=255), dict(y_batch=256), dict(y_batch=767), dict(y_head=300), dict(y_token=64, y_head=64, y_batch=64),
+                                dict(y_head=192, y_token=64, y_batch=500)])
+def test_rotary_refuses_rows_that_meet_across_strides(odla, lib, kw):
+    """Each stride is above a row's channels, but rows of different tokens, heads or batch entries lie on one another, or inside one another's rows."""
+    assert call_rotary(odla, lib, rotary_desc(odla, **kw)) == -1
+
+
+def test_append_and_attention_refuse_rows_that_meet_across_strides(odla, lib):
+    def append(c, **kw):
+        d = odla.AppendDesc(**dict(dict(tokens=3, heads=4, q_token=512, q_head=64, k_token=512, k_head=64, v_token=512, v_head=64, y_token=256, y_head=64), **kw))
+        return lib.b200_paged_append(C.byref(c), A, A, C.byref(d), None, A, A, A, A + 64, None, A, None)
+    for kw in (dict(y_token=64), dict(y_token=192), dict(y_head=256, y_token=255), dict(y_head=256, y_token=256)):
+        assert append(cache(odla), **kw) == -1, kw
+    for kw in (dict(page=1024), dict(page=2040), dict(head=64, token=64), dict(head=64, token=64, page=128), dict(token=128, head=64, page=2040), dict(head=960), dict(head=1 << 20, page=1 << 20)):
+        assert append(cache(odla, **kw)) == -1, kw
+    for kw in (dict(y_head=256), dict(queries=3, y_batch=256), dict(queries=3, y_token=128, y_batch=768), dict(queries=3, y_token=256, y_batch=760)):
+        d = attention_desc(odla, **kw)
+        assert lib.b200_paged_attention_workspace(C.byref(cache(odla)), C.byref(d)) == -1 and call_attention(lib, cache(odla), d) == -1, kw
+
+
+def test_layouts_of_dense_tensors_and_their_slices_are_taken(odla, lib):
+    """Every order of the extents, with room between rows, and strides that no step takes."""
+    import itertools
+    good = [dict(y_batch=1 << 20), dict(queries=1, y_token=0), dict(batch=1, y_batch=0), dict(heads=2, y_head=128), dict(batch=2, y_batch=64, queries=3, y_token=512, y_head=128),
+            dict(batch=3, y_batch=200, queries=2, y_token=5000, y_head=600)]
+    for order in itertools.permutations(("y_batch", "y_token", "y_head")):
+        extent, at, kw = dict(y_batch=2, y_token=5, y_head=4), 64, dict(queries=5)
+        for name in order:
+            kw[name] = at
+            at *= extent[name]
+        good.append(kw)
+    for kw in good:
+        assert lib.b200_paged_attention_workspace(C.byref(cache(odla)), C.byref(attention_desc(odla, **kw))) > 0, kw
+    # caches are only read by attention: they may lie on one another
+    assert lib.b200_paged_attention_workspace(C.byref(cache(odla, page=0, head=0, token=0)), C.byref(attention_desc(odla))) > 0
