@@ -41,6 +41,13 @@ bool apart(int channels, std::initializer_list<std::pair<long long, long long>> 
   }
   return true;
 }
+struct Step { long long extent, from, to; };
+// In place: a result's rows lie where the input's do (an extent of one has no step).
+bool same_rows(std::initializer_list<Step> steps) {
+  for (const Step& s : steps)
+    if (s.extent > 1 && s.from != s.to) return false;
+  return true;
+}
 bool element_aligned(int dtype, std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if ((uintptr_t)p % (dtype == 0 ? 4 : 2)) return false;
@@ -117,7 +124,7 @@ extern "C" int odla_b200_rotary(const odla_b200_rotary_spec* spec, const odla_b2
   if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return 0;
   if (!apart(d->channels, {{d->batch, d->y_batch}, {d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
   if (!x || !y || (spec->pairs && !positions) || !element_aligned(d->dtype, {x, y}) || (uintptr_t)positions % 4) return -1;
-  if (x == y && (d->x_batch != d->y_batch || d->x_token != d->y_token || d->x_head != d->y_head)) return -1;
+  if (x == y && !same_rows({{d->batch, d->x_batch, d->y_batch}, {d->tokens, d->x_token, d->y_token}, {d->heads, d->x_head, d->y_head}})) return -1;
   if (!have_device("odla_b200_rotary")) return -2;
   TurnGeom g{};
   g.src[0] = x; g.dst[0] = y;
@@ -139,7 +146,7 @@ extern "C" int odla_b200_paged_append(const odla_b200_paged_cache* c, void* key_
   if (d->heads && !apart(c->channels, {{d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
   if (!key_cache || !value_cache || !k || !v || !slots || (d->heads && (!q || !q_out)) || (spec && spec->pairs && !positions)) return -1;
   if (!element_aligned(c->dtype, {key_cache, value_cache, q, k, v, q_out}) || (uintptr_t)positions % 4 || (uintptr_t)slots % 8) return -1;
-  if (d->heads && q == q_out && (d->q_token != d->y_token || d->q_head != d->y_head)) return -1;
+  if (d->heads && q == q_out && !same_rows({{d->tokens, d->q_token, d->y_token}, {d->heads, d->q_head, d->y_head}})) return -1;
   if (!have_device("odla_b200_paged_append")) return -2;
   TurnGeom g{};
   g.src[0] = q; g.src[1] = k; g.src[2] = v;

@@ -221,3 +221,32 @@ def test_rotary_any_finite_frequency(odla, gpu_lib):
     # opposite frequencies turn back
     back = turn(odla, gpu_lib, y, torch.tensor(pos, dtype=torch.int32, device="cuda"), [-f for f in frequency])
     R.close(back, x.double(), 4 * R.turn_tolerance(x.double(), size, 0))
+
+
+# --------------------------------------------------------------------- in place ----
+def test_in_place_with_strides_that_no_step_takes(odla, gpu_lib):
+    """A single batch entry or token has no stride to step by: results may go in place whatever the two strides say."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((1, 5, 3, 64), generator=g, device="cuda").half()
+    pos = torch.arange(5, dtype=torch.int32, device="cuda").view(1, 1, 5) + 9
+    f = [10000.0 ** (-i / 32) for i in range(32)]
+    spec = odla.rotary_spec(f)
+    want, size = R.turned(x, pos, f, [0] * 32, False)
+    d = odla.RotaryDesc(dtype=1, batch=1, tokens=5, heads=3, channels=64, x_batch=0, x_token=192, x_head=64, y_batch=960, y_token=192, y_head=64)
+    assert gpu_lib.b200_rotary(C.byref(spec), C.byref(d), x.data_ptr(), x.data_ptr(), pos.data_ptr(), R.stream()) == 0
+    R.close(x, want, R.turn_tolerance(want, size, 1))
+    # one token and one head of it, queries in place inside the projection's row
+    row = torch.randn((1, 3, 64), generator=g, device="cuda").half()
+    kc, vc = (torch.zeros((2, 1, 4, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    at = torch.tensor([[3]], dtype=torch.int32, device="cuda")
+    want, size = R.turned(row, at, f, [0] * 32, False)
+    value = row[0, 2].clone()
+    slot = torch.tensor([6], device="cuda")
+    cache = R.cache_of(odla, kc, 1)
+    d = odla.AppendDesc(tokens=1, heads=1, q_token=192, q_head=64, k_token=192, k_head=64, v_token=192, v_head=64, y_token=64, y_head=0)
+    p = row.data_ptr()
+    assert gpu_lib.b200_paged_append(C.byref(cache), kc.data_ptr(), vc.data_ptr(), C.byref(d), C.byref(spec), p, p + 128, p + 256, p, at.data_ptr(), slot.data_ptr(), R.stream()) == 0
+    tol = R.turn_tolerance(want, size, 1)
+    R.close(row[:, 0], want[:, 0], tol[:, 0])
+    R.close(kc[1, 0, 2], want[0, 1], tol[0, 1])
+    assert torch.equal(vc[1, 0, 2], value)
