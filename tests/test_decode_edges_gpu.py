@@ -250,3 +250,56 @@ def test_in_place_with_strides_that_no_step_takes(odla, gpu_lib):
     R.close(row[:, 0], want[:, 0], tol[:, 0])
     R.close(kc[1, 0, 2], want[0, 1], tol[0, 1])
     assert torch.equal(vc[1, 0, 2], value)
+
+
+# ------------------------------------------------------------- sizes beyond the usual ----
+def random_attention(odla, lib, dtype, batch, queries, heads, kv, channels, page, prefix, lengths, seed, token_major=False):
+    """Own pages in any order, NaN in every slot that no query sees; against the 64-bit form."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    width, shared = max(-(-max(lengths) // page), 1), -(-prefix // page)
+    pages = shared + batch * width + 2
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    pp, table = order[:max(shared, 1)].contiguous(), order[shared:shared + batch * width].view(batch, width).contiguous()
+    caches = []
+    for _ in range(2):
+        full = torch.full((pages, page, kv, channels), float("nan"), device="cuda").to(R.TORCH[dtype])
+        for row, n in [(pp, prefix)] + list(zip(table, lengths)):
+            for j in range(-(-n // page)):
+                m = min(page, n - j * page)
+                full[int(row[j]), :m] = torch.randn((m, kv, channels), generator=g, device="cuda").to(full.dtype)
+        caches.append((full if token_major else full.transpose(1, 2).contiguous().transpose(1, 2)).transpose(1, 2))
+    q = (2 * torch.randn((batch, queries, heads, channels), generator=g, device="cuda")).to(R.TORCH[dtype])
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want, tol = R.attention(q.cpu(), caches[0].cpu(), caches[1].cpu(), pp.cpu(), prefix, table.cpu(), lens.cpu(), R.scale_of(channels))
+    y = R.call_attention(odla, lib, q, caches[0], caches[1], pp, prefix, table, lens, R.scale_of(channels))
+    R.close(y, want, tol, "attention")
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("batch,queries,heads,kv,channels,page,prefix,lengths", [
+    (1, 260, 2, 1, 64, 16, 0, [260]), (2, 150, 4, 2, 128, 24, 40, [400, 90]), (1, 129, 3, 3, 64, 64, 300, [1]), (3, 33, 4, 1, 64, 7, 0, [33, 500, 0]), (1, 400, 1, 1, 128, 100, 0, [1100]),
+    (2, 1, 256, 1, 64, 16, 0, [700, 40]), (3, 1, 100, 1, 128, 16, 150, [0, 129, 333]), (1, 2, 130, 2, 64, 8, 90, [257]), (1, 1, 1024, 16, 64, 16, 0, [200])])
+def test_attention_hundreds_of_queries_and_large_groups(odla, gpu_lib, dtype, batch, queries, heads, kv, channels, page, prefix, lengths):
+    """More rows of a sequence than two tiles of the tensor cores hold; prompts shorter than their queries; one key head for hundreds of query heads."""
+    random_attention(odla, gpu_lib, dtype, batch, queries, heads, kv, channels, page, prefix, lengths, queries + heads, token_major=dtype == 2)
+
+
+def test_sample_more_rows_than_a_grid_is_high(odla, gpu_lib):
+    g = torch.Generator(device="cuda").manual_seed(11)
+    logits, u = torch.randn((70001, 5), generator=g, device="cuda"), torch.rand(70001, generator=g, device="cuda")
+    check_sample(odla, gpu_lib, logits, (None, torch.full((70001,), 3, dtype=torch.int32, device="cuda"), None, None), u, 0)
+
+
+@pytest.mark.parametrize("channels,heads", [(1024, 1024), (1023, 600), (2, 1024)])
+def test_rotary_the_most_heads_and_channels(odla, gpu_lib, channels, heads):
+    g = torch.Generator(device="cuda").manual_seed(channels)
+    x = torch.randn((1, 3, heads, channels), generator=g, device="cuda").half()
+    y = torch.empty_like(x)
+    pos = torch.tensor([[[7, -3, 100]]], dtype=torch.int32, device="cuda")
+    pairs = min(128, channels // 2)
+    f = [10000.0 ** (-i / pairs) for i in range(pairs)]
+    spec, n = odla.rotary_spec(f), heads * channels
+    d = odla.RotaryDesc(dtype=1, batch=1, tokens=3, heads=heads, channels=channels, x_batch=3 * n, x_token=n, x_head=channels, y_batch=3 * n, y_token=n, y_head=channels)
+    assert gpu_lib.b200_rotary(C.byref(spec), C.byref(d), x.data_ptr(), y.data_ptr(), pos.data_ptr(), R.stream()) == 0
+    want, size = R.turned(x, pos, f, [0] * pairs, False)
+    R.close(y, want, R.turn_tolerance(want, size, 1))
