@@ -5,7 +5,6 @@
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
-#include <utility>
 
 #include "common.h"
 
@@ -14,30 +13,34 @@ using namespace b200;
 namespace {
 
 const int kStorage[3] = {DT_F32, DT_F16, DT_BF16};
-constexpr long long kMaxElements = 1ll << 46;   // bound on strides, so that offsets stay inside 63 bits
 
 bool have_device(const char* what) {
   if (visible_devices() > 0) return true;
   fprintf(stderr, "[odla_b200] %s: no CUDA device (there is no CPU fallback)\n", what);
   return false;
 }
-bool strides_ok(std::initializer_list<long long> s) {
-  for (long long v : s)
-    if (v < 0 || v > kMaxElements) return false;
-  return true;
+struct Extent { long long n, stride; };
+// Strides of one tensor: none negative or above 2^46, and no row 2^60 elements or more behind the first, so that offsets stay inside 63 bits.
+bool strides_ok(std::initializer_list<Extent> extents) {
+  __int128 reach = 0;
+  for (const Extent& e : extents) {
+    if (e.stride < 0 || e.stride > (1ll << 46)) return false;
+    if (e.n > 1) reach += (__int128)(e.n - 1) * e.stride;
+  }
+  return reach < ((__int128)1 << 60);
 }
 // Rows that are written must not lie on one another: sorted by stride, each extent above 1 steps over all that the smaller strides reach.  Every dense
 // tensor, in any order of its extents, and every slice of one is laid out like that.
-bool apart(int channels, std::initializer_list<std::pair<long long, long long>> extents) {
-  std::pair<long long, long long> by_stride[3];   // (stride, extent)
+bool apart(int channels, std::initializer_list<Extent> extents) {
+  Extent sorted[3];
   int n = 0;
-  for (const auto& e : extents)
-    if (e.first > 1) by_stride[n++] = {e.second, e.first};
-  std::sort(by_stride, by_stride + n);
+  for (const Extent& e : extents)
+    if (e.n > 1) sorted[n++] = e;
+  std::sort(sorted, sorted + n, [](const Extent& a, const Extent& b) { return a.stride < b.stride; });
   __int128 reach = channels;
   for (int i = 0; i < n; ++i) {
-    if (by_stride[i].first < reach) return false;
-    reach += (__int128)by_stride[i].first * (by_stride[i].second - 1);
+    if (sorted[i].stride < reach) return false;
+    reach += (__int128)(sorted[i].n - 1) * sorted[i].stride;
   }
   return true;
 }
@@ -96,13 +99,14 @@ void put_spec(TurnGeom& g, const odla_b200_rotary_spec* s) {
 }
 bool cache_ok(const odla_b200_paged_cache* c) {
   return c && c->dtype >= 0 && c->dtype <= 2 && c->pages >= 1 && c->page_size >= 1 && c->heads >= 1 && c->heads <= 1024 && c->channels >= 1 && c->channels <= 1024 &&
-         strides_ok({c->page, c->head, c->token});
+         strides_ok({{c->pages, c->page}, {c->heads, c->head}, {c->page_size, c->token}});
 }
 
 bool attention_args(const odla_b200_paged_cache* c, const odla_b200_paged_attention_desc* d, PagedAttention& a) {
   if (!cache_ok(c) || !d || c->dtype == 0 || (c->channels != 64 && c->channels != 128)) return false;
   if (d->batch < 0 || d->queries < 1 || d->heads < 1 || d->heads > 1024 || d->heads % c->heads || d->prefix_length < 0 || d->table_width < 0 || !std::isfinite(d->scale)) return false;
-  if (!strides_ok({d->q_batch, d->q_token, d->q_head, d->y_batch, d->y_token, d->y_head})) return false;
+  if (!strides_ok({{d->batch, d->q_batch}, {d->queries, d->q_token}, {d->heads, d->q_head}}) || !strides_ok({{d->batch, d->y_batch}, {d->queries, d->y_token}, {d->heads, d->y_head}}))
+    return false;
   if (!apart(c->channels, {{d->batch, d->y_batch}, {d->queries, d->y_token}, {d->heads, d->y_head}})) return false;
   for (long long s : {c->page, c->head, c->token, d->q_batch, d->q_token, d->q_head, d->y_batch, d->y_token, d->y_head})
     if (s % 8) return false;
@@ -120,7 +124,8 @@ bool attention_args(const odla_b200_paged_cache* c, const odla_b200_paged_attent
 extern "C" int odla_b200_rotary(const odla_b200_rotary_spec* spec, const odla_b200_rotary_desc* d, const void* x, void* y, const int* positions, void* stream) {
   if (!spec || !d || d->dtype < 0 || d->dtype > 2 || d->batch < 0 || d->tokens < 0 || d->heads < 0 || d->heads > 1024 || d->channels < 1 || d->channels > 1024) return -1;
   if (!spec_ok(spec, d->channels) || (long long)d->batch * d->tokens >= (1ll << 31)) return -1;
-  if (!strides_ok({d->x_batch, d->x_token, d->x_head, d->y_batch, d->y_token, d->y_head})) return -1;
+  if (!strides_ok({{d->batch, d->x_batch}, {d->tokens, d->x_token}, {d->heads, d->x_head}}) || !strides_ok({{d->batch, d->y_batch}, {d->tokens, d->y_token}, {d->heads, d->y_head}}))
+    return -1;
   if (d->batch == 0 || d->tokens == 0 || d->heads == 0) return 0;
   if (!apart(d->channels, {{d->batch, d->y_batch}, {d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
   if (!x || !y || (spec->pairs && !positions) || !element_aligned(d->dtype, {x, y}) || (uintptr_t)positions % 4) return -1;
@@ -140,7 +145,9 @@ extern "C" int odla_b200_rotary(const odla_b200_rotary_spec* spec, const odla_b2
 extern "C" int odla_b200_paged_append(const odla_b200_paged_cache* c, void* key_cache, void* value_cache, const odla_b200_append_desc* d, const odla_b200_rotary_spec* spec,
                                       const void* q, const void* k, const void* v, void* q_out, const int* positions, const long long* slots, void* stream) {
   if (!cache_ok(c) || !d || d->tokens < 0 || d->heads < 0 || d->heads > 1024 || (spec && !spec_ok(spec, c->channels))) return -1;
-  if (!strides_ok({d->q_token, d->q_head, d->k_token, d->k_head, d->v_token, d->v_head, d->y_token, d->y_head})) return -1;
+  if (!strides_ok({{d->tokens, d->q_token}, {d->heads, d->q_head}}) || !strides_ok({{d->tokens, d->k_token}, {c->heads, d->k_head}}) ||
+      !strides_ok({{d->tokens, d->v_token}, {c->heads, d->v_head}}) || !strides_ok({{d->tokens, d->y_token}, {d->heads, d->y_head}}))
+    return -1;
   if (d->tokens == 0) return 0;
   if (!apart(c->channels, {{c->pages, c->page}, {c->page_size, c->token}, {c->heads, c->head}})) return -1;
   if (d->heads && !apart(c->channels, {{d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
@@ -181,7 +188,7 @@ extern "C" int odla_b200_paged_attention(const odla_b200_paged_cache* c, const v
 
 extern "C" int odla_b200_sample(const odla_b200_sample_desc* d, const void* logits, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                                 const float* uniform, int* tokens, void* stream) {
-  if (!d || d->dtype < 0 || d->dtype > 2 || d->rows < 0 || d->rows > (1 << 24) || d->vocab < 1 || d->vocab > kMaxVocab || !strides_ok({d->row})) return -1;
+  if (!d || d->dtype < 0 || d->dtype > 2 || d->rows < 0 || d->rows > (1 << 24) || d->vocab < 1 || d->vocab > kMaxVocab || !strides_ok({{d->rows, d->row}})) return -1;
   if (d->rows == 0) return 0;
   if (!logits || !uniform || !tokens || !element_aligned(d->dtype, {logits})) return -1;
   for (const void* p : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p, (const void*)uniform, (const void*)tokens})

@@ -105,3 +105,23 @@ def test_layouts_of_dense_tensors_and_their_slices_are_taken(odla, lib):
         assert lib.b200_paged_attention_workspace(C.byref(cache(odla)), C.byref(attention_desc(odla, **kw))) > 0, kw
     # caches are only read by attention: they may lie on one another
     assert lib.b200_paged_attention_workspace(C.byref(cache(odla, page=0, head=0, token=0)), C.byref(attention_desc(odla))) > 0
+
+
+def test_offsets_that_pass_63_bits_are_refused(odla, lib):
+    """No stride is too large by itself, but the last row would lie 2^60 elements or more behind the first."""
+    far = 1 << 46
+    assert call_rotary(odla, lib, rotary_desc(odla, batch=1, tokens=1 << 30, x_token=far)) == -1
+    assert call_rotary(odla, lib, rotary_desc(odla, batch=1, tokens=1 << 30, y_token=far)) == -1
+    assert call_rotary(odla, lib, rotary_desc(odla, batch=1 << 20, tokens=1 << 10, x_batch=far)) == -1
+
+    def append(c, **kw):
+        d = odla.AppendDesc(**dict(dict(tokens=1 << 20, heads=4, q_token=512, q_head=64, k_token=512, k_head=64, v_token=512, v_head=64, y_token=256, y_head=64), **kw))
+        return lib.b200_paged_append(C.byref(c), A, A, C.byref(d), None, A, A, A, A + 64, None, A, None)
+    for kw in (dict(q_token=far), dict(k_token=far), dict(v_token=far), dict(y_token=far)):
+        assert append(cache(odla), **kw) == -1, kw
+    assert append(cache(odla, pages=1 << 30, page=far)) == -1
+    for c, kw in ((dict(pages=1 << 30, page=far), {}), ({}, dict(batch=1 << 20, q_batch=far)), ({}, dict(batch=1 << 20, y_batch=far)), ({}, dict(batch=1, queries=1 << 20, q_token=far))):
+        d = attention_desc(odla, **kw)
+        assert lib.b200_paged_attention_workspace(C.byref(cache(odla, **c)), C.byref(d)) == -1 and call_attention(lib, cache(odla, **c), d) == -1, kw
+    d = odla.SampleDesc(dtype=2, rows=1 << 20, vocab=1000, row=far)
+    assert lib.b200_sample(C.byref(d), A, None, None, None, None, A, A, None) == -1
