@@ -886,9 +886,10 @@ template <typename T, int RANKS> struct Part {
 
 // One cluster of CTAs takes one row, each CTA `slice` consecutive logits, which it reads once and keeps in shared memory; where they do not fit
 // (`keep` is 0) the passes after the first read them from the caller's memory again, mostly from L2.  Two CTAs share an SM, so that one
-// computes while the other waits: what a row costs beside its loads and weights is a chain of barriers.
+// computes while the other waits: what a row costs beside its loads and weights is a chain of barriers.  The logits are no __restrict__ constants: the
+// kernel may begin while the one in front still writes them, and loads that count on memory which nobody writes are not for it.
 template <typename T, int RANKS>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* __restrict__ logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const T* logits, int64_t row_stride, int vocab, int slice, int vec, int keep, const __grid_constant__ Powers powers,
                                                           const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* tokens) {
   using L = Logits<T>;
   using P = Part<T, RANKS>;

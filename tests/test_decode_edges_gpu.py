@@ -303,3 +303,32 @@ def test_rotary_the_most_heads_and_channels(odla, gpu_lib, channels, heads):
     assert gpu_lib.b200_rotary(C.byref(spec), C.byref(d), x.data_ptr(), y.data_ptr(), pos.data_ptr(), R.stream()) == 0
     want, size = R.turned(x, pos, f, [0] * pairs, False)
     R.close(y, want, R.turn_tolerance(want, size, 1))
+
+
+# -------------------------------------------------------------- one call after another ----
+@pytest.mark.parametrize("dtype,rows,vocab", [(0, 300, 1000), (2, 40, 1024), (1, 3, 512)])
+def test_a_call_reads_what_the_one_in_front_writes(odla, gpu_lib, dtype, rows, vocab):
+    """Turned rows are the logits of the next call, over and over in the same memory with nothing in between: no call may begin to read before the one in front has written."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    n = 24
+    x = (3 * torch.randn((n, rows, vocab), generator=g, device="cuda")).to(R.TORCH[dtype])
+    pos = torch.randint(0, 1000, (n, rows), generator=g, device="cuda", dtype=torch.int32)
+    u = torch.rand((n, rows), generator=g, device="cuda")
+    k = torch.full((rows,), 5, dtype=torch.int32, device="cuda")
+    spec = odla.rotary_spec([1.0 / (i + 1) for i in range(64)])
+    d = odla.RotaryDesc(dtype=dtype, batch=1, tokens=rows, heads=1, channels=vocab, x_batch=rows * vocab, x_token=vocab, x_head=vocab, y_batch=rows * vocab, y_token=vocab, y_head=vocab)
+
+    def turn_into(y, i):
+        assert gpu_lib.b200_rotary(C.byref(spec), C.byref(d), x[i].data_ptr(), y.data_ptr(), pos[i].data_ptr(), R.stream()) == 0
+    shared, apart = torch.empty_like(x[0]), torch.empty_like(x)
+    tokens = torch.full((n, rows), -7, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(n):
+        turn_into(shared, i)
+        R.call_sample(odla, gpu_lib, shared, None, k if i % 2 else None, None, None, u[i], dtype, tokens=tokens[i])
+    torch.cuda.synchronize()
+    for i in range(n):
+        turn_into(apart[i], i)
+        torch.cuda.synchronize()
+        want = R.sample(apart[i].double().cpu().numpy(), None, k.cpu().numpy() if i % 2 else None, None, None, u[i].cpu().numpy())
+        assert (tokens[i].cpu().numpy() == want).all()
