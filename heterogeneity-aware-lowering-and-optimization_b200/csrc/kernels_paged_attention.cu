@@ -108,12 +108,12 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 // Up to TEAM tiles of 16 rows (query, query head) of one cache head against one chunk of positions, of the prefix or of one sequence.
 // The cache's bytes are the least it has to do: 16 rows do 16 products for each two bytes read, far below what the tensor cores could do.  What
 // bounds it is a warp's chain of latencies, about 2000 clocks for a step of 32 positions of 128 channels (loads asked for 500, Q K^T 400, softmax 450,
-// P V 420), with the two warps per scheduler that 250 registers allow: 128 sequences of up to 900 positions, 236 MB, take 53 us, 4.5 TB/s.
+// P V 420), with the two warps per scheduler that 250 registers allow: 128 sequences of up to 900 positions, 236 MB, take 50 us, 4.7 TB/s.
 // With one tile each warp has positions and a ring of its own: no warp waits for another until
 // the end.  The ring's units alternate keys and values of 32 positions; two of the three are always in flight.  With more tiles the warps that take
 // them over the same positions are a team, which shares its warps' rings, loads and a barrier for each unit, so that a sequence's
 // cache is read once (64 rows of 8 sequences of up to 2500 positions: 35.6 us, a tile for each block 43.9; 24 of 32 of up to 1500: 26.8 and 30).
-// Copies of 16 bytes by all lanes, not one bulk copy for each position: of those an SM starts one in some 25 clocks (53 -> 73 us).
+// Copies of 16 bytes by all lanes, not one bulk copy for each position: of those an SM starts one in some 25 clocks (73 us).
 // Softmax runs over positions with maximum and sum per row; the weights are rounded to the cache's type for the second product, and the
 // sum is taken of the rounded ones, so that the result is an average of values with weights that add up to one.
 template <typename T, int D, int TEAM>

@@ -564,7 +564,7 @@ int odla_b200_paged_append(const odla_b200_paged_cache* cache, void* key_cache, 
  * Every sequence begins with the same prefix_length positions, which lie on prefix_pages[0 ...]; sequence b goes on with
  * lengths[b] positions of its own on page_table[b * table_width ...], the last `queries` of them the tokens that ask.  Query j
  * sees the prefix and own positions 0 ... lengths[b] - queries + j.  Query heads come in equal groups, one for each head
- * of the cache. */
+ * of the cache.  The kernels are made for few queries (up to some tens) and for tables not much wider than the lengths; more of either is right, but slower. */
 typedef struct {
   int batch, queries, heads;
   int prefix_length, table_width;
