@@ -332,3 +332,36 @@ def test_a_call_reads_what_the_one_in_front_writes(odla, gpu_lib, dtype, rows, v
         torch.cuda.synchronize()
         want = R.sample(apart[i].double().cpu().numpy(), None, k.cpu().numpy() if i % 2 else None, None, None, u[i].cpu().numpy())
         assert (tokens[i].cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("batch,queries,heads,kv,prefix,own", [(40, 1, 8, 2, 500, 90), (6, 5, 8, 1, 300, 400), (2, 70, 4, 1, 0, 300), (3, 1, 4, 4, 40, 70)])
+def test_attention_reads_what_the_kernels_in_front_write(odla, gpu_lib, dtype, batch, queries, heads, kv, prefix, own):
+    """Caches, tables, lengths and queries change in place between calls with nothing in between: every call has the bits that it has alone."""
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    page, D, n = 16, 64, 12
+    shared, width = -(-prefix // page), -(-own // page)
+    pages = shared + batch * width
+    sets = []
+    for _ in range(n):
+        order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+        sets.append([torch.randn((batch, queries, heads, D), generator=g, device="cuda").to(R.TORCH[dtype])] +
+                    [torch.randn((pages, kv, page, D), generator=g, device="cuda").to(R.TORCH[dtype]) for _ in range(2)] +
+                    [order[:max(shared, 1)].contiguous(), order[shared:].view(batch, width).contiguous(), torch.randint(0, own + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)])
+    alone = []
+    for q, kc, vc, pp, table, lengths in sets:
+        alone.append(R.call_attention(odla, gpu_lib, q, kc, vc, pp, prefix, table, lengths, 0.125))
+        torch.cuda.synchronize()
+    live = [t.clone() for t in sets[0]]
+    size = 1 << 26
+    workspace, results = torch.empty(size, dtype=torch.uint8, device="cuda"), [torch.empty_like(sets[0][0]) for _ in range(n)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i in range(n):
+            for to, of in zip(live, sets[i]):
+                to.copy_(of)
+            R.call_attention(odla, gpu_lib, *live[:4], prefix, *live[4:], 0.125, y=results[i], workspace=workspace)
+        torch.cuda.synchronize()
+        for i in range(n):
+            assert torch.equal(results[i], alone[i]), i
+            results[i].fill_(7.0)
