@@ -1,4 +1,4 @@
-// The entry points of a decoder's serving step (declared in include/odla_b200.h): their arguments are checked here, completely,
+// The entry points of a decoder's serving step and of its prompts (declared in include/odla_b200.h): their arguments are checked here, completely,
 // before anything is enqueued; the kernels check what only they can see (slots, page numbers, lengths).
 #include <algorithm>
 #include <cmath>
@@ -195,4 +195,69 @@ extern "C" int odla_b200_sample(const odla_b200_sample_desc* d, const void* logi
     if ((uintptr_t)p % 4) return -1;
   if (!have_device("odla_b200_sample")) return -2;
   return sample(kStorage[d->dtype], d->rows, d->vocab, d->row, logits, temperature, top_k, top_p, min_p, uniform, tokens, (cudaStream_t)stream);
+}
+
+extern "C" int odla_b200_rms_norm(const odla_b200_rms_norm_desc* d, const void* x, const void* residual, const void* weight, void* sum, void* y, void* quantised, float* scales,
+                                  void* stream) {
+  if (!d || d->dtype < 0 || d->dtype > 2 || d->weight_dtype < 0 || d->weight_dtype > 2 || d->rows < 0 || d->heads < 0 || d->heads > 1024 || d->channels < 1 || d->channels > 32768) return -1;
+  if (d->quant < 0 || d->quant > 2 || d->group < 0 || !(d->epsilon >= 0.f) || !std::isfinite(d->epsilon) || !std::isfinite(d->weight_offset) || (long long)d->rows * d->heads >= (1ll << 31)) return -1;
+  if (d->quant && d->group && (d->channels % d->group || (d->group % 8 && d->group != d->channels))) return -1;
+  const long long steps[5][2] = {{d->x_row, d->x_head}, {d->residual_row, d->residual_head}, {d->sum_row, d->sum_head}, {d->y_row, d->y_head}, {d->quant_row, d->quant_head}};
+  void* const out[3] = {sum, y, d->quant ? quantised : nullptr};
+  const void* const in[2] = {x, residual};
+  for (int i = 0; i < 5; ++i)
+    if ((i < 2 ? in[i] || i == 0 : out[i - 2] != nullptr) && !strides_ok({{d->rows, steps[i][0]}, {d->heads, steps[i][1]}})) return -1;
+  if (d->rows == 0 || d->heads == 0) return 0;
+  for (int i = 0; i < 3; ++i)
+    if (out[i] && !apart(d->channels, {{d->rows, steps[i + 2][0]}, {d->heads, steps[i + 2][1]}})) return -1;
+  if (!x || (sum && !residual) || (!sum && !y && !d->quant) || (d->quant && (!quantised || !scales)) || (!d->quant && quantised)) return -1;
+  if (!element_aligned(d->dtype, {x, residual, sum, y}) || !element_aligned(d->weight_dtype, {weight}) || (uintptr_t)scales % 4) return -1;
+  // in place: where the input's rows lie; two results never share memory
+  for (int i = 0; i < 2; ++i)
+    for (int o = 0; o < 3; ++o)
+      if (in[i] && in[i] == out[o] && (o == 2 || !same_rows({{d->rows, steps[i][0], steps[o + 2][0]}, {d->heads, steps[i][1], steps[o + 2][1]}}))) return -1;
+  if ((sum && sum == y) || (out[2] && (out[2] == sum || out[2] == y))) return -1;
+  if (!have_device("odla_b200_rms_norm")) return -2;
+  RmsNorm n{};
+  n.dt = kStorage[d->dtype]; n.weight_dt = kStorage[d->weight_dtype];
+  n.heads = d->heads; n.channels = d->channels; n.quant = d->quant; n.group = d->group;
+  n.total = (unsigned)((long long)d->rows * d->heads);
+  n.epsilon = d->epsilon; n.weight_offset = d->weight_offset;
+  for (int i = 0; i < 5; ++i) { n.row[i] = steps[i][0]; n.head[i] = steps[i][1]; }
+  n.x = x; n.residual = residual; n.weight = weight; n.sum = sum; n.y = y; n.quantised = quantised; n.scales = scales;
+  return rms_norm(n, (cudaStream_t)stream);
+}
+
+extern "C" int odla_b200_chunk_attention(const odla_b200_paged_cache* c, const void* key_cache, const void* value_cache, const odla_b200_chunk_attention_desc* d, const void* q,
+                                         const int* starts, const int* prefix_pages, const int* page_table, const int* lengths, void* y, void* stream) {
+  if (!cache_ok(c) || !d || c->dtype == 0 || (c->channels != 64 && c->channels != 128)) return -1;
+  if (d->batch < 0 || d->tokens < 0 || d->heads < 1 || d->heads > 1024 || d->heads % c->heads || d->prefix_length < 0 || d->table_width < 0 || !std::isfinite(d->scale)) return -1;
+  if (!strides_ok({{d->tokens, d->q_token}, {d->heads, d->q_head}}) || !strides_ok({{d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
+  if (!apart(c->channels, {{d->tokens, d->y_token}, {d->heads, d->y_head}})) return -1;
+  for (long long s : {c->page, c->head, c->token, d->q_token, d->q_head, d->y_token, d->y_head})
+    if (s % 8) return -1;
+  // positions and rows (tokens and query heads) are counted in 32 bits
+  if ((long long)d->table_width * c->page_size + d->prefix_length >= (1ll << 30) || d->batch >= (1 << 20) || d->tokens >= (1 << 24) || (long long)d->tokens * d->heads >= (1ll << 28)) return -1;
+  if (d->batch == 0 || d->tokens == 0) return 0;
+  if (!key_cache || !value_cache || !q || !y || !starts || !lengths || (d->prefix_length && !prefix_pages) || (d->table_width && !page_table)) return -1;
+  if (!aligned16({key_cache, value_cache, q, y}) || (uintptr_t)starts % 4 || (uintptr_t)prefix_pages % 4 || (uintptr_t)page_table % 4 || (uintptr_t)lengths % 4) return -1;
+  if (q == y && !same_rows({{d->tokens, d->q_token, d->y_token}, {d->heads, d->q_head, d->y_head}})) return -1;
+  if (!have_device("odla_b200_chunk_attention")) return -2;
+  const ChunkAttention a{kStorage[c->dtype], d->batch, d->tokens, d->heads, c->heads, c->channels, c->pages, c->page_size, d->prefix_length, d->table_width, d->scale,
+                         c->page, c->head, c->token, d->q_token, d->q_head, d->y_token, d->y_head, key_cache, value_cache, q, starts, prefix_pages, page_table, lengths, y};
+  return chunk_attention(a, (cudaStream_t)stream);
+}
+
+extern "C" int odla_b200_log_probs(const odla_b200_log_probs_desc* d, const void* logits, const float* temperature, const int* tokens, float* token_log_probs, float* entropy,
+                                   int* top_tokens, float* top_log_probs, void* stream) {
+  if (!d || d->dtype < 0 || d->dtype > 2 || d->rows < 0 || d->rows > (1 << 24) || d->vocab < 1 || d->vocab > kMaxVocab || d->given < 0 || d->given > kMaxVocab || d->top < 0 ||
+      d->top > kMaxTop || !strides_ok({{d->rows, d->row}}))
+    return -1;
+  if (d->rows == 0) return 0;
+  if (!logits || !element_aligned(d->dtype, {logits}) || (d->given && (!tokens || !token_log_probs)) || (d->top && (!top_tokens || !top_log_probs))) return -1;
+  for (const void* p : {(const void*)temperature, (const void*)tokens, (const void*)token_log_probs, (const void*)entropy, (const void*)top_tokens, (const void*)top_log_probs})
+    if ((uintptr_t)p % 4) return -1;
+  if (!have_device("odla_b200_log_probs")) return -2;
+  return log_probs(LogProbs{kStorage[d->dtype], d->rows, d->vocab, d->given, d->top, d->row, logits, temperature, tokens, token_log_probs, entropy, top_tokens, top_log_probs},
+                   (cudaStream_t)stream);
 }

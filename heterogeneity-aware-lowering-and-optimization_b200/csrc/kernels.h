@@ -304,4 +304,41 @@ constexpr int kMaxVocab = 1 << 18;
 int sample(int dt, int rows, int vocab, int64_t row, const void* logits, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
            const float* uniform, int* tokens, cudaStream_t stream);
 
+// Root-mean-square norm of total = rows * heads rows (kernels_norm.cu); part 0: x, 1: residual, 2: sum, 3: y, 4: quantised.
+struct RmsNorm {
+  int dt, weight_dt, heads, channels, quant, group;
+  unsigned total;
+  float epsilon, weight_offset;
+  int64_t row[5], head[5];
+  const void *x, *residual, *weight;
+  void *sum, *y, *quantised;
+  float* scales;
+};
+int rms_norm(const RmsNorm& n, cudaStream_t stream);
+
+// Attention of the new tokens of each sequence over a paged cache (kernels_chunk_attention.cu); strides in elements.
+struct ChunkAttention {
+  int dt, batch, tokens, heads, kv_heads, channels, pages, page_size, prefix_length, table_width;
+  float scale;
+  int64_t c_page, c_head, c_token, q_token, q_head, y_token, y_head;
+  const void *k, *v, *q;
+  const int *starts, *prefix_pages, *page_table, *lengths;
+  void* y;
+};
+int chunk_attention(const ChunkAttention& a, cudaStream_t stream);
+
+// Log probabilities, entropy and the largest logits of each row (kernels_log_probs.cu).
+constexpr int kMaxTop = 64;
+struct LogProbs {
+  int dt, rows, vocab, given, top;
+  int64_t row;
+  const void* logits;
+  const float* temperature;
+  const int* tokens;
+  float *token_log_probs, *entropy;
+  int* top_tokens;
+  float* top_log_probs;
+};
+int log_probs(const LogProbs& l, cudaStream_t stream);
+
 }  // namespace b200

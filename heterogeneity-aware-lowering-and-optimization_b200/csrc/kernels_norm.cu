@@ -1,0 +1,256 @@
+// Root-mean-square norm, with the residual's addition in front of it and an output in 8 bits behind.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kMaxThreads = 1024, kShort = 32;   // threads of a row; of a row that shares its block with others
+
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+template <> struct Raw<4> { typedef uint32_t type; };
+template <> struct Raw<2> { typedef uint16_t type; };
+template <> struct Raw<1> { typedef uint8_t type; };
+// VEC elements that lie side by side, moved at once.
+template <typename T, int VEC> union Piece {
+  typename Raw<sizeof(T) * VEC>::type raw;
+  T e[VEC];
+  __device__ __forceinline__ Piece() {}
+};
+template <typename T> __device__ __forceinline__ float widen(T v);
+template <> __device__ __forceinline__ float widen<float>(float v) { return v; }
+template <> __device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint8_t e4m3(float v) { return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint8_t int8(float v) { return (uint8_t)(int8_t)min(127, max(-128, __float2int_rn(v))); }   // (NaN: 0)
+
+struct Params {
+  RmsNorm n;
+  int pieces, lanes;      // VEC channels each; threads of a row
+  int rows_of_block;      // 1, or rows of up to 32 threads each
+  int group_shift;        // a group is 1 << group_shift pieces of neighbouring threads; -1: the row; -2: any, counted in shared memory; -3: no scales to find
+};
+
+// h = round(x + residual), y = h / sqrt(mean(h h) + epsilon) * (w + offset), and y in 8 bits with scales.
+// Bound by memory: x and residual are read once and stay in registers (NP pieces of 16 bytes a thread), each result is written once.  Sums of squares
+// are 32-bit, by thread, then by warp, then by block.  A row of few pieces takes `lanes` threads of a warp and shares the block.
+// Largest magnitudes are compared as whole numbers, which order them and keep a NaN.
+template <typename T, int VEC, int NP>
+__global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint32_t tops[];      // of each group (group_shift -2)
+  __shared__ float sums[32];
+  __shared__ uint32_t largest[32];
+  const RmsNorm& n = p.n;
+  const int t = p.rows_of_block == 1 ? threadIdx.x : threadIdx.x % p.lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned at = p.rows_of_block == 1 ? blockIdx.x : blockIdx.x * p.rows_of_block + threadIdx.x / p.lanes;
+  const bool live = at < n.total;
+  const unsigned row = n.heads == 1 ? at : at / n.heads, head = at - row * n.heads;
+  auto place = [&](const void* base, int part) { return (T*)base + (int64_t)row * n.row[part] + (int64_t)head * n.head[part]; };
+  float h[NP][VEC];
+  float square = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  {
+    Piece<T, VEC> x[NP], r[NP];
+    const T *xp = place(n.x, 0), *rp = place(n.residual, 1);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = t + i * p.lanes;
+      const bool there = live && c < p.pieces;
+      if (there) x[i].raw = *(const decltype(x[i].raw)*)(xp + (int64_t)c * VEC);
+      if (there && n.residual) r[i].raw = *(const decltype(x[i].raw)*)(rp + (int64_t)c * VEC);
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = t + i * p.lanes;
+      const bool there = live && c < p.pieces;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        h[i][k] = there ? widen<T>(x[i].e[k]) : 0.f;
+        if (there && n.residual) {
+          x[i].e[k] = narrow<T>(h[i][k] + widen<T>(r[i].e[k]));
+          h[i][k] = widen<T>(x[i].e[k]);
+        }
+        square += h[i][k] * h[i][k];
+      }
+      if (there && n.sum) *(decltype(x[i].raw)*)(place(n.sum, 2) + (int64_t)c * VEC) = x[i].raw;
+    }
+  }
+  if (!n.y && !n.quant) return;
+  const int among = min(p.lanes, 32);
+  for (int o = among / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+  if (p.lanes > 32) {
+    if (lane == 0) sums[warp] = square;
+    if (p.group_shift == -2)
+      for (int g = threadIdx.x; g < n.channels / n.group; g += blockDim.x) tops[g] = 0;
+    __syncthreads();
+    square = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+  }
+  const float factor = 1.f / sqrtf(square / (float)n.channels + n.epsilon);
+  uint32_t top[NP];
+  uint32_t row_top = 0;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = t + i * p.lanes;
+    const bool there = live && c < p.pieces;
+    top[i] = 0;
+    if (!there) continue;
+    float w[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] = 1.f;
+    if (n.weight) {
+      if (n.weight_dt == DT_F32) {
+#pragma unroll
+        for (int k = 0; k < VEC; k += VEC >= 4 ? 4 : 1) {
+          constexpr int W = VEC >= 4 ? 4 : 1;
+          Piece<float, W> v;
+          v.raw = *(const decltype(v.raw)*)((const float*)n.weight + (int64_t)c * VEC + k);
+#pragma unroll
+          for (int e = 0; e < W; ++e) w[k + e] = v.e[e];
+        }
+      } else {
+        Piece<uint16_t, VEC> v;
+        v.raw = *(const decltype(v.raw)*)((const uint16_t*)n.weight + (int64_t)c * VEC);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) w[k] = n.weight_dt == DT_F16 ? __half2float(__ushort_as_half(v.e[k])) : __uint_as_float((uint32_t)v.e[k] << 16);
+      }
+    }
+    Piece<T, VEC> y;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      h[i][k] = h[i][k] * factor * (w[k] + n.weight_offset);
+      y.e[k] = narrow<T>(h[i][k]);
+      top[i] = max(top[i], __float_as_uint(h[i][k]) & 0x7fffffffu);
+    }
+    row_top = max(row_top, top[i]);
+    if (n.y) *(decltype(y.raw)*)(place(n.y, 3) + (int64_t)c * VEC) = y.raw;
+  }
+  if (!n.quant) return;
+  const float most = n.quant == 1 ? 127.f : 448.f;
+  const int64_t groups = n.group ? n.channels / n.group : 1;
+  if (p.group_shift == -1) {
+    for (int o = among / 2; o; o >>= 1) row_top = max(row_top, __shfl_xor_sync(~0u, row_top, o));
+    if (p.lanes > 32) {
+      if (lane == 0) largest[warp] = row_top;
+      __syncthreads();
+      row_top = __reduce_max_sync(~0u, lane < (int)(blockDim.x >> 5) ? largest[lane] : 0u);
+    }
+    if (live && t == 0) n.scales[at] = __uint_as_float(row_top) / most;
+  } else if (p.group_shift >= 0) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      for (int o = 1; o < 1 << p.group_shift; o <<= 1) top[i] = max(top[i], __shfl_xor_sync(~0u, top[i], o));
+      const int c = t + i * p.lanes;
+      if (live && c < p.pieces && (c & ((1 << p.group_shift) - 1)) == 0) n.scales[at * groups + (c >> p.group_shift)] = __uint_as_float(top[i]) / most;
+    }
+  } else if (p.group_shift == -2) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = t + i * p.lanes;
+      if (c < p.pieces) atomicMax(&tops[c * VEC / n.group], top[i]);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) n.scales[at * groups + g] = __uint_as_float(tops[g]) / most;
+  }
+  const float given = p.group_shift == -3 ? n.scales[0] : 0.f;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int c = t + i * p.lanes;
+    if (!live || c >= p.pieces) continue;
+    float inverse = 0.f;
+    if (p.group_shift != -3) {
+      const uint32_t u = p.group_shift == -1 ? row_top : p.group_shift == -2 ? tops[c * VEC / n.group] : top[i];
+      inverse = most / __uint_as_float(u);
+      if (u == 0 || u >= 0x7f800000u || inverse == INFINITY) inverse = u > 0x7f800000u ? __uint_as_float(u) : 0.f;
+    }
+    Piece<uint8_t, VEC> q;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float v = p.group_shift == -3 ? h[i][k] / given : h[i][k] * inverse;
+      q.e[k] = n.quant == 1 ? int8(v) : e4m3(v);
+    }
+    *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)row * n.row[4] + (int64_t)head * n.head[4] + (int64_t)c * VEC) = q.raw;
+  }
+}
+
+template <typename T> int launch(const RmsNorm& n, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  bool wide = n.channels % VEC == 0;
+  auto row = [&](const void* p, int part, int bytes) {
+    if (p) wide = wide && (uintptr_t)p % bytes == 0 && n.row[part] % VEC == 0 && n.head[part] % VEC == 0;
+  };
+  row(n.x, 0, 16); row(n.residual, 1, 16); row(n.sum, 2, 16); row(n.y, 3, 16);
+  if (n.quant) row(n.quantised, 4, VEC);
+  if (n.weight) wide = wide && (uintptr_t)n.weight % (n.weight_dt == DT_F32 ? 16 : 2 * VEC) == 0;
+  Params p{};
+  p.n = n;
+  const int vec = wide ? VEC : 1;
+  p.pieces = n.channels / vec;
+  if (n.quant && n.group == 0) p.group_shift = -3;
+  else if (!n.quant || n.group == n.channels) p.group_shift = -1;
+  else {
+    const int of = n.group / vec;
+    int shift = 0;
+    while (1 << shift < of) ++shift;
+    p.group_shift = n.group % vec == 0 && 1 << shift == of && of <= 32 ? shift : -2;
+  }
+  int threads;
+  if (wide && p.pieces <= kShort && p.group_shift != -2) {
+    p.lanes = 1;
+    while (p.lanes < p.pieces) p.lanes *= 2;
+    threads = 256;
+    p.rows_of_block = threads / p.lanes;
+  } else {
+    // one piece for each thread, up to 1024
+    p.rows_of_block = 1;
+    threads = std::max(64, std::min(kMaxThreads, (p.pieces + 31) / 32 * 32));
+    p.lanes = threads;
+  }
+  const int each = (p.pieces + p.lanes - 1) / p.lanes;
+  const size_t smem = p.group_shift == -2 ? sizeof(uint32_t) * (size_t)(n.channels / n.group) : 0;
+  void (*fn)(Params);
+  if (!wide) fn = each <= 8 ? norm_kernel<T, 1, 8> : norm_kernel<T, 1, 32>;
+  else if (each == 1) fn = norm_kernel<T, VEC, 1>;
+  else if (each == 2) fn = norm_kernel<T, VEC, 2>;
+  else if (each <= 4) fn = norm_kernel<T, VEC, 4>;
+  else fn = norm_kernel<T, VEC, VEC == 4 ? 8 : 4>;   // (32768 channels of two bytes are four pieces for each of 1024 threads)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((n.total + p.rows_of_block - 1) / p.rows_of_block);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, p) == cudaSuccess) return 0;
+  cudaGetLastError();
+  return -2;
+}
+
+}  // namespace
+
+int rms_norm(const RmsNorm& n, cudaStream_t stream) {
+  switch (n.dt) {
+    case DT_F32: return launch<float>(n, stream);
+    case DT_F16: return launch<__half>(n, stream);
+    case DT_BF16: return launch<__nv_bfloat16>(n, stream);
+  }
+  return -1;
+}
+
+}  // namespace b200

@@ -109,6 +109,20 @@ class SampleDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dtype", "rows", "vocab")] + [("row", C.c_longlong)]
 
 
+class RmsNormDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "weight_dtype", "rows", "heads", "channels", "quant", "group")] + [("epsilon", C.c_float), ("weight_offset", C.c_float)] + \
+               [(n, C.c_longlong) for n in ("x_row", "x_head", "residual_row", "residual_head", "sum_row", "sum_head", "y_row", "y_head", "quant_row", "quant_head")]
+
+
+class ChunkAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "tokens", "heads", "prefix_length", "table_width")] + [("scale", C.c_float)] + \
+               [(n, C.c_longlong) for n in ("q_token", "q_head", "y_token", "y_head")]
+
+
+class LogProbsDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "rows", "vocab", "given", "top")] + [("row", C.c_longlong)]
+
+
 def rotary_spec(frequency, axis=None, interleaved=False):
     """The odla_b200_rotary_spec whose pair i turns by position[axis[i]] * frequency[i] radians (axis None: one axis)."""
     frequency = [float(f) for f in frequency]
@@ -235,6 +249,9 @@ _OPTIONAL = {
     "odla_b200_paged_attention_workspace": (C.c_longlong, [C.POINTER(PagedCache), C.POINTER(PagedAttentionDesc)]),
     "odla_b200_paged_attention": (C.c_int, [C.POINTER(PagedCache), _V, _V, C.POINTER(PagedAttentionDesc), _V, _V, _V, _V, _V, _V, C.c_longlong, _V]),
     "odla_b200_sample": (C.c_int, [C.POINTER(SampleDesc), _V, _V, _V, _V, _V, _V, _V, _V]),
+    "odla_b200_rms_norm": (C.c_int, [C.POINTER(RmsNormDesc), _V, _V, _V, _V, _V, _V, _V, _V]),
+    "odla_b200_chunk_attention": (C.c_int, [C.POINTER(PagedCache), _V, _V, C.POINTER(ChunkAttentionDesc), _V, _V, _V, _V, _V, _V, _V]),
+    "odla_b200_log_probs": (C.c_int, [C.POINTER(LogProbsDesc), _V, _V, _V, _V, _V, _V, _V, _V]),
     "odla_cpuref_UsesReference": (C.c_int, []),
     "odla_cpuref_Threads": (C.c_int, []),
     "odla_cpuref_GetAccumulators": (C.c_longlong, [_V, C.c_char_p, _V, C.c_longlong]),

@@ -604,6 +604,68 @@ typedef struct {
 int odla_b200_sample(const odla_b200_sample_desc* desc, const void* logits, const float* temperature, const int* top_k,
                      const float* top_p, const float* min_p, const float* uniform, int* tokens, void* stream);
 
+/* ---- a prompt, beside the steps ------------------------------------------------------------
+ * Three more raw entry points under the same rules (device pointers on the current device, kernels only enqueued on `stream`, nothing
+ * allocated, no workspace, capturable; dtypes 0 = fp32, 1 = fp16, 2 = bf16; strides in elements; 0, -1 or -2; no rows is a valid call
+ * that does nothing): the norm in front of a decoder's products, attention of whole prompts or parts of them, and what a prompt's or a sampled
+ * token's probability was. */
+
+/* Root-mean-square norm of rows x heads rows of `channels` values (1 ... 32768), x[r * x_row + h * x_head + channel]; heads 1 for a hidden state, more for the query
+ * or key heads inside a projection's rows.
+ *   h = x + residual, rounded to dtype (residual NULL: h = x), stored to `sum` if that is not NULL;
+ *   y = h / sqrt(mean of h h over the row + epsilon) * (weight + weight_offset), 32 bits throughout, rounded once; stored to `y` if that is not NULL.
+ * weight: [channels] of weight_dtype, NULL: all ones (weight_offset is added to them, too).
+ * quant 1 or 2 stores y (not the rounded one) in 8 bits to `quantised`: int8 to the nearest, or e4m3 to the nearest.
+ *   group > 0 (a divisor of channels, a multiple of 8 or all of them): a scale for each group of channels, scales[(r * heads + h) * (channels / group) + g] =
+ *     max |y| / 127 (e4m3: / 448), and values y * (127 / max |y|).  A group of zeros has the scale 0 and values of 0, and so have values where
+ *     127 / max |y| passes the range of fp32.  A group with an infinity or a NaN has a scale that is none.
+ *   group 0: scales[0] is given (positive), values y / scales[0], saturated to -128 ... 127 (e4m3: -448 ... 448).
+ * sum, y may be x or residual with the same strides; other overlaps are not allowed.  At least one of sum (with residual), y, quantised is asked for. */
+typedef struct {
+  int dtype, weight_dtype;
+  int rows, heads, channels;
+  int quant, group;
+  float epsilon, weight_offset;
+  long long x_row, x_head, residual_row, residual_head, sum_row, sum_head, y_row, y_head, quant_row, quant_head;
+} odla_b200_rms_norm_desc;
+int odla_b200_rms_norm(const odla_b200_rms_norm_desc* desc, const void* x, const void* residual, const void* weight, void* sum, void* y, void* quantised,
+                       float* scales, void* stream);
+
+/* Attention of any number of new tokens of each sequence: prompts, parts of prompts and single tokens in one call.  Sequence b's new tokens are rows starts[b] ... starts[b + 1] - 1
+ * of q and y (starts: [batch + 1], from 0 to at most `tokens`, not falling), q[row * q_token + head * q_head].  They are the last of its lengths[b] own positions, which
+ * lie on page_table[b * table_width ...] behind the prefix_length positions that all sequences share (prefix_pages), as for
+ * odla_b200_paged_attention: token i of n sees the prefix and own positions 0 ... lengths[b] - n + i.  The cache holds the new tokens' keys and values
+ * already (odla_b200_paged_append in front).  Rows of y behind starts[batch] are left as they are.
+ * A token that sees nothing gets zeros, and so does one whose scores are all minus infinity; pages that the cache does not have are not
+ * seen, lengths beyond the table count as the table; what lies in slots that a token does not see may be anything, infinities and NaN included, and leaves its row alone.
+ * dtype fp16 or bf16, channels 64 or 128, 16-byte alignment as there.  starts, lengths, page_table, prefix_pages are device memory and are read when the kernel runs: a captured
+ * call follows them, and serves any batch of no more sequences and rows (unused sequences: starts[b] = starts[b + 1]).
+ * A bounded wait inside the kernel that expires gives rows of NaN. */
+typedef struct {
+  int batch, tokens, heads;
+  int prefix_length, table_width;
+  float scale;
+  long long q_token, q_head, y_token, y_head;
+} odla_b200_chunk_attention_desc;
+int odla_b200_chunk_attention(const odla_b200_paged_cache* cache, const void* key_cache, const void* value_cache, const odla_b200_chunk_attention_desc* desc,
+                              const void* q, const int* starts, const int* prefix_pages, const int* page_table, const int* lengths, void* y, void* stream);
+
+/* Log probabilities in rows of logits, logits[r * row + i], i < vocab (at most 262144), at a temperature (temperature: [rows], NULL or a value that is not above 0: 1):
+ *   log p_i = (l_i - max l) / T - log(sum over j of exp((l_j - max l) / T)), with sums in 32 bits: good to about 2^-20, absolutely or relatively.
+ * tokens: [rows][given] token numbers -> token_log_probs [rows][given], minus infinity for numbers that are no tokens (the tokens of odla_b200_sample, of a prompt,
+ * -1 in a padded batch).  entropy: [rows], -sum of p log p, or NULL.  top_tokens, top_log_probs: [rows][top], the top (0 ... 64) largest logits in descending
+ * order, ties in favour of the lower index; -1 and minus infinity where no token is left.
+ * A logit that is NaN or minus infinity has probability 0 (entropy: p log p = 0); infinities share all probability.  A row without any other than those of probability 0 gives minus infinity
+ * throughout and an entropy of 0. */
+#define ODLA_B200_MAX_TOP 64
+typedef struct {
+  int dtype;
+  int rows, vocab, given, top;
+  long long row;
+} odla_b200_log_probs_desc;
+int odla_b200_log_probs(const odla_b200_log_probs_desc* desc, const void* logits, const float* temperature, const int* tokens, float* token_log_probs, float* entropy,
+                        int* top_tokens, float* top_log_probs, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
