@@ -319,6 +319,21 @@ def test_chunk_bad_pages_are_not_seen(odla, gpu_lib, prefix, page):
     check_chunk(odla, gpu_lib, case)
 
 
+@pytest.mark.parametrize("new,cached", [([200], [600]), ([900] * 12, [1000] * 12)])
+def test_chunk_a_wait_that_runs_out_gives_nan_and_the_next_call_is_exact(odla, gpu_lib, monkeypatch, new, cached):
+    """The hook leaves one unit of the first block's ring unannounced; the products' wait for it ends after 256 attempts."""
+    case = chunk_case(1, new, [n + c for n, c in zip(new, cached)], 8, 2, 128, 16, 0, behind=0)
+    monkeypatch.setenv("ODLA_B200_TEST_SKIP_STAGE", "1")
+    monkeypatch.setenv("ODLA_B200_TEST_SPIN_LIMIT", "256")
+    y = P.call_chunk(odla, gpu_lib, *case, 0.09)
+    torch.cuda.synchronize()
+    bad = y.isnan().all(-1)
+    assert torch.equal(bad, y.isnan().any(-1)) and 0 < int(bad.sum()) <= 256
+    monkeypatch.delenv("ODLA_B200_TEST_SKIP_STAGE")
+    monkeypatch.delenv("ODLA_B200_TEST_SPIN_LIMIT")
+    check_chunk(odla, gpu_lib, case, scale=0.09)
+
+
 def test_chunk_sees_nothing(odla, gpu_lib):
     case = list(chunk_case(1, [3, 1, 20], [0, 1, 5], 4, 2, 64, 16, 0))
     case[7][0] = -5
