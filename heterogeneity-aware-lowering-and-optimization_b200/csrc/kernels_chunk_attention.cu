@@ -8,28 +8,34 @@
 namespace b200 {
 namespace {
 
-constexpr int kRows = 256, kStep = 128, kRing = 4, kLoaders = 2, kThreads = 12 * 32, kMaxShare = 16;
+constexpr int kRows = 256, kStep = 128, kSoftmax = 8, kLoaders = 2, kThreads = (kSoftmax + kLoaders + 2) * 32, kMaxShare = 16, kMostRing = 5, kSeen = 8;
+template <int D> constexpr int kRing = D == 128 ? 2 : 4;   // units of 128 keys, and as many of values; one more of values where a tile has no second half
+
 constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
 
 struct Params {
   ChunkAttention a;
   int group;                       // query heads of a cache head; rows of a sequence = its new tokens * group
-  int tiles, share;                // tiles of 256 rows that the batch can have; CTAs (a cluster) that share a tile's positions
+  int tile_rows, tiles, share;     // rows of a tile (128 or 256); tiles that the batch can have; CTAs (a cluster) that share a tile's positions
   float scale_log2e;
+  uint32_t group_factor, group_shift, page_factor, page_shift;   // n / group = n * factor >> shift for n < 2^30, n / page_size likewise
   int box_shift;                   // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
+  uint32_t group_bytes, half_bytes;   // in a unit: from eight positions to the next eight, from 64 channels to the next 64
   uint32_t spin_limit;
   int test_skip_stage;             // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
 
 struct Shared {
   float2 stat[kRows];       // reference (a base-2 exponent) and sum of each row
-  uint64_t full[kRing], empty[kRing], clean[kRing], q_full, s_full[2], p_half[2], p_full[2], o_done[2], handed, drained;
-  uint32_t seen[4][4];      // which of a step's positions lie on pages that are there; a step's words are written at most two steps ahead
+  uint64_t k_full[kMostRing], k_empty[kMostRing], v_full[kMostRing], v_empty[kMostRing], q_full, s_full[2], s_read[2], p_most[2], p_full[2], o_done[2], handed, all_done, drained[2];
+  uint32_t seen[kSeen][4];  // which of a step's positions lie on pages that are there; written at most a ring ahead of the step that is read
   uint32_t tmem;
   int abort, odd;           // odd: values that not all rows see, infinite or no numbers, were taken out of the products
-  int scan[kThreads / 32], found, sequence, tile;
+  int scan[kThreads / 32], found, sequence, tile, first_row, count, length;
 };
 
+__device__ __forceinline__ int token_of(const Params& p, int row) { return (int)((uint64_t)(uint32_t)row * p.group_factor >> p.group_shift); }
+__device__ __forceinline__ int page_of(const Params& p, int n) { return (int)((uint64_t)(uint32_t)n * p.page_factor >> p.page_shift); }
 __device__ __forceinline__ float2 load_remote2(uint32_t at) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
@@ -46,7 +52,7 @@ __device__ __forceinline__ bool odd16(uint32_t u, bool bf16) {   // one of two e
 
 // What a row sees of values that are infinite or no numbers, and that stay out of the products of a step that not all rows see whole: position for
 // position, from memory, onto its result (a weight is not zero, so that an infinity remains one).  Rare, and slow.
-template <typename T, int D> __device__ __noinline__ void add_odd(const Params& p, uint32_t row_at, bool wide, int head, const int* pages, int from, int to) {
+template <typename T, int D> __device__ __noinline__ void add_odd(const Params& p, uint32_t row_at, bool wide, int swizzle, int head, const int* pages, int from, int to) {
   for (int pos = from; pos < to; ++pos) {
     const int page = pages[pos / p.a.page_size];
     if (page < 0 || page >= p.a.pages) continue;
@@ -64,50 +70,89 @@ template <typename T, int D> __device__ __noinline__ void add_odd(const Params& 
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(row_at + (2 * c + h) * 4), "f"(y + x) : "memory");
         } else {
           unsigned short y;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(row_at + (2 * c + h) * 2) : "memory");
+          const uint32_t at = row_at + (uint32_t)(((c >> 2) ^ swizzle) << 4) + (uint32_t)((2 * c + h) & 7) * 2;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at) : "memory");
           const float z = (Mma<T>::kBf16 ? __uint_as_float((uint32_t)y << 16) : __half2float(__ushort_as_half(y))) + x;
-          asm volatile("st.shared.u16 [%0], %1;" ::"r"(row_at + (2 * c + h) * 2), "h"((unsigned short)(Mma<T>::pack(z, 0.f) & 0xffffu)) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((unsigned short)(Mma<T>::pack(z, 0.f) & 0xffffu)) : "memory");
         }
       }
     }
   }
 }
 
+// All 128 channels of a box's positions: eight positions of the first 64, then of the others.
+__device__ __forceinline__ void load_box_all(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int position, int head, int page) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(dst), "l"((uint64_t)map),
+               "r"(smem_u32(bar)), "r"(0), "r"(position), "r"(head), "r"(page)
+               : "memory");
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  asm("max.f32 %0, %0, %1, %2;" : "+f"(x) : "f"(y), "f"(z));
+  return x;
+}
+__device__ __forceinline__ void tie32(uint32_t (&r)[32]) {   // (no read of these registers comes before what stands in front)
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+
 // Up to 256 rows (token, query head of one cache head's group; two tiles of 128) of one sequence against the positions that they see, 128 at a
-// time: first the prefix's, then the sequence's own.  S = Q K^T goes to tensor memory; a thread per row turns it into weights, which replace it there
-// as the A operand of O += P V, and O stays in tensor memory.  A row's reference is not its running maximum but one that follows it only when it
-// has been passed by more than 2^8, so that O is rarely rescaled; in fp16, which has no numbers below 2^-24, it lies 2^7 lower, so that the many small weights
-// of a long context count together.
+// time: first the prefix's, then the sequence's own.  S = Q K^T goes to tensor memory, a thread per row takes it into registers and turns it into
+// weights, which go back as the A operand of O += P V, and O stays in tensor memory.  A row's reference is not its running maximum but one that
+// follows it only when it has been passed by more than 2^8, so that O is rarely rescaled; in fp16, which has no numbers below 2^-24, it lies 2^7
+// lower, so that the many small weights of a long context count together.
+// Tensor memory (512 columns, 128 channels): weights of the first tile 64, scores 128, weights of the second 64, O 128 each.  Both tiles use the same
+// columns for their scores, one after the other: they are free again as soon as they are in registers, so that the next scores never
+// wait for a softmax or for the products with its weights.  (Weights over each tile's own scores, two reads of them, no wait for registers: 3500
+// clocks a step of 2 x 128 x 128, 1420 of them a softmax warp's wait for scores that stood behind the last products.)
 // Rows are counted token by token, the heads of the group side by side: a tile covers few tokens, and little of its last steps is hidden from it.  Up to 128
 // rows leave the second tile free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
 // Where tiles are few, the CTAs of a cluster share the positions of each, by the lengths that they find, and every one joins some of the rows
 // out of the others' shared memory.
 // A weight of zero does not hide an infinity: in steps that some rows see less of than others, values that are infinite or no numbers are taken
 // out of shared memory before the product (and positions behind the last one, whatever lies there), and added to the rows that see them at the end.
-// Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products; 11: values of steps that not all see.
+// Warps 0-3 and 4-7: softmax of a tile each; 8 and 9: loads; 10: products for scores; 11: products with values, and
+// what they must not see.  A row's scores are 128 of the 168
+// registers that twelve warps leave a thread.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared w;
   constexpr int kBoxes = D / 64, kPieces = D / 8;
-  constexpr uint32_t kUnit = kBoxes * kBox;
-  const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem, s_ring = smem + 2 * kUnit;
+  constexpr uint32_t kUnit = kBoxes * kBox, kColumns = 512;
+  const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int item = blockIdx.x / p.share, rank = blockIdx.x - item * p.share, head = item % p.a.kv_heads;
+  if (threadIdx.x == 0) {
+    if (p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
+    for (int i = 0; i < kMostRing; ++i) { mbar_init(&w.k_full[i], kLoaders * 33); mbar_init(&w.k_empty[i], 1); mbar_init(&w.v_full[i], kLoaders * 33); mbar_init(&w.v_empty[i], 1); }
+
+    mbar_init(&w.q_full, kSoftmax);
+    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.s_read[t], 4); mbar_init(&w.p_most[t], 4); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
+    mbar_init(&w.handed, 4);
+    mbar_init(&w.all_done, 1);
+    for (int t = 0; t < 2; ++t) mbar_init(&w.drained[t], 1);
+    w.abort = 0;
+    w.odd = 0;
+    w.found = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_proxy();
+  }
   grid_dependency_wait();
   launch_dependents();
   // ---- the sequence that this tile is of: the last ones, which see the most, begin first ----
   {
     const int flat = p.tiles - 1 - item / p.a.kv_heads;
     int before = 0;
-    if (threadIdx.x == 0) w.found = 0;
     for (int b0 = 0; b0 < p.a.batch; b0 += kThreads) {
       const int b = b0 + threadIdx.x;
-      int n = 0;
+      int n = 0, lo = 0, hi = 0, length = 0;
       if (b < p.a.batch) {
-        const int lo = max(0, min(p.a.starts[b], p.a.tokens)), hi = max(lo, min(p.a.starts[b + 1], p.a.tokens));
-        n = ((hi - lo) * p.group + kRows - 1) / kRows;
+        lo = max(0, min(p.a.starts[b], p.a.tokens));
+        hi = max(lo, min(p.a.starts[b + 1], p.a.tokens));
+        length = (int)min((long long)max(p.a.lengths[b], 0), (long long)p.a.table_width * p.a.page_size);
+        n = ((hi - lo) * p.group + p.tile_rows - 1) / p.tile_rows;
       }
       int upto = n;
 #pragma unroll
@@ -115,197 +160,201 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         const int x = __shfl_up_sync(~0u, upto, o);
         if (lane >= o) upto += x;
       }
-      __syncthreads();
+      if (b0) __syncthreads();   // (the sums of the last turn have been read)
       if (lane == 31) w.scan[warp] = upto;
       __syncthreads();
       int all = 0;
+#pragma unroll
       for (int i = 0; i < kThreads / 32; ++i) {
         if (i < warp) upto += w.scan[i];
         all += w.scan[i];
       }
-      if (flat >= before + upto - n && flat < before + upto) { w.found = 1; w.sequence = b; w.tile = flat - (before + upto - n); }
+      if (flat >= before + upto - n && flat < before + upto) {
+        w.found = 1; w.sequence = b; w.tile = flat - (before + upto - n);
+        w.first_row = lo; w.count = hi - lo; w.length = length;
+      }
       before += all;
       if (before > flat) break;
     }
     __syncthreads();
     if (!w.found) return;   // (all of a cluster)
   }
-  const int b = w.sequence, first_row = max(0, min(p.a.starts[b], p.a.tokens)), count = max(first_row, min(p.a.starts[b + 1], p.a.tokens)) - first_row;
-  const int row0 = w.tile * kRows, n_rows = min(kRows, count * p.group - row0);
-  const int length = (int)min((long long)max(p.a.lengths[b], 0), (long long)p.a.table_width * p.a.page_size);
-  const int* own_pages = p.a.page_table + (int64_t)b * p.a.table_width;
+  const int first_row = w.first_row, count = w.count, length = w.length;
+  const int row0 = w.tile * p.tile_rows, n_rows = min(p.tile_rows, count * p.group - row0);
+  const int* own_pages = p.a.page_table + (int64_t)w.sequence * p.a.table_width;
   // own positions that row r of the sequence sees
-  auto limit_of = [&](int r) { return max(0, length - count + r / p.group + 1); };
+  auto limit_of = [&](int r) { return max(0, length - count + token_of(p, r) + 1); };
   const int prefix_steps = (p.a.prefix_length + kStep - 1) / kStep;
   const int least = limit_of(row0), most = limit_of(row0 + n_rows - 1);   // of this tile's first and last row
   const bool split = n_rows <= 128;
+  // Keys and values have rings of their own: whoever waits for one of them follows every turn of its place.
+  constexpr int kKeys = kRing<D>;
+  const int n_values = kRing<D> + split;
+  const uint32_t s_keys = smem + (split ? kUnit : 2 * kUnit), s_values = s_keys + kKeys * kUnit;
+  struct Place { int slot; uint32_t turn; };   // in a ring; the parity of the turn
+  auto next = [](Place& at, int ring) { if (++at.slot == ring) { at.slot = 0; at.turn ^= 1u; } };
   // steps of the whole tile, this CTA's share of them, and how many of those each half of the rows takes part in
   const int all_steps = prefix_steps + (most + kStep - 1) / kStep;
   const int first = (int)((int64_t)all_steps * rank / p.share), steps = (int)((int64_t)all_steps * (rank + 1) / p.share) - first;
-  int takes_part[2];
-  if (split) {
-    takes_part[0] = (steps + 1) / 2;
-    takes_part[1] = steps / 2;
-  } else {
-    takes_part[0] = max(0, min(steps, prefix_steps + (limit_of(row0 + 127) + kStep - 1) / kStep - first));
-    takes_part[1] = steps;
-  }
+  const int takes0 = split ? (steps + 1) / 2 : max(0, min(steps, prefix_steps + (limit_of(row0 + 127) + kStep - 1) / kStep - first)), takes1 = split ? steps / 2 : steps;
   // step i of this CTA: where it begins in its segment, where the segment ends (for the last row), its pages
   auto begin_of = [&](int i) { return (first + i < prefix_steps ? first + i : first + i - prefix_steps) * kStep; };
   auto end_of = [&](int i) { return first + i < prefix_steps ? p.a.prefix_length : most; };
   auto pages_of = [&](int i) { return first + i < prefix_steps ? p.a.prefix_pages : own_pages; };
-  constexpr uint32_t kColumns = 512;
-  if (threadIdx.x == 0) {
-    if (p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
-    for (int i = 0; i < kRing; ++i) { mbar_init(&w.full[i], kLoaders * 33); mbar_init(&w.empty[i], 1); mbar_init(&w.clean[i], 1); }
-    mbar_init(&w.q_full, split ? 4 : 8);
-    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.p_half[t], 4); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
-    mbar_init(&w.handed, 4);
-    mbar_init(&w.drained, 1);
-    w.abort = 0;
-    w.odd = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    fence_async_proxy();
-  }
-  if (warp == 8 + kLoaders) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = w.tmem;
   volatile int* abort_flag = &w.abort;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, nullptr, 0, p.spin_limit); };
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, wait(bar, parity)); };   // one answer for the warp
-  constexpr uint32_t kWideRow = D * 4 + 16, kNarrowRow = D * 2 + 16;   // (16 bytes apart from each other's banks)
+  constexpr uint32_t kWideRow = D * 4 + 16;   // (16 bytes apart from each other's banks)
+  const uint32_t wide_base = split ? s_keys : smem;
 
-  if (warp < 8) {
+  if (warp < kSoftmax) {
     // ------------------------------------------------------------------- softmax ----
     const int tile = warp >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane, r = split ? in_tile : tile * 128 + in_tile;
-    const bool live = r < n_rows;
-    const int row = row0 + (live ? r : n_rows - 1), j = row / p.group, g = row - j * p.group;
-    const int limit = limit_of(row);
-    // (a negative scale becomes the sign of the queries: the largest score is then the largest product)
-    if (!(split && tile)) {
-      const uint4* q = (const uint4*)((const T*)p.a.q + (int64_t)(first_row + j) * p.a.q_token + (int64_t)(head * p.group + g) * p.a.q_head);
-      const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u;
-      const uint32_t s_row = s_q + tile * kUnit + in_tile * 128;
+    const bool live = r < n_rows, any_live = r - lane < n_rows;   // of this thread, of its warp
+    {
+      // queries: sixteen (or eight) threads for a row.  A negative scale becomes the sign of the queries, the largest score is then the largest product; a scale
+      // of zero makes all products zero.
+      const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u, any = p.scale_log2e == 0.f ? 0u : ~0u;
+      const int per = split ? 16 : 32, c = lane % kPieces;
+      uint4 u[32 * kPieces / 32];
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        uint4 u = live ? q[c] : make_uint4(0, 0, 0, 0);
-        u.x ^= sign; u.y ^= sign; u.z ^= sign; u.w ^= sign;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_row + (c >> 3) * kBox + (((c & 7) ^ (r & 7)) << 4)), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+      for (int i = 0; i < kPieces; ++i) {
+        const int at = i * (32 / kPieces) + lane / kPieces, row = row0 + warp * per + at, j = token_of(p, row);
+        u[i] = make_uint4(0, 0, 0, 0);
+        if (at < per && warp * per + at < n_rows)
+          u[i] = *((const uint4*)((const T*)p.a.q + (int64_t)(first_row + j) * p.a.q_token + (int64_t)(head * p.group + row - j * p.group) * p.a.q_head) + c);
+      }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int at = i * (32 / kPieces) + lane / kPieces, q_row = warp * per + at;
+        if (at < per)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_q + (q_row >> 7) * kUnit + (c >> 3) * kBox + (q_row & 127) * 128 + (((c & 7) ^ (q_row & 7)) << 4)),
+                       "r"((u[i].x ^ sign) & any), "r"((u[i].y ^ sign) & any), "r"((u[i].z ^ sign) & any), "r"((u[i].w ^ sign) & any) : "memory");
       }
       fence_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&w.q_full);
     }
-    const float scale = fabsf(p.scale_log2e);
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, t_s = tmem + tile * 128 + lanes, t_o = tmem + 256 + tile * D + lanes;
+    const int row = row0 + (live ? r : n_rows - 1), j = token_of(p, row), limit = limit_of(row);
+    const float scale = p.scale_log2e == 0.f ? 1.f : fabsf(p.scale_log2e);
+    uint32_t tmem = 0;   // (of these lanes; known once the first scores are there)
+    const uint32_t to_p = tile * 192, to_o = 256 + tile * D;
     float reference = -INFINITY, sum = 0.f;
     bool ok = true;
-    const int own_steps = takes_part[tile];
+    const int own_steps = tile ? takes1 : takes0;
+    Place ku{0, 0}, vu{0, 0};
+    if (split && tile) next(ku, kKeys);
+    const bool frees = (split || tile) && quarter == 0 && lane == 0;
     for (int i = 0; i < own_steps; ++i) {
       const int step = split ? 2 * i + tile : i;
       if (!warp_wait(&w.s_full[tile], i & 1)) { ok = false; break; }
       tc_fence_after();
-      uint32_t seen[4];
-      const int sees = (first + step < prefix_steps ? p.a.prefix_length : limit) - begin_of(step);   // positions of this step, if their pages are there
+      if (i == 0) tmem = *(volatile uint32_t*)&w.tmem + ((uint32_t)(quarter * 32) << 16);
+      if (frees) mbar_arrive(&w.k_empty[ku.slot]);   // (the last scores with these keys)
+      next(ku, kKeys);
+      if (split) next(ku, kKeys);
+      uint32_t v[4][32];
+      if (any_live) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        seen[c] = *(volatile uint32_t*)&w.seen[step & 3][c];
-        seen[c] &= sees >= 32 * (c + 1) ? ~0u : sees <= 32 * c ? 0u : (1u << (sees - 32 * c)) - 1u;
+        for (int c = 0; c < 4; ++c) tmem_ld32(tmem + 64 + c * 32, v[c]);
+        tmem_ld_wait32(v[0]);
+#pragma unroll
+        for (int c = 1; c < 4; ++c) tie32(v[c]);
       }
-      const bool whole = __all_sync(~0u, (seen[0] & seen[1] & seen[2] & seen[3]) == ~0u);
-      float mx = -INFINITY;
-      auto largest = [&](auto all) {
-        uint32_t v[2][32];
-        tmem_ld32(t_s, v[0]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w.s_read[tile]);
+      if (any_live) {
+        // positions of this step that the row sees, if their pages are there
+        const int sees = (first + step < prefix_steps ? p.a.prefix_length : limit) - begin_of(step);
+        uint32_t seen[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait32(v[c & 1]);
-          if (c < 3) tmem_ld32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
-          float m4[4] = {mx, mx, mx, mx};
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float x[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] = decltype(all)::value || (seen[c] >> (k + h) & 1) ? __uint_as_float(v[c & 1][k + h]) : -INFINITY;
-            m4[k >> 1 & 3] = fmaxf(m4[k >> 1 & 3], fmaxf(x[0], x[1]));
-          }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          seen[c] = *(volatile uint32_t*)&w.seen[step % kSeen][c];
+          seen[c] &= sees >= 32 * (c + 1) ? ~0u : sees <= 32 * c ? 0u : (1u << (sees - 32 * c)) - 1u;
         }
-      };
-      if (whole) largest(True()); else largest(False());
-      mx = mx == -INFINITY ? mx : mx * scale - Mma<T>::kLift;   // (a scale of zero keeps it a number)
-      const bool passed = mx > (i ? reference + 8.f : -INFINITY);
-      if (__any_sync(~0u, passed)) {
-        const float next = passed ? mx : reference, corr = passed ? exp2_fast(reference - mx) : 1.f;
-        reference = next;
-        sum *= corr;
+        if (!__all_sync(~0u, (seen[0] & seen[1] & seen[2] & seen[3]) == ~0u)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!(seen[c] >> k & 1)) v[c][k] = 0xff800000u;
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) m4[k >> 1 & 3] = max3(m4[k >> 1 & 3], __uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1]));
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        mx = mx * scale - Mma<T>::kLift;
+        const bool passed = mx > (i ? reference + 8.f : -INFINITY);
+        // the last products with this tile's weights are done: theirs are the columns that the next weights go to
         if (i) {
+          if (!warp_wait(&w.o_done[tile], (i - 1) & 1)) { ok = false; break; }
+          if (frees && !split) mbar_arrive(&w.v_empty[vu.slot]);
+          next(vu, n_values);
+        }
+        if (__any_sync(~0u, passed)) {
+          const float next = passed ? mx : reference, corr = passed ? exp2_fast(reference - mx) : 1.f;
+          reference = next;
+          sum *= corr;
+          if (i) {
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld32(t_o + c * 32, v);
-            tmem_ld_wait32(v);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tmem + to_o + c * 16, o);
+              tmem_ld_wait_regs<16>(o);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t u[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(v[h * 16 + k]) * corr);
-              tmem_st16(t_o + c * 32 + h * 16, u);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+              tmem_st16(tmem + to_o + c * 16, o);
             }
           }
-          tmem_st_wait();
         }
-      }
-      const float base = reference == -INFINITY ? 0.f : reference;
-      const uint64_t scale2 = pair_of(scale, scale), base2 = pair_of(-base, -base);
-      auto weights = [&](auto all) {
-        uint32_t v[2][32], u[16];
-        uint64_t part = 0;   // two zeros
-        tmem_ld32(t_s, v[0]);
+        const float base = reference == -INFINITY ? 0.f : reference;
+        const uint64_t scale2 = pair_of(scale, scale), base2 = pair_of(-base, -base);
+        uint64_t part[2] = {0, 0};
+        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait32(v[c & 1]);
-          if (c < 3) tmem_ld32(t_s + (c + 1) * 32, v[(c + 1) & 1]);
+          uint32_t u[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             float e[2];
-            const uint64_t x = fma2(pair_of(v[c & 1][2 * k], v[c & 1][2 * k + 1]), scale2, base2);
-            if (k % 4 == 3) exp2_pair(x, e); else { unpack(x, e); e[0] = exp2_fast(e[0]); e[1] = exp2_fast(e[1]); }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (!decltype(all)::value && !(seen[c] >> (2 * k + h) & 1)) e[h] = 0.f;
-            part = add2(part, pair_of(e[0], e[1]));
+            const uint64_t x = fma2(pair_of(v[c][2 * k], v[c][2 * k + 1]), scale2, base2);
+            unpack(x, e);
+            e[0] = exp2_fast(e[0]);
+            e[1] = exp2_fast(e[1]);
+            part[k & 1] = add2(part[k & 1], pair_of(e[0], e[1]));
             u[k] = Mma<T>::pack(e[0], e[1]);
           }
-          tmem_st16(t_s + c * 16, u);   // (over scores that have been read)
-          if (c == 1) {   // the first half of the weights can be multiplied
+          tmem_st16(tmem + to_p + c * 16, u);
+          if (c == 2) {   // three quarters of the weights can be multiplied
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&w.p_half[tile]);
+            if (lane == 0) mbar_arrive(&w.p_most[tile]);
           }
         }
         float e[2];
-        unpack(part, e);
+        unpack(add2(part[0], part[1]), e);
         sum += e[0] + e[1];
-      };
-      if (whole) weights(True()); else weights(False());
-      tmem_st_wait();
+        tmem_st_wait();
+      } else {
+        if (i && !warp_wait(&w.o_done[tile], (i - 1) & 1)) { ok = false; break; }
+        if (lane == 0) mbar_arrive(&w.p_most[tile]);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&w.p_full[tile]);
     }
-    // All products done, queries and ring are free: the rows of the result go there, and each on as one copy, or to the CTAs that join them.
-    if (ok && takes_part[0]) ok = warp_wait(&w.o_done[0], 0);
-    if (ok && takes_part[1]) ok = warp_wait(&w.o_done[1], 0);
+    // This tile's products are done, its queries' memory is free: the rows of the result go there, and on in whole rows; or, as 32 bits, to the CTAs that
+    // join them or the other tile, once all products are done.
+    const bool hands = split && tile, takes = split && !tile && takes1, shared = p.share > 1, wide = hands || shared;
+    if (ok && own_steps) ok = warp_wait(&w.o_done[tile], (own_steps - 1) & 1);
+    if (ok && wide && steps) ok = warp_wait(&w.all_done, 0);   // (the other tile's o_done has phases that this one does not follow)
     tc_fence_after();
-    const bool hands = split && tile, takes = split && !tile && steps > 1, shared = p.share > 1;
-    const uint32_t wide_at = smem + (uint32_t)r * kWideRow;
+    const uint32_t wide_at = wide_base + (uint32_t)r * kWideRow;
     if (hands) w.stat[128 + in_tile] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
     float mine = 1.f, theirs = 0.f;
     if (takes) {
@@ -319,35 +368,39 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         reference = top;
       }
     }
-    const float inverse = shared || hands ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-    const bool wide = hands || shared;
-    // narrow rows lie behind the wide ones that the second tile hands over
-    const uint32_t row_at = wide ? wide_at : smem + (split ? 128 * kWideRow : 0) + (uint32_t)r * kNarrowRow;
-    if (ok && (own_steps || !hands)) {   // (nothing to hand over: the first tile does not wait, and its rows lie there)
+    const float inverse = wide ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    const uint32_t row_at = wide ? wide_at : s_q + tile * kUnit + (uint32_t)in_tile * (D * 2);
+    if (ok && any_live && (own_steps || !hands)) {   // (nothing to hand over: the first tile does not wait, and its rows lie there)
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
         if (own_steps) {
-          tmem_ld32(t_o + c * 32, v);
+          tmem_ld32(tmem + to_o + c * 32, v);
           tmem_ld_wait32(v);
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] = 0;
         }
+        if (takes) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float x[4] = {__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])};
-          if (takes) {
+          for (int k = 0; k < 8; ++k) {
             float y[4];
             asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(wide_at + c * 128 + k * 16) : "memory");
 #pragma unroll
-            for (int h = 0; h < 4; ++h) x[h] = x[h] * mine + y[h] * theirs;
+            for (int h = 0; h < 4; ++h) v[4 * k + h] = __float_as_uint(__uint_as_float(v[4 * k + h]) * mine + y[h] * theirs);
           }
-          if (wide) {
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + c * 128 + k * 16), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]) : "memory");
-          } else {
-            const uint32_t lo = Mma<T>::pack(x[0] * inverse, x[1] * inverse), hi = Mma<T>::pack(x[2] * inverse, x[3] * inverse);
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row_at + c * 64 + k * 8), "r"(lo), "r"(hi) : "memory");
+        }
+        if (wide) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + c * 128 + k * 16), "r"(v[4 * k]), "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3]) : "memory");
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t u[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) u[h] = Mma<T>::pack(__uint_as_float(v[8 * k + 2 * h]) * inverse, __uint_as_float(v[8 * k + 2 * h + 1]) * inverse);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((c * 4 + k) ^ (lane & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
           }
         }
       }
@@ -357,61 +410,71 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       if (lane == 0) mbar_arrive(&w.handed);
     } else {
       if (ok && *(volatile int*)&w.odd && live) {   // positions of this CTA's steps that this row sees and others do not
-        const int from = max(least, steps ? (max(first, prefix_steps) - prefix_steps) * kStep : 0), to = min(limit, (first + steps - prefix_steps) * kStep);
-        add_odd<T, D>(p, row_at, wide, head, own_pages, from, to);
+        const int from = max(least, (max(first, prefix_steps) - prefix_steps) * kStep), to = min(limit, (first + steps - prefix_steps) * kStep);
+        add_odd<T, D>(p, row_at, wide, lane & 7, head, own_pages, from, to);
       }
       if (shared) {
         w.stat[r] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
-      } else if (live) {
-        T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + g) * p.a.y_head;
-        if (ok) {
-          fence_async_proxy();
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(y), "r"(row_at), "n"(D * 2) : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        } else {
-          for (int c = 0; c < kPieces; ++c) ((uint4*)y)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);   // (no numbers)
+      } else if (any_live) {
+        __syncwarp();
+        const int64_t y_at = (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
+        const int c = lane % kPieces;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int at = i * (32 / kPieces) + lane / kPieces;
+          const int64_t to = __shfl_sync(~0u, y_at, at);
+          uint32_t u[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(row_at + (uint32_t)(at - lane) * (D * 2) + ((c ^ (at & 7)) << 4)) : "memory");
+          if (!ok) u[0] = u[1] = u[2] = u[3] = ~0u;   // (no numbers)
+          if (r - lane + at < n_rows) *(uint4*)((T*)p.a.y + to + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
         }
       }
     }
     tc_fence_before();
-  } else if (warp < 8 + kLoaders) {
+  } else if (warp < kSoftmax + kLoaders) {
     // --------------------------------------------------------------------- loads ----
-    const int part = warp - 8;
+    const int part = warp - kSoftmax;
     const T *kc = (const T*)p.a.k + (int64_t)head * p.a.c_head, *vc = (const T*)p.a.v + (int64_t)head * p.a.c_head;
     // Page numbers are asked for one step early: of the box that this lane brings, or of the positions whose copies it knows the address of.
     constexpr int kEach = 4 / kLoaders;   // groups of 32 positions
     int page[kEach], box_page = -1;
     int64_t off[kEach];
     const int boxes = p.box_shift ? kStep >> p.box_shift : 0;
+    const bool both = kBoxes == 2 && p.half_bytes == 1024;   // (a box brings all channels of its positions)
     auto position = [&](int step, int h) { return begin_of(step) + (part * kEach + h) * 32 + lane; };
     auto ask = [&](int step) {
       if (step >= steps) return;
       if (p.box_shift) {
         const int at = begin_of(step) + (lane << p.box_shift);
-        box_page = lane < boxes && at < end_of(step) ? pages_of(step)[at / p.a.page_size] : -1;
+        box_page = lane < boxes && at < end_of(step) ? pages_of(step)[page_of(p, at)] : -1;
       } else {
 #pragma unroll
-        for (int h = 0; h < kEach; ++h) page[h] = position(step, h) < end_of(step) ? pages_of(step)[position(step, h) / p.a.page_size] : -1;
+        for (int h = 0; h < kEach; ++h) page[h] = position(step, h) < end_of(step) ? pages_of(step)[page_of(p, position(step, h))] : -1;
       }
     };
-    int box_coord = 0, box_at = 0, loaded = 0;
+    int box_coord = 0, box_at = 0;
+    Place ku{0, 0}, vu{0, 0};
     ask(0);
-    for (int u = 0; u < 2 * steps; loaded = ++u) {
+    for (int u = 0; u < 2 * steps; ++u) {
       const int step = u >> 1;
-      uint64_t* full = &w.full[u % kRing];
-      const uint32_t dst = s_ring + (u % kRing) * kUnit;
-      if (!warp_wait(&w.empty[u % kRing], ((u / kRing) & 1) ^ 1)) break;
+      const Place at = (u & 1) ? vu : ku;
+      uint64_t* full = (u & 1) ? &w.v_full[at.slot] : &w.k_full[at.slot];
+      const uint32_t dst = ((u & 1) ? s_values : s_keys) + at.slot * kUnit;
+      if (!warp_wait((u & 1) ? &w.v_empty[at.slot] : &w.k_empty[at.slot], at.turn ^ 1u)) break;
+      if (u & 1) next(vu, n_values); else next(ku, kKeys);
       const bool skip = p.test_skip_stage && blockIdx.x == 0 && u == 1;
       if (p.box_shift) {
         if (!(u & 1)) {
           const bool there = box_page >= 0 && box_page < p.a.pages;
           box_coord = there ? box_page : p.a.pages;   // (past the last page: zeros)
-          box_at = (begin_of(step) + (lane << p.box_shift)) % p.a.page_size;
+          {
+            const int at = begin_of(step) + (lane << p.box_shift);
+            box_at = at - page_of(p, at) * p.a.page_size;
+          }
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const uint32_t seen = __ballot_sync(~0u, __shfl_sync(~0u, there, (h * 32 + lane) >> p.box_shift));
-            if (lane == 0 && part == 0) *(volatile uint32_t*)&w.seen[step & 3][h] = seen;
+            if (lane == 0 && part == 0) *(volatile uint32_t*)&w.seen[step % kSeen][h] = seen;
           }
           ask(step + 1);
         }
@@ -419,17 +482,22 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         mbar_arrive(full);
         if (lane == 0) { if (part == 0) mbar_expect_tx(full, kUnit); else mbar_arrive(full); }
         if (part == 0 && lane < boxes) {
+          const CUtensorMap* map = (u & 1) ? &values : &keys;
+          const uint32_t to = dst + ((uint32_t)lane << p.box_shift >> 3) * p.group_bytes;
+          if (both) load_box_all(to, map, full, box_at, head, box_coord);
+          else {
 #pragma unroll
-          for (int c = 0; c < kBoxes; ++c) load_box(dst + c * kBox + (lane << p.box_shift) * 128, (u & 1) ? &values : &keys, full, c * 64, box_at, head, box_coord);
+            for (int c = 0; c < kBoxes; ++c) load_box(to + c * p.half_bytes, map, full, c * 64, box_at, head, box_coord);
+          }
         }
         continue;
       }
       if (!(u & 1)) {
 #pragma unroll
         for (int h = 0; h < kEach; ++h) {
-          off[h] = page[h] >= 0 && page[h] < p.a.pages ? page[h] * p.a.c_page + (int64_t)(position(step, h) % p.a.page_size) * p.a.c_token : -1;
+          off[h] = page[h] >= 0 && page[h] < p.a.pages ? page[h] * p.a.c_page + (int64_t)(position(step, h) - page_of(p, position(step, h)) * p.a.page_size) * p.a.c_token : -1;
           const uint32_t seen = __ballot_sync(~0u, off[h] >= 0);
-          if (lane == 0) *(volatile uint32_t*)&w.seen[step & 3][part * kEach + h] = seen;
+          if (lane == 0) *(volatile uint32_t*)&w.seen[step % kSeen][part * kEach + h] = seen;
         }
         ask(step + 1);
       }
@@ -452,168 +520,247 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (*abort_flag && lane == 0)
-      for (int i = 0; i < kRing; ++i) await_landing(&w.full[i], loaded > i ? (uint32_t)((loaded - 1 - i) / kRing & 1) : 1u);   // boxes in flight land before their memory goes
-  } else if (warp == 8 + kLoaders && elect_one()) {
+    if (*abort_flag && lane == 0) {   // boxes in flight land before their memory goes
+      await_stages(w.k_full, kKeys, ku.slot, ku.turn ^ 1u);
+      await_stages(w.v_full, n_values, vu.slot, vu.turn ^ 1u);
+    }
+  } else {
     // ------------------------------------------------------------------ products ----
+    // One thread issues those for scores, one of another warp those with values: what each does between its products would otherwise keep the tensor cores
+    // waiting (one thread for both: 2750 clocks a step with a softmax that computes nothing).
     const uint32_t fmt = Mma<T>::kBf16 ? 1u : 0u, common = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
-    const uint32_t idesc_s = common | ((uint32_t)(kStep >> 3) << 17), idesc_o = common | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // (V lies with channels innermost)
-    const uint64_t hi = (uint64_t)(((8u * 128u) >> 4) | (1u << 14) | (2u << 29)) << 32;
-    // the distance between two boxes of channels is only read for V, whose 64-channel groups are a box apart
-    auto desc = [&](uint32_t at, uint32_t lead) { return hi | ((uint64_t)lead << 16) | (uint64_t)((at & 0x3FFFF) >> 4); };
-    // (keys and values were written by copies or stores of other threads, which the barrier has told of: the fence makes them visible to the products)
-    auto landed = [&](uint64_t* bars, int u) {
-      const bool there = wait(&bars[u % kRing], (u / kRing) & 1);
-      fence_async_proxy();
+    // the distance between groups of eight rows; the distance between 64 channels and the next 64 is only read for values, which lie with channels innermost
+    auto desc = [&](uint32_t at, uint32_t lead, uint32_t group) {
+      return (uint64_t)((group >> 4) | (1u << 14) | (2u << 29)) << 32 | (uint64_t)(lead >> 4) << 16 | (uint64_t)((at & 0x3FFFF) >> 4);
+    };
+    // (16-byte copies of other threads, which the barrier has told of: the fence makes them visible to the products; boxes are)
+    auto landed = [&](uint64_t* full, const Place& at) {
+      const bool there = wait(&full[at.slot], at.turn);
+      if (!p.box_shift) fence_async_proxy();
       return there;
     };
-    bool ok = steps == 0 || wait(&w.q_full, 0);
-    auto scores = [&](int i, int t) {   // S_t = Q_t K_i^T
-      const uint32_t k = s_ring + (2 * i % kRing) * kUnit, q = s_q + (split ? 0u : t * kUnit);
+    // Split, a tile has every other step.
+    if (warp == kSoftmax + kLoaders) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+      const uint32_t tmem = *(volatile uint32_t*)&w.tmem;
+      if (elect_one()) {
+        const uint32_t idesc = common | ((uint32_t)(kStep >> 3) << 17), half = p.half_bytes >> 4;   // (64 channels further)
+        const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_keys, 16, p.group_bytes);
+        int last = -1, last_turn = 0;   // the tile whose scores came last: these wait until they are in registers
+        Place at{0, 0};
+        bool ok = steps == 0 || wait(&w.q_full, 0);
+        for (int i = 0; i < steps && ok; ++i, next(at, kKeys)) {
+          ok = landed(w.k_full, at);
+          const uint64_t k = k_desc + (uint32_t)at.slot * (kUnit >> 4);
+          for (int t = split ? i & 1 : i < takes0 ? 0 : 1; t < 2 && ok; t += split ? 2 : 1) {
+            if (last >= 0) ok = wait(&w.s_read[last], last_turn & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t q = q_desc + (split ? 0u : t * (kUnit >> 4));
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n)
-        umma_f16(tmem + t * 128, desc(q + (n >> 2) * kBox + (n & 3) * 32, 1), desc(k + (n >> 2) * kBox + (n & 3) * 32, 1), idesc_s, n ? 1u : 0u);
-      umma_commit(&w.s_full[t]);
-    };
-    // Every tile takes every step that its rows see any of; split, step i belongs to tile i & 1, whose next one is i + 2.
-    const int ahead = split ? 2 : 1;
-    auto has = [&](int i, int t) { return split ? (i & 1) == t : i < takes_part[t]; };
-    for (int i = 0; i < min(ahead, steps) && ok; ++i) {
-      ok = landed(w.full, 2 * i);
-      if (!ok) break;
-      tc_fence_after();
-      for (int t = 0; t < 2; ++t) if (has(i, t)) scores(i, t);
-      umma_commit(&w.empty[2 * i % kRing]);
-    }
-    for (int i = 0; i < steps && ok; ++i) {
-      const int vu = 2 * i + 1, ku = 2 * (i + ahead), turn = split ? i >> 1 : i;
-      const bool more = i + ahead < steps;
-      ok = landed(w.clean, vu);
-      bool keys_there = false;
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (!has(i, t)) continue;
-        const uint32_t v = s_ring + (vu % kRing) * kUnit;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {   // half of the weights while the other half is worked out
-          ok = ok && wait(h ? &w.p_full[t] : &w.p_half[t], turn & 1);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int n = h * 4; n < h * 4 + 4; ++n)
-            umma_tmem_a(tmem + 256 + t * D, tmem + t * 128 + n * 8, desc(v + n * 2048, kBox >> 4), idesc_o, (turn || n) ? 1u : 0u);
-        }
-        if (!ok) break;
-        if (t == 1 || split) umma_commit(&w.empty[vu % kRing]);
-        if (!more || !has(i + ahead, t)) { umma_commit(&w.o_done[t]); continue; }
-        if (!keys_there) { ok = landed(w.full, ku); keys_there = true; }
-        if (!ok) break;
-        tc_fence_after();
-        scores(i + ahead, t);
-        if (t == 1 || split) umma_commit(&w.empty[ku % kRing]);
-      }
-    }
-    if (!ok) { umma_commit(&w.drained); await_landing(&w.drained, 0); }   // products in flight end before their memory goes
-  } else if (warp == 9 + kLoaders) {
-    // ------------------------------------------- values of steps that not all rows see ----
-    for (int i = 0; i < steps; ++i) {
-      const int u = 2 * i + 1;
-      if (!warp_wait(&w.full[u % kRing], (u / kRing) & 1)) break;
-      const int from = (first + i < prefix_steps ? p.a.prefix_length : least) - begin_of(i), end = end_of(i) - begin_of(i);   // seen by all; by any
-      if (from < kStep) {
-        const uint32_t at = s_ring + (u % kRing) * kUnit;
-        bool any = false;
-        for (int n = max(from, 0) * kPieces + lane; n < kStep * kPieces; n += 32) {
-          const int pos = n / kPieces, c = n % kPieces;
-          const uint32_t to = at + (c >> 3) * kBox + pos * 128 + (((c & 7) ^ (pos & 7)) << 4);
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(to) : "memory");
-          bool store = pos >= end;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (pos >= end) x[k] = 0;
-            else if (odd16(x[k], Mma<T>::kBf16)) {
-              store = any = true;
-              x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
-            }
+            for (int n = 0; n < D / 16; ++n)   // S = Q_t K^T
+              umma_f16(tmem + 64, q + (n >> 2) * (kBox >> 4) + (n & 3) * 2, k + (n >> 2) * half + (n & 3) * 2, idesc, n ? 1u : 0u);
+            umma_commit(&w.s_full[t]);   // (softmax warps tell the loaders, where they know, that keys and values have been used)
+            last = t;
+            last_turn = split ? i >> 1 : i;
           }
-          if (store) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
         }
-        if (any) *(volatile int*)&w.odd = 1;
-        fence_async_proxy();
+        if (!ok) { umma_commit(&w.drained[0]); await_landing(&w.drained[0], 0); }   // products in flight end before their memory goes
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w.clean[u % kRing]);
+    } else {
+      const uint32_t idesc = common | (1u << 16) | ((uint32_t)(D >> 3) << 17), sixteen = p.group_bytes >> 3;   // (16 positions further, in units of 16 bytes)
+      const uint64_t v_desc = desc(s_values, p.half_bytes, p.group_bytes);
+      const bool issues = elect_one();
+      uint32_t tmem = 0;
+      Place at{0, 0};
+      bool ok = true;
+      // (all lanes go through all steps, and leave together: the one that issues skips what is left when a wait has run out)
+      for (int i = 0; i < steps; ++i, next(at, n_values)) {
+        const int seen_by_all = (first + i < prefix_steps ? p.a.prefix_length : least) - begin_of(i), seen_by_any = end_of(i) - begin_of(i);
+        if (seen_by_all < kStep) {
+          // values that some rows do not see: those that are infinite or no numbers, and all behind the last position, go
+          __syncwarp();
+          if (!warp_wait(&w.v_full[at.slot], at.turn)) { ok = false; break; }
+          bool any = false;
+          for (int n = max(seen_by_all, 0) * kPieces + lane; n < kStep * kPieces; n += 32) {
+            const int pos = n / kPieces, c = n % kPieces;
+            const uint32_t to = s_values + at.slot * kUnit + (c >> 3) * p.half_bytes + (pos >> 3) * p.group_bytes + (pos & 7) * 128 + (((c & 7) ^ (pos & 7)) << 4);
+            uint32_t x[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(to) : "memory");
+            bool store = pos >= seen_by_any;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (pos >= seen_by_any) x[k] = 0;
+              else if (odd16(x[k], Mma<T>::kBf16)) {
+                store = any = true;
+                x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
+              }
+            }
+            if (store) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+          if (any) *(volatile int*)&w.odd = 1;
+          fence_async_proxy();
+          __syncwarp();
+        }
+        if (issues && ok) {
+          ok = landed(w.v_full, at);
+          const uint64_t v = v_desc + (uint32_t)at.slot * (kUnit >> 4);
+          const int turn = split ? i >> 1 : i;
+          for (int t = split ? i & 1 : i < takes0 ? 0 : 1; t < 2 && ok; t += split ? 2 : 1) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {   // O_t += P_t V
+              if (n == 0 || n == 6) {   // (most of them while the last quarter of the weights is worked out)
+                ok = ok && wait(n ? &w.p_full[t] : &w.p_most[t], turn & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (i < 2 && n == 0) tmem = *(volatile uint32_t*)&w.tmem;
+              }
+              umma_tmem_a(tmem + 256 + t * D, tmem + t * 192 + n * 8, v + n * sixteen, idesc, (turn || n) ? 1u : 0u);
+            }
+            if (!ok) break;
+            umma_commit(&w.o_done[t]);
+            if (split) umma_commit(&w.v_empty[at.slot]);
+          }
+        }
+      }
+      if (issues) {
+        if (ok) umma_commit(&w.all_done);
+        else { umma_commit(&w.drained[1]); await_landing(&w.drained[1], 0); }
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8 + kLoaders) {
+  if (warp == kSoftmax + kLoaders) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(w.tmem), "r"(kColumns) : "memory");
   }
   if (p.share > 1) {
     // ---- each CTA joins the rows that are its own modulo the cluster's size ----
     cluster_sync_all();
-    constexpr int N = D / 32;
-    const uint32_t stat = smem_u32(w.stat);
-    for (int r = rank + p.share * warp; r < n_rows; r += p.share * (kThreads / 32)) {
-      float2 st[kMaxShare];
-      float top = -INFINITY, sum = 0.f, acc[N];
+    if (warp < kSoftmax) {
+      constexpr int N = D / 32;
+      const uint32_t stat = smem_u32(w.stat);
+      for (int r = rank + p.share * warp; r < n_rows; r += p.share * kSoftmax) {
+        float2 st = make_float2(-INFINITY, 0.f);
+        if (lane < p.share) st = load_remote2(map_to_cta(stat + r * 8, lane));
+        float top = st.x, sum = 0.f, acc[N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] = 0.f;
+        for (int o = kMaxShare / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+        top = __shfl_sync(~0u, top, 0);
+        const float f = st.y != 0.f ? exp2_fast(st.x - (top == -INFINITY ? 0.f : top)) : 0.f;   // (a share without positions wrote no row)
 #pragma unroll
-      for (int i = 0; i < kMaxShare; ++i)
-        if (i < p.share) {
-          st[i] = load_remote2(map_to_cta(stat + r * 8, i));
-          top = fmaxf(top, st[i].x);
-        }
-      const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int i = 0; i < kMaxShare; ++i)
-        if (i < p.share && st[i].y != 0.f) {   // (a share without positions wrote no row)
+        for (int k = 0; k < N; ++k) acc[k] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < p.share; ++i) {
+          const float fi = __shfl_sync(~0u, f, i), si = __shfl_sync(~0u, st.y, i);
+          if (si == 0.f) continue;
           float x[N];
-          load_remote<N>(map_to_cta(smem + (uint32_t)r * kWideRow + lane * (N * 4), i), x);
-          const float f = exp2_fast(st[i].x - base);
-          sum += f * st[i].y;
+          load_remote<N>(map_to_cta(wide_base + (uint32_t)r * kWideRow + lane * (N * 4), i), x);
+          sum += fi * si;
 #pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] += f * x[k];
+          for (int k = 0; k < N; ++k) acc[k] += fi * x[k];
         }
-      const int row = row0 + r, j = row / p.group, g = row - j * p.group;
-      T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + g) * p.a.y_head + lane * N;
-      const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const int row = row0 + r, j = token_of(p, row);
+        T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head + lane * N;
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int k = 0; k < N; k += 2) *(uint32_t*)(y + k) = Mma<T>::pack(acc[k] * inverse, acc[k + 1] * inverse);
+        for (int k = 0; k < N; k += 2) *(uint32_t*)(y + k) = Mma<T>::pack(acc[k] * inverse, acc[k + 1] * inverse);
+      }
     }
     cluster_sync_all();   // (what the others read stays until they have)
   }
 }
+// Boxes of all 128 channels of eight positions of one head and page, as two halves.
+bool whole_box_map(CUtensorMap* m, const ChunkAttention& a, const void* base) {
+  if (!load_driver_entry_points()) return false;
+  auto bytes = [](int64_t stride, int extent) { return extent == 1 && stride == 0 ? (cuuint64_t)16 : (cuuint64_t)stride * 2; };
+  const cuuint64_t dims[5] = {64, (cuuint64_t)a.page_size, 2, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+  const cuuint64_t strides[4] = {bytes(a.c_token, a.page_size), 128, bytes(a.c_head, a.kv_heads), bytes(a.c_page, a.pages)};
+  for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return false;
+  const cuuint32_t box[5] = {64, 8, 2, 1, 1}, step[5] = {1, 1, 1, 1, 1};
+  return g_encode_tiled(m, a.dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, (void*)base, dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Fit {
+  int clusters[kMaxShare + 1];   // of each size, that run at the same time
+};
 
 template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
-  constexpr size_t smem = (size_t)(2 + kRing) * (D / 64) * kBox + 1024;
-  CUtensorMap keys{}, values{};
-  p.box_shift = 0;
-  int shift = 0;
-  while (shift < 7 && p.a.page_size % (2 << shift) == 0) ++shift;
-  if (shift >= 3 && box_map(&keys, p.a, p.a.k, 1 << shift) && box_map(&values, p.a, p.a.v, 1 << shift)) p.box_shift = shift;
+  constexpr size_t smem = (size_t)(2 + 2 * kRing<D>) * (D / 64) * kBox + 1024;
   auto* fn = chunk_kernel<T, D>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) { cudaGetLastError(); return -2; }
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return -2; }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.tiles * p.a.kv_heads * p.share));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.share;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return -2;
+  }
+  // How many clusters of each size fit: the same for every call (GPUs of this kind have the same SMs).
+  static const Fit fit = [&] {
+    Fit f{};
+    cfg.numAttrs = 1;
+    for (int i = 1; i <= kMaxShare; ++i) {
+      cfg.gridDim = dim3((unsigned)(i * 148));
+      attr[0].val.clusterDim.x = (unsigned)i;
+      if (cudaOccupancyMaxActiveClusters(&f.clusters[i], fn, &cfg) != cudaSuccess) { cudaGetLastError(); f.clusters[i] = 0; }
+    }
+    f.clusters[1] = std::max(f.clusters[1], 1);
+    return f;
+  }();
+  // Rows of a tile and CTAs that share it: the shortest estimate of waves of steps (1.2 us, 0.7 for 128 rows) and of what a CTA does before and after them
+  // (6 us, 2 more to join).  Lengths are not known here: the table's width stands for them.
+  const int64_t steps = ((int64_t)p.a.table_width * p.a.page_size + kStep - 1) / kStep + (p.a.prefix_length + kStep - 1) / kStep;
+  double best = 1e30;
+  for (int rows = kRows; rows >= 128; rows /= 2) {
+    // (a sequence's last tile has one row at least)
+    const int64_t tiles = ((int64_t)p.a.tokens * p.group + (int64_t)std::min(p.a.batch, p.a.tokens) * (rows - 1)) / rows, clusters = tiles * p.a.kv_heads;
+    for (int share = 1; share <= kMaxShare; ++share) {
+      if (fit.clusters[share] < 1 || (share > 1 && steps < 2 * share)) continue;
+      const int64_t waves = (clusters + fit.clusters[share] - 1) / fit.clusters[share];
+      const double us = (double)waves * ((double)((steps + share - 1) / share) * (rows == kRows ? 1.2 : 0.7) + (share > 1 ? 8.0 : 6.0));
+      if (us < best) { best = us; p.tile_rows = rows; p.tiles = (int)tiles; p.share = share; }
+    }
+  }
+  CUtensorMap keys{}, values{};
+  p.box_shift = 0;
+  p.group_bytes = 1024;
+  p.half_bytes = kBox;
+  int shift = 0;
+  while (shift < 7 && p.a.page_size % (2 << shift) == 0) ++shift;
+  // (boxes of eight positions bring both halves of the channels: the boxes of an SM begin some 85 clocks after one another, and 64 of them held a step at
+  // 5460 clocks)
+  if (D == 128 && shift == 3 && whole_box_map(&keys, p.a, p.a.k) && whole_box_map(&values, p.a, p.a.v)) {
+    p.box_shift = 3;
+    p.group_bytes = 2048;
+    p.half_bytes = 1024;
+  } else if (shift >= 3 && box_map(&keys, p.a, p.a.k, 1 << shift) && box_map(&values, p.a, p.a.v, 1 << shift)) {
+    p.box_shift = shift;
+  }
+  cfg.gridDim = dim3((unsigned)(p.tiles * p.a.kv_heads * p.share));
+  attr[0].val.clusterDim.x = (unsigned)p.share;
   cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, fn, p, keys, values) == cudaSuccess) return 0;
   cudaGetLastError();
   return -2;
+}
+
+// n / of = n * factor >> shift for n < 2^30: factor * of exceeds 2^shift by at most of <= 2^(shift - 30).
+void quotient(int of, uint32_t& factor, uint32_t& shift) {
+  shift = 0;
+  while ((1ll << shift) < of) ++shift;
+  shift += 30;
+  factor = (uint32_t)((1ull << shift) / of + 1);
 }
 
 }  // namespace
@@ -622,11 +769,8 @@ int chunk_attention(const ChunkAttention& a, cudaStream_t stream) {
   Params p{};
   p.a = a;
   p.group = a.heads / a.kv_heads;
-  // (a sequence's last tile has one row at least)
-  p.tiles = (int)(((int64_t)a.tokens * p.group + (int64_t)std::min(a.batch, a.tokens) * (kRows - 1)) / kRows);
-  const int64_t steps = ((int64_t)a.table_width * a.page_size + kStep - 1) / kStep + (a.prefix_length + kStep - 1) / kStep;
-  p.share = 1;
-  while (p.share < kMaxShare && (int64_t)p.tiles * a.kv_heads * p.share * 2 <= 148 && steps >= 4 * p.share) p.share *= 2;
+  quotient(p.group, p.group_factor, p.group_shift);
+  quotient(a.page_size, p.page_factor, p.page_shift);
   p.scale_log2e = a.scale * kLog2e;
   p.spin_limit = kSpinLimit;
   p.test_skip_stage = getenv("ODLA_B200_TEST_SKIP_STAGE") != nullptr;
