@@ -120,7 +120,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared w;
   constexpr int kBoxes = D / 64, kPieces = D / 8;
-  constexpr uint32_t kUnit = kBoxes * kBox, kColumns = 512;
+  constexpr uint32_t kUnit = kBoxes * kBox, kColumns = 512, tmem = 0;   // (all columns: they begin at the first, whatever a look at the allocation's word says, and when)
   const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int item = blockIdx.x / p.share, rank = blockIdx.x - item * p.share, head = item % p.a.kv_heads;
@@ -237,8 +237,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     }
     const int row = row0 + (live ? r : n_rows - 1), j = token_of(p, row), limit = limit_of(row);
     const float scale = p.scale_log2e == 0.f ? 1.f : fabsf(p.scale_log2e);
-    uint32_t tmem = 0;   // (of these lanes; known once the first scores are there)
-    const uint32_t to_p = tile * 192, to_o = 256 + tile * D;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, t_s = lanes + 64, t_p = lanes + tile * 192, t_o = lanes + 256 + tile * D;
     float reference = -INFINITY, sum = 0.f;
     bool ok = true;
     const int own_steps = tile ? takes1 : takes0;
@@ -249,14 +248,13 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       const int step = split ? 2 * i + tile : i;
       if (!warp_wait(&w.s_full[tile], i & 1)) { ok = false; break; }
       tc_fence_after();
-      if (i == 0) tmem = *(volatile uint32_t*)&w.tmem + ((uint32_t)(quarter * 32) << 16);
       if (frees) mbar_arrive(&w.k_empty[ku.slot]);   // (the last scores with these keys)
       next(ku, kKeys);
       if (split) next(ku, kKeys);
       uint32_t v[4][32];
       if (any_live) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tmem + 64 + c * 32, v[c]);
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, v[c]);
         tmem_ld_wait32(v[0]);
 #pragma unroll
         for (int c = 1; c < 4; ++c) tie32(v[c]);
@@ -303,11 +301,11 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
-              tmem_ld16(tmem + to_o + c * 16, o);
+              tmem_ld16(t_o + c * 16, o);
               tmem_ld_wait_regs<16>(o);
 #pragma unroll
               for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
-              tmem_st16(tmem + to_o + c * 16, o);
+              tmem_st16(t_o + c * 16, o);
             }
           }
         }
@@ -328,7 +326,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
             part[k & 1] = add2(part[k & 1], pair_of(e[0], e[1]));
             u[k] = Mma<T>::pack(e[0], e[1]);
           }
-          tmem_st16(tmem + to_p + c * 16, u);
+          tmem_st16(t_p + c * 16, u);
           if (c == 2) {   // three quarters of the weights can be multiplied
             tmem_st_wait();
             tc_fence_before();
@@ -375,7 +373,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
         if (own_steps) {
-          tmem_ld32(tmem + to_o + c * 32, v);
+          tmem_ld32(t_o + c * 32, v);
           tmem_ld_wait32(v);
         } else {
 #pragma unroll
@@ -543,7 +541,6 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     if (warp == kSoftmax + kLoaders) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-      const uint32_t tmem = *(volatile uint32_t*)&w.tmem;
       if (elect_one()) {
         const uint32_t idesc = common | ((uint32_t)(kStep >> 3) << 17), half = p.half_bytes >> 4;   // (64 channels further)
         const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_keys, 16, p.group_bytes);
@@ -572,7 +569,6 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       const uint32_t idesc = common | (1u << 16) | ((uint32_t)(D >> 3) << 17), sixteen = p.group_bytes >> 3;   // (16 positions further, in units of 16 bytes)
       const uint64_t v_desc = desc(s_values, p.half_bytes, p.group_bytes);
       const bool issues = elect_one();
-      uint32_t tmem = 0;
       Place at{0, 0};
       bool ok = true;
       // (all lanes go through all steps, and leave together: the one that issues skips what is left when a wait has run out)
@@ -614,7 +610,6 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
                 ok = ok && wait(n ? &w.p_full[t] : &w.p_most[t], turn & 1);
                 if (!ok) break;
                 tc_fence_after();
-                if (i < 2 && n == 0) tmem = *(volatile uint32_t*)&w.tmem;
               }
               umma_tmem_a(tmem + 256 + t * D, tmem + t * 192 + n * 8, v + n * sixteen, idesc, (turn || n) ? 1u : 0u);
             }
@@ -634,7 +629,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   __syncthreads();
   if (warp == kSoftmax + kLoaders) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(w.tmem), "r"(kColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
   }
   if (p.share > 1) {
     // ---- each CTA joins the rows that are its own modulo the cluster's size ----
