@@ -24,6 +24,10 @@ template <> struct Mma<__half> {
     const __half2 h = __floats2half2_rn(x, y);
     return *(const uint32_t*)&h;
   }
+  static __device__ __forceinline__ uint32_t times_zero(uint32_t x, uint32_t sum) {   // of two values, plus the sum
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+    return sum;
+  }
   static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {   // adds the values as rounded
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
@@ -41,6 +45,10 @@ template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *(const uint32_t*)&h;
+  }
+  static __device__ __forceinline__ uint32_t times_zero(uint32_t x, uint32_t sum) {
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+    return sum;
   }
   static __device__ __forceinline__ uint32_t pack(float x, float y, float& sum) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);

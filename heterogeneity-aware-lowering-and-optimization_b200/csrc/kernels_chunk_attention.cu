@@ -1,5 +1,6 @@
 // Attention of the new tokens of each sequence of a batch over a paged cache.
 #include <algorithm>
+#include <cstddef>
 #include <cstdlib>
 
 #include "attention.cuh"
@@ -16,6 +17,7 @@ constexpr uint32_t kBox = 16384;   // 128 rows of 128 bytes
 struct Params {
   ChunkAttention a;
   int group;                       // query heads of a cache head; rows of a sequence = its new tokens * group
+  int capacity;                    // positions that a sequence's table has room for
   int tile_rows, tiles, share;     // rows of a tile (128 or 256); tiles that the batch can have; CTAs (a cluster) that share a tile's positions
   float scale_log2e;
   uint32_t group_factor, group_shift, page_factor, page_shift;   // n / group = n * factor >> shift for n < 2^30, n / page_size likewise
@@ -25,9 +27,10 @@ struct Params {
   int test_skip_stage;             // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
 
+constexpr int kBarriers = 4 * kMostRing + 15;
 struct Shared {
   float2 stat[kRows];       // reference (a base-2 exponent) and sum of each row
-  uint64_t k_full[kMostRing], k_empty[kMostRing], v_full[kMostRing], v_empty[kMostRing], q_full, s_full[2], s_read[2], p_most[2], p_full[2], o_done[2], handed, all_done, drained[2];
+  uint64_t k_full[kMostRing], v_full[kMostRing], k_empty[kMostRing], v_empty[kMostRing], q_full, s_full[2], s_read[2], p_most[2], p_full[2], o_done[2], handed, all_done, drained[2];
   uint32_t seen[kSeen][4];  // which of a step's positions lie on pages that are there; written at most a ring ahead of the step that is read
   uint32_t tmem;
   int abort, odd;           // odd: values that not all rows see, infinite or no numbers, were taken out of the products
@@ -123,21 +126,22 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   constexpr uint32_t kUnit = kBoxes * kBox, kColumns = 512, tmem = 0;   // (all columns: they begin at the first, whatever a look at the allocation's word says, and when)
   const uint32_t smem = (shared_address(smem_raw) + 1023u) & ~1023u, s_q = smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int item = blockIdx.x / p.share, rank = blockIdx.x - item * p.share, head = item % p.a.kv_heads;
-  if (threadIdx.x == 0) {
-    if (p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
-    for (int i = 0; i < kMostRing; ++i) { mbar_init(&w.k_full[i], kLoaders * 33); mbar_init(&w.k_empty[i], 1); mbar_init(&w.v_full[i], kLoaders * 33); mbar_init(&w.v_empty[i], 1); }
-
-    mbar_init(&w.q_full, kSoftmax);
-    for (int t = 0; t < 2; ++t) { mbar_init(&w.s_full[t], 1); mbar_init(&w.s_read[t], 4); mbar_init(&w.p_most[t], 4); mbar_init(&w.p_full[t], 4); mbar_init(&w.o_done[t], 1); }
-    mbar_init(&w.handed, 4);
-    mbar_init(&w.all_done, 1);
-    for (int t = 0; t < 2; ++t) mbar_init(&w.drained[t], 1);
-    w.abort = 0;
-    w.odd = 0;
-    w.found = 0;
+  const int item = p.share == 1 ? blockIdx.x : blockIdx.x / p.share, rank = blockIdx.x - item * p.share, head = item % p.a.kv_heads;
+  if (warp == kSoftmax + kLoaders) {
+    // (early: it takes a microsecond, which nobody but this warp waits for.  No other block that holds tensor memory fits beside this one, whose threads take all registers.)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 0) {   // a barrier for each lane, and how often it is arrived at
+    static_assert(offsetof(Shared, drained) + sizeof(w.drained) - offsetof(Shared, k_full) == 8 * kBarriers, "barriers lie side by side");
+    if (lane == 0) { w.abort = 0; w.odd = 0; w.found = 0; }
+    for (int i = lane; i < kBarriers; i += 32) {
+      uint64_t* bar = &w.k_full[0] + i;
+      mbar_init(bar, bar < w.k_empty ? kLoaders * 33 : bar == &w.q_full ? kSoftmax : (bar >= w.s_read && bar < w.o_done) || bar == &w.handed ? 4 : 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_proxy();
+    if (lane == 0 && p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
   }
   grid_dependency_wait();
   launch_dependents();
@@ -151,7 +155,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       if (b < p.a.batch) {
         lo = max(0, min(p.a.starts[b], p.a.tokens));
         hi = max(lo, min(p.a.starts[b + 1], p.a.tokens));
-        length = (int)min((long long)max(p.a.lengths[b], 0), (long long)p.a.table_width * p.a.page_size);
+        length = min(max(p.a.lengths[b], 0), p.capacity);
         n = ((hi - lo) * p.group + p.tile_rows - 1) / p.tile_rows;
       }
       int upto = n;
@@ -177,7 +181,10 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       if (before > flat) break;
     }
     __syncthreads();
-    if (!w.found) return;   // (all of a cluster)
+    if (!w.found) {   // (all of a cluster)
+      if (warp == kSoftmax + kLoaders) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+      return;
+    }
   }
   const int first_row = w.first_row, count = w.count, length = w.length;
   const int row0 = w.tile * p.tile_rows, n_rows = min(p.tile_rows, count * p.group - row0);
@@ -195,7 +202,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   auto next = [](Place& at, int ring) { if (++at.slot == ring) { at.slot = 0; at.turn ^= 1u; } };
   // steps of the whole tile, this CTA's share of them, and how many of those each half of the rows takes part in
   const int all_steps = prefix_steps + (most + kStep - 1) / kStep;
-  const int first = (int)((int64_t)all_steps * rank / p.share), steps = (int)((int64_t)all_steps * (rank + 1) / p.share) - first;
+  const int first = p.share == 1 ? 0 : all_steps * rank / p.share, steps = (p.share == 1 ? all_steps : all_steps * (rank + 1) / p.share) - first;   // (2^23 steps at most)
   const int takes0 = split ? (steps + 1) / 2 : max(0, min(steps, prefix_steps + (limit_of(row0 + 127) + kStep - 1) / kStep - first)), takes1 = split ? steps / 2 : steps;
   // step i of this CTA: where it begins in its segment, where the segment ends (for the last row), its pages
   auto begin_of = [&](int i) { return (first + i < prefix_steps ? first + i : first + i - prefix_steps) * kStep; };
@@ -369,37 +376,40 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     const float inverse = wide ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
     const uint32_t row_at = wide ? wide_at : s_q + tile * kUnit + (uint32_t)in_tile * (D * 2);
     if (ok && any_live && (own_steps || !hands)) {   // (nothing to hand over: the first tile does not wait, and its rows lie there)
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[32];
-        if (own_steps) {
-          tmem_ld32(t_o + c * 32, v);
-          tmem_ld_wait32(v);
-        } else {
+      uint32_t v[D / 32][32];
+      if (own_steps) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = 0;
+        for (int c = 0; c < D / 32; ++c) tmem_ld32(t_o + c * 32, v[c]);
+        tmem_ld_wait32(v[0]);
+#pragma unroll
+        for (int c = 1; c < D / 32; ++c) tie32(v[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[c][k] = 0;
+      }
+      if (takes) {
+#pragma unroll
+        for (int k = 0; k < D / 4; ++k) {
+          float y[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(wide_at + k * 16));
+#pragma unroll
+          for (int h = 0; h < 4; ++h) v[k >> 3][(k & 7) * 4 + h] = __float_as_uint(__uint_as_float(v[k >> 3][(k & 7) * 4 + h]) * mine + y[h] * theirs);
         }
-        if (takes) {
+      }
+      if (wide) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float y[4];
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(wide_at + c * 128 + k * 16) : "memory");
+        for (int k = 0; k < D / 4; ++k)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + k * 16), "r"(v[k >> 3][(k & 7) * 4]), "r"(v[k >> 3][(k & 7) * 4 + 1]), "r"(v[k >> 3][(k & 7) * 4 + 2]),
+                       "r"(v[k >> 3][(k & 7) * 4 + 3]) : "memory");
+      } else {
 #pragma unroll
-            for (int h = 0; h < 4; ++h) v[4 * k + h] = __float_as_uint(__uint_as_float(v[4 * k + h]) * mine + y[h] * theirs);
-          }
-        }
-        if (wide) {
+        for (int k = 0; k < kPieces; ++k) {
+          uint32_t u[4];
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + c * 128 + k * 16), "r"(v[4 * k]), "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3]) : "memory");
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t u[4];
-#pragma unroll
-            for (int h = 0; h < 4; ++h) u[h] = Mma<T>::pack(__uint_as_float(v[8 * k + 2 * h]) * inverse, __uint_as_float(v[8 * k + 2 * h + 1]) * inverse);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (((c * 4 + k) ^ (lane & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
-          }
+          for (int h = 0; h < 4; ++h) u[h] = Mma<T>::pack(__uint_as_float(v[k >> 2][(k & 3) * 8 + 2 * h]) * inverse, __uint_as_float(v[k >> 2][(k & 3) * 8 + 2 * h + 1]) * inverse);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + ((k ^ (lane & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
         }
       }
     }
@@ -417,14 +427,18 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         __syncwarp();
         const int64_t y_at = (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
         const int c = lane % kPieces;
+        uint32_t u[kPieces][4];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int at = i * (32 / kPieces) + lane / kPieces;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[i][0]), "=r"(u[i][1]), "=r"(u[i][2]), "=r"(u[i][3]) : "r"(row_at + (uint32_t)(at - lane) * (D * 2) + ((c ^ (at & 7)) << 4)));
+        }
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
           const int at = i * (32 / kPieces) + lane / kPieces;
           const int64_t to = __shfl_sync(~0u, y_at, at);
-          uint32_t u[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(row_at + (uint32_t)(at - lane) * (D * 2) + ((c ^ (at & 7)) << 4)) : "memory");
-          if (!ok) u[0] = u[1] = u[2] = u[3] = ~0u;   // (no numbers)
-          if (r - lane + at < n_rows) *(uint4*)((T*)p.a.y + to + c * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+          if (!ok) u[i][0] = u[i][1] = u[i][2] = u[i][3] = ~0u;   // (no numbers)
+          if (r - lane + at < n_rows) *(uint4*)((T*)p.a.y + to + c * 8) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
         }
       }
     }
@@ -539,8 +553,6 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     };
     // Split, a tile has every other step.
     if (warp == kSoftmax + kLoaders) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(kColumns) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
       if (elect_one()) {
         const uint32_t idesc = common | ((uint32_t)(kStep >> 3) << 17), half = p.half_bytes >> 4;   // (64 channels further)
         const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_keys, 16, p.group_bytes);
@@ -578,24 +590,36 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
           // values that some rows do not see: those that are infinite or no numbers, and all behind the last position, go
           __syncwarp();
           if (!warp_wait(&w.v_full[at.slot], at.turn)) { ok = false; break; }
-          bool any = false;
-          for (int n = max(seen_by_all, 0) * kPieces + lane; n < kStep * kPieces; n += 32) {
+          const uint32_t unit = s_values + at.slot * kUnit;
+          auto place = [&](int n) {   // of piece n of 16 bytes, position after position
             const int pos = n / kPieces, c = n % kPieces;
-            const uint32_t to = s_values + at.slot * kUnit + (c >> 3) * p.half_bytes + (pos >> 3) * p.group_bytes + (pos & 7) * 128 + (((c & 7) ^ (pos & 7)) << 4);
-            uint32_t x[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(to) : "memory");
-            bool store = pos >= seen_by_any;
+            return unit + (c >> 3) * p.half_bytes + (pos >> 3) * p.group_bytes + (pos & 7) * 128 + (((c & 7) ^ (pos & 7)) << 4);
+          };
+          const int n0 = max(seen_by_all, 0) * kPieces, n1 = min(seen_by_any, kStep) * kPieces;
+          // (times zero, an infinity and what is no number stay no numbers: one instruction for two values)
+          uint32_t none = 0;
+          for (int n = n0 + lane; n < n1; n += 128) {
+            uint32_t x[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (pos >= seen_by_any) x[k] = 0;
-              else if (odd16(x[k], Mma<T>::kBf16)) {
-                store = any = true;
-                x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
-              }
-            }
-            if (store) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            for (int k = 0; k < 4; ++k)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3]) : "r"(place(n + 32 * k < n1 ? n + 32 * k : n)));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) none = Mma<T>::times_zero(x[k][e], none);
           }
-          if (any) *(volatile int*)&w.odd = 1;
+          if (__any_sync(~0u, none & 0x7fff7fffu)) {
+            for (int n = n0 + lane; n < n1; n += 32) {
+              uint32_t x[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(n)) : "memory");
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (odd16(x[k], Mma<T>::kBf16)) x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(n)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            }
+            *(volatile int*)&w.odd = 1;
+          }
+          for (int n = n1 + lane; n < kStep * kPieces; n += 32) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place(n)), "r"(0) : "memory");
           fence_async_proxy();
           __syncwarp();
         }
@@ -764,6 +788,7 @@ int chunk_attention(const ChunkAttention& a, cudaStream_t stream) {
   Params p{};
   p.a = a;
   p.group = a.heads / a.kv_heads;
+  p.capacity = a.table_width * a.page_size;   // (below 2^30)
   quotient(p.group, p.group_factor, p.group_shift);
   quotient(a.page_size, p.page_factor, p.page_shift);
   p.scale_log2e = a.scale * kLog2e;
