@@ -22,15 +22,16 @@ struct Params {
   float scale_log2e;
   uint32_t group_factor, group_shift, page_factor, page_shift;   // n / group = n * factor >> shift for n < 2^30, n / page_size likewise
   int box_shift;                   // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
+  int row_boxes;                   // queries and results of 128 rows move as boxes of whole tokens: the group divides 128
   uint32_t group_bytes, half_bytes;   // in a unit: from eight positions to the next eight, from 64 channels to the next 64
   uint32_t spin_limit;
   int test_skip_stage;             // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
 
-constexpr int kBarriers = 4 * kMostRing + 15;
+constexpr int kBarriers = 4 * kMostRing + 15 + kSeen;
 struct Shared {
   float2 stat[kRows];       // reference (a base-2 exponent) and sum of each row
-  uint64_t k_full[kMostRing], v_full[kMostRing], k_empty[kMostRing], v_empty[kMostRing], q_full, s_full[2], s_read[2], p_most[2], p_full[2], o_done[2], handed, all_done, drained[2];
+  uint64_t k_full[kMostRing], v_full[kMostRing], k_empty[kMostRing], v_empty[kMostRing], q_full, s_full[2], s_read[2], p_most[2], p_full[2], o_done[2], handed, all_done, clean[kSeen], drained[2];
   uint32_t seen[kSeen][4];  // which of a step's positions lie on pages that are there; written at most a ring ahead of the step that is read
   uint32_t tmem;
   int abort, odd;           // odd: values that not all rows see, infinite or no numbers, were taken out of the products
@@ -55,7 +56,7 @@ __device__ __forceinline__ bool odd16(uint32_t u, bool bf16) {   // one of two e
 
 // What a row sees of values that are infinite or no numbers, and that stay out of the products of a step that not all rows see whole: position for
 // position, from memory, onto its result (a weight is not zero, so that an infinity remains one).  Rare, and slow.
-template <typename T, int D> __device__ __noinline__ void add_odd(const Params& p, uint32_t row_at, bool wide, int swizzle, int head, const int* pages, int from, int to) {
+template <typename T, int D> __device__ __noinline__ void add_odd(const Params& p, uint32_t row_at, bool wide, int swizzle, uint32_t second_half, int head, const int* pages, int from, int to) {
   for (int pos = from; pos < to; ++pos) {
     const int page = pages[pos / p.a.page_size];
     if (page < 0 || page >= p.a.pages) continue;
@@ -73,7 +74,7 @@ template <typename T, int D> __device__ __noinline__ void add_odd(const Params& 
           asm volatile("st.shared.f32 [%0], %1;" ::"r"(row_at + (2 * c + h) * 4), "f"(y + x) : "memory");
         } else {
           unsigned short y;
-          const uint32_t at = row_at + (uint32_t)(((c >> 2) ^ swizzle) << 4) + (uint32_t)((2 * c + h) & 7) * 2;
+          const uint32_t at = row_at + (c >= 32 ? second_half : 0u) + (uint32_t)(((c >> 2) ^ swizzle) << 4) + (uint32_t)((2 * c + h) & 7) * 2;
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(at) : "memory");
           const float z = (Mma<T>::kBf16 ? __uint_as_float((uint32_t)y << 16) : __half2float(__ushort_as_half(y))) + x;
           asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((unsigned short)(Mma<T>::pack(z, 0.f) & 0xffffu)) : "memory");
@@ -92,6 +93,15 @@ __device__ __forceinline__ void load_box_all(uint32_t dst, const CUtensorMap* ma
 __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %0, %1, %2;" : "+f"(x) : "f"(y), "f"(z));
   return x;
+}
+// 128 rows of 64 channels: whole tokens of the heads of a group.
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int channel, int head, int token) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map),
+               "r"(smem_u32(bar)), "r"(channel), "r"(head), "r"(token)
+               : "memory");
+}
+__device__ __forceinline__ void store_rows(uint32_t src, const CUtensorMap* map, int channel, int head, int token) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"((uint64_t)map), "r"(src), "r"(channel), "r"(head), "r"(token) : "memory");
 }
 __device__ __forceinline__ void tie32(uint32_t (&r)[32]) {   // (no read of these registers comes before what stands in front)
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
@@ -119,7 +129,8 @@ __device__ __forceinline__ void tie32(uint32_t (&r)[32]) {   // (no read of thes
 // registers that twelve warps leave a thread.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values) {
+chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values, const __grid_constant__ CUtensorMap queries,
+             const __grid_constant__ CUtensorMap results) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared w;
   constexpr int kBoxes = D / 64, kPieces = D / 8;
@@ -137,11 +148,12 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     if (lane == 0) { w.abort = 0; w.odd = 0; w.found = 0; }
     for (int i = lane; i < kBarriers; i += 32) {
       uint64_t* bar = &w.k_full[0] + i;
-      mbar_init(bar, bar < w.k_empty ? kLoaders * 33 : bar == &w.q_full ? kSoftmax : (bar >= w.s_read && bar < w.o_done) || bar == &w.handed ? 4 : 1);
+      mbar_init(bar, bar < w.k_empty ? (p.box_shift ? 33 : kLoaders * 33) : bar == &w.q_full ? (p.row_boxes ? 1 : kSoftmax) : (bar >= w.s_read && bar < w.o_done) || bar == &w.handed ? 4 : 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_proxy();
     if (lane == 0 && p.box_shift) { prefetch_map(&keys); prefetch_map(&values); }
+    if (lane == 0 && p.row_boxes) { prefetch_map(&queries); prefetch_map(&results); }
   }
   grid_dependency_wait();
   launch_dependents();
@@ -214,11 +226,56 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   constexpr uint32_t kWideRow = D * 4 + 16;   // (16 bytes apart from each other's banks)
   const uint32_t wide_base = split ? s_keys : smem;
 
+  // Values that some rows of this tile do not see: of step i, those that are infinite or no numbers, and all behind the last position, go out of the unit where they
+  // have landed.
+  auto seen_by_all = [&](int i) { return (first + i < prefix_steps ? p.a.prefix_length : least) - begin_of(i); };
+  auto hides_any = [&](int i) { return seen_by_all(i) < kStep; };
+  auto hide = [&](int i, int slot) {
+    const int seen_by_any = end_of(i) - begin_of(i);
+    const uint32_t unit = s_values + slot * kUnit;
+    auto place = [&](int n) {   // of piece n of 16 bytes, position after position
+      const int pos = n / kPieces, c = n % kPieces;
+      return unit + (c >> 3) * p.half_bytes + (pos >> 3) * p.group_bytes + (pos & 7) * 128 + (((c & 7) ^ (pos & 7)) << 4);
+    };
+    const int n0 = max(seen_by_all(i), 0) * kPieces, n1 = min(seen_by_any, kStep) * kPieces;
+    // (times zero, an infinity and what is no number stay no numbers: one instruction for two values)
+    uint32_t none = 0;
+    for (int n = n0 + lane; n < n1; n += 128) {
+      uint32_t x[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3]) : "r"(place(n + 32 * k < n1 ? n + 32 * k : n)));
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) none = Mma<T>::times_zero(x[k][e], none);
+    }
+    if (__any_sync(~0u, none & 0x7fff7fffu)) {
+      for (int n = n0 + lane; n < n1; n += 32) {
+        uint32_t x[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(n)) : "memory");
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (odd16(x[k], Mma<T>::kBf16)) x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(n)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+      }
+      *(volatile int*)&w.odd = 1;
+    }
+    for (int n = n1 + lane; n < kStep * kPieces; n += 32) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place(n)), "r"(0) : "memory");
+    fence_async_proxy();
+  };
+
   if (warp < kSoftmax) {
     // ------------------------------------------------------------------- softmax ----
     const int tile = warp >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane, r = split ? in_tile : tile * 128 + in_tile;
     const bool live = r < n_rows, any_live = r - lane < n_rows;   // of this thread, of its warp
-    {
+    if (p.row_boxes) {
+      if (threadIdx.x == 0) {   // (rows behind the sequence's last are other sequences', or zeros, and stay without effect)
+        mbar_expect_tx(&w.q_full, split ? kUnit : 2 * kUnit);
+        for (int t = 0; t < (split ? 1 : 2); ++t)
+          for (int c = 0; c < kBoxes; ++c) load_rows(s_q + t * kUnit + c * kBox, &queries, &w.q_full, c * 64, head * p.group, first_row + token_of(p, row0 + 128 * t));
+      }
+    } else {
       // queries: sixteen (or eight) threads for a row.  A negative scale becomes the sign of the queries, the largest score is then the largest product; a scale
       // of zero makes all products zero.
       const uint32_t sign = p.scale_log2e < 0.f ? 0x80008000u : 0u, any = p.scale_log2e == 0.f ? 0u : ~0u;
@@ -374,7 +431,9 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       }
     }
     const float inverse = wide ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-    const uint32_t row_at = wide ? wide_at : s_q + tile * kUnit + (uint32_t)in_tile * (D * 2);
+    // rows of whole channels, 16-byte pieces swizzled; or, for a tile that leaves as boxes, of 64 channels as boxes have them
+    const bool boxed = !wide && p.row_boxes && n_rows - (split ? 0 : tile * 128) >= 128;
+    const uint32_t row_at = wide ? wide_at : s_q + tile * kUnit + (uint32_t)in_tile * (boxed ? 128 : D * 2), second_half = boxed ? kBox - 128 : 0;
     if (ok && any_live && (own_steps || !hands)) {   // (nothing to hand over: the first tile does not wait, and its rows lie there)
       uint32_t v[D / 32][32];
       if (own_steps) {
@@ -409,7 +468,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
           uint32_t u[4];
 #pragma unroll
           for (int h = 0; h < 4; ++h) u[h] = Mma<T>::pack(__uint_as_float(v[k >> 2][(k & 3) * 8 + 2 * h]) * inverse, __uint_as_float(v[k >> 2][(k & 3) * 8 + 2 * h + 1]) * inverse);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + ((k ^ (lane & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + (k >> 3) * second_half + ((k ^ (lane & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
         }
       }
     }
@@ -419,10 +478,21 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     } else {
       if (ok && *(volatile int*)&w.odd && live) {   // positions of this CTA's steps that this row sees and others do not
         const int from = max(least, (max(first, prefix_steps) - prefix_steps) * kStep), to = min(limit, (first + steps - prefix_steps) * kStep);
-        add_odd<T, D>(p, row_at, wide, lane & 7, head, own_pages, from, to);
+        add_odd<T, D>(p, row_at, wide, lane & 7, second_half, head, own_pages, from, to);
       }
       if (shared) {
         w.stat[r] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
+      } else if (boxed) {
+        fence_async_proxy();
+        asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");   // (the tile's four warps)
+        if (*abort_flag) {
+          T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
+          for (int c = 0; c < kPieces; ++c) ((uint4*)y)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);   // (no numbers)
+        } else if (quarter == 0 && lane == 0) {
+          for (int c = 0; c < kBoxes; ++c) store_rows(s_q + tile * kUnit + c * kBox, &results, c * 64, head * p.group, first_row + token_of(p, row0 + 128 * tile));
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
       } else if (any_live) {
         __syncwarp();
         const int64_t y_at = (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
@@ -443,6 +513,18 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       }
     }
     tc_fence_before();
+  } else if (warp == kSoftmax + 1 && p.box_shift) {
+    // one warp asks for boxes; the other looks at the values of steps that not all rows see (it follows them all, to know the turns)
+    Place at{0, 0};
+    int hidden = 0;
+    for (int i = 0; i < steps; ++i, next(at, n_values)) {
+      if (!warp_wait(&w.v_full[at.slot], at.turn)) break;
+      if (!hides_any(i)) continue;
+      hide(i, at.slot);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w.clean[hidden % kSeen]);
+      ++hidden;
+    }
   } else if (warp < kSoftmax + kLoaders) {
     // --------------------------------------------------------------------- loads ----
     const int part = warp - kSoftmax;
@@ -486,14 +568,14 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const uint32_t seen = __ballot_sync(~0u, __shfl_sync(~0u, there, (h * 32 + lane) >> p.box_shift));
-            if (lane == 0 && part == 0) *(volatile uint32_t*)&w.seen[step % kSeen][h] = seen;
+            if (lane == 0) *(volatile uint32_t*)&w.seen[step % kSeen][h] = seen;
           }
           ask(step + 1);
         }
         if (skip) continue;
         mbar_arrive(full);
-        if (lane == 0) { if (part == 0) mbar_expect_tx(full, kUnit); else mbar_arrive(full); }
-        if (part == 0 && lane < boxes) {
+        if (lane == 0) mbar_expect_tx(full, kUnit);
+        if (lane < boxes) {
           const CUtensorMap* map = (u & 1) ? &values : &keys;
           const uint32_t to = dst + ((uint32_t)lane << p.box_shift >> 3) * p.group_bytes;
           if (both) load_box_all(to, map, full, box_at, head, box_coord);
@@ -581,50 +663,21 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       const uint32_t idesc = common | (1u << 16) | ((uint32_t)(D >> 3) << 17), sixteen = p.group_bytes >> 3;   // (16 positions further, in units of 16 bytes)
       const uint64_t v_desc = desc(s_values, p.half_bytes, p.group_bytes);
       const bool issues = elect_one();
+      int hidden = 0;   // steps that hid values
       Place at{0, 0};
       bool ok = true;
       // (all lanes go through all steps, and leave together: the one that issues skips what is left when a wait has run out)
       for (int i = 0; i < steps; ++i, next(at, n_values)) {
-        const int seen_by_all = (first + i < prefix_steps ? p.a.prefix_length : least) - begin_of(i), seen_by_any = end_of(i) - begin_of(i);
-        if (seen_by_all < kStep) {
-          // values that some rows do not see: those that are infinite or no numbers, and all behind the last position, go
+        const bool hides = hides_any(i);
+        if (hides && !p.box_shift) {
           __syncwarp();
           if (!warp_wait(&w.v_full[at.slot], at.turn)) { ok = false; break; }
-          const uint32_t unit = s_values + at.slot * kUnit;
-          auto place = [&](int n) {   // of piece n of 16 bytes, position after position
-            const int pos = n / kPieces, c = n % kPieces;
-            return unit + (c >> 3) * p.half_bytes + (pos >> 3) * p.group_bytes + (pos & 7) * 128 + (((c & 7) ^ (pos & 7)) << 4);
-          };
-          const int n0 = max(seen_by_all, 0) * kPieces, n1 = min(seen_by_any, kStep) * kPieces;
-          // (times zero, an infinity and what is no number stay no numbers: one instruction for two values)
-          uint32_t none = 0;
-          for (int n = n0 + lane; n < n1; n += 128) {
-            uint32_t x[4][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3]) : "r"(place(n + 32 * k < n1 ? n + 32 * k : n)));
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) none = Mma<T>::times_zero(x[k][e], none);
-          }
-          if (__any_sync(~0u, none & 0x7fff7fffu)) {
-            for (int n = n0 + lane; n < n1; n += 32) {
-              uint32_t x[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(place(n)) : "memory");
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (odd16(x[k], Mma<T>::kBf16)) x[k] &= (odd16(x[k] & 0xffffu, Mma<T>::kBf16) ? 0u : 0xffffu) | (odd16(x[k] >> 16, Mma<T>::kBf16) ? 0u : 0xffff0000u);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(n)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-            }
-            *(volatile int*)&w.odd = 1;
-          }
-          for (int n = n1 + lane; n < kStep * kPieces; n += 32) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(place(n)), "r"(0) : "memory");
-          fence_async_proxy();
+          hide(i, at.slot);
           __syncwarp();
         }
         if (issues && ok) {
-          ok = landed(w.v_full, at);
+          ok = hides && p.box_shift ? wait(&w.clean[hidden % kSeen], hidden / kSeen & 1) : landed(w.v_full, at);
+          hidden += hides;
           const uint64_t v = v_desc + (uint32_t)at.slot * (kUnit >> 4);
           const int turn = split ? i >> 1 : i;
           for (int t = split ? i & 1 : i < takes0 ? 0 : 1; t < 2 && ok; t += split ? 2 : 1) {
@@ -703,6 +756,18 @@ bool whole_box_map(CUtensorMap* m, const ChunkAttention& a, const void* base) {
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Boxes of 64 channels of 128 rows: a group's heads of whole tokens.
+bool row_map(CUtensorMap* m, const Params& p, const void* base, int64_t token, int64_t head) {
+  if (!load_driver_entry_points()) return false;
+  auto bytes = [](int64_t stride, int extent) { return extent == 1 && stride == 0 ? (cuuint64_t)16 : (cuuint64_t)stride * 2; };
+  const cuuint64_t dims[3] = {(cuuint64_t)p.a.channels, (cuuint64_t)p.a.heads, (cuuint64_t)p.a.tokens};
+  const cuuint64_t strides[2] = {bytes(head, p.a.heads), bytes(token, p.a.tokens)};
+  for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return false;
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(128 / p.group)}, step[3] = {1, 1, 1};
+  return g_encode_tiled(m, p.a.dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct Fit {
   int clusters[kMaxShare + 1];   // of each size, that run at the same time
 };
@@ -751,7 +816,7 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
       if (us < best) { best = us; p.tile_rows = rows; p.tiles = (int)tiles; p.share = share; }
     }
   }
-  CUtensorMap keys{}, values{};
+  CUtensorMap keys{}, values{}, queries{}, results{};
   p.box_shift = 0;
   p.group_bytes = 1024;
   p.half_bytes = kBox;
@@ -766,10 +831,11 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   } else if (shift >= 3 && box_map(&keys, p.a, p.a.k, 1 << shift) && box_map(&values, p.a, p.a.v, 1 << shift)) {
     p.box_shift = shift;
   }
+  p.row_boxes = p.scale_log2e > 0.f && 128 % p.group == 0 && row_map(&queries, p, p.a.q, p.a.q_token, p.a.q_head) && row_map(&results, p, p.a.y, p.a.y_token, p.a.y_head);
   cfg.gridDim = dim3((unsigned)(p.tiles * p.a.kv_heads * p.share));
   attr[0].val.clusterDim.x = (unsigned)p.share;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, fn, p, keys, values) == cudaSuccess) return 0;
+  if (cudaLaunchKernelEx(&cfg, fn, p, keys, values, queries, results) == cudaSuccess) return 0;
   cudaGetLastError();
   return -2;
 }
