@@ -18,12 +18,14 @@ struct Params {
   ChunkAttention a;
   int group;                       // query heads of a cache head; rows of a sequence = its new tokens * group
   int capacity;                    // positions that a sequence's table has room for
-  int tile_rows, tiles, share;     // rows of a tile (128 or 256); tiles that the batch can have; CTAs (a cluster) that share a tile's positions
+  int tile_rows, tiles, share;     // rows of a tile (half_rows or twice as many); tiles that the batch can have; CTAs (a cluster) that share a tile's positions
   float scale_log2e;
   uint32_t group_factor, group_shift, page_factor, page_shift;   // n / group = n * factor >> shift for n < 2^30, n / page_size likewise
   int box_shift;                   // keys and values arrive in boxes of 1 << box_shift positions by TMA; 0: by 16-byte copies only
-  int row_boxes;                   // queries and results of 128 rows move as boxes of whole tokens: the group divides 128
+  int half_rows;                   // rows of half a tile: those of as many whole tokens as fit into 128, where they leave few of them empty
+  int row_boxes;                   // queries and results of half a tile move as boxes
   uint32_t group_bytes, half_bytes;   // in a unit: from eight positions to the next eight, from 64 channels to the next 64
+  int fold;                        // boxes bring all 128 channels: 1: pages and heads are counted together, 2: pages and positions are; 0: they bring 64
   uint32_t spin_limit;
   int test_skip_stage;             // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
 };
@@ -84,17 +86,17 @@ template <typename T, int D> __device__ __noinline__ void add_odd(const Params& 
   }
 }
 
-// All 128 channels of a box's positions: eight positions of the first 64, then of the others.
-__device__ __forceinline__ void load_box_all(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int position, int head, int page) {
-  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(dst), "l"((uint64_t)map),
-               "r"(smem_u32(bar)), "r"(0), "r"(position), "r"(head), "r"(page)
+// All 128 channels of a box's positions: eight positions of the first 64 channels, the same of the others, the next eight positions ...
+__device__ __forceinline__ void load_box_all(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int eight, int outer) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map),
+               "r"(smem_u32(bar)), "r"(0), "r"(eight), "r"(outer)
                : "memory");
 }
 __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %0, %1, %2;" : "+f"(x) : "f"(y), "f"(z));
   return x;
 }
-// 128 rows of 64 channels: whole tokens of the heads of a group.
+// Half a tile's rows of 64 channels: whole tokens of the heads of a group.
 __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int channel, int head, int token) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"((uint64_t)map),
                "r"(smem_u32(bar)), "r"(channel), "r"(head), "r"(token)
@@ -118,8 +120,8 @@ __device__ __forceinline__ void tie32(uint32_t (&r)[32]) {   // (no read of thes
 // columns for their scores, one after the other: they are free again as soon as they are in registers, so that the next scores never
 // wait for a softmax or for the products with its weights.  (Weights over each tile's own scores, two reads of them, no wait for registers: 3500
 // clocks a step of 2 x 128 x 128, 1420 of them a softmax warp's wait for scores that stood behind the last products.)
-// Rows are counted token by token, the heads of the group side by side: a tile covers few tokens, and little of its last steps is hidden from it.  Up to 128
-// rows leave the second tile free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
+// Rows are counted token by token, the heads of the group side by side: a tile covers few tokens, and little of its last steps is hidden from it.  Up to half
+// a tile's rows leave the second half free: it takes the same rows against every other step (`split`), and hands its sums to the first at the end.
 // Where tiles are few, the CTAs of a cluster share the positions of each, by the lengths that they find, and every one joins some of the rows
 // out of the others' shared memory.
 // A weight of zero does not hide an infinity: in steps that some rows see less of than others, values that are infinite or no numbers are taken
@@ -205,7 +207,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   auto limit_of = [&](int r) { return max(0, length - count + token_of(p, r) + 1); };
   const int prefix_steps = (p.a.prefix_length + kStep - 1) / kStep;
   const int least = limit_of(row0), most = limit_of(row0 + n_rows - 1);   // of this tile's first and last row
-  const bool split = n_rows <= 128;
+  const bool split = n_rows <= p.half_rows;
   // Keys and values have rings of their own: whoever waits for one of them follows every turn of its place.
   constexpr int kKeys = kRing<D>;
   const int n_values = kRing<D> + split;
@@ -215,7 +217,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
   // steps of the whole tile, this CTA's share of them, and how many of those each half of the rows takes part in
   const int all_steps = prefix_steps + (most + kStep - 1) / kStep;
   const int first = p.share == 1 ? 0 : all_steps * rank / p.share, steps = (p.share == 1 ? all_steps : all_steps * (rank + 1) / p.share) - first;   // (2^23 steps at most)
-  const int takes0 = split ? (steps + 1) / 2 : max(0, min(steps, prefix_steps + (limit_of(row0 + 127) + kStep - 1) / kStep - first)), takes1 = split ? steps / 2 : steps;
+  const int takes0 = split ? (steps + 1) / 2 : max(0, min(steps, prefix_steps + (limit_of(row0 + p.half_rows - 1) + kStep - 1) / kStep - first)), takes1 = split ? steps / 2 : steps;
   // step i of this CTA: where it begins in its segment, where the segment ends (for the last row), its pages
   auto begin_of = [&](int i) { return (first + i < prefix_steps ? first + i : first + i - prefix_steps) * kStep; };
   auto end_of = [&](int i) { return first + i < prefix_steps ? p.a.prefix_length : most; };
@@ -267,13 +269,14 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
 
   if (warp < kSoftmax) {
     // ------------------------------------------------------------------- softmax ----
-    const int tile = warp >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane, r = split ? in_tile : tile * 128 + in_tile;
-    const bool live = r < n_rows, any_live = r - lane < n_rows;   // of this thread, of its warp
+    const int tile = warp >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane, r = split ? in_tile : tile * p.half_rows + in_tile;
+    const int n_live = min(p.half_rows, n_rows - (split ? 0 : tile * p.half_rows));   // rows of this half
+    const bool live = in_tile < n_live, any_live = in_tile - lane < n_live;   // this thread's, its warp's first
     if (p.row_boxes) {
       if (threadIdx.x == 0) {   // (rows behind the sequence's last are other sequences', or zeros, and stay without effect)
-        mbar_expect_tx(&w.q_full, split ? kUnit : 2 * kUnit);
+        mbar_expect_tx(&w.q_full, (split ? 1 : 2) * kBoxes * p.half_rows * 128);
         for (int t = 0; t < (split ? 1 : 2); ++t)
-          for (int c = 0; c < kBoxes; ++c) load_rows(s_q + t * kUnit + c * kBox, &queries, &w.q_full, c * 64, head * p.group, first_row + token_of(p, row0 + 128 * t));
+          for (int c = 0; c < kBoxes; ++c) load_rows(s_q + t * kUnit + c * kBox, &queries, &w.q_full, c * 64, head * p.group, first_row + token_of(p, row0 + p.half_rows * t));
       }
     } else {
       // queries: sixteen (or eight) threads for a row.  A negative scale becomes the sign of the queries, the largest score is then the largest product; a scale
@@ -283,9 +286,9 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
       uint4 u[32 * kPieces / 32];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int at = i * (32 / kPieces) + lane / kPieces, row = row0 + warp * per + at, j = token_of(p, row);
+        const int at = i * (32 / kPieces) + lane / kPieces, q_row = warp * per + at, n = (q_row >> 7) * p.half_rows + (q_row & 127), row = row0 + n, j = token_of(p, row);
         u[i] = make_uint4(0, 0, 0, 0);
-        if (at < per && warp * per + at < n_rows)
+        if (at < per && (q_row & 127) < p.half_rows && n < n_rows)
           u[i] = *((const uint4*)((const T*)p.a.q + (int64_t)(first_row + j) * p.a.q_token + (int64_t)(head * p.group + row - j * p.group) * p.a.q_head) + c);
       }
 #pragma unroll
@@ -432,7 +435,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     }
     const float inverse = wide ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
     // rows of whole channels, 16-byte pieces swizzled; or, for a tile that leaves as boxes, of 64 channels as boxes have them
-    const bool boxed = !wide && p.row_boxes && n_rows - (split ? 0 : tile * 128) >= 128;
+    const bool boxed = !wide && p.row_boxes && n_live == p.half_rows;
     const uint32_t row_at = wide ? wide_at : s_q + tile * kUnit + (uint32_t)in_tile * (boxed ? 128 : D * 2), second_half = boxed ? kBox - 128 : 0;
     if (ok && any_live && (own_steps || !hands)) {   // (nothing to hand over: the first tile does not wait, and its rows lie there)
       uint32_t v[D / 32][32];
@@ -458,9 +461,10 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         }
       }
       if (wide) {
+        // (lanes behind a half's last row have the places of the other half's first ones)
 #pragma unroll
         for (int k = 0; k < D / 4; ++k)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + k * 16), "r"(v[k >> 3][(k & 7) * 4]), "r"(v[k >> 3][(k & 7) * 4 + 1]), "r"(v[k >> 3][(k & 7) * 4 + 2]),
+          if (live) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_at + k * 16), "r"(v[k >> 3][(k & 7) * 4]), "r"(v[k >> 3][(k & 7) * 4 + 1]), "r"(v[k >> 3][(k & 7) * 4 + 2]),
                        "r"(v[k >> 3][(k & 7) * 4 + 3]) : "memory");
       } else {
 #pragma unroll
@@ -481,15 +485,17 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         add_odd<T, D>(p, row_at, wide, lane & 7, second_half, head, own_pages, from, to);
       }
       if (shared) {
-        w.stat[r] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
+        if (live) w.stat[r] = make_float2(ok ? reference : 0.f, ok ? sum : __int_as_float(0x7fc00000));
       } else if (boxed) {
         fence_async_proxy();
         asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");   // (the tile's four warps)
         if (*abort_flag) {
+          if (live) {
           T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
           for (int c = 0; c < kPieces; ++c) ((uint4*)y)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);   // (no numbers)
+          }
         } else if (quarter == 0 && lane == 0) {
-          for (int c = 0; c < kBoxes; ++c) store_rows(s_q + tile * kUnit + c * kBox, &results, c * 64, head * p.group, first_row + token_of(p, row0 + 128 * tile));
+          for (int c = 0; c < kBoxes; ++c) store_rows(s_q + tile * kUnit + c * kBox, &results, c * 64, head * p.group, first_row + token_of(p, row0 + p.half_rows * tile));
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
@@ -508,7 +514,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
           const int at = i * (32 / kPieces) + lane / kPieces;
           const int64_t to = __shfl_sync(~0u, y_at, at);
           if (!ok) u[i][0] = u[i][1] = u[i][2] = u[i][3] = ~0u;   // (no numbers)
-          if (r - lane + at < n_rows) *(uint4*)((T*)p.a.y + to + c * 8) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
+          if (in_tile - lane + at < n_live) *(uint4*)((T*)p.a.y + to + c * 8) = make_uint4(u[i][0], u[i][1], u[i][2], u[i][3]);
         }
       }
     }
@@ -534,7 +540,6 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     int page[kEach], box_page = -1;
     int64_t off[kEach];
     const int boxes = p.box_shift ? kStep >> p.box_shift : 0;
-    const bool both = kBoxes == 2 && p.half_bytes == 1024;   // (a box brings all channels of its positions)
     auto position = [&](int step, int h) { return begin_of(step) + (part * kEach + h) * 32 + lane; };
     auto ask = [&](int step) {
       if (step >= steps) return;
@@ -578,7 +583,8 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         if (lane < boxes) {
           const CUtensorMap* map = (u & 1) ? &values : &keys;
           const uint32_t to = dst + ((uint32_t)lane << p.box_shift >> 3) * p.group_bytes;
-          if (both) load_box_all(to, map, full, box_at, head, box_coord);
+          if (p.fold == 1) load_box_all(to, map, full, box_at >> 3, box_coord == p.a.pages ? p.a.pages * p.a.kv_heads : box_coord * p.a.kv_heads + head);
+          else if (p.fold == 2) load_box_all(to, map, full, box_coord * (p.a.page_size >> 3) + (box_at >> 3), head);
           else {
 #pragma unroll
             for (int c = 0; c < kBoxes; ++c) load_box(to + c * p.half_bytes, map, full, c * 64, box_at, head, box_coord);
@@ -744,26 +750,30 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     cluster_sync_all();   // (what the others read stays until they have)
   }
 }
-// Boxes of all 128 channels of eight positions of one head and page, as two halves.
-bool whole_box_map(CUtensorMap* m, const ChunkAttention& a, const void* base) {
-  if (!load_driver_entry_points()) return false;
-  auto bytes = [](int64_t stride, int extent) { return extent == 1 && stride == 0 ? (cuuint64_t)16 : (cuuint64_t)stride * 2; };
-  const cuuint64_t dims[5] = {64, (cuuint64_t)a.page_size, 2, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
-  const cuuint64_t strides[4] = {bytes(a.c_token, a.page_size), 128, bytes(a.c_head, a.kv_heads), bytes(a.c_page, a.pages)};
-  for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return false;
-  const cuuint32_t box[5] = {64, 8, 2, 1, 1}, step[5] = {1, 1, 1, 1, 1};
+// Boxes of all 128 channels of 8 << shift positions of one head and page.  A tensor map has five dimensions: 64 channels, eight positions, the two halves of
+// the channels, eights of positions, and one for both heads and pages, which dense caches allow: pages of heads are counted through, or, where the heads of a position
+// lie together, pages of positions.
+int whole_box_map(CUtensorMap* m, const ChunkAttention& a, const void* base, int shift) {
+  if (!load_driver_entry_points()) return 0;
+  const int fold = a.c_page == a.kv_heads * a.c_head || a.pages == 1 || a.kv_heads == 1 ? 1 : a.c_page == a.page_size * a.c_token ? 2 : 0;
+  if (!fold || a.c_token == 0 || (int64_t)a.pages * std::max(a.kv_heads, a.page_size) >= (1ll << 31) || (a.kv_heads > 1 && a.c_head == 0)) return 0;
+  const int64_t eights = a.page_size / 8, outer = fold == 1 ? (a.kv_heads > 1 ? a.c_head : a.pages > 1 ? a.c_page : a.channels) : a.kv_heads > 1 ? a.c_head : a.channels;
+  const cuuint64_t dims[5] = {64, 8, 2, (cuuint64_t)(fold == 1 ? eights : eights * a.pages), (cuuint64_t)(fold == 1 ? (int64_t)a.pages * a.kv_heads : a.kv_heads)};
+  const cuuint64_t strides[4] = {(cuuint64_t)a.c_token * 2, 128, (cuuint64_t)a.c_token * 16, (cuuint64_t)outer * 2};
+  for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return 0;
+  const cuuint32_t box[5] = {64, 8, 2, 1u << shift, 1}, step[5] = {1, 1, 1, 1, 1};
   return g_encode_tiled(m, a.dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, (void*)base, dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? fold : 0;
 }
 
-// Boxes of 64 channels of 128 rows: a group's heads of whole tokens.
+// Boxes of 64 channels of half a tile's rows: a group's heads of whole tokens.
 bool row_map(CUtensorMap* m, const Params& p, const void* base, int64_t token, int64_t head) {
   if (!load_driver_entry_points()) return false;
   auto bytes = [](int64_t stride, int extent) { return extent == 1 && stride == 0 ? (cuuint64_t)16 : (cuuint64_t)stride * 2; };
   const cuuint64_t dims[3] = {(cuuint64_t)p.a.channels, (cuuint64_t)p.a.heads, (cuuint64_t)p.a.tokens};
   const cuuint64_t strides[2] = {bytes(head, p.a.heads), bytes(token, p.a.tokens)};
   for (cuuint64_t s : strides) if (s == 0 || s >= (1ull << 40)) return false;
-  const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(128 / p.group)}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(p.half_rows / p.group)}, step[3] = {1, 1, 1};
   return g_encode_tiled(m, p.a.dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -802,17 +812,17 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
     f.clusters[1] = std::max(f.clusters[1], 1);
     return f;
   }();
-  // Rows of a tile and CTAs that share it: the shortest estimate of waves of steps (1.2 us, 0.7 for 128 rows) and of what a CTA does before and after them
+  // Rows of a tile and CTAs that share it: the shortest estimate of waves of steps (1.9 us, 1.2 for half a tile's rows) and of what a CTA does before and after them
   // (6 us, 2 more to join).  Lengths are not known here: the table's width stands for them.
   const int64_t steps = ((int64_t)p.a.table_width * p.a.page_size + kStep - 1) / kStep + (p.a.prefix_length + kStep - 1) / kStep;
   double best = 1e30;
-  for (int rows = kRows; rows >= 128; rows /= 2) {
+  for (int rows = 2 * p.half_rows; rows >= p.half_rows; rows -= p.half_rows) {
     // (a sequence's last tile has one row at least)
     const int64_t tiles = ((int64_t)p.a.tokens * p.group + (int64_t)std::min(p.a.batch, p.a.tokens) * (rows - 1)) / rows, clusters = tiles * p.a.kv_heads;
     for (int share = 1; share <= kMaxShare; ++share) {
       if (fit.clusters[share] < 1 || (share > 1 && steps < 2 * share)) continue;
       const int64_t waves = (clusters + fit.clusters[share] - 1) / fit.clusters[share];
-      const double us = (double)waves * ((double)((steps + share - 1) / share) * (rows == kRows ? 1.2 : 0.7) + (share > 1 ? 8.0 : 6.0));
+      const double us = (double)waves * ((double)((steps + share - 1) / share) * (rows > p.half_rows ? 1.9 : 1.2) + (share > 1 ? 8.0 : 6.0));
       if (us < best) { best = us; p.tile_rows = rows; p.tiles = (int)tiles; p.share = share; }
     }
   }
@@ -822,16 +832,16 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   p.half_bytes = kBox;
   int shift = 0;
   while (shift < 7 && p.a.page_size % (2 << shift) == 0) ++shift;
-  // (boxes of eight positions bring both halves of the channels: the boxes of an SM begin some 85 clocks after one another, and 64 of them held a step at
-  // 5460 clocks)
-  if (D == 128 && shift == 3 && whole_box_map(&keys, p.a, p.a.k) && whole_box_map(&values, p.a, p.a.v)) {
-    p.box_shift = 3;
+  // (an SM's boxes begin some 85 clocks after one another: 64 of eight positions and 64 channels held a step at 5460 clocks)
+  if (D == 128 && shift >= 3 && (p.fold = whole_box_map(&keys, p.a, p.a.k, shift - 3)) != 0 && whole_box_map(&values, p.a, p.a.v, shift - 3)) {
+    p.box_shift = shift;
     p.group_bytes = 2048;
     p.half_bytes = 1024;
   } else if (shift >= 3 && box_map(&keys, p.a, p.a.k, 1 << shift) && box_map(&values, p.a, p.a.v, 1 << shift)) {
     p.box_shift = shift;
+    p.fold = 0;
   }
-  p.row_boxes = p.scale_log2e > 0.f && 128 % p.group == 0 && row_map(&queries, p, p.a.q, p.a.q_token, p.a.q_head) && row_map(&results, p, p.a.y, p.a.y_token, p.a.y_head);
+  p.row_boxes = p.scale_log2e > 0.f && p.half_rows % p.group == 0 && row_map(&queries, p, p.a.q, p.a.q_token, p.a.q_head) && row_map(&results, p, p.a.y, p.a.y_token, p.a.y_head);
   cfg.gridDim = dim3((unsigned)(p.tiles * p.a.kv_heads * p.share));
   attr[0].val.clusterDim.x = (unsigned)p.share;
   cfg.numAttrs = 2;
@@ -854,6 +864,7 @@ int chunk_attention(const ChunkAttention& a, cudaStream_t stream) {
   Params p{};
   p.a = a;
   p.group = a.heads / a.kv_heads;
+  p.half_rows = p.group <= 128 && 128 / p.group * p.group >= 112 ? 128 / p.group * p.group : 128;
   p.capacity = a.table_width * a.page_size;   // (below 2^30)
   quotient(p.group, p.group_factor, p.group_shift);
   quotient(a.page_size, p.page_factor, p.page_shift);

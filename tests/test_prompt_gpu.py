@@ -226,6 +226,9 @@ CHUNKS = [  # new tokens, own lengths, heads, kv heads, channels, page, prefix
     ([17, 0, 0, 128], [17, 10, 0, 128], 64, 2, 64, 48, 1),
     ([1024], [1024], 4, 1, 128, 64, 0),
     ([1000, 24], [1500, 2000], 20, 4, 64, 40, 77),
+    ([3, 2], [50, 400], 192, 1, 64, 16, 0),               # more heads in a group than a tile has rows, and groups that leave many of its rows empty
+    ([9], [300], 100, 1, 128, 24, 10),
+    ([140], [300], 36, 2, 128, 256, 0),
 ]
 
 
