@@ -22,17 +22,22 @@ struct Params {
   int batches;      // of a thread, at most
 };
 
-// What a row's CTA says to the others: sums relative to its own maximum, its best logits.
+constexpr int kMaxShare = 8, kWarps = kThreads / 32;
+// A row's largest logit (of a warp, of a CTA), and relative to it the sums of w and of w log2 w.
+struct Sums { float top, sum, mean; };
 struct Shared {
-  float top, sum, mean;                         // largest logit; sum of w; sum of w log2 w
-  int found;                                    // its alternatives
-  float best[kMaxTop];
-  int best_at[kMaxTop];
-  float red[3][kThreads / 32];
-  int count, above, kept;
-  uint32_t bins[256], key;
-  float candidate[kCandidates];
-  int candidate_at[kCandidates];
+  // what a row's first CTA is told by the others
+  Sums all[kMaxShare];
+  int found[kMaxShare];
+  unsigned long long best[kMaxShare][kMaxTop];   // alternatives of each slice in descending order: key and complement of the index
+  // a CTA's own
+  Sums warp[kWarps];
+  float log_sum, base, top;
+  uint32_t key[kThreads];                        // of the threads' largest logits
+  int above[2][16];
+  int count, left, kept;
+  uint32_t bins[256], prefix;
+  unsigned long long candidate[kCandidates];
 };
 
 template <typename T> struct alignas(16) Sixteen { T e[16 / sizeof(T)]; };
@@ -50,6 +55,9 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
+// Its number (0: the lowest; a key between two numbers: one of them or nothing that is below it).
+__device__ __forceinline__ float value_of(uint32_t key) { return key < 0x00800000u ? -FLT_MAX : __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ unsigned long long entry(float v, int index) { return (unsigned long long)key_of(v) << 32 | (uint32_t)~index; }   // larger: in front
 __device__ __forceinline__ float below_infinity(float v) { return fminf(v, FLT_MAX); }
 
 // A row's slice: pieces lo ... hi - 1 of 16 aligned bytes, the first and last of the row perhaps partly outside it.
@@ -71,25 +79,24 @@ template <typename T> struct Slice {
   }
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & (kThreads / 32 - 1)];
-#pragma unroll
-  for (int o = kThreads / 64; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
+// Relative to a larger maximum.
+__device__ __forceinline__ void lower(float& sum, float& mean, float top, float to, float k2) {
+  const float shift = top > -INFINITY ? fmaxf((below_infinity(top) - below_infinity(to)) * k2, -200.f) : 0.f, f = exp2f(shift);
+  mean = f * (mean + shift * sum);
+  sum *= f;
 }
-__device__ __forceinline__ float block_sum(float v, float* red) {
+template <int LANES> __device__ __forceinline__ Sums together(Sums x, float k2) {
+  float top = x.top;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & (kThreads / 32 - 1)];
+  for (int o = LANES / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  lower(x.sum, x.mean, x.top, top, k2);
 #pragma unroll
-  for (int o = kThreads / 64; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+  for (int o = LANES / 2; o; o >>= 1) {
+    x.sum += __shfl_xor_sync(~0u, x.sum, o);
+    x.mean += __shfl_xor_sync(~0u, x.mean, o);
+  }
+  x.top = top;
+  return x;
 }
 
 // The n largest logits of a slice where more than kCandidates are no smaller than the bound (long runs of equal logits): the n-th largest key bit
@@ -113,12 +120,12 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
     if (threadIdx.x == 0) {
       int bin = 255, more = left;
       while (bin > 0 && (int)w.bins[bin] < more) more -= w.bins[bin--];
-      w.key = prefix | (uint32_t)bin << shift;
-      w.above = more;
+      w.prefix = prefix | (uint32_t)bin << shift;
+      w.left = more;
     }
     __syncthreads();
-    prefix = w.key;
-    left = w.above;
+    prefix = w.prefix;
+    left = w.left;
   }
   // `left` equals of the key `prefix` are wanted
   if (threadIdx.x == 0) { w.count = 0; w.kept = 0; }
@@ -132,7 +139,7 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
       const uint32_t key = key_of(v[k]);
       if (key > prefix) {
         const int at = atomicAdd(&w.count, 1);
-        if (at < kCandidates) { w.candidate[at] = v[k]; w.candidate_at[at] = s.first(p) + k; }
+        if (at < kCandidates) w.candidate[at] = entry(v[k], s.first(p) + k);
       }
       equal += key == prefix && key;
     }
@@ -157,7 +164,7 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
     for (int k = 0; k < VEC; ++k)
       if (key_of(v[k]) == prefix && prefix && before++ < left) {
         const int at = atomicAdd(&w.count, 1);
-        if (at < kCandidates) { w.candidate[at] = v[k]; w.candidate_at[at] = s.first(p) + k; }
+        if (at < kCandidates) w.candidate[at] = entry(v[k], s.first(p) + k);
       }
     __syncthreads();
     if (threadIdx.x == 0) w.kept = kept + all;
@@ -166,41 +173,58 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
 }
 
 // One pass over a row's logits: each thread keeps its largest one and, relative to it, the sums of w = 2^t and of w t, t = (l - max) / T in
-// base 2; then threads, and the CTAs that share the row, are put together.
+// base 2; then lanes, warps, and the CTAs that share the row, are put together.
 // Alternatives: the n-th largest of the threads' maxima is no larger than the n-th largest logit, so that only logits from there on can be among the n; they
-// are few, and are found again through the remembered maximum of each batch of pieces.
+// are few, and are found again through the remembered maximum of each batch of pieces.  The sixteen upper bits of the bound are enough; four at a
+// time, each warp counts for one of their sixteen values (bit by bit, 32 barriers and lists that the first CTA fetched entry by entry
+// made up 22 of 32 us for 64 rows of 128000 logits).  A candidate's place is the number of those in front of it.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_constant__ Params p) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ float group_top[];      // [batches][threads]
   __shared__ Shared w;
   const LogProbs& l = p.l;
-  const int t = threadIdx.x, rank = blockIdx.x % p.share;
-  const int64_t r = blockIdx.x / p.share;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = p.share == 1 ? 0 : blockIdx.x % p.share;
+  const int64_t r = p.share == 1 ? blockIdx.x : blockIdx.x / p.share;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (p.share > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");   // (the first CTA is there before others write to it)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Slice<T> s;
   s.row = (const T*)l.logits + r * l.row;
   s.off = (int)((uintptr_t)s.row % 16 / sizeof(T));
   s.vocab = l.vocab;
-  const int pieces = (s.off + l.vocab + VEC - 1) / VEC, each = (pieces + p.share - 1) / p.share;
+  const int pieces = (s.off + l.vocab + VEC - 1) / VEC, each = p.share == 1 ? pieces : (pieces + p.share - 1) / p.share;
   s.lo = min(pieces, rank * each);
   s.hi = min(pieces, s.lo + each);
   const float temperature = l.temperature ? l.temperature[r] : 1.f, T1 = temperature > 0.f ? temperature : 1.f;
   const float k2 = fminf(kLog2e / T1, FLT_MAX);
+  if (t == 0) w.count = 0;
 
   float top = -INFINITY, sum = 0.f, mean = 0.f;
-  for (int b = 0; b < p.batches; ++b) {
+  auto load = [&](int b, float (&v)[kBatch][VEC]) {
     const int piece = s.lo + b * (kThreads * kBatch) + t;
-    if (s.lo + b * (kThreads * kBatch) >= s.hi) break;
-    float v[kBatch][VEC];
+    if (s.lo + (b + 1) * (kThreads * kBatch) < s.hi && s.first(s.lo + b * (kThreads * kBatch)) >= 0) {   // all inside the row
+      Sixteen<T> x[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) s.load(piece + j * kThreads, v[j]);
+      for (int j = 0; j < kBatch; ++j) x[j] = *(const Sixteen<T>*)(s.row + s.first(piece + j * kThreads));
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[j][k] = widen<T>(x[j].e[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) s.load(piece + j * kThreads, v[j]);
+    }
+  };
+  for (int b = 0; s.lo + b * (kThreads * kBatch) < s.hi; ++b) {
+    float v[kBatch][VEC];
+    load(b, v);
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) mx = fmaxf(mx, v[j][k]);
+      for (int k = 0; k < VEC; k += 2) mx = fmaxf(mx, fmaxf(v[j][k], v[j][k + 1]));
     if (l.top) group_top[b * kThreads + t] = mx;
     if (mx > below_infinity(top)) {     // (infinities share all probability: each counts as the largest number)
       if (mx == INFINITY) {
@@ -209,120 +233,137 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
 #pragma unroll
           for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] == INFINITY ? FLT_MAX : v[j][k];
       }
-      if (top > -INFINITY) {
-        const float shift = fmaxf((below_infinity(top) - below_infinity(mx)) * k2, -200.f), f = exp2_fast(shift);
-        mean = f * (mean + shift * sum);
-        sum *= f;
-      }
+      if (top > -INFINITY) lower(sum, mean, top, mx, k2);
       top = mx;
     }
     const float base = below_infinity(top);
+    float sums[4] = {}, means[4] = {};
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         const float x = fmaxf((v[j][k] - base) * k2, -150.f), e = exp2_fast(x);   // (2^-150 is 0; NaN becomes that, too)
-        sum += e;
-        mean += e * x;
+        sums[k & 3] += e;
+        means[k & 3] += e * x;
       }
+    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    mean += (means[0] + means[1]) + (means[2] + means[3]);
   }
-  // ---- the block's, then the row's ----
-  const float block_top = block_max(top, w.red[0]);
+  // ---- the warp's, the block's ----
+  w.key[t] = key_of(top);
   {
-    const float shift = top > -INFINITY ? fmaxf((below_infinity(top) - below_infinity(block_top)) * k2, -200.f) : 0.f, f = exp2_fast(shift);
-    mean = f * (mean + shift * sum);
-    sum *= f;
+    const Sums mine = together<32>(Sums{top, sum, mean}, k2);
+    if (lane == 0) w.warp[warp] = mine;
   }
-  sum = block_sum(sum, w.red[1]);
-  mean = block_sum(mean, w.red[2]);
-  if (t == 0) { w.top = block_top; w.sum = sum; w.mean = mean; w.found = 0; w.count = 0; }
   __syncthreads();
+  Sums block{};
+  if (warp == 0) block = together<kWarps>(w.warp[lane & (kWarps - 1)], k2);
+  int found = 0;
   if (l.top) {
-    // the n-th largest of the threads' maxima, bit by bit
-    const uint32_t key = key_of(top);
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t next = bound | 1u << bit;
-      if (__syncthreads_count(key >= next) >= l.top) bound = next;
-    }
-    bound = max(bound, 1u);      // (0: logits of probability 0)
-    if (key >= bound)
-      for (int b = 0; b < p.batches; ++b) {
-        const int piece = s.lo + b * (kThreads * kBatch) + t;
-        if (piece >= s.hi) break;
-        if (key_of(group_top[b * kThreads + t]) < bound) continue;
-        for (int j = 0; j < kBatch; ++j) {
-          float v[VEC];
-          s.load(piece + j * kThreads, v);
+    uint32_t keys[kThreads / 32];
 #pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (key_of(v[k]) >= bound) {
+    for (int i = 0; i < kThreads / 32; ++i) keys[i] = w.key[i * 32 + lane];
+    uint32_t bound = 0;
+#pragma unroll
+    for (int shift = 28; shift >= 16; shift -= 4) {
+      const uint32_t at = bound | (uint32_t)warp << shift;
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) above += keys[i] >= at;
+      above = __reduce_add_sync(~0u, above);
+      int* counts = w.above[shift >> 2 & 1];
+      if (lane == 0) counts[warp] = above;
+      __syncthreads();
+      const uint32_t enough = __ballot_sync(~0u, lane < 16 && counts[lane & 15] >= l.top) | 1u;   // (falling counts)
+      bound |= (uint32_t)(31 - __clz(enough)) << shift;
+    }
+    const float least = value_of(bound);
+    if (top >= least)
+      for (int b = 0; s.lo + b * (kThreads * kBatch) < s.hi; ++b) {
+        if (!(group_top[b * kThreads + t] >= least)) continue;
+        float v[kBatch][VEC];
+        load(b, v);
+#pragma unroll 1
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            float x = v[0][k];
+#pragma unroll
+            for (int i = 1; i < kBatch; ++i) x = j == i ? v[i][k] : x;
+            if (x >= least) {
               const int at = atomicAdd(&w.count, 1);
-              if (at < kCandidates) { w.candidate[at] = v[k]; w.candidate_at[at] = s.first(piece + j * kThreads) + k; }
+              if (at < kCandidates) w.candidate[at] = entry(x, s.first(s.lo + b * (kThreads * kBatch) + t + j * kThreads) + k);
             }
-        }
+          }
       }
     __syncthreads();
     if (w.count > kCandidates) gather_exactly(s, l.top, w);
     __syncthreads();
     const int n = min(w.count, kCandidates);
+    found = min(n, l.top);
     for (int c = t; c < n; c += kThreads) {
-      const uint32_t mine = key_of(w.candidate[c]);
-      const int at = w.candidate_at[c];
+      const unsigned long long mine = w.candidate[c];
       int place = 0;
-      for (int i = 0; i < n; ++i) {
-        const uint32_t other = key_of(w.candidate[i]);
-        place += other > mine || (other == mine && w.candidate_at[i] < at);
-      }
-      if (place < l.top) { w.best[place] = w.candidate[c]; w.best_at[place] = at; }
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) place += w.candidate[i] > mine;
+      if (place < l.top) w.best[rank][place] = mine;
     }
-    if (t == 0) w.found = min(n, l.top);
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (p.share > 1) cluster.sync(); else __syncthreads();
-  if (rank == 0) {
-    float row_top = -INFINITY, row_sum = 0.f, row_mean = 0.f;
-    for (int i = 0; i < p.share; ++i) row_top = fmaxf(row_top, p.share > 1 ? cluster.map_shared_rank(&w, i)->top : w.top);
-    const float base = below_infinity(row_top);
-    for (int i = 0; i < p.share; ++i) {
-      const Shared* o = p.share > 1 ? cluster.map_shared_rank(&w, i) : &w;
-      const float shift = o->top > -INFINITY ? fmaxf((below_infinity(o->top) - base) * k2, -200.f) : 0.f, f = exp2_fast(shift);
-      row_mean += f * (o->mean + shift * o->sum);
-      row_sum += f * o->sum;
-    }
-    const float log_sum = logf(row_sum);
-    auto log_prob = [&](float v) {
-      if (!(v > -INFINITY) || (row_top == INFINITY && v < INFINITY)) return -INFINITY;
-      return (below_infinity(v) - base) / T1 - log_sum;
-    };
-    if (t == 0 && l.entropy) l.entropy[r] = row_sum > 0.f ? log_sum - kLn2 * row_mean / row_sum : 0.f;
-    for (int i = t; i < l.given; i += kThreads) {
-      const int token = l.tokens[r * l.given + i];
-      l.token_log_probs[r * l.given + i] = token >= 0 && token < l.vocab ? log_prob(widen<T>(s.row[token])) : -INFINITY;
-    }
-    // the CTAs' alternatives, each in order: a place is the number of those in front
-    int all = 0;
-    for (int i = 0; i < p.share; ++i) all += p.share > 1 ? cluster.map_shared_rank(&w, i)->found : w.found;
-    for (int c = t; c < p.share * l.top; c += kThreads) {
-      const int i = c / l.top, k = c - i * l.top;
-      const Shared* o = p.share > 1 ? cluster.map_shared_rank(&w, i) : &w;
-      if (k >= o->found) continue;
-      const float v = o->best[k];
-      const uint32_t mine = key_of(v);
-      int place = k;
-      for (int j = 0; j < p.share; ++j) {
-        if (j == i) continue;
-        const Shared* q = cluster.map_shared_rank(&w, j);
-        for (int m = 0; m < q->found; ++m) {
-          const uint32_t other = key_of(q->best[m]);
-          if (other > mine || (other == mine && j < i)) ++place; else break;
-        }
-      }
-      if (place < l.top) { l.top_tokens[r * l.top + place] = o->best_at[k]; l.top_log_probs[r * l.top + place] = log_prob(v); }
-    }
-    for (int k = all + t; k < l.top; k += kThreads) { l.top_tokens[r * l.top + k] = -1; l.top_log_probs[r * l.top + k] = -INFINITY; }
+  Shared* first = &w;
+  if (p.share > 1) {
+    first = cluster.map_shared_rank(&w, 0);
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    __syncthreads();
+    if (rank)
+      for (int k = t; k < found; k += kThreads) first->best[rank][k] = w.best[rank][k];
   }
-  if (p.share > 1) cluster.sync();   // (what the others read stays until they have)
+  if (t == 0) { first->all[rank] = block; first->found[rank] = found; }
+  if (p.share > 1) {
+    cluster.sync();
+    if (rank) return;
+  } else if (l.top) {
+    __syncthreads();
+  }
+  // ---- the row's ----
+  if (warp == 0) {
+    if (p.share > 1) block = together<kMaxShare>(lane % kMaxShare < p.share ? w.all[lane % kMaxShare] : Sums{-INFINITY, 0.f, 0.f}, k2);
+    const float log_sum = logf(block.sum);
+    if (lane == 0) {
+      w.top = block.top; w.log_sum = log_sum;
+      if (l.entropy) l.entropy[r] = block.sum > 0.f ? log_sum - kLn2 * block.mean / block.sum : 0.f;
+    }
+  }
+  if (!l.given && !l.top) return;
+  __syncthreads();
+  const float row_top = w.top, base = below_infinity(row_top), log_sum = w.log_sum;
+  auto log_prob = [&](float v) {
+    if (!(v > -INFINITY) || (row_top == INFINITY && v < INFINITY)) return -INFINITY;
+    return (below_infinity(v) - base) / T1 - log_sum;
+  };
+  for (int i = t; i < l.given; i += kThreads) {
+    const int token = l.tokens[r * l.given + i];
+    l.token_log_probs[r * l.given + i] = token >= 0 && token < l.vocab ? log_prob(widen<T>(s.row[token])) : -INFINITY;
+  }
+  int all = 0;
+  for (int i = 0; i < p.share; ++i) all += w.found[i];
+  for (int c = t; c < p.share * l.top; c += kThreads) {
+    const int i = p.share == 1 ? 0 : c / l.top, k = c - i * l.top;
+    if (k >= w.found[i]) continue;
+    const unsigned long long mine = w.best[i][k];
+    int place = k;
+    for (int j = 0; j < p.share; ++j)
+      if (j != i) {
+        const int n = w.found[j];
+#pragma unroll 4
+        for (int m = 0; m < n; ++m) place += w.best[j][m] > mine;
+      }
+    if (place < l.top) {
+      const uint32_t key = (uint32_t)(mine >> 32);
+      l.top_tokens[r * l.top + place] = (int)~(uint32_t)mine;
+      l.top_log_probs[r * l.top + place] = log_prob(__uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key));
+    }
+  }
+  for (int k = all + t; k < l.top; k += kThreads) { l.top_tokens[r * l.top + k] = -1; l.top_log_probs[r * l.top + k] = -INFINITY; }
 }
 
 template <typename T> int launch(const LogProbs& l, cudaStream_t stream) {
