@@ -12,8 +12,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kBatch = 4;       // 16-byte pieces that a thread has in flight, whose largest logit it remembers
-constexpr int kCandidates = 2048;               // logits that may be sorted for the alternatives
+constexpr int kThreads = 256, kBatch = 4;       // 16-byte pieces that a thread has in flight, whose largest logit it remembers
+constexpr int kCandidates = 1024;               // logits that may be sorted for the alternatives
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -40,11 +40,56 @@ struct Shared {
   unsigned long long candidate[kCandidates];
 };
 
-template <typename T> struct alignas(16) Sixteen { T e[16 / sizeof(T)]; };
+template <typename T> union alignas(16) Sixteen {
+  uint4 raw;
+  uint32_t u[4];
+  T e[16 / sizeof(T)];
+  __device__ __forceinline__ Sixteen() {}
+};
 template <typename T> __device__ __forceinline__ float widen(T v);
 template <> __device__ __forceinline__ float widen<float>(float v) { return v; }
 template <> __device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T minus_infinity();
+template <> __device__ __forceinline__ float minus_infinity<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ __half minus_infinity<__half>() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+// The largest of a few pieces' numbers (NaN where there is none but that); two-byte ones by pairs.
+template <int N> __device__ __forceinline__ float largest(const Sixteen<float> (&x)[N]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < N; ++j) m = fmaxf(m, fmaxf(fmaxf(x[j].e[0], x[j].e[1]), fmaxf(x[j].e[2], x[j].e[3])));
+  return m;
+}
+template <int N> __device__ __forceinline__ float largest(const Sixteen<__half> (&x)[N]) {
+  uint32_t m = x[0].u[0];
+#pragma unroll
+  for (int i = 1; i < 4 * N; ++i) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(x[i >> 2].u[i & 3]));
+  const float2 f = __half22float2(*(const __half2*)&m);
+  return fmaxf(f.x, f.y);
+}
+template <int N> __device__ __forceinline__ float largest(const Sixteen<__nv_bfloat16> (&x)[N]) {
+  uint32_t m = x[0].u[0];
+#pragma unroll
+  for (int i = 1; i < 4 * N; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(x[i >> 2].u[i & 3]));
+  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
   return x;
@@ -66,16 +111,21 @@ template <typename T> struct Slice {
   const T* row;       // (logit 0)
   int off, vocab, lo, hi;
   __device__ __forceinline__ int first(int piece) const { return piece * VEC - off; }   // index of its first logit
-  __device__ __forceinline__ void load(int piece, float (&v)[VEC]) const {
+  __device__ __forceinline__ Sixteen<T> load(int piece) const {   // (minus infinity outside)
+    Sixteen<T> x;
     const int i = first(piece);
     if (piece < hi && i >= 0 && i + VEC <= vocab) {
-      const Sixteen<T> x = *(const Sixteen<T>*)(row + i);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = widen<T>(x.e[k]);
+      x.raw = *(const uint4*)(row + i);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = piece < hi && i + k >= 0 && i + k < vocab ? widen<T>(row[i + k]) : -INFINITY;
+      for (int k = 0; k < VEC; ++k) x.e[k] = piece < hi && i + k >= 0 && i + k < vocab ? row[i + k] : minus_infinity<T>();
     }
+    return x;
+  }
+  __device__ __forceinline__ void load(int piece, float (&v)[VEC]) const {
+    const Sixteen<T> x = load(piece);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = widen<T>(x.e[k]);
   }
 };
 
@@ -179,7 +229,7 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
 // time, each warp counts for one of their sixteen values (bit by bit, 32 barriers and lists that the first CTA fetched entry by entry
 // made up 22 of 32 us for 64 rows of 128000 logits).  A candidate's place is the number of those in front of it.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_constant__ Params p) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ float group_top[];      // [batches][threads]
   __shared__ Shared w;
@@ -202,52 +252,59 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
   if (t == 0) w.count = 0;
 
   float top = -INFINITY, sum = 0.f, mean = 0.f;
-  auto load = [&](int b, float (&v)[kBatch][VEC]) {
+  auto load = [&](int b, Sixteen<T> (&x)[kBatch]) {
     const int piece = s.lo + b * (kThreads * kBatch) + t;
     if (s.lo + (b + 1) * (kThreads * kBatch) < s.hi && s.first(s.lo + b * (kThreads * kBatch)) >= 0) {   // all inside the row
-      Sixteen<T> x[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) x[j] = *(const Sixteen<T>*)(s.row + s.first(piece + j * kThreads));
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[j][k] = widen<T>(x[j].e[k]);
+      for (int j = 0; j < kBatch; ++j) x[j].raw = *(const uint4*)(s.row + s.first(piece + j * kThreads));
     } else {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) s.load(piece + j * kThreads, v[j]);
+      for (int j = 0; j < kBatch; ++j) x[j] = s.load(piece + j * kThreads);
     }
   };
-  for (int b = 0; s.lo + b * (kThreads * kBatch) < s.hi; ++b) {
-    float v[kBatch][VEC];
-    load(b, v);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-      for (int k = 0; k < VEC; k += 2) mx = fmaxf(mx, fmaxf(v[j][k], v[j][k + 1]));
+  const int batches = (s.hi - s.lo + kThreads * kBatch - 1) / (kThreads * kBatch);
+  Sixteen<T> x[kBatch];
+  if (batches) load(0, x);
+  for (int b = 0; b < batches; ++b) {
+    Sixteen<T> next[kBatch];
+    if (b + 1 < batches) load(b + 1, next);
+    const float mx = largest(x);
     if (l.top) group_top[b * kThreads + t] = mx;
     if (mx > below_infinity(top)) {     // (infinities share all probability: each counts as the largest number)
-      if (mx == INFINITY) {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] == INFINITY ? FLT_MAX : v[j][k];
-      }
       if (top > -INFINITY) lower(sum, mean, top, mx, k2);
       top = mx;
     }
     const float base = below_infinity(top);
-    float sums[4] = {}, means[4] = {};
+    float2 sums[2] = {}, means[2] = {};
+    if (top < INFINITY) {
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
+      for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float x = fmaxf((v[j][k] - base) * k2, -150.f), e = exp2_fast(x);   // (2^-150 is 0; NaN becomes that, too)
-        sums[k & 3] += e;
-        means[k & 3] += e * x;
+        for (int k = 0; k < VEC; k += 2) {
+          float2 y = mul2(add2(make_float2(widen<T>(x[j].e[k]), widen<T>(x[j].e[k + 1])), make_float2(-base, -base)), make_float2(k2, k2));
+          y.x = fmaxf(y.x, -150.f);   // (2^-150 is 0; NaN becomes that, too)
+          y.y = fmaxf(y.y, -150.f);
+          const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+          sums[k >> 1 & 1] = add2(sums[k >> 1 & 1], e);
+          means[k >> 1 & 1] = fma2(e, y, means[k >> 1 & 1]);
+        }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kBatch * VEC; ++i) {
+        float v = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v = i == j * VEC + k ? widen<T>(x[j].e[k]) : v;
+        const float y = fmaxf((below_infinity(v) - base) * k2, -150.f), e = v > -INFINITY ? exp2_fast(y) : 0.f;
+        sums[0].x += e;
+        means[0].x += e * y;
       }
-    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    mean += (means[0] + means[1]) + (means[2] + means[3]);
+    }
+    sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+    mean += (means[0].x + means[0].y) + (means[1].x + means[1].y);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j].raw = next[j].raw;
   }
   // ---- the warp's, the block's ----
   w.key[t] = key_of(top);
@@ -266,35 +323,41 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
     uint32_t bound = 0;
 #pragma unroll
     for (int shift = 28; shift >= 16; shift -= 4) {
-      const uint32_t at = bound | (uint32_t)warp << shift;
-      int above = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) above += keys[i] >= at;
-      above = __reduce_add_sync(~0u, above);
       int* counts = w.above[shift >> 2 & 1];
-      if (lane == 0) counts[warp] = above;
+#pragma unroll
+      for (int e = 0; e < 16; e += kWarps) {
+        const uint32_t at = bound | (uint32_t)(warp + e) << shift;
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i) above += keys[i] >= at;
+        above = __reduce_add_sync(~0u, above);
+        if (lane == 0) counts[warp + e] = above;
+      }
       __syncthreads();
       const uint32_t enough = __ballot_sync(~0u, lane < 16 && counts[lane & 15] >= l.top) | 1u;   // (falling counts)
       bound |= (uint32_t)(31 - __clz(enough)) << shift;
     }
     const float least = value_of(bound);
     if (top >= least)
-      for (int b = 0; s.lo + b * (kThreads * kBatch) < s.hi; ++b) {
+      for (int b = 0; b < batches; ++b) {
         if (!(group_top[b * kThreads + t] >= least)) continue;
-        float v[kBatch][VEC];
-        load(b, v);
+        load(b, x);
 #pragma unroll 1
-        for (int j = 0; j < kBatch; ++j)
+        for (int j = 0; j < kBatch; ++j) {
+          Sixteen<T> y;
+          y.raw = x[0].raw;
+#pragma unroll
+          for (int i = 1; i < kBatch; ++i)
+            if (j == i) y.raw = x[i].raw;
 #pragma unroll
           for (int k = 0; k < VEC; ++k) {
-            float x = v[0][k];
-#pragma unroll
-            for (int i = 1; i < kBatch; ++i) x = j == i ? v[i][k] : x;
-            if (x >= least) {
+            const float v = widen<T>(y.e[k]);
+            if (v >= least) {
               const int at = atomicAdd(&w.count, 1);
-              if (at < kCandidates) w.candidate[at] = entry(x, s.first(s.lo + b * (kThreads * kBatch) + t + j * kThreads) + k);
+              if (at < kCandidates) w.candidate[at] = entry(v, s.first(s.lo + b * (kThreads * kBatch) + t + j * kThreads) + k);
             }
           }
+        }
       }
     __syncthreads();
     if (w.count > kCandidates) gather_exactly(s, l.top, w);
