@@ -12,7 +12,7 @@ namespace {
 
 constexpr unsigned kMany = 4 * 148;
 constexpr int kEach = 2;
-constexpr int kMaxThreads = 1024, kShort = 32;   // threads of a row; of a row that shares its block with others
+constexpr int kMaxThreads = 1024, kShort = 32, kShortThreads = 256, kRows = 2;   // threads of a row; of a row that shares its block with others
 
 template <int BYTES> struct Raw;
 template <> struct Raw<16> { typedef uint4 type; };
@@ -51,26 +51,54 @@ template <int VEC> __device__ __forceinline__ void to_e4m3(const float (&v)[VEC]
     }
 }
 
+template <int VEC> __device__ __forceinline__ void load_weight(const RmsNorm& n, int c, float (&w)[VEC]) {   // of piece c, with the offset
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) w[k] = 1.f;
+  if (n.weight && n.weight_dt == DT_F32) {
+    constexpr int W = VEC >= 4 ? 4 : 1;
+#pragma unroll
+    for (int k = 0; k < VEC; k += W) {
+      Piece<float, W> v;
+      v.raw = *(const decltype(v.raw)*)((const float*)n.weight + (int64_t)c * VEC + k);
+#pragma unroll
+      for (int e = 0; e < W; ++e) w[k + e] = v.e[e];
+    }
+  } else if (n.weight) {
+    Piece<uint16_t, VEC> v;
+    v.raw = *(const decltype(v.raw)*)((const uint16_t*)n.weight + (int64_t)c * VEC);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] = n.weight_dt == DT_F16 ? __half2float(__ushort_as_half(v.e[k])) : __uint_as_float((uint32_t)v.e[k] << 16);
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) w[k] += n.weight_offset;
+}
+// What values of a group are multiplied by, for its largest magnitude as a whole number.
+__device__ __forceinline__ float inverse_of(uint32_t top, float most) {
+  const float inverse = most / __uint_as_float(top);
+  if (top == 0 || top >= 0x7f800000u || inverse == INFINITY) return top > 0x7f800000u ? __uint_as_float(top) : 0.f;
+  return inverse;
+}
+
 struct Params {
   RmsNorm n;
+  float per_channel;      // 1 / channels
   int pieces, lanes;      // VEC channels each; threads of a row
-  int rows_of_block;      // 1, or rows of up to 32 threads each
+  int rows_of_block, step_row, step_head;   // short rows of a block at a time, and what that is in rows and heads
   int group_shift;        // a group is 1 << group_shift pieces of neighbouring threads; -1: the row; -2: any, counted in shared memory; -3: no scales to find
 };
 
 // h = round(x + residual), y = h / sqrt(mean(h h) + epsilon) * (w + offset), and y in 8 bits with scales.
 // Bound by memory: x and residual are read once and stay in registers (NP pieces of 16 bytes a thread), each result is written once.  Sums of squares
-// are 32-bit, by thread, then by warp, then by block.  A row of few pieces takes `lanes` threads of a warp and shares the block.
+// are 32-bit, by thread, then by warp, then by block.
 // Largest magnitudes are compared as whole numbers, which order them and keep a NaN.
 template <typename T, int VEC, int NP>
-__global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) norm_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint32_t tops[];      // of each group (group_shift -2)
   __shared__ float sums[32];
   __shared__ uint32_t largest[32];
   const RmsNorm& n = p.n;
-  const int t = p.rows_of_block == 1 ? threadIdx.x : threadIdx.x % p.lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned at = p.rows_of_block == 1 ? blockIdx.x : blockIdx.x * p.rows_of_block + threadIdx.x / p.lanes;
-  const bool live = at < n.total;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const unsigned at = blockIdx.x;
   const unsigned row = n.heads == 1 ? at : at / n.heads, head = at - row * n.heads;
   auto place = [&](const void* base, int part) { return (T*)base + (int64_t)row * n.row[part] + (int64_t)head * n.head[part]; };
   float h[NP][VEC];
@@ -82,7 +110,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = t + i * p.lanes;
-      const bool there = live && c < p.pieces;
+      const bool there = c < p.pieces;
       if (there) x[i].raw = *(const decltype(x[i].raw)*)(xp + (int64_t)c * VEC);
       if (there && n.residual) r[i].raw = *(const decltype(x[i].raw)*)(rp + (int64_t)c * VEC);
     }
@@ -90,7 +118,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int c = t + i * p.lanes;
-      const bool there = live && c < p.pieces;
+      const bool there = c < p.pieces;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         h[i][k] = there ? widen<T>(x[i].e[k]) : 0.f;
@@ -104,50 +132,30 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
     }
   }
   if (!n.y && !n.quant) return;
-  const int among = min(p.lanes, 32);
-  for (int o = among / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
-  if (p.lanes > 32) {
-    if (lane == 0) sums[warp] = square;
-    if (p.group_shift == -2)
-      for (int g = threadIdx.x; g < n.channels / n.group; g += blockDim.x) tops[g] = 0;
-    __syncthreads();
-    square = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
-  }
-  const float factor = 1.f / sqrtf(square / (float)n.channels + n.epsilon);
+  for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+  if (lane == 0) sums[warp] = square;
+  if (p.group_shift == -2)
+    for (int g = threadIdx.x; g < n.channels / n.group; g += blockDim.x) tops[g] = 0;
+  __syncthreads();
+  square = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+  const float factor = rsqrtf(square * p.per_channel + n.epsilon);
   uint32_t top[NP];
   uint32_t row_top = 0;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int c = t + i * p.lanes;
-    const bool there = live && c < p.pieces;
+    const bool there = c < p.pieces;
     top[i] = 0;
     if (!there) continue;
     float w[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) w[k] = 1.f;
-    if (n.weight) {
-      if (n.weight_dt == DT_F32) {
-#pragma unroll
-        for (int k = 0; k < VEC; k += VEC >= 4 ? 4 : 1) {
-          constexpr int W = VEC >= 4 ? 4 : 1;
-          Piece<float, W> v;
-          v.raw = *(const decltype(v.raw)*)((const float*)n.weight + (int64_t)c * VEC + k);
-#pragma unroll
-          for (int e = 0; e < W; ++e) w[k + e] = v.e[e];
-        }
-      } else {
-        Piece<uint16_t, VEC> v;
-        v.raw = *(const decltype(v.raw)*)((const uint16_t*)n.weight + (int64_t)c * VEC);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) w[k] = n.weight_dt == DT_F16 ? __half2float(__ushort_as_half(v.e[k])) : __uint_as_float((uint32_t)v.e[k] << 16);
-      }
-    }
+    load_weight<VEC>(n, c, w);
     Piece<T, VEC> y;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      h[i][k] = h[i][k] * factor * (w[k] + n.weight_offset);
+      h[i][k] = h[i][k] * factor * w[k];
       y.e[k] = narrow<T>(h[i][k]);
       top[i] = max(top[i], __float_as_uint(h[i][k]) & 0x7fffffffu);
     }
@@ -158,19 +166,17 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
   const float most = n.quant == 1 ? 127.f : 448.f;
   const int64_t groups = n.group ? n.channels / n.group : 1;
   if (p.group_shift == -1) {
-    for (int o = among / 2; o; o >>= 1) row_top = max(row_top, __shfl_xor_sync(~0u, row_top, o));
-    if (p.lanes > 32) {
-      if (lane == 0) largest[warp] = row_top;
-      __syncthreads();
-      row_top = __reduce_max_sync(~0u, lane < (int)(blockDim.x >> 5) ? largest[lane] : 0u);
-    }
-    if (live && t == 0) n.scales[at] = __uint_as_float(row_top) / most;
+    row_top = __reduce_max_sync(~0u, row_top);
+    if (lane == 0) largest[warp] = row_top;
+    __syncthreads();
+    row_top = __reduce_max_sync(~0u, lane < (int)(blockDim.x >> 5) ? largest[lane] : 0u);
+    if (t == 0) n.scales[at] = __uint_as_float(row_top) / most;
   } else if (p.group_shift >= 0) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       for (int o = 1; o < 1 << p.group_shift; o <<= 1) top[i] = max(top[i], __shfl_xor_sync(~0u, top[i], o));
       const int c = t + i * p.lanes;
-      if (live && c < p.pieces && (c & ((1 << p.group_shift) - 1)) == 0) n.scales[at * groups + (c >> p.group_shift)] = __uint_as_float(top[i]) / most;
+      if (c < p.pieces && (c & ((1 << p.group_shift) - 1)) == 0) n.scales[at * groups + (c >> p.group_shift)] = __uint_as_float(top[i]) / most;
     }
   } else if (p.group_shift == -2) {
 #pragma unroll
@@ -185,12 +191,11 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int c = t + i * p.lanes;
-    if (!live || c >= p.pieces) continue;
+    if (c >= p.pieces) continue;
     float inverse = 0.f;
     if (p.group_shift != -3) {
       const uint32_t u = p.group_shift == -1 ? row_top : p.group_shift == -2 ? tops[c * VEC / n.group] : top[i];
-      inverse = most / __uint_as_float(u);
-      if (u == 0 || u >= 0x7f800000u || inverse == INFINITY) inverse = u > 0x7f800000u ? __uint_as_float(u) : 0.f;
+      inverse = inverse_of(u, most);
     }
     Piece<uint8_t, VEC> q;
     float v[VEC];
@@ -198,6 +203,75 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const __grid_constant
     for (int k = 0; k < VEC; ++k) v[k] = p.group_shift == -3 ? h[i][k] / given : h[i][k] * inverse;
     if (n.quant == 1) to_int8<VEC>(v, q.e); else to_e4m3<VEC>(v, q.e);
     *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)row * n.row[4] + (int64_t)head * n.head[4] + (int64_t)c * VEC) = q.raw;
+  }
+}
+
+// The same for rows of up to 32 pieces (heads): `lanes` threads of a warp have a piece each, of ROWS rows, whose loads are under way together and which
+// share the weight (a row for each: 27.7 us for 4097 tokens of 32 heads of 128).
+template <typename T, int VEC, int ROWS>
+__global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_constant__ Params p) {
+  const RmsNorm& n = p.n;
+  const int c = threadIdx.x & (p.lanes - 1);
+  unsigned at = blockIdx.x * (unsigned)(p.rows_of_block * ROWS) + threadIdx.x / p.lanes;
+  unsigned row = n.heads == 1 ? at : at / n.heads, head = at - row * n.heads;
+  unsigned rows[ROWS], heads[ROWS];
+  bool there[ROWS];
+  Piece<T, VEC> x[ROWS], r[ROWS];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    rows[i] = row;
+    heads[i] = head;
+    there[i] = at + i * p.rows_of_block < n.total && c < p.pieces;
+    if (there[i]) x[i].raw = *(const decltype(x[i].raw)*)((const T*)n.x + (int64_t)row * n.row[0] + (int64_t)head * n.head[0] + c * VEC);
+    if (there[i] && n.residual) r[i].raw = *(const decltype(x[i].raw)*)((const T*)n.residual + (int64_t)row * n.row[1] + (int64_t)head * n.head[1] + c * VEC);
+    row += p.step_row;
+    head += p.step_head;
+    if (head >= (unsigned)n.heads) { head -= n.heads; ++row; }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  float w[VEC];
+  if (c < p.pieces) load_weight<VEC>(n, c, w);
+  const float most = n.quant == 1 ? 127.f : 448.f, given = p.group_shift == -3 ? n.scales[0] : 0.f;
+  const int groups = n.group ? n.channels / n.group : 1;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    auto place = [&](void* base, int part) { return (T*)base + (int64_t)rows[i] * n.row[part] + (int64_t)heads[i] * n.head[part] + c * VEC; };
+    float h[VEC], square = 0.f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      h[k] = there[i] ? widen<T>(x[i].e[k]) : 0.f;
+      if (there[i] && n.residual) {
+        x[i].e[k] = narrow<T>(h[k] + widen<T>(r[i].e[k]));
+        h[k] = widen<T>(x[i].e[k]);
+      }
+      square += h[k] * h[k];
+    }
+    if (there[i] && n.sum) *(decltype(x[i].raw)*)place(n.sum, 2) = x[i].raw;
+    for (int o = p.lanes / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+    const float factor = rsqrtf(square * p.per_channel + n.epsilon);
+    uint32_t top = 0;
+    Piece<T, VEC> y;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      h[k] = there[i] ? h[k] * factor * w[k] : 0.f;
+      y.e[k] = narrow<T>(h[k]);
+      top = max(top, __float_as_uint(h[k]) & 0x7fffffffu);
+    }
+    if (there[i] && n.y) *(decltype(y.raw)*)place(n.y, 3) = y.raw;
+    if (!n.quant) continue;
+    float inverse = 0.f;
+    if (p.group_shift != -3) {
+      const int across = p.group_shift == -1 ? p.lanes : 1 << p.group_shift;
+      for (int o = 1; o < across; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+      inverse = inverse_of(top, most);
+      if (there[i] && (c & (across - 1)) == 0) n.scales[(int64_t)(at + i * p.rows_of_block) * groups + c / across] = __uint_as_float(top) / most;
+    }
+    Piece<uint8_t, VEC> q;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) h[k] = p.group_shift == -3 ? h[k] / given : h[k] * inverse;
+    if (n.quant == 1) to_int8<VEC>(h, q.e); else to_e4m3<VEC>(h, q.e);
+    if (there[i]) *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)rows[i] * n.row[4] + (int64_t)heads[i] * n.head[4] + c * VEC) = q.raw;
   }
 }
 
@@ -212,6 +286,7 @@ template <typename T> int launch(const RmsNorm& n, cudaStream_t stream) {
   if (n.weight) wide = wide && (uintptr_t)n.weight % (n.weight_dt == DT_F32 ? 16 : 2 * VEC) == 0;
   Params p{};
   p.n = n;
+  p.per_channel = 1.f / (float)n.channels;
   const int vec = wide ? VEC : 1;
   p.pieces = n.channels / vec;
   if (n.quant && n.group == 0) p.group_shift = -3;
@@ -222,29 +297,34 @@ template <typename T> int launch(const RmsNorm& n, cudaStream_t stream) {
     while (1 << shift < of) ++shift;
     p.group_shift = n.group % vec == 0 && 1 << shift == of && of <= 32 ? shift : -2;
   }
-  int threads;
+  int threads, each;   // rows of a thread
+  void (*fn)(Params);
   if (wide && p.pieces <= kShort && p.group_shift != -2) {
     p.lanes = 1;
     while (p.lanes < p.pieces) p.lanes *= 2;
-    threads = 256;
+    threads = kShortThreads;
     p.rows_of_block = threads / p.lanes;
+    p.step_row = p.rows_of_block / n.heads;
+    p.step_head = p.rows_of_block % n.heads;
+    each = n.total / p.rows_of_block >= kMany * kRows ? kRows : 1;
+    fn = each == 1 ? short_kernel<T, VEC, 1> : short_kernel<T, VEC, kRows>;
   } else {
     // one piece for each thread, up to 1024; two where rows are many, so that more of them are under way
     p.rows_of_block = 1;
     const int wanted = wide && n.total >= kMany ? (p.pieces + kEach - 1) / kEach : p.pieces;
     threads = std::max(64, std::min(kMaxThreads, (wanted + 31) / 32 * 32));
     p.lanes = threads;
+    const int pieces = (p.pieces + threads - 1) / threads;
+    if (!wide) fn = pieces <= 8 ? norm_kernel<T, 1, 8> : norm_kernel<T, 1, 32>;
+    else if (pieces == 1) fn = norm_kernel<T, VEC, 1>;
+    else if (pieces == 2 && threads <= 512) fn = norm_kernel<T, VEC, 2>;
+    else if (pieces <= 4) fn = norm_kernel<T, VEC, 4>;
+    else fn = norm_kernel<T, VEC, VEC == 4 ? 8 : 4>;   // (32768 channels of two bytes are four pieces for each of 1024 threads)
+    each = 1;
   }
-  const int each = (p.pieces + p.lanes - 1) / p.lanes;
   const size_t smem = p.group_shift == -2 ? sizeof(uint32_t) * (size_t)(n.channels / n.group) : 0;
-  void (*fn)(Params);
-  if (!wide) fn = each <= 8 ? norm_kernel<T, 1, 8> : norm_kernel<T, 1, 32>;
-  else if (each == 1) fn = norm_kernel<T, VEC, 1>;
-  else if (each == 2) fn = norm_kernel<T, VEC, 2>;
-  else if (each <= 4) fn = norm_kernel<T, VEC, 4>;
-  else fn = norm_kernel<T, VEC, VEC == 4 ? 8 : 4>;   // (32768 channels of two bytes are four pieces for each of 1024 threads)
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((n.total + p.rows_of_block - 1) / p.rows_of_block);
+  cfg.gridDim = dim3((n.total + p.rows_of_block * each - 1) / (p.rows_of_block * each));
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
