@@ -5,6 +5,7 @@
 
 #include "attention.cuh"
 #include "kernels.h"
+#include "per_device.h"
 
 namespace b200 {
 namespace {
@@ -795,11 +796,12 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    cudaGetLastError();
+  static std::atomic<uint64_t> told{0};
+  if (!once_per_device(told, [&] {
+        return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+               cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+      }))
     return -2;
-  }
   // How many clusters of each size fit: the same for every call (GPUs of this kind have the same SMs).
   static const Fit fit = [&] {
     Fit f{};

@@ -6,6 +6,7 @@
 #include <cfloat>
 
 #include "kernels.h"
+#include "per_device.h"
 
 namespace b200 {
 namespace {
@@ -13,6 +14,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kBatch = 4;       // 16-byte pieces that a thread has in flight, whose largest logit it remembers
+constexpr size_t kMostSmem = 96 * 1024;         // for the batches' largest logits: 66 KB for 262144 of four bytes
 constexpr int kCandidates = 1024;               // logits that may be sorted for the alternatives
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -439,7 +441,8 @@ template <typename T> int launch(const LogProbs& l, cudaStream_t stream) {
   p.batches = ((pieces + p.share - 1) / p.share + kThreads * kBatch - 1) / (kThreads * kBatch);
   const size_t smem = l.top ? sizeof(float) * (size_t)p.batches * kThreads : 0;
   auto* fn = log_probs_kernel<T>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != cudaSuccess) { cudaGetLastError(); return -2; }
+  static std::atomic<uint64_t> told{0};
+  if (smem > kMostSmem || !once_per_device(told, [&] { return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) == cudaSuccess; })) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(l.rows * p.share));
   cfg.blockDim = dim3(kThreads);
