@@ -116,11 +116,15 @@ template <typename T> struct Slice {
   __device__ __forceinline__ Sixteen<T> load(int piece) const {   // (minus infinity outside)
     Sixteen<T> x;
     const int i = first(piece);
-    if (piece < hi && i >= 0 && i + VEC <= vocab) {
-      x.raw = *(const uint4*)(row + i);
-    } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x.e[k] = piece < hi && i + k >= 0 && i + k < vocab ? row[i + k] : minus_infinity<T>();
+    for (int k = 0; k < VEC; ++k) x.e[k] = minus_infinity<T>();
+    if (piece < hi) {
+      if (i >= 0 && i + VEC <= vocab) x.raw = *(const uint4*)(row + i);
+      else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (i + k >= 0 && i + k < vocab) x.e[k] = row[i + k];
+      }
     }
     return x;
   }

@@ -4,6 +4,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -34,23 +35,81 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-// VEC values in 8 bits, to the nearest.  int8: 1.5 * 2^23 more, a number's lowest bits are the whole number (a conversion is issued at a
-// quarter of the rate of a sum); NaN: 0.
-template <int VEC> __device__ __forceinline__ void to_int8(const float (&v)[VEC], uint8_t (&q)[VEC]) {
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) q[k] = (uint8_t)(__float_as_uint(fminf(fmaxf(v[k] == v[k] ? v[k] : 0.f, -128.f), 127.f) + 12582912.f) & 0xffu);
-}
-template <int VEC> __device__ __forceinline__ void to_e4m3(const float (&v)[VEC], uint8_t (&q)[VEC]) {
-  if constexpr (VEC == 1) q[0] = (uint8_t)__nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
-  else
+// A piece's values, and back, rounded; two-byte types by pairs.
+template <typename T, int VEC> __device__ __forceinline__ void unpack(const Piece<T, VEC>& p, float (&v)[VEC]) {
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
 #pragma unroll
     for (int k = 0; k < VEC; k += 2) {
-      const uint16_t two = (uint16_t)__nv_cvt_float2_to_fp8x2(make_float2(v[k], v[k + 1]), __NV_SATFINITE, __NV_E4M3);
-      q[k] = (uint8_t)two;
-      q[k + 1] = (uint8_t)(two >> 8);
+      const uint32_t u = ((const uint32_t*)&p.raw)[k / 2];
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*(const __half2*)&u);
+        v[k] = f.x;
+        v[k + 1] = f.y;
+      } else {
+        v[k] = __uint_as_float(u << 16);
+        v[k + 1] = __uint_as_float(u & 0xffff0000u);
+      }
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = widen<T>(p.e[k]);
+  }
 }
-
+template <typename T, int VEC> __device__ __forceinline__ void pack(const float (&v)[VEC], Piece<T, VEC>& p) {
+  if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(v[k], v[k + 1]);
+        ((uint32_t*)&p.raw)[k / 2] = *(const uint32_t*)&h;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
+        ((uint32_t*)&p.raw)[k / 2] = *(const uint32_t*)&h;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) p.e[k] = narrow<T>(v[k]);
+  }
+}
+// The largest magnitude; a NaN stays one.
+template <int VEC> __device__ __forceinline__ float magnitude(const float (&v)[VEC]) {
+  float m = fabsf(v[0]);
+#pragma unroll
+  for (int k = 1; k < VEC; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[k])));
+  return m;
+}
+// Values in 8 bits, to the nearest.  int8: 1.5 * 2^23 more, a number's lowest bits are the whole number (a conversion is issued at a quarter of the rate of
+// a sum); `bounded` values are numbers of no more than 127.
+template <int VEC> __device__ __forceinline__ void to_int8(float (&v)[VEC], bool bounded, Piece<uint8_t, VEC>& q) {
+  if (!bounded) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = fminf(fmaxf(v[k] == v[k] ? v[k] : 0.f, -128.f), 127.f);
+  }
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(v[k + e] + 12582912.f);
+      ((uint32_t*)&q.raw)[k / 4] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q.e[k] = (uint8_t)(__float_as_uint(v[k] + 12582912.f) & 0xffu);
+  }
+}
+template <int VEC> __device__ __forceinline__ void to_e4m3(const float (&v)[VEC], Piece<uint8_t, VEC>& q) {
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4)
+      ((uint32_t*)&q.raw)[k / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[k], v[k + 1]), __NV_SATFINITE, __NV_E4M3) |
+                                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[k + 2], v[k + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q.e[k] = (uint8_t)__nv_cvt_float_to_fp8(v[k], __NV_SATFINITE, __NV_E4M3);
+  }
+}
 template <int VEC> __device__ __forceinline__ void load_weight(const RmsNorm& n, int c, float (&w)[VEC]) {   // of piece c, with the offset
 #pragma unroll
   for (int k = 0; k < VEC; ++k) w[k] = 1.f;
@@ -119,14 +178,18 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
     for (int i = 0; i < NP; ++i) {
       const int c = t + i * p.lanes;
       const bool there = c < p.pieces;
+      if (there) {
+        unpack<T, VEC>(x[i], h[i]);
+        if (n.residual) {
+          float v[VEC];
+          unpack<T, VEC>(r[i], v);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        h[i][k] = there ? widen<T>(x[i].e[k]) : 0.f;
-        if (there && n.residual) {
-          x[i].e[k] = narrow<T>(h[i][k] + widen<T>(r[i].e[k]));
-          h[i][k] = widen<T>(x[i].e[k]);
+          for (int k = 0; k < VEC; ++k) v[k] += h[i][k];
+          pack<T, VEC>(v, x[i]);
+          unpack<T, VEC>(x[i], h[i]);
         }
-        square += h[i][k] * h[i][k];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) square += h[i][k] * h[i][k];
       }
       if (there && n.sum) *(decltype(x[i].raw)*)(place(n.sum, 2) + (int64_t)c * VEC) = x[i].raw;
     }
@@ -154,12 +217,12 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
     load_weight<VEC>(n, c, w);
     Piece<T, VEC> y;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      h[i][k] = h[i][k] * factor * w[k];
-      y.e[k] = narrow<T>(h[i][k]);
-      top[i] = max(top[i], __float_as_uint(h[i][k]) & 0x7fffffffu);
+    for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * factor * w[k];
+    pack<T, VEC>(h[i], y);
+    if (n.quant) {
+      top[i] = __float_as_uint(magnitude<VEC>(h[i]));
+      row_top = max(row_top, top[i]);
     }
-    row_top = max(row_top, top[i]);
     if (n.y) *(decltype(y.raw)*)(place(n.y, 3) + (int64_t)c * VEC) = y.raw;
   }
   if (!n.quant) return;
@@ -193,15 +256,16 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
     const int c = t + i * p.lanes;
     if (c >= p.pieces) continue;
     float inverse = 0.f;
+    uint32_t u = 0xffffffffu;
     if (p.group_shift != -3) {
-      const uint32_t u = p.group_shift == -1 ? row_top : p.group_shift == -2 ? tops[c * VEC / n.group] : top[i];
+      u = p.group_shift == -1 ? row_top : p.group_shift == -2 ? tops[c * VEC / n.group] : top[i];
       inverse = inverse_of(u, most);
     }
     Piece<uint8_t, VEC> q;
     float v[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) v[k] = p.group_shift == -3 ? h[i][k] / given : h[i][k] * inverse;
-    if (n.quant == 1) to_int8<VEC>(v, q.e); else to_e4m3<VEC>(v, q.e);
+    if (n.quant == 1) to_int8<VEC>(v, u < 0x7f800000u, q); else to_e4m3<VEC>(v, q);
     *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)row * n.row[4] + (int64_t)head * n.head[4] + (int64_t)c * VEC) = q.raw;
   }
 }
@@ -238,28 +302,29 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
   for (int i = 0; i < ROWS; ++i) {
     auto place = [&](void* base, int part) { return (T*)base + (int64_t)rows[i] * n.row[part] + (int64_t)heads[i] * n.head[part] + c * VEC; };
     float h[VEC], square = 0.f;
+    if (there[i]) {
+      unpack<T, VEC>(x[i], h);
+      if (n.residual) {
+        float v[VEC];
+        unpack<T, VEC>(r[i], v);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      h[k] = there[i] ? widen<T>(x[i].e[k]) : 0.f;
-      if (there[i] && n.residual) {
-        x[i].e[k] = narrow<T>(h[k] + widen<T>(r[i].e[k]));
-        h[k] = widen<T>(x[i].e[k]);
+        for (int k = 0; k < VEC; ++k) v[k] += h[k];
+        pack<T, VEC>(v, x[i]);
+        unpack<T, VEC>(x[i], h);
       }
-      square += h[k] * h[k];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) square += h[k] * h[k];
     }
     if (there[i] && n.sum) *(decltype(x[i].raw)*)place(n.sum, 2) = x[i].raw;
     for (int o = p.lanes / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
     const float factor = rsqrtf(square * p.per_channel + n.epsilon);
-    uint32_t top = 0;
     Piece<T, VEC> y;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      h[k] = there[i] ? h[k] * factor * w[k] : 0.f;
-      y.e[k] = narrow<T>(h[k]);
-      top = max(top, __float_as_uint(h[k]) & 0x7fffffffu);
-    }
+    for (int k = 0; k < VEC; ++k) h[k] = h[k] * factor * w[k];
+    pack<T, VEC>(h, y);
     if (there[i] && n.y) *(decltype(y.raw)*)place(n.y, 3) = y.raw;
     if (!n.quant) continue;
+    uint32_t top = there[i] ? __float_as_uint(magnitude<VEC>(h)) : 0u;
     float inverse = 0.f;
     if (p.group_shift != -3) {
       const int across = p.group_shift == -1 ? p.lanes : 1 << p.group_shift;
@@ -270,7 +335,7 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
     Piece<uint8_t, VEC> q;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) h[k] = p.group_shift == -3 ? h[k] / given : h[k] * inverse;
-    if (n.quant == 1) to_int8<VEC>(h, q.e); else to_e4m3<VEC>(h, q.e);
+    if (n.quant == 1) to_int8<VEC>(h, p.group_shift != -3 && top < 0x7f800000u, q); else to_e4m3<VEC>(h, q);
     if (there[i]) *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)rows[i] * n.row[4] + (int64_t)heads[i] * n.head[4] + c * VEC) = q.raw;
   }
 }
