@@ -15,6 +15,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kBatch = 4;       // 16-byte pieces that a thread has in flight, whose largest logit it remembers
 constexpr size_t kMostSmem = 96 * 1024;         // for the batches' largest logits: 66 KB for 262144 of four bytes
+constexpr int kHits = 512;                      // batches that may hold some of them
 constexpr int kCandidates = 1024;               // logits that may be sorted for the alternatives
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -37,7 +38,7 @@ struct Shared {
   float log_sum, base, top;
   uint32_t key[kThreads];                        // of the threads' largest logits
   int above[2][16];
-  int count, left, kept;
+  int count, left, kept, hits, hit[kHits];
   uint32_t bins[256], prefix;
   unsigned long long candidate[kCandidates];
 };
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
   s.hi = min(pieces, s.lo + each);
   const float temperature = l.temperature ? l.temperature[r] : 1.f, T1 = temperature > 0.f ? temperature : 1.f;
   const float k2 = fminf(kLog2e / T1, FLT_MAX);
-  if (t == 0) w.count = 0;
+  if (t == 0) { w.count = 0; w.hits = 0; }
 
   float top = -INFINITY, sum = 0.f, mean = 0.f;
   auto load = [&](int b, Sixteen<T> (&x)[kBatch]) {
@@ -343,28 +344,33 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
       const uint32_t enough = __ballot_sync(~0u, lane < 16 && counts[lane & 15] >= l.top) | 1u;   // (falling counts)
       bound |= (uint32_t)(31 - __clz(enough)) << shift;
     }
+    // batches that hold one, then their pieces, a thread for each
     const float least = value_of(bound);
-    if (top >= least)
-      for (int b = 0; b < batches; ++b) {
-        if (!(group_top[b * kThreads + t] >= least)) continue;
-        load(b, x);
-#pragma unroll 1
-        for (int j = 0; j < kBatch; ++j) {
-          Sixteen<T> y;
-          y.raw = x[0].raw;
-#pragma unroll
-          for (int i = 1; i < kBatch; ++i)
-            if (j == i) y.raw = x[i].raw;
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const float v = widen<T>(y.e[k]);
-            if (v >= least) {
-              const int at = atomicAdd(&w.count, 1);
-              if (at < kCandidates) w.candidate[at] = entry(v, s.first(s.lo + b * (kThreads * kBatch) + t + j * kThreads) + k);
-            }
-          }
+    if (top >= least) {
+#pragma unroll 4
+      for (int b = 0; b < batches; ++b)
+        if (group_top[b * kThreads + t] >= least) {
+          const int at = atomicAdd(&w.hits, 1);
+          if (at < kHits) w.hit[at] = s.lo + b * (kThreads * kBatch) + t;
         }
+    }
+    __syncthreads();
+    const int hits = w.hits;
+    if (hits > kHits) {
+      if (t == 0) w.count = kCandidates + 1;
+    } else {
+      for (int i = t; i < hits * kBatch; i += kThreads) {
+        const int piece = w.hit[i / kBatch] + i % kBatch * kThreads;
+        float v[VEC];
+        s.load(piece, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (v[k] >= least) {
+            const int at = atomicAdd(&w.count, 1);
+            if (at < kCandidates) w.candidate[at] = entry(v[k], s.first(piece) + k);
+          }
       }
+    }
     __syncthreads();
     if (w.count > kCandidates) gather_exactly(s, l.top, w);
     __syncthreads();
