@@ -14,7 +14,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kBatch = 4;       // 16-byte pieces that a thread has in flight, whose largest logit it remembers
-constexpr size_t kMostSmem = 96 * 1024;         // for the batches' largest logits: 66 KB for 262144 of four bytes
+constexpr size_t kMostSmem = 96 * 1024;         // for the batches' largest logits: 33 KB for 262144 of four bytes
 constexpr int kHits = 512;                      // batches that may hold some of them
 constexpr int kCandidates = 1024;               // logits that may be sorted for the alternatives
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -238,7 +238,7 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_constant__ Params p) {
   constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ float group_top[];      // [batches][threads]
+  extern __shared__ uint16_t group_top[];   // [batches][threads]: the upper halves of their keys
   __shared__ Shared w;
   const LogProbs& l = p.l;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = p.share == 1 ? 0 : blockIdx.x % p.share;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     Sixteen<T> next[kBatch];
     if (b + 1 < batches) load(b + 1, next);
     const float mx = largest(x);
-    if (l.top) group_top[b * kThreads + t] = mx;
+    if (l.top) group_top[b * kThreads + t] = (uint16_t)(key_of(mx) >> 16);
     if (mx > below_infinity(top)) {     // (infinities share all probability: each counts as the largest number)
       if (top > -INFINITY) lower(sum, mean, top, mx, k2);
       top = mx;
@@ -346,10 +346,11 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     }
     // batches that hold one, then their pieces, a thread for each
     const float least = value_of(bound);
+    const uint16_t upper = (uint16_t)max(bound >> 16, 1u);
     if (top >= least) {
 #pragma unroll 4
       for (int b = 0; b < batches; ++b)
-        if (group_top[b * kThreads + t] >= least) {
+        if (group_top[b * kThreads + t] >= upper) {
           const int at = atomicAdd(&w.hits, 1);
           if (at < kHits) w.hit[at] = s.lo + b * (kThreads * kBatch) + t;
         }
@@ -449,7 +450,7 @@ template <typename T> int launch(const LogProbs& l, cudaStream_t stream) {
   p.share = 1;
   while (p.share < 8 && l.rows * p.share < 148 && pieces / p.share > 2 * kThreads) p.share *= 2;
   p.batches = ((pieces + p.share - 1) / p.share + kThreads * kBatch - 1) / (kThreads * kBatch);
-  const size_t smem = l.top ? sizeof(float) * (size_t)p.batches * kThreads : 0;
+  const size_t smem = l.top ? sizeof(uint16_t) * (size_t)p.batches * kThreads : 0;
   auto* fn = log_probs_kernel<T>;
   static std::atomic<uint64_t> told{0};
   if (smem > kMostSmem || !once_per_device(told, [&] { return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) == cudaSuccess; })) return -2;
