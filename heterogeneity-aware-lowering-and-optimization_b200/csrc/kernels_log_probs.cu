@@ -258,6 +258,13 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
   const float k2 = fminf(kLog2e / T1, FLT_MAX);
   if (t == 0) { w.count = 0; w.hits = 0; }
 
+  // the first given tokens' logits, on their way while the row is read
+  float given = -INFINITY;
+  if (rank == 0 && t < l.given) {
+    const int token = l.tokens[r * l.given + t];
+    if (token >= 0 && token < l.vocab) given = widen<T>(s.row[token]);
+  }
+
   float top = -INFINITY, sum = 0.f, mean = 0.f;
   auto load = [&](int b, Sixteen<T> (&x)[kBatch]) {
     const int piece = s.lo + b * (kThreads * kBatch) + t;
@@ -328,21 +335,27 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) keys[i] = w.key[i * 32 + lane];
     uint32_t bound = 0;
+    if (l.top == 1) {          // (the largest logit itself)
 #pragma unroll
-    for (int shift = 28; shift >= 16; shift -= 4) {
-      int* counts = w.above[shift >> 2 & 1];
+      for (int i = 0; i < kThreads / 32; ++i) bound = max(bound, keys[i]);
+      bound = __reduce_max_sync(~0u, bound);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 16; e += kWarps) {
-        const uint32_t at = bound | (uint32_t)(warp + e) << shift;
-        int above = 0;
+      for (int shift = 28; shift >= 16; shift -= 4) {
+        int* counts = w.above[shift >> 2 & 1];
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) above += keys[i] >= at;
-        above = __reduce_add_sync(~0u, above);
-        if (lane == 0) counts[warp + e] = above;
+        for (int e = 0; e < 16; e += kWarps) {
+          const uint32_t at = bound | (uint32_t)(warp + e) << shift;
+          int above = 0;
+#pragma unroll
+          for (int i = 0; i < kThreads / 32; ++i) above += keys[i] >= at;
+          above = __reduce_add_sync(~0u, above);
+          if (lane == 0) counts[warp + e] = above;
+        }
+        __syncthreads();
+        const uint32_t enough = __ballot_sync(~0u, lane < 16 && counts[lane & 15] >= l.top) | 1u;   // (falling counts)
+        bound |= (uint32_t)(31 - __clz(enough)) << shift;
       }
-      __syncthreads();
-      const uint32_t enough = __ballot_sync(~0u, lane < 16 && counts[lane & 15] >= l.top) | 1u;   // (falling counts)
-      bound |= (uint32_t)(31 - __clz(enough)) << shift;
     }
     // batches that hold one, then their pieces, a thread for each
     const float least = value_of(bound);
@@ -416,7 +429,8 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     if (!(v > -INFINITY) || (row_top == INFINITY && v < INFINITY)) return -INFINITY;
     return (below_infinity(v) - base) / T1 - log_sum;
   };
-  for (int i = t; i < l.given; i += kThreads) {
+  if (t < l.given) l.token_log_probs[r * l.given + t] = log_prob(given);
+  for (int i = t + kThreads; i < l.given; i += kThreads) {
     const int token = l.tokens[r * l.given + i];
     l.token_log_probs[r * l.given + i] = token >= 0 && token < l.vocab ? log_prob(widen<T>(s.row[token])) : -INFINITY;
   }
