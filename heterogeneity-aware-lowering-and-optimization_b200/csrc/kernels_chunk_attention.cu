@@ -418,6 +418,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     // join them or the other tile, once all products are done.
     const bool hands = split && tile, takes = split && !tile && takes1, shared = p.share > 1, wide = hands || shared;
     if (ok && own_steps) ok = warp_wait(&w.o_done[tile], (own_steps - 1) & 1);
+    else if (ok && p.row_boxes) ok = warp_wait(&w.q_full, 0);   // (nobody else may have waited for queries without positions, and they must not land on the zeros)
     if (ok && wide && steps) ok = warp_wait(&w.all_done, 0);   // (the other tile's o_done has phases that this one does not follow)
     tc_fence_after();
     const uint32_t wide_at = wide_base + (uint32_t)r * kWideRow;
@@ -491,10 +492,9 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
         fence_async_proxy();
         asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");   // (the tile's four warps)
         if (*abort_flag) {
-          if (live) {
           T* y = (T*)p.a.y + (int64_t)(first_row + j) * p.a.y_token + (int64_t)(head * p.group + row - j * p.group) * p.a.y_head;
-          for (int c = 0; c < kPieces; ++c) ((uint4*)y)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);   // (no numbers)
-          }
+          if (live)
+            for (int c = 0; c < kPieces; ++c) ((uint4*)y)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);   // (no numbers)
         } else if (quarter == 0 && lane == 0) {
           for (int c = 0; c < kBoxes; ++c) store_rows(s_q + tile * kUnit + c * kBox, &results, c * 64, head * p.group, first_row + token_of(p, row0 + p.half_rows * tile));
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -664,7 +664,11 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
             last_turn = split ? i >> 1 : i;
           }
         }
-        if (!ok) { umma_commit(&w.drained[0]); await_landing(&w.drained[0], 0); }   // products in flight end before their memory goes
+        if (!ok) {   // products and queries in flight end before their memory goes
+          umma_commit(&w.drained[0]);
+          await_landing(&w.drained[0], 0);
+          if (p.row_boxes) await_landing(&w.q_full, 0);
+        }
       }
     } else {
       const uint32_t idesc = common | (1u << 16) | ((uint32_t)(D >> 3) << 17), sixteen = p.group_bytes >> 3;   // (16 positions further, in units of 16 bytes)
@@ -699,13 +703,14 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
             }
             if (!ok) break;
             umma_commit(&w.o_done[t]);
-            if (split) umma_commit(&w.v_empty[at.slot]);
+            if (split && i + n_values < steps) umma_commit(&w.v_empty[at.slot]);
           }
         }
       }
       if (issues) {
-        if (ok) umma_commit(&w.all_done);
-        else { umma_commit(&w.drained[1]); await_landing(&w.drained[1], 0); }
+        uint64_t* last = ok ? &w.all_done : &w.drained[1];
+        umma_commit(last);
+        await_landing(last, 0);   // (no arrival is under way when the block ends)
       }
     }
   }

@@ -193,3 +193,20 @@ def test_log_probs_over_and_over_have_the_same_bits(odla, gpu_lib):
         for _ in range(20):
             again = P.call_log_probs(odla, gpu_lib, logits, torch.zeros((rows, 1), dtype=torch.int32, device="cuda"), 20)
             assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv,channels,page,prefix", [
+    ([512, 256], [0, 0], 4, 4, 128, 32, 0),                  # whole tiles of tokens that see nothing
+    ([700], [100], 8, 8, 64, 16, 0),                         # the first halves of tiles, and the halves of one
+    ([300, 128, 700], [44, 0, 700], 8, 2, 128, 16, 0),
+    ([112] * 6, [0, 60, 0, 5, 0, 2000], 8, 8, 128, 64, 0),   # few positions for many blocks, behind a wide table
+])
+def test_chunk_queries_without_positions_leave_zeros(odla, gpu_lib, new, lengths, heads, kv, channels, page, prefix):
+    case = T.chunk_case(2, new, lengths, heads, kv, channels, page, prefix, q_scale=100.0)
+    y = T.check_chunk(odla, gpu_lib, case)
+    at = 0
+    for n, own in zip(new, lengths):
+        assert (y[at:at + max(0, n - own)] == 0).all()
+        at += n
+    for _ in range(10):
+        assert torch.equal(T.P.call_chunk(odla, gpu_lib, *case, T.R.scale_of(channels), y=torch.full_like(y, 7.0)), y)
