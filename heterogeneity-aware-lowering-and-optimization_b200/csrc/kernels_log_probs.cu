@@ -93,9 +93,23 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
+// Two numbers, raised to the lowest (minus infinity and NaN become that): of fp16, and a power of two that leaves a difference of two bf16 numbers finite.
+template <typename T> __device__ __forceinline__ float lowest() { return 0.f; }
+template <> __device__ __forceinline__ float lowest<__half>() { return -65504.f; }
+template <> __device__ __forceinline__ float lowest<__nv_bfloat16>() { return -0x1p122f; }
+template <typename T> __device__ __forceinline__ float2 pair_above(uint32_t u) { return make_float2(0.f, 0.f); }
+template <> __device__ __forceinline__ float2 pair_above<__half>(uint32_t u) {
+  asm("max.f16x2 %0, %0, %1;" : "+r"(u) : "r"(0xfbfffbffu));
+  return __half22float2(*(const __half2*)&u);
+}
+template <> __device__ __forceinline__ float2 pair_above<__nv_bfloat16>(uint32_t u) {
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(u) : "r"(0xfc80fc80u));
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
 __device__ __forceinline__ float exp2_fast(float x) {
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
-  return x;
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // Whole numbers in the order of the floats; minus infinity, and NaN, which counts as that, are 0.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -254,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
   const int pieces = (s.off + l.vocab + VEC - 1) / VEC, each = p.share == 1 ? pieces : (pieces + p.share - 1) / p.share;
   s.lo = min(pieces, rank * each);
   s.hi = min(pieces, s.lo + each);
-  const float temperature = l.temperature ? l.temperature[r] : 1.f, T1 = temperature > 0.f ? temperature : 1.f;
+  const float temperature = l.temperature ? l.temperature[r] : 1.f, T1 = temperature > 0.f ? fminf(temperature, 0x1p100f) : 1.f;   // (up to there a difference beyond fp32 weighs nothing)
   const float k2 = fminf(kLog2e / T1, FLT_MAX);
   if (t == 0) { w.count = 0; w.hits = 0; }
 
@@ -279,6 +293,8 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
   const int batches = (s.hi - s.lo + kThreads * kBatch - 1) / (kThreads * kBatch);
   Sixteen<T> x[kBatch];
   if (batches) load(0, x);
+  // (two at a time save four-byte types a twentieth and cost two-byte ones, with their longer code, a tenth)
+#pragma unroll (sizeof(T) == 4 ? 2 : 1)
   for (int b = 0; b < batches; ++b) {
     Sixteen<T> next[kBatch];
     if (b + 1 < batches) load(b + 1, next);
@@ -290,7 +306,18 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     }
     const float base = below_infinity(top);
     float2 sums[2] = {}, means[2] = {};
-    if (top < INFINITY) {
+    const float far = (base - lowest<T>()) * k2;
+    if (sizeof(T) == 2 && far >= 64.f && far <= 1e30f) {   // (the lowest stands for what has no probability)
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 y = mul2(add2(pair_above<T>(x[j].u[k]), make_float2(-base, -base)), make_float2(k2, k2));
+          const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+          sums[k & 1] = add2(sums[k & 1], e);
+          means[k & 1] = fma2(e, y, means[k & 1]);
+        }
+    } else if (top < INFINITY) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
 #pragma unroll
@@ -427,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
   const float row_top = w.top, base = below_infinity(row_top), log_sum = w.log_sum;
   auto log_prob = [&](float v) {
     if (!(v > -INFINITY) || (row_top == INFINITY && v < INFINITY)) return -INFINITY;
-    return (below_infinity(v) - base) / T1 - log_sum;
+    return (below_infinity(v) * 0.5f - base * 0.5f) / T1 * 2.f - log_sum;   // (halves: the difference may pass fp32's range, the quotient not)
   };
   if (t < l.given) l.token_log_probs[r * l.given + t] = log_prob(given);
   for (int i = t + kThreads; i < l.given; i += kThreads) {

@@ -650,8 +650,8 @@ typedef struct {
 int odla_b200_chunk_attention(const odla_b200_paged_cache* cache, const void* key_cache, const void* value_cache, const odla_b200_chunk_attention_desc* desc,
                               const void* q, const int* starts, const int* prefix_pages, const int* page_table, const int* lengths, void* y, void* stream);
 
-/* Log probabilities in rows of logits, logits[r * row + i], i < vocab (at most 262144), at a temperature (temperature: [rows], NULL or a value that is not above 0: 1):
- *   log p_i = (l_i - max l) / T - log(sum over j of exp((l_j - max l) / T)), with sums in 32 bits: good to 2^-17, absolutely or relatively (measured: 2^-21).
+/* Log probabilities in rows of logits, logits[r * row + i], i < vocab (at most 262144), at a temperature (temperature: [rows], NULL or a value that is not above 0: 1; more than 2^100: 2^100):
+ *   log p_i = (l_i - max l) / T - log(sum over j of exp((l_j - max l) / T)), with sums in 32 bits: good to 2^-17, absolutely or relatively (measured: 2^-21); below the lowest fp32 number: minus infinity.
  * tokens: [rows][given] token numbers -> token_log_probs [rows][given], minus infinity for numbers that are no tokens (the tokens of odla_b200_sample, of a prompt,
  * -1 in a padded batch).  entropy: [rows], -sum of p log p, or NULL.  top_tokens, top_log_probs: [rows][top], the top (0 ... 64) largest logits in descending
  * order, ties in favour of the lower index; -1 and minus infinity where no token is left.

@@ -210,3 +210,30 @@ def test_chunk_queries_without_positions_leave_zeros(odla, gpu_lib, new, lengths
         at += n
     for _ in range(10):
         assert torch.equal(T.P.call_chunk(odla, gpu_lib, *case, T.R.scale_of(channels), y=torch.full_like(y, 7.0)), y)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("middle", [0.0, 3e4, -3e4, -6.5e4, 1e36, -4e36, 1e38, -3e38])
+def test_log_probs_far_from_what_has_no_probability(odla, gpu_lib, dtype, middle):
+    """Logits around a middle near either end of their type, between minus infinities, NaN and the type's lowest, hot and cold."""
+    if dtype == 1 and abs(middle) > 65504:
+        pytest.skip("not a number of fp16")
+    g = T.gen(dtype, int(abs(middle)) % 1000003)
+    rows, vocab = 9, 5003
+    z = T.randn(g, (rows, vocab), 0).double() * (abs(middle) / 64 + 1) + middle
+    z = z.clamp(-torch.finfo(R.TORCH[dtype]).max, torch.finfo(R.TORCH[dtype]).max).to(R.TORCH[dtype])
+    kind = torch.randint(0, 8, (rows, vocab), generator=g, device="cuda")
+    z[kind == 0], z[kind == 1], z[kind == 2] = -float("inf"), float("nan"), torch.finfo(R.TORCH[dtype]).min
+    z[3, 100:] = -float("inf")
+    z[4, :4000] = -float("inf")
+    z[5, :4000] = torch.finfo(R.TORCH[dtype]).min
+    temperature = torch.tensor([1.0, 300.0, 1400.0, 1.0, 1.0, 1.0, 1500.0, 1e5, 1e-3], device="cuda")
+    tokens = torch.randint(0, vocab, (rows, 40), generator=g, device="cuda", dtype=torch.int32)
+    got = P.call_log_probs(odla, gpu_lib, z, tokens, 20, temperature)
+    given, given_tol, entropy, entropy_tol, order, lp, lp_tol = P.log_probs(z, tokens, 20, temperature)
+    # (what lies half a step or more below the lowest fp32 number rounds to minus infinity: -3.4e38 at a temperature of 1e-3)
+    beyond = -torch.finfo(torch.float32).max * (1 + 2.0 ** -25)
+    P.near(got[0], torch.where(given < beyond, -float("inf"), given), given_tol, "given")
+    P.near(got[1], entropy, entropy_tol, "entropy")
+    assert torch.equal(got[2], order)
+    P.near(got[3], torch.where(lp < beyond, -float("inf"), lp), lp_tol, "alternatives")
