@@ -249,6 +249,8 @@ template <typename T> __device__ __noinline__ void gather_exactly(const Slice<T>
 // are few, and are found again through the remembered maximum of each batch of pieces.  The sixteen upper bits of the bound are enough; four at a
 // time, each warp counts for one of their sixteen values (bit by bit, 32 barriers and lists that the first CTA fetched entry by entry
 // made up 22 of 32 us for 64 rows of 128000 logits).  A candidate's place is the number of those in front of it.
+// 1024 rows of 131072 fp32 logits: 100 us, 5.4 TB/s, 90 without alternatives.  Two-byte logits are bound by the issue slots, some nine instructions each: 2048 rows of 128000 bf16 97 us
+// (5.4 TB/s), 113 with 20 alternatives.  64 such rows take 11.5 us, 7 without, a chain of barriers; four CTAs share each.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_constant__ Params p) {
   constexpr int VEC = 16 / sizeof(T);

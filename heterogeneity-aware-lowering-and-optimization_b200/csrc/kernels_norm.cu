@@ -11,7 +11,7 @@
 namespace b200 {
 namespace {
 
-constexpr unsigned kMany = 4 * 148;
+constexpr unsigned kMany = 4 * 148;   // rows from which on a thread has kEach pieces of each (four blocks for each SM)
 constexpr int kEach = 2;
 constexpr int kMaxThreads = 1024, kShort = 32, kShortThreads = 256, kRows = 2;   // threads of a row; of a row that shares its block with others
 
@@ -149,7 +149,9 @@ struct Params {
 // h = round(x + residual), y = h / sqrt(mean(h h) + epsilon) * (w + offset), and y in 8 bits with scales.
 // Bound by memory: x and residual are read once and stay in registers (NP pieces of 16 bytes a thread), each result is written once.  Sums of squares
 // are 32-bit, by thread, then by warp, then by block.
-// Largest magnitudes are compared as whole numbers, which order them and keep a NaN.
+// Largest magnitudes are compared as whole numbers across threads, which order them and keep a NaN.
+// 8191 rows of 5120 fp16 values with residual, sum and int8: 69 us, 5.5 TB/s and three quarters of the issue slots; without the 8 bits 52 us.
+// 64 rows of 4096: 2.5 us, a chain of loads, two sums over the block and stores.
 template <typename T, int VEC, int NP>
 __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) norm_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint32_t tops[];      // of each group (group_shift -2)
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
 }
 
 // The same for rows of up to 32 pieces (heads): `lanes` threads of a warp have a piece each, of ROWS rows, whose loads are under way together and which
-// share the weight (a row for each: 27.7 us for 4097 tokens of 32 heads of 128).
+// share the weight (4097 tokens of 32 heads of 128: 17.5 us, three quarters of the issue slots; 18.7 with a row for each).
 template <typename T, int VEC, int ROWS>
 __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_constant__ Params p) {
   const RmsNorm& n = p.n;
@@ -374,7 +376,8 @@ template <typename T> int launch(const RmsNorm& n, cudaStream_t stream) {
     each = n.total / p.rows_of_block >= kMany * kRows ? kRows : 1;
     fn = each == 1 ? short_kernel<T, VEC, 1> : short_kernel<T, VEC, kRows>;
   } else {
-    // one piece for each thread, up to 1024; two where rows are many, so that more of them are under way
+    // one piece for each thread, up to 1024; two where rows are many, so that more of them are under way (rows of 4096 bf16 with
+    // a residual and e4m3, one and two: 64 rows 2.5 and 2.8 us, 512 5.0 and 5.7, 1024 7.8 both, 2048 17.0 and 14.2)
     p.rows_of_block = 1;
     const int wanted = wide && n.total >= kMany ? (p.pieces + kEach - 1) / kEach : p.pieces;
     threads = std::max(64, std::min(kMaxThreads, (wanted + 31) / 32 * 32));
