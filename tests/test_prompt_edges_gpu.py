@@ -237,3 +237,30 @@ def test_log_probs_far_from_what_has_no_probability(odla, gpu_lib, dtype, middle
     P.near(got[1], entropy, entropy_tol, "entropy")
     assert torch.equal(got[2], order)
     P.near(got[3], torch.where(lp < beyond, -float("inf"), lp), lp_tol, "alternatives")
+
+
+def test_chunk_many_sequences(odla, gpu_lib):
+    """More sequences than a block has threads, some without new tokens, one with many."""
+    rng = random.Random(5)
+    new = [rng.choice([0, 1, 1, 1, 2, 3]) for _ in range(1000)]
+    new[900] = 200
+    lengths = [n + rng.randint(0, 60) for n in new]
+    T.check_chunk(odla, gpu_lib, T.chunk_case(1, new, lengths, 4, 2, 64, 16, 0, poison=False))
+    T.check_chunk(odla, gpu_lib, T.chunk_case(2, new[:700] + [70, 0, 0], lengths[:700] + [70, 3, 0], 2, 1, 128, 24, 20, poison=False))
+
+
+@pytest.mark.parametrize("page", [16, 24])
+def test_chunk_lengths_beyond_the_table(odla, gpu_lib, page):
+    case = list(T.chunk_case(2, [40, 3, 200], [300, 20, 200], 8, 2, 128, page, 0, poison=False))
+    case[6] = case[6].clamp(min=0)          # (every entry a page that is there)
+    case[7] = torch.tensor([100000, 2 ** 31 - 1, 333], dtype=torch.int32, device="cuda")
+    T.check_chunk(odla, gpu_lib, case)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("rows,vocab,given", [(1, 60000, 1000), (2, 300, 257), (160, 5001, 512), (3, 262144, 300)])
+def test_log_probs_of_many_tokens(odla, gpu_lib, dtype, rows, vocab, given):
+    g = T.gen(dtype, rows, vocab, given)
+    z = T.logits_of(g, rows, vocab, dtype)
+    tokens = torch.randint(-2, vocab + 2, (rows, given), generator=g, device="cuda", dtype=torch.int32)
+    T.check_log_probs(odla, gpu_lib, z, tokens, 7, torch.full((rows,), 0.8, device="cuda"))
