@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     }
     const float base = below_infinity(top);
     float2 sums[2] = {}, means[2] = {};
-    const float far = (base - lowest<T>()) * k2;
+    const float far = (top - lowest<T>()) * k2;   // (infinite with the largest logit, whatever the temperature)
     if (sizeof(T) == 2 && far >= 64.f && far <= 1e30f) {   // (the lowest stands for what has no probability)
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
