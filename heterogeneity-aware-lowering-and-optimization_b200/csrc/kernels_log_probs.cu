@@ -150,9 +150,9 @@ template <typename T> struct Slice {
   }
 };
 
-// Relative to a larger maximum.
+// Relative to a larger maximum.  (Below an infinite one nothing is left of finite logits.)
 __device__ __forceinline__ void lower(float& sum, float& mean, float top, float to, float k2) {
-  const float shift = top > -INFINITY ? fmaxf((below_infinity(top) - below_infinity(to)) * k2, -200.f) : 0.f, f = exp2f(shift);
+  const float shift = top == to || !(top > -INFINITY) ? 0.f : to < INFINITY ? fmaxf((top - to) * k2, -200.f) : -200.f, f = exp2f(shift);
   mean = f * (mean + shift * sum);
   sum *= f;
 }
@@ -302,11 +302,10 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
     if (b + 1 < batches) load(b + 1, next);
     const float mx = largest(x);
     if (l.top) group_top[b * kThreads + t] = (uint16_t)(key_of(mx) >> 16);
-    if (mx > below_infinity(top)) {     // (infinities share all probability: each counts as the largest number)
+    if (mx > top) {     // (infinities share all probability)
       if (top > -INFINITY) lower(sum, mean, top, mx, k2);
       top = mx;
     }
-    const float base = below_infinity(top);
     float2 sums[2] = {}, means[2] = {};
     const float far = (top - lowest<T>()) * k2;   // (infinite with the largest logit, whatever the temperature)
     if (sizeof(T) == 2 && far >= 64.f && far <= 1e30f) {   // (the lowest stands for what has no probability)
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
       for (int j = 0; j < kBatch; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float2 y = mul2(add2(pair_above<T>(x[j].u[k]), make_float2(-base, -base)), make_float2(k2, k2));
+          const float2 y = mul2(add2(pair_above<T>(x[j].u[k]), make_float2(-top, -top)), make_float2(k2, k2));
           const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
           sums[k & 1] = add2(sums[k & 1], e);
           means[k & 1] = fma2(e, y, means[k & 1]);
@@ -324,25 +323,18 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const __grid_con
       for (int j = 0; j < kBatch; ++j)
 #pragma unroll
         for (int k = 0; k < VEC; k += 2) {
-          float2 y = mul2(add2(make_float2(widen<T>(x[j].e[k]), widen<T>(x[j].e[k + 1])), make_float2(-base, -base)), make_float2(k2, k2));
+          float2 y = mul2(add2(make_float2(widen<T>(x[j].e[k]), widen<T>(x[j].e[k + 1])), make_float2(-top, -top)), make_float2(k2, k2));
           y.x = fmaxf(y.x, -150.f);   // (2^-150 is 0; NaN becomes that, too)
           y.y = fmaxf(y.y, -150.f);
           const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
           sums[k >> 1 & 1] = add2(sums[k >> 1 & 1], e);
           means[k >> 1 & 1] = fma2(e, y, means[k >> 1 & 1]);
         }
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < kBatch * VEC; ++i) {
-        float v = -INFINITY;
+    } else {   // (infinities alone have a weight, of 1)
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j)
+      for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) v = i == j * VEC + k ? widen<T>(x[j].e[k]) : v;
-        const float y = fmaxf((below_infinity(v) - base) * k2, -150.f), e = v > -INFINITY ? exp2_fast(y) : 0.f;
-        sums[0].x += e;
-        means[0].x += e * y;
-      }
+        for (int k = 0; k < VEC; ++k) sums[k & 1].x += widen<T>(x[j].e[k]) == INFINITY ? 1.f : 0.f;
     }
     sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
     mean += (means[0].x + means[0].y) + (means[1].x + means[1].y);

@@ -29,3 +29,18 @@ def test_log_probs_infinities_at_high_temperatures(odla, gpu_lib, dtype, rows, v
     P.near(got[1], entropy, entropy_tol, "entropy")
     assert torch.equal(got[2], order)
     P.near(got[3], lp, lp_tol, "alternatives")
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows", [4, 200])     # rows that several blocks share, and rows of a block each
+def test_log_probs_infinities_beside_the_largest_number(odla, gpu_lib, dtype, rows):
+    """A finite logit has no probability beside an infinite one, the type's largest number included: in the same piece, another turn of its thread, another thread, another block."""
+    vocab, most = 20011, torch.finfo(R.TORCH[dtype]).max
+    for infinite, finite in (([9001], [9000, 9003]), ([9001], [9001 - 8192, 9001 - 4096]), ([9001], [9001 + 4096, 9001 + 8192]), ([9001, 9002], [5]), ([3], [19990]), ([20010], [0]), ([9001], range(vocab))):
+        z = T.logits_of(T.gen(dtype, rows), rows, vocab, dtype)
+        z[:, list(finite)] = most
+        z[1::2, list(finite)[-1]] = most * (1 - 2.0 ** -20) if dtype == 0 else most
+        z[:, infinite] = T.INF
+        tokens = torch.tensor([infinite[:1] + list(finite)[:2] + [7777]], dtype=torch.int32, device="cuda").expand(rows, -1).contiguous()
+        for temperature in (None, torch.full((rows,), 1e-3, device="cuda"), torch.full((rows,), HOTTEST, device="cuda")):
+            T.check_log_probs(odla, gpu_lib, z, tokens, 4, temperature, str((infinite, temperature is not None)))
