@@ -420,7 +420,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     // join them or the other tile, once all products are done.
     const bool hands = split && tile, takes = split && !tile && takes1, shared = p.share > 1, wide = hands || shared;
     if (ok && own_steps) ok = warp_wait(&w.o_done[tile], (own_steps - 1) & 1);
-    else if (ok && p.row_boxes) ok = warp_wait(&w.q_full, 0);   // (nobody else may have waited for queries without positions, and they must not land on the zeros)
+    else if (ok) ok = warp_wait(&w.q_full, 0);   // (nobody else may have waited for queries without positions: neither boxes nor another warp's rows must land on the zeros)
     if (ok && wide && steps) ok = warp_wait(&w.all_done, 0);   // (the other tile's o_done has phases that this one does not follow)
     tc_fence_after();
     const uint32_t wide_at = wide_base + (uint32_t)r * kWideRow;

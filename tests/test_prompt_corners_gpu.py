@@ -44,3 +44,20 @@ def test_log_probs_infinities_beside_the_largest_number(odla, gpu_lib, dtype, ro
         tokens = torch.tensor([infinite[:1] + list(finite)[:2] + [7777]], dtype=torch.int32, device="cuda").expand(rows, -1).contiguous()
         for temperature in (None, torch.full((rows,), 1e-3, device="cuda"), torch.full((rows,), HOTTEST, device="cuda")):
             T.check_log_probs(odla, gpu_lib, z, tokens, 4, temperature, str((infinite, temperature is not None)))
+
+
+@pytest.mark.parametrize("channels", [64, 128])
+@pytest.mark.parametrize("heads,kv,scale", [(8, 2, -0.1), (8, 8, 0.0), (33, 1, 0.1), (48, 1, 0.1), (8, 2, 0.1)])
+@pytest.mark.parametrize("new,lengths", [([512, 256], [0, 0]), ([700], [100]), ([300, 128, 700], [44, 0, 700]), ([112] * 6, [0, 60, 0, 5, 0, 2000]), ([3, 2, 1], [0, 0, 0])])
+def test_chunk_queries_that_are_no_boxes_leave_zeros(odla, gpu_lib, channels, heads, kv, scale, new, lengths):
+    """Tokens that see nothing where queries come by plain loads: a scale that is not positive, groups of heads that leave much of half a tile empty, strides of zero."""
+    case = list(T.chunk_case(2, new, lengths, heads, kv, channels, 16, 0, q_scale=100.0))
+    if (heads, scale) == (8, 0.1):
+        case[0] = case[0][:1].expand(case[0].shape)
+    y = T.check_chunk(odla, gpu_lib, case, scale=scale)
+    at = 0
+    for n, own in zip(new, lengths):
+        assert (y[at:at + max(0, n - own)] == 0).all()
+        at += n
+    for _ in range(10):
+        assert torch.equal(P.call_chunk(odla, gpu_lib, *case, scale, y=torch.full(y.shape, 7.0, dtype=y.dtype, device="cuda")), y)
