@@ -29,6 +29,7 @@ struct Params {
   int fold;                        // boxes bring all 128 channels: 1: pages and heads are counted together, 2: pages and positions are; 0: they bring 64
   uint32_t spin_limit;
   int test_skip_stage;             // test hook, as in kernels_umma.cu: block 0's second unit is neither loaded nor announced
+  int test_late;                   // test hook: the warp that hides values comes to each step some steps' time late
 };
 
 constexpr int kBarriers = 4 * kMostRing + 15 + kSeen;
@@ -153,7 +154,7 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     if (lane == 0) { w.abort = 0; w.odd = 0; w.found = 0; }
     for (int i = lane; i < kBarriers; i += 32) {
       uint64_t* bar = &w.k_full[0] + i;
-      mbar_init(bar, bar < w.k_empty ? (p.box_shift ? 33 : kLoaders * 33) : bar == &w.q_full ? (p.row_boxes ? 1 : kSoftmax) : (bar >= w.s_read && bar < w.o_done) || bar == &w.handed ? 4 : 1);
+      mbar_init(bar, bar < w.k_empty ? (p.box_shift ? 33 : kLoaders * 33) : bar == &w.q_full ? (p.row_boxes ? 1 : kSoftmax) : bar >= w.v_empty && bar < &w.q_full ? (p.box_shift ? 2 : 1) : (bar >= w.s_read && bar < w.o_done) || bar == &w.handed ? 4 : 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_proxy();
@@ -523,16 +524,20 @@ chunk_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorM
     }
     tc_fence_before();
   } else if (warp == kSoftmax + 1 && p.box_shift) {
-    // one warp asks for boxes; the other looks at the values of steps that not all rows see (it follows them all, to know the turns)
+    // one warp asks for boxes; the other looks at the values of steps that not all rows see.  It follows them all, and a place is filled again only when it has
+    // been here, too: two turns further the barrier's parity would be the same.
     Place at{0, 0};
     int hidden = 0;
     for (int i = 0; i < steps; ++i, next(at, n_values)) {
+      if (p.test_late) __nanosleep(20000);
       if (!warp_wait(&w.v_full[at.slot], at.turn)) break;
-      if (!hides_any(i)) continue;
-      hide(i, at.slot);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w.clean[hidden % kSeen]);
-      ++hidden;
+      if (hides_any(i)) {
+        hide(i, at.slot);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w.clean[hidden % kSeen]);
+        ++hidden;
+      }
+      if (lane == 0) mbar_arrive(&w.v_empty[at.slot]);
     }
   } else if (warp < kSoftmax + kLoaders) {
     // --------------------------------------------------------------------- loads ----
@@ -880,6 +885,7 @@ int chunk_attention(const ChunkAttention& a, cudaStream_t stream) {
   p.scale_log2e = a.scale * kLog2e;
   p.spin_limit = kSpinLimit;
   p.test_skip_stage = getenv("ODLA_B200_TEST_SKIP_STAGE") != nullptr;
+  p.test_late = getenv("ODLA_B200_TEST_LATE_WARP") != nullptr;
   if (const char* e = getenv("ODLA_B200_TEST_SPIN_LIMIT")) { const long v = atol(e); if (v >= 64 && v <= (1l << 18)) p.spin_limit = (uint32_t)v; }
   if (a.dt == DT_F16) return a.channels == 64 ? launch<__half, 64>(p, stream) : launch<__half, 128>(p, stream);
   return a.channels == 64 ? launch<__nv_bfloat16, 64>(p, stream) : launch<__nv_bfloat16, 128>(p, stream);

@@ -61,3 +61,17 @@ def test_chunk_queries_that_are_no_boxes_leave_zeros(odla, gpu_lib, channels, he
         at += n
     for _ in range(10):
         assert torch.equal(P.call_chunk(odla, gpu_lib, *case, scale, y=torch.full(y.shape, 7.0, dtype=y.dtype, device="cuda")), y)
+
+
+@pytest.mark.parametrize("new,cached,heads,kv,channels,page,prefix", [
+    ([600], [3000], 4, 1, 128, 16, 0),           # rings of two places
+    ([40], [6000], 2, 1, 128, 64, 300),          # of three, and positions that blocks share
+    ([300, 1, 77], [900, 2000, 0], 8, 2, 64, 32, 100),
+    ([1000] * 4, [1500] * 4, 8, 8, 64, 16, 0),
+])
+def test_chunk_a_warp_that_comes_late_misses_nothing(odla, gpu_lib, monkeypatch, new, cached, heads, kv, channels, page, prefix):
+    """The warp that takes hidden values out of the boxes is held up for several steps' time in front of each step, also of those that hide nothing."""
+    case = T.chunk_case(2, new, [n + c for n, c in zip(new, cached)], heads, kv, channels, page, prefix)
+    y = T.check_chunk(odla, gpu_lib, case)
+    monkeypatch.setenv("ODLA_B200_TEST_LATE_WARP", "1")
+    assert torch.equal(T.check_chunk(odla, gpu_lib, case), y)
