@@ -814,8 +814,9 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
                cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
       }))
     return -2;
-  // How many clusters of each size fit: the same for every call (GPUs of this kind have the same SMs).
-  static const Fit fit = [&] {
+  // How many clusters of each size fit: GPUs of one kind have the same number of SMs, but not in the same groups.
+  static PerDevice<Fit> fits;
+  const Fit fit = fits([&] {
     Fit f{};
     cfg.numAttrs = 1;
     for (int i = 1; i <= kMaxShare; ++i) {
@@ -825,7 +826,7 @@ template <typename T, int D> int launch(Params& p, cudaStream_t stream) {
     }
     f.clusters[1] = std::max(f.clusters[1], 1);
     return f;
-  }();
+  });
   // Rows of a tile and CTAs that share it: the shortest estimate of waves of steps (1.9 us, 1.2 for half a tile's rows) and of what a CTA does before and after them
   // (6 us, 2 more to join).  Lengths are not known here: the table's width stands for them.
   const int64_t steps = ((int64_t)p.a.table_width * p.a.page_size + kStep - 1) / kStep + (p.a.prefix_length + kStep - 1) / kStep;
