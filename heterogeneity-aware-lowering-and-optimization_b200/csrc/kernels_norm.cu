@@ -138,6 +138,13 @@ __device__ __forceinline__ float inverse_of(uint32_t top, float most) {
   return inverse;
 }
 
+// A mean of squares below 2^-90 or beyond fp32 (fp16 has none): the row is multiplied by a power of two that brings the sum of up to 32768 squares into range, epsilon
+// likewise, and summed again.  Of a row around 2^56 or more, values below 2^-54 lose bits then, of which less than 2^-126 is left in the result.
+template <typename T> __device__ __forceinline__ bool out_of_range(float mean) {
+  return !std::is_same<T, __half>::value && __float_as_uint(mean) - 0x12800000u > 0x7f7fffffu - 0x12800000u;
+}
+__device__ __forceinline__ float into_range(float mean) { return mean < 0x1p-90f ? 0x1p90f : 0x1p-72f; }
+
 struct Params {
   RmsNorm n;
   float per_channel;      // 1 / channels
@@ -206,7 +213,30 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
   square = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0.f;
 #pragma unroll
   for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
-  const float factor = rsqrtf(square * p.per_channel + n.epsilon);
+  float mean = square * p.per_channel + n.epsilon;
+  if (out_of_range<T>(mean)) {   // (all threads have the same)
+    const float by = into_range(mean);
+    square = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (t + i * p.lanes < p.pieces) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          h[i][k] *= by;
+          square += h[i][k] * h[i][k];
+        }
+      }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+    __syncthreads();   // (the first sums have been read)
+    if (lane == 0) sums[warp] = square;
+    __syncthreads();
+    square = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+    mean = square * p.per_channel + n.epsilon * by * by;
+  }
+  const float factor = rsqrtf(mean);
   uint32_t top[NP];
   uint32_t row_top = 0;
 #pragma unroll
@@ -300,33 +330,54 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
   if (c < p.pieces) load_weight<VEC>(n, c, w);
   const float most = n.quant == 1 ? 127.f : 448.f, given = p.group_shift == -3 ? n.scales[0] : 0.f;
   const int groups = n.group ? n.channels / n.group : 1;
+  float h[ROWS][VEC], mean[ROWS];
+  bool odd = false;
+  auto mean_of = [&](int i, float by) {
+    float square = 0.f;
+    if (there[i]) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) square += h[i][k] * h[i][k];
+    }
+    for (int o = p.lanes / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+    return square * p.per_channel + n.epsilon * by * by;
+  };
+  auto place = [&](int i, void* base, int part) { return (T*)base + (int64_t)rows[i] * n.row[part] + (int64_t)heads[i] * n.head[part] + c * VEC; };
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    auto place = [&](void* base, int part) { return (T*)base + (int64_t)rows[i] * n.row[part] + (int64_t)heads[i] * n.head[part] + c * VEC; };
-    float h[VEC], square = 0.f;
     if (there[i]) {
-      unpack<T, VEC>(x[i], h);
+      unpack<T, VEC>(x[i], h[i]);
       if (n.residual) {
         float v[VEC];
         unpack<T, VEC>(r[i], v);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] += h[k];
+        for (int k = 0; k < VEC; ++k) v[k] += h[i][k];
         pack<T, VEC>(v, x[i]);
-        unpack<T, VEC>(x[i], h);
+        unpack<T, VEC>(x[i], h[i]);
       }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) square += h[k] * h[k];
     }
-    if (there[i] && n.sum) *(decltype(x[i].raw)*)place(n.sum, 2) = x[i].raw;
-    for (int o = p.lanes / 2; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
-    const float factor = rsqrtf(square * p.per_channel + n.epsilon);
+    if (there[i] && n.sum) *(decltype(x[i].raw)*)place(i, n.sum, 2) = x[i].raw;
+    mean[i] = mean_of(i, 1.f);
+    odd = odd || out_of_range<T>(mean[i]);
+  }
+  if (__any_sync(~0u, odd)) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const float by = out_of_range<T>(mean[i]) ? into_range(mean[i]) : 1.f;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] *= by;
+      mean[i] = mean_of(i, by);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const float factor = rsqrtf(mean[i]);
     Piece<T, VEC> y;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) h[k] = h[k] * factor * w[k];
-    pack<T, VEC>(h, y);
-    if (there[i] && n.y) *(decltype(y.raw)*)place(n.y, 3) = y.raw;
+    for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * factor * w[k];
+    pack<T, VEC>(h[i], y);
+    if (there[i] && n.y) *(decltype(y.raw)*)place(i, n.y, 3) = y.raw;
     if (!n.quant) continue;
-    uint32_t top = there[i] ? __float_as_uint(magnitude<VEC>(h)) : 0u;
+    uint32_t top = there[i] ? __float_as_uint(magnitude<VEC>(h[i])) : 0u;
     float inverse = 0.f;
     if (p.group_shift != -3) {
       const int across = p.group_shift == -1 ? p.lanes : 1 << p.group_shift;
@@ -336,8 +387,8 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_const
     }
     Piece<uint8_t, VEC> q;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) h[k] = p.group_shift == -3 ? h[k] / given : h[k] * inverse;
-    if (n.quant == 1) to_int8<VEC>(h, p.group_shift != -3 && top < 0x7f800000u, q); else to_e4m3<VEC>(h, q);
+    for (int k = 0; k < VEC; ++k) h[i][k] = p.group_shift == -3 ? h[i][k] / given : h[i][k] * inverse;
+    if (n.quant == 1) to_int8<VEC>(h[i], p.group_shift != -3 && top < 0x7f800000u, q); else to_e4m3<VEC>(h[i], q);
     if (there[i]) *(decltype(q.raw)*)((uint8_t*)n.quantised + (int64_t)rows[i] * n.row[4] + (int64_t)heads[i] * n.head[4] + c * VEC) = q.raw;
   }
 }

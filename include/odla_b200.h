@@ -614,6 +614,7 @@ int odla_b200_sample(const odla_b200_sample_desc* desc, const void* logits, cons
  * or key heads inside a projection's rows.
  *   h = x + residual, rounded to dtype (residual NULL: h = x), stored to `sum` if that is not NULL;
  *   y = h / sqrt(mean of h h over the row + epsilon) * (weight + weight_offset), 32 bits throughout, rounded once; stored to `y` if that is not NULL.
+ *     Rows of any magnitude are right, those whose squares pass fp32's range included.
  * weight: [channels] of weight_dtype, NULL: all ones (weight_offset is added to them, too).
  * quant 1 or 2 stores y (not the rounded one) in 8 bits to `quantised`: int8 to the nearest, or e4m3 to the nearest.
  *   group > 0 (a divisor of channels, a multiple of 8 or all of them): a scale for each group of channels, scales[(r * heads + h) * (channels / group) + g] =

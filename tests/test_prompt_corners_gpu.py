@@ -75,3 +75,33 @@ def test_chunk_a_warp_that_comes_late_misses_nothing(odla, gpu_lib, monkeypatch,
     y = T.check_chunk(odla, gpu_lib, case)
     monkeypatch.setenv("ODLA_B200_TEST_LATE_WARP", "1")
     assert torch.equal(T.check_chunk(odla, gpu_lib, case), y)
+
+
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("rows,heads,channels", [(5, 1, 4096), (700, 1, 4096), (3, 1, 1001), (9, 5, 128), (3000, 4, 64), (2, 1, 32768), (2, 1, 20001), (700, 1, 5)])
+def test_norm_squares_beyond_fp32(odla, gpu_lib, dtype, rows, heads, channels):
+    """Rows whose squares pass fp32's range at either end, beside rows of ordinary size, without an epsilon and with one."""
+    g = T.gen(dtype, rows, channels)
+    size = 2.0 ** torch.tensor([0, 70, 126, -70, -120, 60, 10], dtype=torch.float64, device="cuda")[torch.randint(0, 7, (rows, heads, 1), generator=g, device="cuda")]
+    size[0, 0], size[-1, -1] = 2.0 ** 125, 2.0 ** -110
+    x = ((1 + torch.rand((rows, heads, channels), generator=g, device="cuda").double()) * size * (torch.randint(0, 2, (rows, heads, channels), generator=g, device="cuda") * 2 - 1)).to(R.TORCH[dtype])
+    w = (1 + 0.3 * torch.randn(channels, generator=g, device="cuda"))
+    for epsilon in (0.0, 1e-6, 1e30):
+        y, total = torch.empty_like(x), torch.empty_like(x)
+        q, scales = torch.empty(x.shape, dtype=torch.uint8, device="cuda"), torch.empty((rows, heads, 1), device="cuda")
+        assert P.call_norm(odla, gpu_lib, x, torch.zeros_like(x), w, total, y, q, scales, 1, channels, epsilon) == 0
+        want = P.norm(x, None, w, epsilon, 0.0)[1]
+        P.near(y, want, P.norm_tolerance(want, dtype) + 2.0 ** -126, "y")      # (below the smallest normal number of fp32, as much may be lost)
+        values, tol = P.eight_bits(want, 1, scales, False)
+        P.near(torch.where(scales >= 2.0 ** -119, q.view(torch.int8).double() * scales.double(), values), values, tol + 2.0 ** -126, "8 bits")   # (127 / max |y| beyond fp32: zeros)
+        assert torch.equal(total, x)
+
+
+@pytest.mark.parametrize("channels", [128, 4096])
+def test_norm_of_infinities_beside_large_numbers(odla, gpu_lib, channels):
+    x = torch.full((4, 1, channels), 3e38, device="cuda")
+    x[1, 0, 3], x[2, 0, 5] = T.INF, float("nan")
+    y = torch.empty_like(x)
+    assert P.call_norm(odla, gpu_lib, x, y=y) == 0
+    P.near(y[[0, 3]], torch.ones_like(y[[0, 3]]).double(), torch.full_like(y[[0, 3]], P.NORM).double())
+    assert y[1, 0, 3].isnan() and (y[1, 0, :3] == 0).all() and (y[1, 0, 4:] == 0).all() and y[2].isnan().all()
