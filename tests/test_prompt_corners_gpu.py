@@ -105,3 +105,17 @@ def test_norm_of_infinities_beside_large_numbers(odla, gpu_lib, channels):
     assert P.call_norm(odla, gpu_lib, x, y=y) == 0
     P.near(y[[0, 3]], torch.ones_like(y[[0, 3]]).double(), torch.full_like(y[[0, 3]], P.NORM).double())
     assert y[1, 0, 3].isnan() and (y[1, 0, :3] == 0).all() and (y[1, 0, 4:] == 0).all() and y[2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("new,cached,heads,kv,channels,page", [([40, 3], 300, 4, 2, 64, 16), ([700], 300, 8, 8, 128, 32), ([300, 130], 60, 4, 4, 64, 7), ([5], 6000, 8, 2, 128, 16)])
+def test_chunk_no_weight_at_all_gives_zeros_whatever_the_values(odla, gpu_lib, dtype, new, cached, heads, kv, channels, page):
+    """Scores of minus infinity throughout, values that are infinite or no numbers among those that all tokens see and among those that the later ones do."""
+    case = T.chunk_case(dtype, new, [n + cached for n in new], heads, kv, channels, page, 0, poison=False, behind=0)
+    q, starts, kc, vc, pp, prefix, table, lengths = case
+    q[..., 0] = 1.0
+    kc[..., 0] = -T.INF
+    for b, n in enumerate(new):
+        for p in (3, cached - 1, cached + n // 2, cached + n - 1):
+            vc[int(table[b, p // page]), :, p % page, ::3], vc[int(table[b, p // page]), :, p % page, 1::3] = T.INF, float("nan")
+    assert (P.call_chunk(odla, gpu_lib, *case, 0.125) == 0).all()
