@@ -93,7 +93,8 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
-// Two numbers, raised to the lowest (minus infinity and NaN become that): of fp16, and a power of two that leaves a difference of two bf16 numbers finite.
+// Two numbers, raised to the lowest (minus infinity and NaN become that): fp16's own, -2^122 for bf16.  (The largest bf16 numbers less that pass fp32: `far` is
+// infinite then, and the other way is taken.)
 template <typename T> __device__ __forceinline__ float lowest() { return 0.f; }
 template <> __device__ __forceinline__ float lowest<__half>() { return -65504.f; }
 template <> __device__ __forceinline__ float lowest<__nv_bfloat16>() { return -0x1p122f; }

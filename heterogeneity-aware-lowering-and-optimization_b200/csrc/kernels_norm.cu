@@ -159,6 +159,8 @@ struct Params {
 // Largest magnitudes are compared as whole numbers across threads, which order them and keep a NaN.
 // 8191 rows of 5120 fp16 values with residual, sum and int8: 69 us, 5.5 TB/s and three quarters of the issue slots; without the 8 bits 52 us.
 // 64 rows of 4096: 2.5 us, a chain of loads, two sums over the block and stores.
+// Rows that are no whole pieces of 16 bytes, or lie off them, go element by element: 2048 x 4001 bf16 52 us where 2048 x 4096 take 10 (in L2), 512 x 20001 117 us
+// (up to 32 elements a thread, which do not all stay in registers).
 template <typename T, int VEC, int NP>
 __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) norm_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint32_t tops[];      // of each group (group_shift -2)
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : kMaxThreads, NP == 2 ? 3 : 1) 
 }
 
 // The same for rows of up to 32 pieces (heads): `lanes` threads of a warp have a piece each, of ROWS rows, whose loads are under way together and which
-// share the weight (4097 tokens of 32 heads of 128: 17.5 us, three quarters of the issue slots; 18.7 with a row for each).
+// share the weight (4097 tokens of 32 heads of 128 bf16: 14.8 us out of a graph, three quarters of the issue slots; fp32 29 us).
 template <typename T, int VEC, int ROWS>
 __global__ void __launch_bounds__(kShortThreads) short_kernel(const __grid_constant__ Params p) {
   const RmsNorm& n = p.n;
